@@ -625,6 +625,93 @@ int ls_dense_attn_kvcache(const void* q, int64_t q_row_stride, const int32_t* cu
                           float softmax_scale, int32_t causal, int32_t n_splits, void* out,
                           float* softmax_lse, void* ws, size_t ws_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Decode over a KV cache held in 8 bits (no counterpart in the reference, whose
+ * cache is 16-bit: leanselect/models/minicpm.py:1188-1490).  A page is 64 tokens
+ * of one KV head, head_dim 128:
+ *   k8 [batch][pages][G][64 tokens][128]  e4m3
+ *   v8 [batch][pages][G][128][64 tokens]  e4m3, token 16 t + 4 q + i of a channel
+ *                                         at place 16 q + 4 t + i
+ *   k_scale, v_scale [batch][pages][G]    uint8, code c standing for 2^(c - 127)
+ * with the given batch strides (elements; the same for K and V).  An element
+ * stands for its e4m3 value times its page's power of two.
+ * ------------------------------------------------------------------------ */
+
+/*
+ * Append packed new tokens (k_new / v_new [total_new, G, 128] bf16 or fp16, rows
+ * new_row_stride apart; sequence b's rows are [cu_seqlens_new[b],
+ * cu_seqlens_new[b+1])) at positions cache_seqlens[b] + i.  A page's code becomes
+ * the least c >= 1 with max |x| <= 448 2^(c - 127) over its finite new rows, and
+ * at least the old code where it holds older rows (from before cache_seqlens[b]),
+ * which are then brought under the new one; rows after the new ones are left as
+ * they are.  Infinities and NaN are stored as NaN.  With kc_cache [batch]
+ * [kc_rows][G][128] (the dtype of k_new), the first max_new_windows windows that
+ * the new tokens complete are written: window w is the mean of the stored keys
+ * [16 w, 16 w + 32), float32 sums, one rounding.  Rows past `pages` pages and
+ * windows past kc_rows are not written.  cache_seqlens is not advanced.
+ */
+int ls_kvcache_append_q8(void* k8, void* v8, int64_t cache_batch_stride, uint8_t* k_scale,
+                         uint8_t* v_scale, int64_t scale_batch_stride, int64_t pages,
+                         const int32_t* cache_seqlens, const void* k_new, const void* v_new,
+                         int64_t new_row_stride, const int32_t* cu_seqlens_new, int64_t total_new,
+                         int32_t batch, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+                         void* kc_cache, int64_t kc_batch_stride, int64_t kc_row_stride,
+                         int64_t kc_rows, int64_t max_new_windows, void* stream);
+
+/*
+ * Attention of packed decode rows over the 8-bit cache: ls_sparse_attn_kvcache
+ * over the values it stands for, or ls_dense_attn_kvcache where topk_idx is NULL
+ * (topk is then not read).  A repeated plan id counts once.  Rows at and after
+ * cu_seqlens_q[batch] are left as they are.  A row without a visible key gets
+ * out = 0 and lse = +inf.  At most 16 query heads per KV head, topk <= 256,
+ * 1 <= n_splits <= 256; the workspace may be NULL for n_splits = 1.
+ */
+size_t ls_attn_kvcache_q8_workspace_size(int64_t total_q, int32_t num_kv_heads, int32_t n_splits);
+int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int32_t* cu_seqlens_q,
+                       int64_t total_q, const void* k8, const void* v8,
+                       int64_t cache_batch_stride, const uint8_t* k_scale, const uint8_t* v_scale,
+                       int64_t scale_batch_stride, int64_t pages, const int32_t* cache_seqlens,
+                       int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                       int32_t dtype, const int32_t* topk_idx, int32_t topk, float softmax_scale,
+                       int32_t causal, int32_t n_splits, void* out, float* softmax_lse,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Products of a few rows with 4-bit weights (no counterpart in the reference,
+ * whose projections are 16-bit: leanselect/models/minicpm.py:2176-2222,
+ * 1098-1135, 3987-4090).  A weight [N, K] (K a multiple of 8) is held as E2M1
+ * values with a power-of-two scale per 32 inputs, zero-padded, in the order
+ *   codes  [ceil(N/16)][ceil(K/128)][64][16] bytes: of each tile of 16 outputs by
+ *          128 inputs, lane 16 q + r holds inputs 32 q .. 32 q + 31 of output r,
+ *          the even input in a byte's low half
+ *   scales [ceil(N/16)][ceil(K/512)][64][4] bytes: the same lanes, byte i for the
+ *          i-th of four tiles; code c in [8, 252] stands for 2^(c - 127)
+ * ------------------------------------------------------------------------ */
+
+/*
+ * Lay out weight [N, K] (any dtype, finite, rows weight_row_stride apart): a
+ * group's code is the least c >= 8 with max |w| <= 6 2^(c - 127) (127 for zeros),
+ * at most 252 (larger magnitudes saturate); values to the nearest, ties to the
+ * even code.
+ */
+int ls_quantize_mx4(const void* weight, int64_t weight_row_stride, int64_t out_features,
+                    int64_t in_features, int32_t dtype, void* codes, void* scales, void* stream);
+
+/* The values [N, K] in bf16 (exact) or fp16 (rounded), rows out_row_stride apart. */
+int ls_dequantize_mx4(const void* codes, const void* scales, int64_t out_features,
+                      int64_t in_features, int32_t dtype, void* out, int64_t out_row_stride,
+                      void* stream);
+
+/*
+ * out[m][n] = sum_k x[m][k] w[n][k] in float32, rounded once to dtype (bf16 or
+ * fp16, also the type w's values are taken in); x [rows, K], out [rows, N].  With
+ * silu_mul, w is [gate; up] (N a multiple of 32) and out [rows, N / 2] is
+ * silu(gate) * up, float32 up to the rounding.
+ */
+int ls_linear_mx4(const void* x, int64_t x_row_stride, int64_t rows, int64_t in_features,
+                  const void* codes, const void* scales, int64_t out_features, int32_t silu_mul,
+                  int32_t dtype, void* out, int64_t out_row_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

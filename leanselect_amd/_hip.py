@@ -110,6 +110,17 @@ SIGNATURES = {
     "ls_dense_attn_kvcache": (
         _i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _i32, _i32, _i32, _i32, _i32, _f32,
                _i32, _i32, _p, _p, _p, _sz, _p]),
+    "ls_kvcache_append_q8": (
+        _i32, [_p, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _i32, _i32, _i32,
+               _i32, _p, _i64, _i64, _i64, _i64, _p]),
+    "ls_attn_kvcache_q8_workspace_size": (_sz, [_i64, _i32, _i32]),
+    "ls_attn_kvcache_q8": (
+        _i32, [_p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _p, _i32, _i32, _i32, _i32,
+               _i32, _p, _i32, _f32, _i32, _i32, _p, _p, _p, _sz, _p]),
+    "ls_quantize_mx4": (_i32, [_p, _i64, _i64, _i64, _i32, _p, _p, _p]),
+    "ls_dequantize_mx4": (_i32, [_p, _p, _i64, _i64, _i32, _p, _i64, _p]),
+    "ls_linear_mx4": (
+        _i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _i32, _i32, _p, _i64, _p]),
 }
 
 _lib = None
@@ -274,6 +285,19 @@ def stream_of(device: torch.device) -> int:
     # without an index is the current one.
     index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+def launch(device: torch.device, name: str, *args) -> None:
+    """Call entry point ``name`` on ``device``'s current stream (appended to ``args``), with that
+    device current while it launches."""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        rc = getattr(lib(), name)(*args, stream_of(device))
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(lib(), name)(*args, stream_of(device))
+    if rc != LS_OK:
+        check(rc, name)
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

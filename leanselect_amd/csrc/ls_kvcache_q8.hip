@@ -1,0 +1,676 @@
+// Decode over a KV cache held in 8 bits: quantising append and attention.
+//
+// Cache layout (the caller's tensors), a page being 64 tokens of one KV head:
+//   k8 [batch][pages][G][64 tokens][128]  e4m3
+//   v8 [batch][pages][G][128][64 tokens]  e4m3, a channel's 64 tokens together,
+//                                          token 16 t + 4 q + i at place 16 q + 4 t + i
+//   k_scale, v_scale [batch][pages][G]    uint8 codes, code c standing for 2^(c - 127)
+// An element stands for its e4m3 value times its page's power of two.  The code of a
+// page is the least c >= 1 with max |x| <= 448 2^(c - 127) over the finite rows it has
+// held since its first token, so nothing saturates; a power of two costs no precision
+// (e4m3 is a float) and changing it leaves a stored row exact unless it becomes subnormal.
+// Infinities and NaN are stored as NaN (e4m3 has no infinity) and do not count for the code.
+//
+// The orders are those in which the attention's matrix instructions read a page, so a
+// wave takes it from memory to registers in 16-byte loads without LDS:
+// S^T = K Q^T (rows are keys) gives lane (r, q) = (lane & 15, lane >> 4) the scores of head
+// r and tokens 16 t + 4 q + i, and P^T is the right operand of O^T = V^T P^T as it stands
+// when lane (r, q)'s 16 bytes of a channel's values are the tokens 16 t + 4 q + i.
+//
+// Extends ls_kvcache_append, ls_sparse_attn_kvcache and ls_dense_attn_kvcache (the
+// reference's cache is 16-bit: leanselect/models/minicpm.py:1188-1490).
+#include <algorithm>
+
+#include "ls_common.h"
+
+namespace {
+
+constexpr int kPage = 64;
+constexpr int kDim = 128;
+constexpr int kPageBytes = kPage * kDim;
+
+typedef float Q8F2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ int64_t q8_windows(int64_t len, int ks, int stride) {
+  return len >= ks ? (len - ks) / stride + 1 : 0;
+}
+
+// Largest finite magnitude of eight 16-bit values as 16 bits (their order is that of the
+// values); an infinity or NaN counts as zero.
+template <int DT>
+__device__ __forceinline__ uint32_t q8_abs_max(ls_u32x4 x, uint32_t top) {
+  constexpr uint32_t kInf = DT == LS_BF16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t lo = x[e] & 0x7fffu, hi = (x[e] >> 16) & 0x7fffu;
+    top = max(top, lo < kInf ? lo : 0u);
+    top = max(top, hi < kInf ? hi : 0u);
+  }
+  return top;
+}
+
+// The least code c >= 1 with m <= 448 2^(c - 127): 448 = 1.75 2^8.
+template <int DT>
+__device__ __forceinline__ uint32_t q8_code(uint32_t top16) {
+  const uint32_t bits = __float_as_uint(LsElem<DT>::to_f((uint16_t)top16));
+  const int c = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return (uint32_t)max(c, 1);
+}
+
+// 2^(e - 127) for e in [1, 254].
+__device__ __forceinline__ float q8_pow(int e) { return __uint_as_float((uint32_t)e << 23); }
+
+// Four floats as four e4m3 bytes, to nearest even (overflow and non-finite: NaN).
+__device__ __forceinline__ uint32_t q8_pack(float a, float b, float c, float d) {
+  uint32_t v = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, (int)v, true);
+}
+
+// Four stored bytes under a smaller power: times f, rounded to e4m3 again.
+__device__ __forceinline__ uint32_t q8_rescale(uint32_t v, float f) {
+  const Q8F2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)v, false);
+  const Q8F2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)v, true);
+  return q8_pack(lo[0] * f, lo[1] * f, hi[0] * f, hi[1] * f);
+}
+
+// The sequence that holds work unit `unit` when sequence b has count(b) units, in order:
+// a wave scans 64 sequences at a time.  Every lane gets the sequence and the unit's number
+// in it; -1 past the last unit.
+template <class Count>
+__device__ __forceinline__ int q8_find(int64_t& unit, int batch, Count count) {
+  const int lane = ls_lane();
+  for (int s0 = 0; s0 < batch; s0 += 64) {
+    const int64_t mine = s0 + lane < batch ? count(s0 + lane) : 0;
+    int64_t upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t y = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += y;
+    }
+    const uint64_t past = __ballot(unit < upto);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      unit -= __shfl(upto - mine, at, 64);
+      return s0 + at;
+    }
+    unit -= __shfl(upto, 63, 64);
+  }
+  return -1;
+}
+
+// ---------------------------------------------------------------------------
+// Append: a workgroup per (page that gets new rows, KV head).  It finds the largest
+// magnitude of the page's new rows, takes the page's code (at least the old one where the
+// page holds older rows), brings older rows under a raised code, and writes the new rows.
+// A page of a sequence belongs to one workgroup, so nothing is shared between them.
+// K: thread (row, c) takes the 8-channel pieces c, c + 4, c + 8, c + 12 of its row.
+// V: thread (quad, octet) takes 8 channels of the four tokens that share a 4-byte word.
+// ---------------------------------------------------------------------------
+template <int DT>
+__global__ __launch_bounds__(256) void ls_q8_append_kernel(
+    uint8_t* __restrict__ k8, uint8_t* __restrict__ v8, int64_t cbs, uint8_t* __restrict__ ks,
+    uint8_t* __restrict__ vs, int64_t sbs, int64_t pages, const int32_t* __restrict__ cache_seqlens,
+    const uint16_t* __restrict__ kn, const uint16_t* __restrict__ vn, int64_t nrs,
+    const int32_t* __restrict__ cu_new, int64_t total_new, int batch, int G) {
+  __shared__ uint32_t s_top[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int g = blockIdx.y;
+  int64_t unit = blockIdx.x;
+  const int b = q8_find(unit, batch, [&](int i) -> int64_t {
+    const int64_t len = cache_seqlens[i], n = cu_new[i + 1] - cu_new[i];
+    return n > 0 && len >= 0 ? (len + n + kPage - 1) / kPage - len / kPage : 0;
+  });
+  if (b < 0) return;
+  const int64_t len = cache_seqlens[b], n0 = cu_new[b];
+  const int64_t n1 = min((int64_t)cu_new[b + 1], total_new);
+  const int64_t page = len / kPage + unit;
+  if (page >= pages || n0 < 0) return;
+  const int64_t base = page * kPage;
+  const int r0 = (int)max<int64_t>(0, len - base);              // first new row of the page
+  const int r1 = (int)min<int64_t>(kPage, len + (n1 - n0) - base);
+  const int64_t at = (int64_t)b * cbs + (page * G + g) * kPageBytes;
+  const int64_t sat = (int64_t)b * sbs + page * G + g;
+  const int64_t first = (n0 + base - len) * nrs + (int64_t)g * kDim;  // the page's row 0, if it were new
+
+  const int krow = tid >> 2, kc = 8 * (tid & 3);
+  const bool knew = krow >= r0 && krow < r1;
+  const int quad = tid >> 4, oct = tid & 15;                    // quad = 4 q + t
+  const int tok = 16 * (quad & 3) + 4 * (quad >> 2);
+  ls_u32x4 kx[4], vx[4];
+  uint32_t ktop = 0, vtop = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    kx[j] = knew ? ls_load16(kn + first + krow * nrs + 32 * j + kc) : ls_u32x4{0u, 0u, 0u, 0u};
+    const bool vnew = tok + j >= r0 && tok + j < r1;
+    vx[j] = vnew ? ls_load16(vn + first + (tok + j) * nrs + 8 * oct) : ls_u32x4{0u, 0u, 0u, 0u};
+  }
+  uint32_t kold = 1, vold = 1;
+  if (r0 > 0) {
+    kold = ks[sat];
+    vold = vs[sat];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    ktop = q8_abs_max<DT>(kx[j], ktop);
+    vtop = q8_abs_max<DT>(vx[j], vtop);
+  }
+  ktop = ls_wave_max_u32(ktop);
+  vtop = ls_wave_max_u32(vtop);
+  if (lane == 0) {
+    s_top[0][w] = ktop;
+    s_top[1][w] = vtop;
+  }
+  __syncthreads();
+  ktop = max(max(s_top[0][0], s_top[0][1]), max(s_top[0][2], s_top[0][3]));
+  vtop = max(max(s_top[1][0], s_top[1][1]), max(s_top[1][2], s_top[1][3]));
+  const uint32_t kcode = max(q8_code<DT>(ktop), kold), vcode = max(q8_code<DT>(vtop), vold);
+  if (tid == 0) {
+    ks[sat] = (uint8_t)kcode;
+    vs[sat] = (uint8_t)vcode;
+  }
+  const float kinv = q8_pow(254 - (int)kcode), vinv = q8_pow(254 - (int)vcode);
+  const float kdown = q8_pow(max(127 + (int)kold - (int)kcode, 0));
+  const float vdown = q8_pow(max(127 + (int)vold - (int)vcode, 0));
+
+  uint8_t* kp = k8 + at + krow * kDim + kc;
+  if (knew) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[2 * e] = LsElem<DT>::to_f((uint16_t)(kx[j][e] & 0xffffu)) * kinv;
+        f[2 * e + 1] = LsElem<DT>::to_f((uint16_t)(kx[j][e] >> 16)) * kinv;
+      }
+      *reinterpret_cast<uint2*>(kp + 32 * j) =
+          make_uint2(q8_pack(f[0], f[1], f[2], f[3]), q8_pack(f[4], f[5], f[6], f[7]));
+    }
+  } else if (krow < r0 && kcode > kold) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint2* p = reinterpret_cast<uint2*>(kp + 32 * j);
+      const uint2 v = *p;
+      *p = make_uint2(q8_rescale(v.x, kdown), q8_rescale(v.y, kdown));
+    }
+  }
+
+  // Bytes of the word that are new, and those that are older.
+  uint32_t is_new = 0, is_old = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (tok + j >= r0 && tok + j < r1) is_new |= 0xffu << (8 * j);
+    if (tok + j < r0) is_old |= 0xffu << (8 * j);
+  }
+  const bool lower = vcode > vold && is_old != 0;
+  if (is_new != 0 || lower) {
+    uint8_t* vp = v8 + at + (8 * oct) * kPage + 4 * quad;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        f[j] = LsElem<DT>::to_f((uint16_t)(vx[j][e >> 1] >> (16 * (e & 1)))) * vinv;
+      uint32_t* p = reinterpret_cast<uint32_t*>(vp + e * kPage);
+      uint32_t v = q8_pack(f[0], f[1], f[2], f[3]);
+      if (is_new != 0xffffffffu) {
+        const uint32_t o = *p;
+        const uint32_t l = lower ? q8_rescale(o, vdown) : o;
+        v = (v & is_new) | (l & is_old) | (o & ~(is_new | is_old));
+      }
+      *p = v;
+    }
+  }
+}
+
+// Compressed keys: a wave per (window, KV head), after the rows are stored.  Window w is
+// the mean of the 32 stored keys from token 16 w, as the cache holds them; lane (c, part)
+// sums 8 channels of 8 rows in float32, then the parts are added in order.
+template <int DT>
+__global__ __launch_bounds__(256) void ls_q8_windows_kernel(
+    const uint8_t* __restrict__ k8, int64_t cbs, const uint8_t* __restrict__ ks, int64_t sbs,
+    int64_t pages, const int32_t* __restrict__ cache_seqlens, const int32_t* __restrict__ cu_new,
+    int batch, int G, int64_t max_windows, uint16_t* __restrict__ kcc, int64_t kbs, int64_t krs,
+    int64_t kc_rows) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int g = blockIdx.y;
+  int64_t unit = (int64_t)blockIdx.x * 4 + (tid >> 6);
+  if (unit >= max_windows) return;
+  const int b = q8_find(unit, batch, [&](int i) -> int64_t {
+    const int64_t len = cache_seqlens[i], n = cu_new[i + 1] - cu_new[i];
+    return n > 0 ? q8_windows(len + n, 32, 16) - q8_windows(len, 32, 16) : 0;
+  });
+  if (b < 0) return;
+  const int64_t win = q8_windows(cache_seqlens[b], 32, 16) + unit;
+  const int c = lane & 15, part = lane >> 4;
+  const int64_t tok = 16 * win + 8 * part;
+  const int64_t page = tok / kPage;  // eight rows from a multiple of eight: one page
+  if (page >= pages || win >= kc_rows) return;
+  const uint8_t* p = k8 + (int64_t)b * cbs + (page * G + g) * kPageBytes + (tok & 63) * kDim + 8 * c;
+  const float f = q8_pow(ks[(int64_t)b * sbs + page * G + g]);
+  float s[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s[e] = 0.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p + r * kDim);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int x = (int)(h ? v.y : v.x);
+      const Q8F2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(x, false);
+      const Q8F2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(x, true);
+      s[4 * h] += lo[0];
+      s[4 * h + 1] += lo[1];
+      s[4 * h + 2] += hi[0];
+      s[4 * h + 3] += hi[1];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    s[e] *= f;  // the four parts may lie in two pages
+    s[e] += ls_shfl_xor(s[e], 16);
+    s[e] += ls_shfl_xor(s[e], 32);
+    s[e] *= 1.f / 32.f;
+  }
+  if (part == 0) {
+    ls_u32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o[e] = ls_pack2(LsElem<DT>::from_f(s[2 * e]), LsElem<DT>::from_f(s[2 * e + 1]));
+    *reinterpret_cast<ls_u32x4*>(kcc + (int64_t)b * kbs + win * krs + (int64_t)g * kDim + 8 * c) = o;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attention of decode rows.  Workgroup (slice s, row t, KV head g): four waves, each a
+// share of the row's pages with a running maximum and sum, joined through LDS; with
+// several slices, partial results go to the workspace and a second kernel joins them.
+// Row i of sequence b sees keys j < len_b, or j <= len_b - len_q(b) + i (causal).
+// K's bytes become the query's type (exact) for S^T = K Q^T, V's become fp16 (exact) for
+// O^T = V^T P^T with P <= 1 rounded to fp16 (2^-12 of each weight; the sum of the weights
+// is taken of the rounded ones, so the result is an exact mean with those weights).
+// A page's powers of two go into the scores' scale and into the sum of O.
+// ---------------------------------------------------------------------------
+#define LS_Q8_MAX_SPLITS 256
+#define LS_Q8_PART (16 * 128 + 32)  // floats per partial: O [16][128], m [16], l [16]
+#define LS_Q8_PITCH 132             // floats per head of a wave's O in LDS
+#define LS_Q8_ID_REGS 4             // plan ids held in registers: topk <= 256
+
+// Eight e4m3 bytes as eight values of the query's type.
+template <int DT>
+__device__ __forceinline__ ls_u32x4 q8_expand(uint32_t lo, uint32_t hi) {
+  ls_u32x4 o;
+  if constexpr (DT == LS_BF16) {
+    o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false));
+    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
+    o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
+    o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
+  } else {
+    o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false));
+    o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true));
+    o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false));
+    o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true));
+  }
+  return o;
+}
+
+template <int DT, bool DENSE>
+__global__ __launch_bounds__(256) void ls_q8_attn_kernel(
+    const uint16_t* __restrict__ q, int64_t qrs, const int32_t* __restrict__ cu_q, int batch,
+    int64_t total_q, const uint8_t* __restrict__ k8, const uint8_t* __restrict__ v8, int64_t cbs,
+    const uint8_t* __restrict__ ks, const uint8_t* __restrict__ vs, int64_t sbs, int64_t pages,
+    const int32_t* __restrict__ cache_seqlens, int gs, const int32_t* __restrict__ topk_idx,
+    int topk, int ppw, int n_splits, float scale_log2, int causal, float* __restrict__ part,
+    uint16_t* __restrict__ out, float* __restrict__ lse) {
+  __shared__ __attribute__((aligned(16))) float s_o[4][16 * LS_Q8_PITCH];
+  __shared__ float s_ml[4][2][16];
+  const int64_t t = blockIdx.x / (unsigned)n_splits;
+  const int s = (int)(blockIdx.x - (unsigned)t * (unsigned)n_splits);
+  const int g = blockIdx.y, G = gridDim.y;
+  if (t >= cu_q[batch]) return;  // a row behind the last sequence
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, qg = lane >> 4;
+  const int b = ls_find_segment(cu_q, batch, t);
+  const int64_t len_b = min((int64_t)cache_seqlens[b], pages * kPage);
+  const int64_t limit =
+      causal ? len_b - (cu_q[b + 1] - cu_q[b]) + (t - cu_q[b]) + 1 : len_b;  // keys j < limit
+  // Queries: step k4 of the product takes channels 32 qg + 8 k4 + [0, 8), as K's loads do.
+  ls_u32x4 qf[4];
+  const uint16_t* qrow = q + t * qrs + ((int64_t)g * gs + r) * kDim + 32 * qg;
+#pragma unroll
+  for (int k4 = 0; k4 < 4; ++k4)
+    qf[k4] = r < gs ? ls_load16(qrow + 8 * k4) : ls_u32x4{0u, 0u, 0u, 0u};
+  const uint8_t* kseq = k8 + (int64_t)b * cbs + (int64_t)g * kPageBytes;
+  const uint8_t* vseq = v8 + (int64_t)b * cbs + (int64_t)g * kPageBytes;
+  const uint8_t* kss = ks + (int64_t)b * sbs + g;
+  const uint8_t* vss = vs + (int64_t)b * sbs + g;
+
+  typedef int IdRegs __attribute__((ext_vector_type(LS_Q8_ID_REGS)));
+  IdRegs idr = -1;
+  int slot, slot1;  // the wave's next plan slot (DENSE: page) and the end of its share
+  if constexpr (DENSE) {
+    const int64_t n_vis = limit <= 0 ? 0 : (limit + kPage - 1) / kPage;
+    const int share = (int)((n_vis + 4 * n_splits - 1) / (4 * n_splits));
+    slot = (4 * s + w) * share;
+    slot1 = (int)min<int64_t>(n_vis, slot + share);
+  } else {
+    const int32_t* idrow = topk_idx + ((int64_t)g * total_q + t) * topk;
+#pragma unroll
+    for (int k = 0; k < LS_Q8_ID_REGS; ++k)
+      if (64 * k + lane < topk) idr[k] = idrow[64 * k + lane];
+    slot = (4 * s + w) * ppw;
+    slot1 = min(topk, slot + ppw);
+  }
+  // The page of the next valid slot (-1 at the end of the share).
+  auto next_page = [&]() -> int {
+    int found = -1;
+    while (found < 0 && slot < slot1) {
+      const int at = slot++;
+      if constexpr (DENSE) {
+        found = at;
+      } else {
+        const int held = at < 128 ? (at < 64 ? idr[0] : idr[1]) : (at < 192 ? idr[2] : idr[3]);
+        const int id = __builtin_amdgcn_readlane(held, at & 63);
+        if (id < 0 || (int64_t)kPage * id >= limit) continue;  // limit <= pages * 64
+        bool dup = false;  // a repeated id counts once, as a bitmask of pages would have it
+#pragma unroll
+        for (int k = 0; k < LS_Q8_ID_REGS; ++k)
+          dup |= __ballot(64 * k + lane < at && idr[k] == id) != 0ull;
+        if (!dup) found = id;
+      }
+    }
+    return found;
+  };
+
+  float m_run = -INFINITY, l_run = 0.f;
+  ls_f32x4 o[8];
+#pragma unroll
+  for (int db = 0; db < 8; ++db) o[db] = ls_f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int page = next_page(); page >= 0; page = next_page()) {
+    const int64_t left = limit - (int64_t)kPage * page;
+    const int nvis = left < kPage ? (int)left : kPage;
+    const uint8_t* kp = kseq + (int64_t)page * G * kPageBytes + r * kDim + 32 * qg;
+    const uint8_t* vp = vseq + (int64_t)page * G * kPageBytes + r * kPage + 16 * qg;
+    ls_u32x4 kf[4][2], vf[8];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      kf[kb][0] = ls_load16(kp + kb * 16 * kDim);
+      kf[kb][1] = ls_load16(kp + kb * 16 * kDim + 16);
+    }
+#pragma unroll
+    for (int db = 0; db < 8; ++db) vf[db] = ls_load16(vp + db * 16 * kPage);
+    const float kscale = scale_log2 * q8_pow(kss[(int64_t)page * G]);
+    const float vscale = q8_pow(vss[(int64_t)page * G]);
+
+    float sv[16], pm = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) {
+      ls_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k4 = 0; k4 < 4; ++k4) {
+        const ls_u32x4 kk = kf[kb][k4 >> 1];
+        acc = LsElem<DT>::mfma(q8_expand<DT>(kk[2 * (k4 & 1)], kk[2 * (k4 & 1) + 1]), qf[k4], acc);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = 16 * kb + 4 * qg + i < nvis ? acc[i] * kscale : -INFINITY;
+        sv[4 * kb + i] = x;
+        pm = fmaxf(pm, x);
+      }
+    }
+    if (nvis < kPage) {  // values past the end may be anything: zeros
+#pragma unroll
+      for (int kb = 0; kb < 4; ++kb) {
+        const int n = min(4, max(0, nvis - 16 * kb - 4 * qg));
+        const uint32_t keep = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
+#pragma unroll
+        for (int db = 0; db < 8; ++db) vf[db][kb] &= keep;
+      }
+    }
+    pm = fmaxf(pm, ls_shfl_xor(pm, 16));
+    pm = fmaxf(pm, ls_shfl_xor(pm, 32));
+    const float m_new = fmaxf(m_run, pm);
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+    m_run = m_new;
+    l_run *= alpha;
+    ls_u32x4 pf[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint16_t h0 = ls_f32_to_f16(__builtin_amdgcn_exp2f(sv[8 * c + 2 * e] - m_new));
+        const uint16_t h1 = ls_f32_to_f16(__builtin_amdgcn_exp2f(sv[8 * c + 2 * e + 1] - m_new));
+        l_run += ls_f16_to_f32(h0) + ls_f16_to_f32(h1);
+        pf[c][e] = ls_pack2(h0, h1);
+      }
+#pragma unroll
+    for (int db = 0; db < 8; ++db) {
+      ls_f32x4 pv = {0.f, 0.f, 0.f, 0.f};
+      pv = LsElem<LS_F16>::mfma(q8_expand<LS_F16>(vf[db][0], vf[db][1]), pf[0], pv);
+      pv = LsElem<LS_F16>::mfma(q8_expand<LS_F16>(vf[db][2], vf[db][3]), pf[1], pv);
+      o[db] = o[db] * alpha + pv * vscale;
+    }
+  }
+  l_run += ls_shfl_xor(l_run, 16);
+  l_run += ls_shfl_xor(l_run, 32);
+#pragma unroll
+  for (int db = 0; db < 8; ++db)  // o[db][i]: head r, channel 16 db + 4 qg + i
+    *reinterpret_cast<ls_f32x4*>(&s_o[w][r * LS_Q8_PITCH + 16 * db + 4 * qg]) = o[db];
+  if (qg == 0) {
+    s_ml[w][0][r] = m_run;
+    s_ml[w][1][r] = l_run;
+  }
+  __syncthreads();
+  // Join the four waves: thread e takes channel e & 127 of heads e >> 7, + 2, ...  A wave
+  // without a page has sum 0 and is left out; one whose sum is NaN is not.
+  float* pp = part + (((int64_t)g * total_q + t) * n_splits + s) * LS_Q8_PART;
+  for (int e = tid; e < gs * kDim; e += 256) {
+    const int h = e >> 7, d = e & 127;
+    float M = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) M = fmaxf(M, s_ml[i][0][h]);
+    float acc = 0.f, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (s_ml[i][1][h] == 0.f) continue;
+      const float wt = __builtin_amdgcn_exp2f(s_ml[i][0][h] - M);
+      acc += wt * s_o[i][h * LS_Q8_PITCH + d];
+      L += wt * s_ml[i][1][h];
+    }
+    if (n_splits == 1) {
+      out[(t * G + g) * (int64_t)gs * kDim + e] = LsElem<DT>::from_f(L == 0.f ? 0.f : acc / L);
+      if (lse && d == 0)
+        lse[((int64_t)g * gs + h) * total_q + t] =
+            L == 0.f ? INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
+    } else {
+      pp[e] = acc;
+      if (d == 0) {
+        pp[16 * 128 + h] = M;
+        pp[16 * 128 + 16 + h] = L;
+      }
+    }
+  }
+}
+
+// out[t][g*gs + h] = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s; a row that sees no key
+// gives zeros and lse = +inf.  A workgroup per (row, KV head, query head), a thread per channel;
+// the weights of the slices (one a thread) are formed in LDS.
+template <int DT>
+__global__ __launch_bounds__(128) void ls_q8_join_kernel(
+    const float* __restrict__ part, const int32_t* __restrict__ cu_q, int batch, int64_t total_q,
+    int gs, int n_splits, uint16_t* __restrict__ out, float* __restrict__ lse) {
+  __shared__ float s_w[LS_Q8_MAX_SPLITS];
+  const int64_t t = blockIdx.x;
+  const int g = blockIdx.y, h = blockIdx.z, G = gridDim.y;
+  if (t >= cu_q[batch]) return;
+  const int tid = threadIdx.x;
+  const float* pr = part + ((int64_t)g * total_q + t) * n_splits * LS_Q8_PART;
+  // Every wave goes over all slices (at most four a lane), so no value is exchanged but weights.
+  float ms[4], ls[4], M = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int i = 64 * k + (tid & 63);
+    ms[k] = i < n_splits ? pr[(int64_t)i * LS_Q8_PART + 16 * 128 + h] : -INFINITY;
+    ls[k] = i < n_splits ? pr[(int64_t)i * LS_Q8_PART + 16 * 128 + 16 + h] : 0.f;
+    M = fmaxf(M, ms[k]);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, ls_shfl_xor(M, o));
+  float L = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    ms[k] = ls[k] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ms[k] - M);
+    L += ms[k] * ls[k];
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) L += ls_shfl_xor(L, o);
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  if (tid < 64) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (64 * k + tid < n_splits) s_w[64 * k + tid] = ms[k] * inv;
+  }
+  __syncthreads();
+  float acc = 0.f;
+  for (int sp = 0; sp < n_splits; ++sp) {
+    const float x = pr[(int64_t)sp * LS_Q8_PART + h * 128 + tid];
+    if (s_w[sp] != 0.f) acc += s_w[sp] * x;
+  }
+  out[((t * G + g) * (int64_t)gs + h) * kDim + tid] = LsElem<DT>::from_f(acc);
+  if (lse && tid == 0)
+    lse[((int64_t)g * gs + h) * total_q + t] =
+        L == 0.f ? INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+extern "C" int ls_kvcache_append_q8(void* k8, void* v8, int64_t cache_batch_stride,
+                                    uint8_t* k_scale, uint8_t* v_scale,
+                                    int64_t scale_batch_stride, int64_t pages,
+                                    const int32_t* cache_seqlens, const void* k_new,
+                                    const void* v_new, int64_t new_row_stride,
+                                    const int32_t* cu_seqlens_new, int64_t total_new,
+                                    int32_t batch, int32_t num_kv_heads, int32_t head_dim,
+                                    int32_t dtype, void* kc_cache, int64_t kc_batch_stride,
+                                    int64_t kc_row_stride, int64_t kc_rows,
+                                    int64_t max_new_windows, void* stream) {
+  const char* who = "ls_kvcache_append_q8";
+  LS_REQUIRE(batch >= 0 && total_new >= 0 && num_kv_heads > 0 && pages >= 0 && kc_rows >= 0,
+             LS_ERR_INVALID, "%s: bad sizes", who);
+  LS_REQUIRE(head_dim == kDim, LS_ERR_UNSUPPORTED, "%s: head_dim must be 128", who);
+  LS_REQUIRE(dtype == LS_BF16 || dtype == LS_F16, LS_ERR_UNSUPPORTED,
+             "%s: new keys and values are bf16 or fp16", who);
+  LS_REQUIRE(num_kv_heads <= 65535, LS_ERR_INVALID, "%s: too many heads", who);
+  LS_REQUIRE(new_row_stride % 8 == 0 && cache_batch_stride % 16 == 0, LS_ERR_UNSUPPORTED,
+             "%s: rows must be 16-byte aligned", who);
+  if (total_new == 0 || batch == 0) return LS_OK;
+  LS_REQUIRE(k8 && v8 && k_scale && v_scale && k_new && v_new && cache_seqlens && cu_seqlens_new,
+             LS_ERR_INVALID, "%s: null pointer", who);
+  LS_REQUIRE(ls_aligned16(k8) && ls_aligned16(v8) && ls_aligned16(k_new) && ls_aligned16(v_new),
+             LS_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned", who);
+  // A sequence's n > 0 new tokens touch at most (n + 126) / 64 <= n pages.
+  const int64_t nb = std::min<int64_t>(batch, total_new);
+  const int64_t units = std::min(total_new, (total_new + 126 * nb) / 64);
+  LS_REQUIRE(units <= 0x7fffffffLL, LS_ERR_UNSUPPORTED, "%s: too many new tokens", who);
+  const bool windows = kc_cache && max_new_windows > 0;
+  if (windows) {
+    LS_REQUIRE(ls_aligned16(kc_cache) && kc_row_stride % 8 == 0 && kc_batch_stride % 8 == 0,
+               LS_ERR_UNSUPPORTED, "%s: compressed cache must be 16-byte aligned", who);
+    LS_REQUIRE(max_new_windows <= 0x7fffffffLL, LS_ERR_UNSUPPORTED, "%s: too many windows", who);
+  }
+  hipStream_t s = (hipStream_t)stream;
+  auto append = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)units, num_kv_heads), dim3(256), 0, s, (uint8_t*)k8,
+                       (uint8_t*)v8, cache_batch_stride, k_scale, v_scale, scale_batch_stride,
+                       pages, cache_seqlens, (const uint16_t*)k_new, (const uint16_t*)v_new,
+                       new_row_stride, cu_seqlens_new, total_new, batch, num_kv_heads);
+    return ls_check_launch("ls_q8_append_kernel");
+  };
+  int rc = dtype == LS_BF16 ? append(ls_q8_append_kernel<LS_BF16>)
+                            : append(ls_q8_append_kernel<LS_F16>);
+  if (rc || !windows) return rc;
+  auto pool = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((max_new_windows + 3) / 4), num_kv_heads),
+                       dim3(256), 0, s, (const uint8_t*)k8, cache_batch_stride, k_scale,
+                       scale_batch_stride, pages, cache_seqlens, cu_seqlens_new, batch,
+                       num_kv_heads, max_new_windows, (uint16_t*)kc_cache, kc_batch_stride,
+                       kc_row_stride, kc_rows);
+    return ls_check_launch("ls_q8_windows_kernel");
+  };
+  return dtype == LS_BF16 ? pool(ls_q8_windows_kernel<LS_BF16>)
+                          : pool(ls_q8_windows_kernel<LS_F16>);
+}
+
+extern "C" size_t ls_attn_kvcache_q8_workspace_size(int64_t total_q, int32_t num_kv_heads,
+                                                    int32_t n_splits) {
+  if (n_splits <= 1 || total_q <= 0 || num_kv_heads <= 0) return 0;
+  return ls_align256(4 * (size_t)total_q * num_kv_heads * n_splits * LS_Q8_PART);
+}
+
+extern "C" int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int32_t* cu_seqlens_q,
+                                  int64_t total_q, const void* k8, const void* v8,
+                                  int64_t cache_batch_stride, const uint8_t* k_scale,
+                                  const uint8_t* v_scale, int64_t scale_batch_stride,
+                                  int64_t pages, const int32_t* cache_seqlens, int32_t batch,
+                                  int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                  int32_t dtype, const int32_t* topk_idx, int32_t topk,
+                                  float softmax_scale, int32_t causal, int32_t n_splits, void* out,
+                                  float* softmax_lse, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  const char* who = "ls_attn_kvcache_q8";
+  LS_REQUIRE(batch > 0 && total_q >= 0 && num_kv_heads > 0 && num_heads > 0 &&
+                 num_heads % num_kv_heads == 0 && pages >= 0,
+             LS_ERR_INVALID, "%s: bad sizes", who);
+  const int gs = num_heads / num_kv_heads;
+  LS_REQUIRE(head_dim == kDim && gs <= 16, LS_ERR_UNSUPPORTED,
+             "%s: head_dim 128 and at most 16 query heads per KV head", who);
+  LS_REQUIRE(dtype == LS_BF16 || dtype == LS_F16, LS_ERR_UNSUPPORTED,
+             "%s: queries are bf16 or fp16", who);
+  const bool dense = topk_idx == nullptr;
+  LS_REQUIRE((dense || topk >= 1) && n_splits >= 1 && n_splits <= LS_Q8_MAX_SPLITS, LS_ERR_INVALID,
+             "%s: need topk >= 1 and 1 <= n_splits <= %d", who, LS_Q8_MAX_SPLITS);
+  LS_REQUIRE(dense || topk <= 64 * LS_Q8_ID_REGS, LS_ERR_UNSUPPORTED,
+             "%s: at most %d plan ids per row (got %d)", who, 64 * LS_Q8_ID_REGS, topk);
+  LS_REQUIRE(total_q <= 0x7fffffffLL / n_splits && num_kv_heads <= 65535, LS_ERR_UNSUPPORTED,
+             "%s: too many rows or KV heads", who);
+  LS_REQUIRE(pages <= 0x1000000, LS_ERR_UNSUPPORTED, "%s: at most 2^24 pages a sequence", who);
+  LS_REQUIRE(q_row_stride % 8 == 0 && cache_batch_stride % 16 == 0, LS_ERR_UNSUPPORTED,
+             "%s: rows must be 16-byte aligned", who);
+  if (total_q == 0) return LS_OK;
+  LS_REQUIRE(q && k8 && v8 && k_scale && v_scale && cu_seqlens_q && cache_seqlens && out,
+             LS_ERR_INVALID, "%s: null pointer", who);
+  LS_REQUIRE(ls_aligned16(q) && ls_aligned16(k8) && ls_aligned16(v8), LS_ERR_UNSUPPORTED,
+             "%s: tensors must be 16-byte aligned", who);
+  // Four waves a slice, ppw plan slots a wave.
+  const int ppw = dense ? 0 : (topk + 4 * n_splits - 1) / (4 * n_splits);
+  const int splits = dense ? n_splits : (topk + 4 * ppw - 1) / (4 * ppw);
+  const size_t need = ls_attn_kvcache_q8_workspace_size(total_q, num_kv_heads, splits);
+  LS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), LS_ERR_WORKSPACE,
+             "%s: workspace %zu < %zu", who, workspace ? workspace_bytes : (size_t)0, need);
+  hipStream_t s = (hipStream_t)stream;
+  const float scale_log2 = softmax_scale * 1.4426950408889634f;
+  float* part = (float*)workspace;
+  auto attend = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(total_q * splits), num_kv_heads), dim3(256), 0,
+                       s, (const uint16_t*)q, q_row_stride, cu_seqlens_q, batch, total_q,
+                       (const uint8_t*)k8, (const uint8_t*)v8, cache_batch_stride, k_scale,
+                       v_scale, scale_batch_stride, pages, cache_seqlens, gs, topk_idx, topk, ppw,
+                       splits, scale_log2, causal, part, (uint16_t*)out, softmax_lse);
+    return ls_check_launch("ls_q8_attn_kernel");
+  };
+  int rc;
+  if (dtype == LS_BF16)
+    rc = dense ? attend(ls_q8_attn_kernel<LS_BF16, true>) : attend(ls_q8_attn_kernel<LS_BF16, false>);
+  else
+    rc = dense ? attend(ls_q8_attn_kernel<LS_F16, true>) : attend(ls_q8_attn_kernel<LS_F16, false>);
+  if (rc || splits == 1) return rc;
+  auto join = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)total_q, num_kv_heads, gs), dim3(128), 0, s, part,
+                       cu_seqlens_q, batch, total_q, gs, splits, (uint16_t*)out, softmax_lse);
+    return ls_check_launch("ls_q8_join_kernel");
+  };
+  return dtype == LS_BF16 ? join(ls_q8_join_kernel<LS_BF16>) : join(ls_q8_join_kernel<LS_F16>);
+}
