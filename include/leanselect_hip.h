@@ -660,19 +660,21 @@ int ls_kvcache_append_q8(void* k8, void* v8, int64_t cache_batch_stride, uint8_t
 
 /*
  * Attention of packed decode rows over the 8-bit cache: ls_sparse_attn_kvcache
- * over the values it stands for, or ls_dense_attn_kvcache where topk_idx is NULL
- * (topk is then not read).  A repeated plan id counts once.  Rows at and after
+ * over the values it stands for with plans topk_idx [G, total_q, n_pages], or
+ * ls_dense_attn_kvcache where topk_idx is NULL (n_pages, the pages of the longest
+ * row, then only decides how the work is cut).  A repeated plan id counts once.  Rows at and after
  * cu_seqlens_q[batch] are left as they are.  A row without a visible key gets
- * out = 0 and lse = +inf.  At most 16 query heads per KV head, topk <= 256,
- * 1 <= n_splits <= 256; the workspace may be NULL for n_splits = 1.
+ * out = 0 and lse = +inf.  At most 16 query heads per KV head, at most 256 plan
+ * ids, 1 <= n_splits <= 256; out, like the other tensors, is 16-byte aligned; the
+ * workspace (16-byte aligned) may be NULL for n_splits = 1.
  */
-size_t ls_attn_kvcache_q8_workspace_size(int64_t total_q, int32_t num_kv_heads, int32_t n_splits);
+size_t ls_attn_kvcache_q8_workspace_size(int64_t total_q, int32_t num_heads, int32_t n_splits);
 int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int32_t* cu_seqlens_q,
                        int64_t total_q, const void* k8, const void* v8,
                        int64_t cache_batch_stride, const uint8_t* k_scale, const uint8_t* v_scale,
                        int64_t scale_batch_stride, int64_t pages, const int32_t* cache_seqlens,
                        int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                       int32_t dtype, const int32_t* topk_idx, int32_t topk, float softmax_scale,
+                       int32_t dtype, const int32_t* topk_idx, int32_t n_pages, float softmax_scale,
                        int32_t causal, int32_t n_splits, void* out, float* softmax_lse,
                        void* workspace, size_t workspace_bytes, void* stream);
 
@@ -706,11 +708,15 @@ int ls_dequantize_mx4(const void* codes, const void* scales, int64_t out_feature
  * out[m][n] = sum_k x[m][k] w[n][k] in float32, rounded once to dtype (bf16 or
  * fp16, also the type w's values are taken in); x [rows, K], out [rows, N].  With
  * silu_mul, w is [gate; up] (N a multiple of 32) and out [rows, N / 2] is
- * silu(gate) * up, float32 up to the rounding.
+ * silu(gate) * up, float32 up to the rounding.  The workspace (16-byte aligned) may
+ * be NULL where its size is 0.
  */
+size_t ls_linear_mx4_workspace_size(int64_t rows, int64_t in_features, int64_t out_features,
+                                    int32_t silu_mul);
 int ls_linear_mx4(const void* x, int64_t x_row_stride, int64_t rows, int64_t in_features,
                   const void* codes, const void* scales, int64_t out_features, int32_t silu_mul,
-                  int32_t dtype, void* out, int64_t out_row_stride, void* stream);
+                  int32_t dtype, void* out, int64_t out_row_stride, void* workspace,
+                  size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -119,8 +119,9 @@ SIGNATURES = {
                _i32, _p, _i32, _f32, _i32, _i32, _p, _p, _p, _sz, _p]),
     "ls_quantize_mx4": (_i32, [_p, _i64, _i64, _i64, _i32, _p, _p, _p]),
     "ls_dequantize_mx4": (_i32, [_p, _p, _i64, _i64, _i32, _p, _i64, _p]),
+    "ls_linear_mx4_workspace_size": (_sz, [_i64, _i64, _i64, _i32]),
     "ls_linear_mx4": (
-        _i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _i32, _i32, _p, _i64, _p]),
+        _i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _i32, _i32, _p, _i64, _p, _sz, _p]),
 }
 
 _lib = None
@@ -287,15 +288,26 @@ def stream_of(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
-def launch(device: torch.device, name: str, *args) -> None:
-    """Call entry point ``name`` on ``device``'s current stream (appended to ``args``), with that
-    device current while it launches."""
-    index = device.index
-    if index is None or index == torch.cuda.current_device():
-        rc = getattr(lib(), name)(*args, stream_of(device))
+def gpu_index(first: torch.Tensor, *rest: torch.Tensor | None) -> int:
+    """``require_gpu`` as a device number, without building device objects on every call."""
+    index = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        require_gpu(first, *rest)  # raises
+    return index
+
+
+def launch(index: int, name: str, *args) -> None:
+    """Call entry point ``name`` on GPU ``index``'s current stream (appended to ``args``), with
+    that GPU current while it launches."""
+    fn = getattr(lib(), name)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            rc = getattr(lib(), name)(*args, stream_of(device))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc != LS_OK:
         check(rc, name)
 

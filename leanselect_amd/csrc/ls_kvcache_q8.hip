@@ -20,6 +20,7 @@
 // Extends ls_kvcache_append, ls_sparse_attn_kvcache and ls_dense_attn_kvcache (the
 // reference's cache is 16-bit: leanselect/models/minicpm.py:1188-1490).
 #include <algorithm>
+#include <type_traits>
 
 #include "ls_common.h"
 
@@ -289,11 +290,65 @@ __global__ __launch_bounds__(256) void ls_q8_windows_kernel(
 // O^T = V^T P^T with P <= 1 rounded to fp16 (2^-12 of each weight; the sum of the weights
 // is taken of the rounded ones, so the result is an exact mean with those weights).
 // A page's powers of two go into the scores' scale and into the sum of O.
+//
+// A wave takes ppw plan slots, or (DENSE) pages, or more of a row that is longer than the
+// caller said; a row's later slices, past its last page, end at once.  The next page's K is loaded as soon as this page's scores are formed,
+// its V as soon as this page's sum is, into the same registers.
 // ---------------------------------------------------------------------------
 #define LS_Q8_MAX_SPLITS 256
-#define LS_Q8_PART (16 * 128 + 32)  // floats per partial: O [16][128], m [16], l [16]
 #define LS_Q8_PITCH 132             // floats per head of a wave's O in LDS
 #define LS_Q8_ID_REGS 4             // plan ids held in registers: topk <= 256
+
+// Workspace: O float [G][total_q][n_splits][gs][128], then (m, l) float2 [G][total_q][gs][n_splits].
+struct Q8Part {
+  float* o;
+  float2* ml;
+};
+
+// The decode row: its sequence's length, and the keys j < limit it sees (<= 0: none).
+struct Q8Row {
+  int b;
+  int64_t limit;
+};
+
+// Row t of the batch (t < cu_q[batch]).  A batch of at most 64 is read by the lanes at once.
+__device__ __forceinline__ Q8Row q8_row(const int32_t* __restrict__ cu_q,
+                                        const int32_t* __restrict__ lens, int batch, int64_t t,
+                                        int64_t capacity, int causal) {
+  int b, c0, c1, len;
+  if (batch <= 64) {
+    const int i = min(ls_lane(), batch - 1);
+    const int lo = cu_q[i], hi = cu_q[i + 1], n = lens[i];
+    b = __popcll(__ballot(ls_lane() < batch && t >= hi));  // sequences that end at or before t
+    b = min(b, batch - 1);
+    c0 = __builtin_amdgcn_readlane(lo, b);
+    c1 = __builtin_amdgcn_readlane(hi, b);
+    len = __builtin_amdgcn_readlane(n, b);
+  } else {
+    b = ls_find_segment(cu_q, batch, t);
+    c0 = cu_q[b];
+    c1 = cu_q[b + 1];
+    len = lens[b];
+  }
+  Q8Row r;
+  r.b = b;
+  const int64_t held = min((int64_t)len, capacity);
+  r.limit = causal ? held - (c1 - c0) + (t - c0) + 1 : held;
+  return r;
+}
+
+// Pages a wave takes of a dense row, at least ppw and enough for n_splits slices of four waves,
+// and the slices that the row's pages then fill.
+struct Q8Share {
+  int pages, share, slices;
+};
+__device__ __forceinline__ Q8Share q8_share(int64_t limit, int ppw, int n_splits) {
+  Q8Share x;
+  x.pages = limit <= 0 ? 0 : (int)((limit + kPage - 1) / kPage);
+  x.share = max(ppw, (x.pages + 4 * n_splits - 1) / (4 * n_splits));
+  x.slices = (x.pages + 4 * x.share - 1) / (4 * x.share);
+  return x;
+}
 
 // Eight e4m3 bytes as eight values of the query's type.
 template <int DT>
@@ -319,48 +374,47 @@ __global__ __launch_bounds__(256) void ls_q8_attn_kernel(
     int64_t total_q, const uint8_t* __restrict__ k8, const uint8_t* __restrict__ v8, int64_t cbs,
     const uint8_t* __restrict__ ks, const uint8_t* __restrict__ vs, int64_t sbs, int64_t pages,
     const int32_t* __restrict__ cache_seqlens, int gs, const int32_t* __restrict__ topk_idx,
-    int topk, int ppw, int n_splits, float scale_log2, int causal, float* __restrict__ part,
+    int topk, int ppw, int n_splits, float scale_log2, int causal, Q8Part part,
     uint16_t* __restrict__ out, float* __restrict__ lse) {
   __shared__ __attribute__((aligned(16))) float s_o[4][16 * LS_Q8_PITCH];
   __shared__ float s_ml[4][2][16];
   const int64_t t = blockIdx.x / (unsigned)n_splits;
   const int s = (int)(blockIdx.x - (unsigned)t * (unsigned)n_splits);
   const int g = blockIdx.y, G = gridDim.y;
-  if (t >= cu_q[batch]) return;  // a row behind the last sequence
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, qg = lane >> 4;
-  const int b = ls_find_segment(cu_q, batch, t);
-  const int64_t len_b = min((int64_t)cache_seqlens[b], pages * kPage);
-  const int64_t limit =
-      causal ? len_b - (cu_q[b + 1] - cu_q[b]) + (t - cu_q[b]) + 1 : len_b;  // keys j < limit
+  // The row's plan ids, 64 per register.  (A vector: an array indexed in the lambda below
+  // would be kept in LDS.)
+  typedef int IdRegs __attribute__((ext_vector_type(LS_Q8_ID_REGS)));
+  IdRegs idr = -1;
+  if constexpr (!DENSE) {
+    const int32_t* idrow = topk_idx + ((int64_t)g * total_q + t) * topk;
+#pragma unroll
+    for (int k = 0; k < LS_Q8_ID_REGS; ++k)
+      if (64 * k + lane < topk) idr[k] = idrow[64 * k + lane];
+  }
   // Queries: step k4 of the product takes channels 32 qg + 8 k4 + [0, 8), as K's loads do.
   ls_u32x4 qf[4];
   const uint16_t* qrow = q + t * qrs + ((int64_t)g * gs + r) * kDim + 32 * qg;
 #pragma unroll
   for (int k4 = 0; k4 < 4; ++k4)
     qf[k4] = r < gs ? ls_load16(qrow + 8 * k4) : ls_u32x4{0u, 0u, 0u, 0u};
-  const uint8_t* kseq = k8 + (int64_t)b * cbs + (int64_t)g * kPageBytes;
-  const uint8_t* vseq = v8 + (int64_t)b * cbs + (int64_t)g * kPageBytes;
-  const uint8_t* kss = ks + (int64_t)b * sbs + g;
-  const uint8_t* vss = vs + (int64_t)b * sbs + g;
-
-  typedef int IdRegs __attribute__((ext_vector_type(LS_Q8_ID_REGS)));
-  IdRegs idr = -1;
-  int slot, slot1;  // the wave's next plan slot (DENSE: page) and the end of its share
+  if (t >= cu_q[batch]) return;  // a row behind the last sequence
+  const Q8Row row = q8_row(cu_q, cache_seqlens, batch, t, pages * kPage, causal);
+  const int64_t limit = row.limit;
+  Q8Share cut = {topk, ppw, n_splits};
   if constexpr (DENSE) {
-    const int64_t n_vis = limit <= 0 ? 0 : (limit + kPage - 1) / kPage;
-    const int share = (int)((n_vis + 4 * n_splits - 1) / (4 * n_splits));
-    slot = (4 * s + w) * share;
-    slot1 = (int)min<int64_t>(n_vis, slot + share);
-  } else {
-    const int32_t* idrow = topk_idx + ((int64_t)g * total_q + t) * topk;
-#pragma unroll
-    for (int k = 0; k < LS_Q8_ID_REGS; ++k)
-      if (64 * k + lane < topk) idr[k] = idrow[64 * k + lane];
-    slot = (4 * s + w) * ppw;
-    slot1 = min(topk, slot + ppw);
+    cut = q8_share(limit, ppw, n_splits);
+    if (s > 0 && s >= cut.slices) return;
   }
+  const uint8_t* kseq = k8 + (int64_t)row.b * cbs + (int64_t)g * kPageBytes;
+  const uint8_t* vseq = v8 + (int64_t)row.b * cbs + (int64_t)g * kPageBytes;
+  const uint8_t* kss = ks + (int64_t)row.b * sbs + g;
+  const uint8_t* vss = vs + (int64_t)row.b * sbs + g;
+
+  int slot = (4 * s + w) * cut.share;  // the wave's next plan slot (DENSE: page) and its end
+  const int slot1 = min(cut.pages, slot + cut.share);
   // The page of the next valid slot (-1 at the end of the share).
   auto next_page = [&]() -> int {
     int found = -1;
@@ -386,22 +440,31 @@ __global__ __launch_bounds__(256) void ls_q8_attn_kernel(
   ls_f32x4 o[8];
 #pragma unroll
   for (int db = 0; db < 8; ++db) o[db] = ls_f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int page = next_page(); page >= 0; page = next_page()) {
-    const int64_t left = limit - (int64_t)kPage * page;
-    const int nvis = left < kPage ? (int)left : kPage;
+  ls_u32x4 kf[4][2], vf[8];
+  uint32_t kcode, vcode;
+  auto load_k = [&](int page) {
     const uint8_t* kp = kseq + (int64_t)page * G * kPageBytes + r * kDim + 32 * qg;
-    const uint8_t* vp = vseq + (int64_t)page * G * kPageBytes + r * kPage + 16 * qg;
-    ls_u32x4 kf[4][2], vf[8];
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
       kf[kb][0] = ls_load16(kp + kb * 16 * kDim);
       kf[kb][1] = ls_load16(kp + kb * 16 * kDim + 16);
     }
+    kcode = kss[(int64_t)page * G];
+  };
+  auto load_v = [&](int page) {
+    const uint8_t* vp = vseq + (int64_t)page * G * kPageBytes + r * kPage + 16 * qg;
 #pragma unroll
     for (int db = 0; db < 8; ++db) vf[db] = ls_load16(vp + db * 16 * kPage);
-    const float kscale = scale_log2 * q8_pow(kss[(int64_t)page * G]);
-    const float vscale = q8_pow(vss[(int64_t)page * G]);
-
+    vcode = vss[(int64_t)page * G];
+  };
+  // One page whose K and V are in registers (or on their way), with the loads of the page
+  // after it.  The last page is its own copy of this code, so that the loads are on every
+  // path of the loop (a conditional load would be waited for where the paths meet).
+  auto attend = [&](int page, int after, auto more) {
+    constexpr bool kMore = decltype(more)::value;
+    const int64_t left = limit - (int64_t)kPage * page;
+    const int nvis = left < kPage ? (int)left : kPage;
+    const float kscale = scale_log2 * q8_pow(kcode);
     float sv[16], pm = -INFINITY;
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
@@ -412,21 +475,23 @@ __global__ __launch_bounds__(256) void ls_q8_attn_kernel(
         acc = LsElem<DT>::mfma(q8_expand<DT>(kk[2 * (k4 & 1)], kk[2 * (k4 & 1) + 1]), qf[k4], acc);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = 16 * kb + 4 * qg + i < nvis ? acc[i] * kscale : -INFINITY;
-        sv[4 * kb + i] = x;
-        pm = fmaxf(pm, x);
-      }
+      for (int i = 0; i < 4; ++i) sv[4 * kb + i] = acc[i] * kscale;
     }
-    if (nvis < kPage) {  // values past the end may be anything: zeros
+    if constexpr (kMore) load_k(after);
+    if (nvis < kPage) {  // keys past the end: no weight; their values may be anything: zeros
 #pragma unroll
       for (int kb = 0; kb < 4; ++kb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * kb + 4 * qg + i >= nvis) sv[4 * kb + i] = -INFINITY;
         const int n = min(4, max(0, nvis - 16 * kb - 4 * qg));
         const uint32_t keep = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
 #pragma unroll
         for (int db = 0; db < 8; ++db) vf[db][kb] &= keep;
       }
     }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) pm = fmaxf(pm, sv[i]);
     pm = fmaxf(pm, ls_shfl_xor(pm, 16));
     pm = fmaxf(pm, ls_shfl_xor(pm, 32));
     const float m_new = fmaxf(m_run, pm);
@@ -443,6 +508,7 @@ __global__ __launch_bounds__(256) void ls_q8_attn_kernel(
         l_run += ls_f16_to_f32(h0) + ls_f16_to_f32(h1);
         pf[c][e] = ls_pack2(h0, h1);
       }
+    const float vscale = q8_pow(vcode);
 #pragma unroll
     for (int db = 0; db < 8; ++db) {
       ls_f32x4 pv = {0.f, 0.f, 0.f, 0.f};
@@ -450,6 +516,19 @@ __global__ __launch_bounds__(256) void ls_q8_attn_kernel(
       pv = LsElem<LS_F16>::mfma(q8_expand<LS_F16>(vf[db][2], vf[db][3]), pf[1], pv);
       o[db] = o[db] * alpha + pv * vscale;
     }
+    if constexpr (kMore) load_v(after);
+  };
+  int page = next_page();
+  if (page >= 0) {
+    load_k(page);
+    load_v(page);
+    for (;;) {
+      const int after = next_page();
+      if (after < 0) break;
+      attend(page, after, std::true_type());
+      page = after;
+    }
+    attend(page, -1, std::false_type());
   }
   l_run += ls_shfl_xor(l_run, 16);
   l_run += ls_shfl_xor(l_run, 32);
@@ -461,57 +540,73 @@ __global__ __launch_bounds__(256) void ls_q8_attn_kernel(
     s_ml[w][1][r] = l_run;
   }
   __syncthreads();
-  // Join the four waves: thread e takes channel e & 127 of heads e >> 7, + 2, ...  A wave
-  // without a page has sum 0 and is left out; one whose sum is NaN is not.
-  float* pp = part + (((int64_t)g * total_q + t) * n_splits + s) * LS_Q8_PART;
-  for (int e = tid; e < gs * kDim; e += 256) {
-    const int h = e >> 7, d = e & 127;
-    float M = -INFINITY;
+  // Join the four waves, eight channels of a head a thread.  A wave without a page has sum 0
+  // and is left out; one whose sum is NaN is not.
+  const int h = tid >> 4, d = 8 * (tid & 15);
+  if (h >= gs) return;
+  float M = -INFINITY, L = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) M = fmaxf(M, s_ml[i][0][h]);
-    float acc = 0.f, L = 0.f;
+  for (int i = 0; i < 4; ++i) M = fmaxf(M, s_ml[i][0][h]);
+  ls_f32x4 a[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (s_ml[i][1][h] == 0.f) continue;
-      const float wt = __builtin_amdgcn_exp2f(s_ml[i][0][h] - M);
-      acc += wt * s_o[i][h * LS_Q8_PITCH + d];
-      L += wt * s_ml[i][1][h];
-    }
-    if (n_splits == 1) {
-      out[(t * G + g) * (int64_t)gs * kDim + e] = LsElem<DT>::from_f(L == 0.f ? 0.f : acc / L);
-      if (lse && d == 0)
-        lse[((int64_t)g * gs + h) * total_q + t] =
-            L == 0.f ? INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
-    } else {
-      pp[e] = acc;
-      if (d == 0) {
-        pp[16 * 128 + h] = M;
-        pp[16 * 128 + 16 + h] = L;
-      }
-    }
+  for (int i = 0; i < 4; ++i) {
+    const float l = s_ml[i][1][h];
+    const float wt = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(s_ml[i][0][h] - M);
+    const float* so = &s_o[i][h * LS_Q8_PITCH + d];
+    a[0] += wt * *reinterpret_cast<const ls_f32x4*>(so);
+    a[1] += wt * *reinterpret_cast<const ls_f32x4*>(so + 4);
+    L += wt * l;
+  }
+  const int64_t tg = (int64_t)g * total_q + t;
+  if (n_splits == 1) {
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    ls_u32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      x[e] = ls_pack2(LsElem<DT>::from_f(a[e >> 1][2 * (e & 1)] * inv),
+                      LsElem<DT>::from_f(a[e >> 1][2 * (e & 1) + 1] * inv));
+    *reinterpret_cast<ls_u32x4*>(out + ((t * G + g) * (int64_t)gs + h) * kDim + d) = x;
+    if (lse && d == 0)
+      lse[((int64_t)g * gs + h) * total_q + t] =
+          L == 0.f ? INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
+  } else {
+    float* po = part.o + ((tg * n_splits + s) * gs + h) * kDim + d;
+    *reinterpret_cast<ls_f32x4*>(po) = a[0];
+    *reinterpret_cast<ls_f32x4*>(po + 4) = a[1];
+    if (d == 0) part.ml[(tg * gs + h) * n_splits + s] = make_float2(M, L);
   }
 }
 
-// out[t][g*gs + h] = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s; a row that sees no key
-// gives zeros and lse = +inf.  A workgroup per (row, KV head, query head), a thread per channel;
-// the weights of the slices (one a thread) are formed in LDS.
-template <int DT>
-__global__ __launch_bounds__(128) void ls_q8_join_kernel(
-    const float* __restrict__ part, const int32_t* __restrict__ cu_q, int batch, int64_t total_q,
-    int gs, int n_splits, uint16_t* __restrict__ out, float* __restrict__ lse) {
+// out[t][g*gs + h] = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the slices that the
+// row fills; a row that sees no key gives zeros and lse = +inf.  A workgroup per (row, KV head,
+// query head): each wave forms the maximum and sum of all slices (at most four a lane), then
+// thread (part, c) sums four channels of every eighth slice, and the eight parts are added in
+// LDS in order.
+template <int DT, bool DENSE>
+__global__ __launch_bounds__(256) void ls_q8_join_kernel(
+    Q8Part part, const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cache_seqlens,
+    int batch, int64_t pages, int causal, int ppw, int64_t total_q, int gs, int n_splits,
+    uint16_t* __restrict__ out, float* __restrict__ lse) {
   __shared__ float s_w[LS_Q8_MAX_SPLITS];
+  __shared__ ls_f32x4 s_a[8][32];
   const int64_t t = blockIdx.x;
   const int g = blockIdx.y, h = blockIdx.z, G = gridDim.y;
+  const int tid = threadIdx.x, lane = tid & 63;
   if (t >= cu_q[batch]) return;
-  const int tid = threadIdx.x;
-  const float* pr = part + ((int64_t)g * total_q + t) * n_splits * LS_Q8_PART;
-  // Every wave goes over all slices (at most four a lane), so no value is exchanged but weights.
-  float ms[4], ls[4], M = -INFINITY;
+  int n = n_splits;
+  if constexpr (DENSE) {
+    const Q8Row row = q8_row(cu_q, cache_seqlens, batch, t, pages * kPage, causal);
+    n = max(1, __builtin_amdgcn_readfirstlane(q8_share(row.limit, ppw, n_splits).slices));
+  }
+  const int64_t tg = (int64_t)g * total_q + t;
+  const float2* ml = part.ml + (tg * gs + h) * n_splits;
+  float ms[4], sum[4], M = -INFINITY;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const int i = 64 * k + (tid & 63);
-    ms[k] = i < n_splits ? pr[(int64_t)i * LS_Q8_PART + 16 * 128 + h] : -INFINITY;
-    ls[k] = i < n_splits ? pr[(int64_t)i * LS_Q8_PART + 16 * 128 + 16 + h] : 0.f;
+    const int i = 64 * k + lane;
+    const float2 x = i < n ? ml[i] : make_float2(-INFINITY, 0.f);
+    ms[k] = x.x;
+    sum[k] = x.y;
     M = fmaxf(M, ms[k]);
   }
 #pragma unroll
@@ -519,27 +614,38 @@ __global__ __launch_bounds__(128) void ls_q8_join_kernel(
   float L = 0.f;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    ms[k] = ls[k] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ms[k] - M);
-    L += ms[k] * ls[k];
+    ms[k] = sum[k] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ms[k] - M);
+    L += ms[k] * sum[k];
   }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) L += ls_shfl_xor(L, o);
-  const float inv = L == 0.f ? 0.f : 1.f / L;
   if (tid < 64) {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (64 * k + tid < n_splits) s_w[64 * k + tid] = ms[k] * inv;
+      if (64 * k + lane < n) s_w[64 * k + lane] = ms[k];
   }
   __syncthreads();
-  float acc = 0.f;
-  for (int sp = 0; sp < n_splits; ++sp) {
-    const float x = pr[(int64_t)sp * LS_Q8_PART + h * 128 + tid];
-    if (s_w[sp] != 0.f) acc += s_w[sp] * x;
+  const int c = tid & 31, p = tid >> 5;
+  ls_f32x4 a = {0.f, 0.f, 0.f, 0.f};
+  const float* po = part.o + (tg * n_splits * gs + h) * kDim + 4 * c;
+#pragma unroll 8
+  for (int sp = p; sp < n; sp += 8)
+    a += s_w[sp] * *reinterpret_cast<const ls_f32x4*>(po + (int64_t)sp * gs * kDim);
+  s_a[p][c] = a;
+  __syncthreads();
+  if (tid < 32) {
+    a = s_a[0][c];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) a += s_a[i][c];
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    uint2 x;
+    x.x = ls_pack2(LsElem<DT>::from_f(a[0] * inv), LsElem<DT>::from_f(a[1] * inv));
+    x.y = ls_pack2(LsElem<DT>::from_f(a[2] * inv), LsElem<DT>::from_f(a[3] * inv));
+    *reinterpret_cast<uint2*>(out + ((t * G + g) * (int64_t)gs + h) * kDim + 4 * c) = x;
+    if (lse && tid == 0)
+      lse[((int64_t)g * gs + h) * total_q + t] =
+          L == 0.f ? INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
   }
-  out[((t * G + g) * (int64_t)gs + h) * kDim + tid] = LsElem<DT>::from_f(acc);
-  if (lse && tid == 0)
-    lse[((int64_t)g * gs + h) * total_q + t] =
-        L == 0.f ? INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
 }
 
 }  // namespace
@@ -604,10 +710,10 @@ extern "C" int ls_kvcache_append_q8(void* k8, void* v8, int64_t cache_batch_stri
                           : pool(ls_q8_windows_kernel<LS_F16>);
 }
 
-extern "C" size_t ls_attn_kvcache_q8_workspace_size(int64_t total_q, int32_t num_kv_heads,
+extern "C" size_t ls_attn_kvcache_q8_workspace_size(int64_t total_q, int32_t num_heads,
                                                     int32_t n_splits) {
-  if (n_splits <= 1 || total_q <= 0 || num_kv_heads <= 0) return 0;
-  return ls_align256(4 * (size_t)total_q * num_kv_heads * n_splits * LS_Q8_PART);
+  if (n_splits <= 1 || total_q <= 0 || num_heads <= 0) return 0;
+  return 4 * (size_t)total_q * num_heads * n_splits * (kDim + 2);
 }
 
 extern "C" int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int32_t* cu_seqlens_q,
@@ -616,7 +722,7 @@ extern "C" int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int
                                   const uint8_t* v_scale, int64_t scale_batch_stride,
                                   int64_t pages, const int32_t* cache_seqlens, int32_t batch,
                                   int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                                  int32_t dtype, const int32_t* topk_idx, int32_t topk,
+                                  int32_t dtype, const int32_t* topk_idx, int32_t n_pages,
                                   float softmax_scale, int32_t causal, int32_t n_splits, void* out,
                                   float* softmax_lse, void* workspace, size_t workspace_bytes,
                                   void* stream) {
@@ -630,10 +736,10 @@ extern "C" int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int
   LS_REQUIRE(dtype == LS_BF16 || dtype == LS_F16, LS_ERR_UNSUPPORTED,
              "%s: queries are bf16 or fp16", who);
   const bool dense = topk_idx == nullptr;
-  LS_REQUIRE((dense || topk >= 1) && n_splits >= 1 && n_splits <= LS_Q8_MAX_SPLITS, LS_ERR_INVALID,
-             "%s: need topk >= 1 and 1 <= n_splits <= %d", who, LS_Q8_MAX_SPLITS);
-  LS_REQUIRE(dense || topk <= 64 * LS_Q8_ID_REGS, LS_ERR_UNSUPPORTED,
-             "%s: at most %d plan ids per row (got %d)", who, 64 * LS_Q8_ID_REGS, topk);
+  LS_REQUIRE(n_pages >= 1 && n_splits >= 1 && n_splits <= LS_Q8_MAX_SPLITS, LS_ERR_INVALID,
+             "%s: need n_pages >= 1 and 1 <= n_splits <= %d", who, LS_Q8_MAX_SPLITS);
+  LS_REQUIRE(dense || n_pages <= 64 * LS_Q8_ID_REGS, LS_ERR_UNSUPPORTED,
+             "%s: at most %d plan ids per row (got %d)", who, 64 * LS_Q8_ID_REGS, n_pages);
   LS_REQUIRE(total_q <= 0x7fffffffLL / n_splits && num_kv_heads <= 65535, LS_ERR_UNSUPPORTED,
              "%s: too many rows or KV heads", who);
   LS_REQUIRE(pages <= 0x1000000, LS_ERR_UNSUPPORTED, "%s: at most 2^24 pages a sequence", who);
@@ -642,22 +748,26 @@ extern "C" int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int
   if (total_q == 0) return LS_OK;
   LS_REQUIRE(q && k8 && v8 && k_scale && v_scale && cu_seqlens_q && cache_seqlens && out,
              LS_ERR_INVALID, "%s: null pointer", who);
-  LS_REQUIRE(ls_aligned16(q) && ls_aligned16(k8) && ls_aligned16(v8), LS_ERR_UNSUPPORTED,
-             "%s: tensors must be 16-byte aligned", who);
-  // Four waves a slice, ppw plan slots a wave.
-  const int ppw = dense ? 0 : (topk + 4 * n_splits - 1) / (4 * n_splits);
-  const int splits = dense ? n_splits : (topk + 4 * ppw - 1) / (4 * ppw);
-  const size_t need = ls_attn_kvcache_q8_workspace_size(total_q, num_kv_heads, splits);
+  LS_REQUIRE(ls_aligned16(q) && ls_aligned16(k8) && ls_aligned16(v8) && ls_aligned16(out) &&
+                 ls_aligned16(workspace),
+             LS_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned", who);
+  // Four waves a slice, ppw plan slots or pages a wave; with every wave's share rounded up,
+  // fewer slices may do.
+  const int ppw = (int)((n_pages + 4LL * n_splits - 1) / (4 * n_splits));
+  const int splits = (int)((n_pages + 4LL * ppw - 1) / (4 * ppw));
+  const size_t need = ls_attn_kvcache_q8_workspace_size(total_q, num_heads, splits);
   LS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), LS_ERR_WORKSPACE,
              "%s: workspace %zu < %zu", who, workspace ? workspace_bytes : (size_t)0, need);
   hipStream_t s = (hipStream_t)stream;
   const float scale_log2 = softmax_scale * 1.4426950408889634f;
-  float* part = (float*)workspace;
+  Q8Part part;
+  part.o = (float*)workspace;
+  part.ml = (float2*)(part.o + (splits > 1 ? (size_t)total_q * num_heads * splits * kDim : 0));
   auto attend = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)(total_q * splits), num_kv_heads), dim3(256), 0,
                        s, (const uint16_t*)q, q_row_stride, cu_seqlens_q, batch, total_q,
                        (const uint8_t*)k8, (const uint8_t*)v8, cache_batch_stride, k_scale,
-                       v_scale, scale_batch_stride, pages, cache_seqlens, gs, topk_idx, topk, ppw,
+                       v_scale, scale_batch_stride, pages, cache_seqlens, gs, topk_idx, n_pages, ppw,
                        splits, scale_log2, causal, part, (uint16_t*)out, softmax_lse);
     return ls_check_launch("ls_q8_attn_kernel");
   };
@@ -668,9 +778,12 @@ extern "C" int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int
     rc = dense ? attend(ls_q8_attn_kernel<LS_F16, true>) : attend(ls_q8_attn_kernel<LS_F16, false>);
   if (rc || splits == 1) return rc;
   auto join = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)total_q, num_kv_heads, gs), dim3(128), 0, s, part,
-                       cu_seqlens_q, batch, total_q, gs, splits, (uint16_t*)out, softmax_lse);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)total_q, num_kv_heads, gs), dim3(256), 0, s, part,
+                       cu_seqlens_q, cache_seqlens, batch, pages, causal, ppw, total_q, gs, splits,
+                       (uint16_t*)out, softmax_lse);
     return ls_check_launch("ls_q8_join_kernel");
   };
-  return dtype == LS_BF16 ? join(ls_q8_join_kernel<LS_BF16>) : join(ls_q8_join_kernel<LS_F16>);
+  if (dtype == LS_BF16)
+    return dense ? join(ls_q8_join_kernel<LS_BF16, true>) : join(ls_q8_join_kernel<LS_BF16, false>);
+  return dense ? join(ls_q8_join_kernel<LS_F16, true>) : join(ls_q8_join_kernel<LS_F16, false>);
 }

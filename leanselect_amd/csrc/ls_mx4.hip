@@ -40,55 +40,127 @@ __device__ __forceinline__ ls_u32x4 mx4_expand(uint32_t v, float scale) {
   return o;
 }
 
-// Workgroup (tile of outputs, block of 16 MT rows of x): NW waves share the inputs, four tiles
-// (512 inputs) at a time, and are summed through LDS in order.  PAIR: the tile and the one
-// `pair` tiles later are the gate and up projections of the same outputs, and
-// silu(gate) * up is written (float32 up to the one rounding).
-template <int DT, int MT, bool PAIR, int NW>
+// Outputs col .. col + 3 of a row, as far as there are so many.
+template <int DT>
+__device__ __forceinline__ void mx4_store(ls_f32x4 y, uint16_t* row, int64_t col, int64_t n_out) {
+  uint16_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = LsElem<DT>::from_f(y[i]);
+  uint16_t* o = row + col;
+  if (col + 4 <= n_out && ((uintptr_t)o & 7) == 0) {
+    *reinterpret_cast<uint2*>(o) = make_uint2(ls_pack2(h[0], h[1]), ls_pack2(h[2], h[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col + i < n_out) o[i] = h[i];
+  }
+}
+
+__device__ __forceinline__ ls_f32x4 mx4_silu_mul(ls_f32x4 gate, ls_f32x4 up) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) gate[i] = gate[i] / (1.f + __expf(-gate[i])) * up[i];
+  return gate;
+}
+
+// Four registers a lane, [piece][quarter of the wave] -> [quarter][piece]: what lane (r, q) holds
+// as piece p goes to lane (r, p) as piece q.
+__device__ __forceinline__ void mx4_transpose(ls_u32x4 (&x)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    // Halves of the wave, pieces two apart; then odd and even quarters, pieces one apart.
+    const auto a = __builtin_amdgcn_permlane32_swap(x[0][e], x[2][e], false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(x[1][e], x[3][e], false, false);
+    const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+    const auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    x[0][e] = c[0];
+    x[1][e] = c[1];
+    x[2][e] = d[0];
+    x[3][e] = d[1];
+  }
+}
+
+// Workgroup (RT tiles of 16 outputs, block of 16 MT rows of x): NW waves share the inputs, four
+// tiles (512 inputs) at a time, and are summed through LDS in order, so a row's bits depend
+// on neither MT nor RT.  PAIR: half of the tiles are `pair` tiles later, the up projections of
+// the same outputs, and silu(gate) * up is written (float32 up to the one rounding).
+//
+// x is read as it lies, a load's lanes (r, p) taking 16 bytes each of 64 contiguous ones of row
+// r: the operands' own order (64 bytes apart) would touch a cache line per lane, which bounded
+// the kernel at 1.8 TB/s of weights at 16 rows.  Four registers' exchange between the
+// quarters of the wave brings the pieces where the weights' order wants them.
+// A wave's next weights are loaded into the registers of each tile that it has used.
+template <int DT, int MT, int RT, bool PAIR, int NW>
 __global__ __launch_bounds__(64 * NW) void ls_mx4_kernel(
     const uint16_t* __restrict__ x, int64_t xrs, int64_t m, int64_t K,
     const uint8_t* __restrict__ codes, const uint32_t* __restrict__ scales, int64_t kc, int64_t kc4,
-    int64_t pair, int64_t n_out, uint16_t* __restrict__ out, int64_t ors) {
-  constexpr int RT = PAIR ? 2 : 1;
+    int64_t tiles, int64_t n_out, uint16_t* __restrict__ out, int64_t ors) {
+  constexpr int OT = PAIR ? RT / 2 : RT;  // tiles of outputs
   __shared__ __attribute__((aligned(16))) ls_f32x4 s_acc[NW][RT * MT][64];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
-  const int64_t nt = blockIdx.x, m0 = (int64_t)blockIdx.y * (16 * MT);
+  const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
+  // Tile a of the workgroup; past the last one, the last again (not written).
+  int64_t tile[RT];
+#pragma unroll
+  for (int a = 0; a < RT; ++a) {
+    const int64_t t = min((int64_t)blockIdx.x * OT + a % OT, tiles - 1);
+    tile[a] = t + (a / OT) * tiles;
+  }
   ls_f32x4 acc[RT][MT];
 #pragma unroll
   for (int a = 0; a < RT; ++a)
 #pragma unroll
     for (int c = 0; c < MT; ++c) acc[a][c] = ls_f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (int64_t j = w; j < kc4; j += NW) {
-    const int n = (int)min<int64_t>(4, kc - 4 * j);
-    ls_u32x4 wt[RT][4];
-    uint32_t sc[RT];
+  ls_u32x4 wt[RT][4];
+  uint32_t sc[RT];
+  auto load_w = [&](int64_t j, int i) {
+    const int64_t chunk = min(4 * j + i, kc - 1);  // past the last one: x is zero there
 #pragma unroll
-    for (int a = 0; a < RT; ++a) {
-      const int64_t tile = nt + a * pair;
-      sc[a] = scales[(tile * kc4 + j) * 64 + lane];
+    for (int a = 0; a < RT; ++a) wt[a][i] = ls_load16(codes + ((tile[a] * kc + chunk) * 64 + lane) * 16);
+  };
+  auto load_s = [&](int64_t j) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        wt[a][i] = i < n ? ls_load16(codes + ((tile * kc + 4 * j + i) * 64 + lane) * 16)
-                         : ls_u32x4{0u, 0u, 0u, 0u};
+    for (int a = 0; a < RT; ++a) sc[a] = scales[(tile[a] * kc4 + j) * 64 + lane];
+  };
+  const uint16_t* xrow[MT];
+#pragma unroll
+  for (int c = 0; c < MT; ++c) xrow[c] = x + min(m0 + 16 * c + r, m - 1) * xrs;
+  ls_u32x4 xr[MT][4];
+  auto load_x = [&](int64_t j, int i) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const int64_t k = 512 * j + 128 * i + 32 * p + 8 * q;
+#pragma unroll
+      for (int c = 0; c < MT; ++c)
+        xr[c][p] = m0 + 16 * c + r < m && k < K ? ls_load16(xrow[c] + k) : ls_u32x4{0u, 0u, 0u, 0u};
     }
+  };
+  // 512 inputs whose weights are in registers (or on their way), with the loads of the wave's
+  // next ones.
+  auto group = [&](int64_t j, auto more) {
+    constexpr bool kMore = decltype(more)::value;
+    uint32_t s4[RT];
+#pragma unroll
+    for (int a = 0; a < RT; ++a) s4[a] = sc[a];
+    if constexpr (kMore) load_s(j + NW);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       ls_u32x4 xf[MT][4];
-      const int64_t k0 = 512 * j + 128 * i + 32 * q;
 #pragma unroll
       for (int c = 0; c < MT; ++c) {
-        const int64_t row = m0 + 16 * c + r;
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-          xf[c][s] = row < m && k0 + 8 * s < K ? ls_load16(x + row * xrs + k0 + 8 * s)
-                                               : ls_u32x4{0u, 0u, 0u, 0u};
+        for (int p = 0; p < 4; ++p) xf[c][p] = xr[c][p];
+        mx4_transpose(xf[c]);
       }
+      if (i < 3)
+        load_x(j, i + 1);
+      else if constexpr (kMore)
+        load_x(j + NW, 0);
 #pragma unroll
       for (int a = 0; a < RT; ++a) {
-        const float f = __uint_as_float(((sc[a] >> (8 * i)) & 0xffu) << 23);
+        const float f = __uint_as_float(((s4[a] >> (8 * i)) & 0xffu) << 23);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           const ls_u32x4 wf = mx4_expand<DT>(wt[a][i][s], f);
@@ -96,40 +168,194 @@ __global__ __launch_bounds__(64 * NW) void ls_mx4_kernel(
           for (int c = 0; c < MT; ++c) acc[a][c] = LsElem<DT>::mfma(wf, xf[c][s], acc[a][c]);
         }
       }
+      if constexpr (kMore) load_w(j + NW, i);
     }
+  };
+  int64_t j = w;
+  if (j < kc4) {
+    load_s(j);
+    load_w(j, 0);
+    load_x(j, 0);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) load_w(j, i);
+    for (; j + NW < kc4; j += NW) group(j, std::true_type());
+    group(j, std::false_type());
   }
 #pragma unroll
   for (int a = 0; a < RT; ++a)
 #pragma unroll
     for (int c = 0; c < MT; ++c) s_acc[w][a * MT + c][lane] = acc[a][c];
   __syncthreads();
-  // acc[c][i]: output 16 nt + 4 q + i of row m0 + 16 c + r.
-  for (int c = w; c < MT; c += NW) {
-    ls_f32x4 y[RT];
+  // acc[a][c][i]: output 16 tile + 4 q + i of row m0 + 16 c + r.  A wave a (tile, 16 rows).
+  for (int u = w; u < OT * MT; u += NW) {
+    const int a = u / MT, c = u - a * MT;
+    ls_f32x4 y = s_acc[0][u][lane];
 #pragma unroll
-    for (int a = 0; a < RT; ++a) {
-      y[a] = s_acc[0][a * MT + c][lane];
-#pragma unroll
-      for (int i = 1; i < NW; ++i) y[a] += s_acc[i][a * MT + c][lane];
-    }
+    for (int i = 1; i < NW; ++i) y += s_acc[i][u][lane];
     if constexpr (PAIR) {
+      ls_f32x4 up = s_acc[0][u + OT * MT][lane];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[0][i] = y[0][i] / (1.f + __expf(-y[0][i])) * y[1][i];
+      for (int i = 1; i < NW; ++i) up += s_acc[i][u + OT * MT][lane];
+      y = mx4_silu_mul(y, up);
     }
-    const int64_t row = m0 + 16 * c + r, col = 16 * nt + 4 * q;
-    if (row >= m) continue;
-    uint16_t h[4];
+    const int64_t t = (int64_t)blockIdx.x * OT + a, row = m0 + 16 * c + r;
+    if (t < tiles && row < m) mx4_store<DT>(y, out + row * ors, 16 * t + 4 * q, n_out);
+  }
+}
+
+// More rows: what x costs a compute unit then bounds the product (16 rows of x are 4 KB for
+// every 1 KB of a tile), so eight tiles of outputs share it through LDS.  Workgroup (eight
+// tiles, or four and their up projections; block of 16 MT rows; slice z of the inputs): eight
+// waves, wave (n, h) two tiles over the h-th half of the slice.  256 inputs of each half are
+// staged at a time, in two buffers: the four waves of a half load x as it lies (wave n the n-th
+// 64 bytes of each 256), and an operand is read back across the pieces, 256 contiguous bytes
+// for 16 lanes.  The halves are summed through LDS; with several slices float32 parts go to the
+// workspace, [slice][row][16 tiles], and a second kernel adds them in order.
+template <int DT, int MT, bool PAIR>
+__global__ __launch_bounds__(512) void ls_mx4_rows_kernel(
+    const uint16_t* __restrict__ x, int64_t xrs, int64_t m, int64_t K,
+    const uint8_t* __restrict__ codes, const uint32_t* __restrict__ scales, int64_t kc, int64_t kc4,
+    int64_t tiles, int64_t per_half, int64_t n_out, uint16_t* __restrict__ out, int64_t ors,
+    float* __restrict__ part) {
+  constexpr int OT = PAIR ? 4 : 8;  // tiles of outputs of the workgroup
+  // [buffer][half][128 inputs][16 rows][32 inputs][16 p + r]: 16 bytes, piece p of row r
+  __shared__ __attribute__((aligned(16))) ls_u32x4 s_x[2][2][2][MT][4][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = w & 3, h = w >> 2;
+  const int r = lane & 15, q = lane >> 4;
+  const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
+  int64_t ot[2], tile[2];  // tile of outputs, tile of the weight (past the last: the last again)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = LsElem<DT>::from_f(y[0][i]);
-    uint16_t* o = out + row * ors + col;
-    if (col + 4 <= n_out && ((uintptr_t)o & 7) == 0) {
-      *reinterpret_cast<uint2*>(o) = make_uint2(ls_pack2(h[0], h[1]), ls_pack2(h[2], h[3]));
-    } else {
+  for (int a = 0; a < 2; ++a) {
+    ot[a] = (int64_t)blockIdx.x * OT + (PAIR ? wn : 2 * wn + a);
+    tile[a] = min(ot[a], tiles - 1) + (PAIR ? a * tiles : 0);
+  }
+  const int64_t g0 = (2 * (int64_t)blockIdx.z + h) * per_half;  // groups of 512 inputs
+  const int64_t g1 = min(kc4, g0 + per_half);
+  ls_f32x4 acc[2][MT];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (col + i < n_out) o[i] = h[i];
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int c = 0; c < MT; ++c) acc[a][c] = ls_f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // Past the half's end weights are those of the last group, and x is zero.
+  ls_u32x4 wt[2][4];
+  uint32_t sc[2];
+  auto load_w = [&](int64_t g, int i) {
+    const int64_t chunk = min(4 * g + i, kc - 1);
+#pragma unroll
+    for (int a = 0; a < 2; ++a) wt[a][i] = ls_load16(codes + ((tile[a] * kc + chunk) * 64 + lane) * 16);
+  };
+  auto load_s = [&](int64_t g) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) sc[a] = scales[(tile[a] * kc4 + min(g, kc4 - 1)) * 64 + lane];
+  };
+  ls_u32x4 xs[2 * MT];
+  auto load_x = [&](int64_t g, int st) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t k = 512 * g + 256 * st + 128 * i + 32 * wn + 8 * q;
+#pragma unroll
+      for (int c = 0; c < MT; ++c) {
+        const int64_t row = m0 + 16 * c + r;
+        xs[i * MT + c] = row < m && k < K && g < g1 ? ls_load16(x + row * xrs + k)
+                                                    : ls_u32x4{0u, 0u, 0u, 0u};
+      }
+    }
+  };
+  auto store_x = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int c = 0; c < MT; ++c) s_x[buf][h][i][c][wn][lane] = xs[i * MT + c];
+  };
+  load_s(g0);
+  load_x(g0, 0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) load_w(g0, i);
+  store_x(0);
+  for (int64_t j = 0; j < per_half; ++j) {
+    const int64_t g = g0 + j;
+    const uint32_t s4[2] = {sc[0], sc[1]};
+    load_s(g + 1);
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      __syncthreads();  // buffer st is whole, and nobody reads the other any more
+      load_x(g + st, st ^ 1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float f[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+          f[a] = __uint_as_float(((s4[a] >> (16 * st + 8 * i)) & 0xffu) << 23);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          ls_u32x4 xf[MT];
+#pragma unroll
+          for (int c = 0; c < MT; ++c) xf[c] = s_x[st][h][i][c][q][16 * s + r];
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            const ls_u32x4 wf = mx4_expand<DT>(wt[a][2 * st + i][s], f[a]);
+#pragma unroll
+            for (int c = 0; c < MT; ++c) acc[a][c] = LsElem<DT>::mfma(wf, xf[c], acc[a][c]);
+          }
+        }
+        load_w(g + 1, 2 * st + i);
+      }
+      store_x(st ^ 1);
     }
   }
+  __syncthreads();
+  ls_f32x4(*s_acc)[2][MT][64] = reinterpret_cast<ls_f32x4(*)[2][MT][64]>(&s_x[0][0][0][0][0][0]);
+  if (h == 1) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int c = 0; c < MT; ++c) s_acc[wn][a][c][lane] = acc[a][c];
+  }
+  __syncthreads();
+  if (h == 1) return;
+  // acc[a][c][i]: output 16 tile + 4 q + i of row m0 + 16 c + r.
+#pragma unroll
+  for (int c = 0; c < MT; ++c) {
+    const int64_t row = m0 + 16 * c + r;
+    if (row >= m) continue;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) acc[a][c] += s_acc[wn][a][c][lane];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      if (ot[a] >= tiles) continue;
+      if (gridDim.z > 1) {
+        const int64_t cols = 16 * tiles * (PAIR ? 2 : 1);
+        *reinterpret_cast<ls_f32x4*>(part + ((int64_t)blockIdx.z * m + row) * cols + 16 * tile[a] + 4 * q) =
+            acc[a][c];
+      } else if (!PAIR) {
+        mx4_store<DT>(acc[a][c], out + row * ors, 16 * ot[a] + 4 * q, n_out);
+      } else if (a == 0) {
+        mx4_store<DT>(mx4_silu_mul(acc[0][c], acc[1][c]), out + row * ors, 16 * ot[a] + 4 * q, n_out);
+      }
+    }
+  }
+}
+
+// The slices' parts, added in order: a thread per four outputs of a row.
+template <int DT, bool PAIR>
+__global__ __launch_bounds__(256) void ls_mx4_join_kernel(const float* __restrict__ part,
+                                                          int64_t slices, int64_t m, int64_t tiles,
+                                                          int64_t n_out, uint16_t* __restrict__ out,
+                                                          int64_t ors) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = at / (4 * tiles), col = 4 * (at - row * 4 * tiles);
+  if (row >= m) return;
+  const int64_t cols = 16 * tiles * (PAIR ? 2 : 1);
+  ls_f32x4 y[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll 8
+  for (int64_t z = 0; z < slices; ++z)
+#pragma unroll
+    for (int a = 0; a < (PAIR ? 2 : 1); ++a)
+      y[a] += *reinterpret_cast<const ls_f32x4*>(part + (z * m + row) * cols + a * 16 * tiles + col);
+  mx4_store<DT>(PAIR ? mx4_silu_mul(y[0], y[1]) : y[0], out + row * ors, col, n_out);
 }
 
 // ---------------------------------------------------------------------------
@@ -199,10 +425,64 @@ bool mx4_sizes(int64_t n, int64_t k) {
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
+namespace {
+// How a product is cut.
+struct Mx4Cut {
+  bool shared;       // ls_mx4_rows_kernel, else ls_mx4_kernel
+  int mt;            // 16-row blocks of x a workgroup
+  int nw, rt;        // ls_mx4_kernel: waves and tiles of the weight a workgroup
+  int64_t slices;    // ls_mx4_rows_kernel: of the inputs
+  int64_t per_half;  // and groups of 512 inputs for each half of a slice
+  int64_t tiles;     // of outputs (16 each)
+  int64_t kc, kc4;   // tiles and groups of four tiles along the inputs
+  int64_t blocks;    // of rows
+};
+
+// Measured with weights from memory (us; floor at 5.13 TB/s), outputs x inputs, rows:
+//   waves and tiles a workgroup (8/1, 8/2, 4/4), one row: 4096 x 4096 5.2, 6.1, 9.0; 4608 x 4096
+//   6.9, 6.2, 9.1; 16384 x 4096 12.6, 11.5, 12.7; 73448 x 4096 47, 36.5, 35.3 (floor 31).  So
+//   eight waves up to 1024 tiles of the weight, one tile up to 256 (all workgroups in one round).
+//   ls_mx4_kernel, ls_mx4_rows_kernel, above 16 rows: 4608 x 4096, 40 rows 14.7, 13.1; [gate; up]
+//   32768 x 4096, 33 rows 33.9, 23.7 (floor 13.9); 4096 x 16384, 33 rows 37.8, 18.2; but 3000 x 600,
+//   24 rows 4.3, 5.7: the second for weights from 2 MB.  Up to 16 rows: [gate; up] 32768 x 4096, one
+//   row 18.6, 17.4, 16 rows 20.1, 17.6; 4096 x 16384, one row 15.0, 12.6, 16 rows 20.1, 13.7; but
+//   4608 x 4096, 16 rows 8.0, 9.7; 73448 x 4096, one row 35.3, 41.1: the second where its
+//   workgroups just fill the chip's 256 units without slices, or where the inputs are long and
+//   the tiles few.
+Mx4Cut mx4_cut(int64_t rows, int64_t K, int64_t N, bool silu) {
+  Mx4Cut c;
+  const int64_t tiles = (N + 15) / 16;  // of the weight
+  c.kc = (K + 127) / 128;
+  c.kc4 = (c.kc + 3) / 4;
+  c.tiles = silu ? tiles / 2 : tiles;
+  c.mt = rows > 64 ? 4 : (int)((rows + 15) / 16);
+  c.blocks = (rows + 16 * c.mt - 1) / (16 * c.mt);
+  c.nw = tiles <= 1024 ? 8 : 4;
+  c.rt = c.nw == 4 ? 4 : silu || tiles > 256 ? 2 : 1;
+  const int64_t per_wg = silu ? 4 : 8;
+  const int64_t wgs = (c.tiles + per_wg - 1) / per_wg * c.blocks;
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(c.kc4 / 2, 256 / wgs));
+  c.per_half = (c.kc4 + 2 * want - 1) / (2 * want);
+  c.slices = (c.kc4 + 2 * c.per_half - 1) / (2 * c.per_half);
+  c.shared = rows > 16 ? tiles * c.kc >= 2048
+                       : (c.slices == 1 && wgs > 128 && wgs <= 256) || (c.kc4 >= 16 && tiles <= 256);
+  return c;
+}
+}  // namespace
+
+extern "C" size_t ls_linear_mx4_workspace_size(int64_t rows, int64_t in_features,
+                                               int64_t out_features, int32_t silu_mul) {
+  if (rows <= 0 || !mx4_sizes(out_features, in_features)) return 0;
+  const Mx4Cut c = mx4_cut(rows, in_features, out_features, silu_mul != 0);
+  if (!c.shared || c.slices == 1) return 0;
+  return 4 * (size_t)c.slices * rows * c.tiles * 16 * (silu_mul ? 2 : 1);
+}
+
 extern "C" int ls_linear_mx4(const void* x, int64_t x_row_stride, int64_t rows,
                              int64_t in_features, const void* codes, const void* scales,
                              int64_t out_features, int32_t silu_mul, int32_t dtype, void* out,
-                             int64_t out_row_stride, void* stream) {
+                             int64_t out_row_stride, void* workspace, size_t workspace_bytes,
+                             void* stream) {
   const char* who = "ls_linear_mx4";
   LS_REQUIRE(rows >= 0 && mx4_sizes(out_features, in_features), LS_ERR_INVALID,
              "%s: need rows >= 0, out_features >= 1 and in_features a multiple of 8", who);
@@ -213,34 +493,66 @@ extern "C" int ls_linear_mx4(const void* x, int64_t x_row_stride, int64_t rows,
              who);
   if (rows == 0) return LS_OK;
   LS_REQUIRE(x && codes && scales && out, LS_ERR_INVALID, "%s: null pointer", who);
-  LS_REQUIRE(ls_aligned16(x) && ls_aligned16(codes) && ((uintptr_t)scales & 3) == 0,
-             LS_ERR_UNSUPPORTED, "%s: x and codes must be 16-byte aligned", who);
-  const int64_t tiles = (out_features + 15) / 16, kc = (in_features + 127) / 128, kc4 = (kc + 3) / 4;
+  LS_REQUIRE(ls_aligned16(x) && ls_aligned16(codes) && ((uintptr_t)scales & 3) == 0 &&
+                 ls_aligned16(workspace),
+             LS_ERR_UNSUPPORTED, "%s: x, codes and workspace must be 16-byte aligned", who);
+  const Mx4Cut cut = mx4_cut(rows, in_features, out_features, silu_mul != 0);
+  const size_t need = ls_linear_mx4_workspace_size(rows, in_features, out_features, silu_mul);
+  LS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), LS_ERR_WORKSPACE,
+             "%s: workspace %zu < %zu", who, workspace ? workspace_bytes : (size_t)0, need);
+  LS_REQUIRE(cut.blocks <= 65535, LS_ERR_UNSUPPORTED, "%s: too many rows", who);
   const int64_t n_out = silu_mul ? out_features / 2 : out_features;
-  const int64_t grid_x = silu_mul ? tiles / 2 : tiles;
-  const int mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const int64_t grid_y = (rows + 16 * mt - 1) / (16 * mt);
-  LS_REQUIRE(grid_y <= 65535, LS_ERR_UNSUPPORTED, "%s: too many rows", who);
-  auto launch = [&](auto dt, auto mtc, auto pr) {
-    constexpr int NW = 4;
-    hipLaunchKernelGGL((ls_mx4_kernel<decltype(dt)::value, decltype(mtc)::value,
-                                      decltype(pr)::value, NW>),
-                       dim3((unsigned)grid_x, (unsigned)grid_y), dim3(64 * NW), 0,
-                       (hipStream_t)stream, (const uint16_t*)x, x_row_stride, rows, in_features,
-                       (const uint8_t*)codes, (const uint32_t*)scales, kc, kc4, grid_x, n_out,
-                       (uint16_t*)out, out_row_stride);
+  hipStream_t stm = (hipStream_t)stream;
+  using std::integral_constant;
+  auto few = [&](auto dt, auto mtc, auto pr, auto rt, auto nw) {
+    constexpr int RT = decltype(rt)::value, NW = decltype(nw)::value;
+    constexpr bool PAIR = decltype(pr)::value;
+    constexpr int OT = PAIR ? RT / 2 : RT;
+    hipLaunchKernelGGL((ls_mx4_kernel<decltype(dt)::value, decltype(mtc)::value, RT, PAIR, NW>),
+                       dim3((unsigned)((cut.tiles + OT - 1) / OT), (unsigned)cut.blocks),
+                       dim3(64 * NW), 0, stm, (const uint16_t*)x, x_row_stride, rows, in_features,
+                       (const uint8_t*)codes, (const uint32_t*)scales, cut.kc, cut.kc4, cut.tiles,
+                       n_out, (uint16_t*)out, out_row_stride);
     return ls_check_launch("ls_mx4_kernel");
   };
+  auto by_waves = [&](auto dt, auto mtc, auto pr) {
+    constexpr int P = decltype(pr)::value ? 2 : 1;
+    if (cut.nw == 4) return few(dt, mtc, pr, integral_constant<int, 4>(), integral_constant<int, 4>());
+    if (cut.rt == 2) return few(dt, mtc, pr, integral_constant<int, 2>(), integral_constant<int, 8>());
+    return few(dt, mtc, pr, integral_constant<int, P>(), integral_constant<int, 8>());
+  };
+  auto shared = [&](auto dt, auto mtc, auto pr) {
+    constexpr int DT = decltype(dt)::value;
+    constexpr bool PAIR = decltype(pr)::value;
+    constexpr int OT = PAIR ? 4 : 8;
+    hipLaunchKernelGGL((ls_mx4_rows_kernel<DT, decltype(mtc)::value, PAIR>),
+                       dim3((unsigned)((cut.tiles + OT - 1) / OT), (unsigned)cut.blocks,
+                            (unsigned)cut.slices),
+                       dim3(512), 0, stm, (const uint16_t*)x, x_row_stride, rows, in_features,
+                       (const uint8_t*)codes, (const uint32_t*)scales, cut.kc, cut.kc4, cut.tiles,
+                       cut.per_half, n_out, (uint16_t*)out, out_row_stride, (float*)workspace);
+    const int rc = ls_check_launch("ls_mx4_rows_kernel");
+    if (rc || cut.slices == 1) return rc;
+    hipLaunchKernelGGL((ls_mx4_join_kernel<DT, PAIR>),
+                       dim3((unsigned)((rows * cut.tiles * 4 + 255) / 256)), dim3(256), 0, stm,
+                       (const float*)workspace, cut.slices, rows, cut.tiles, n_out, (uint16_t*)out,
+                       out_row_stride);
+    return ls_check_launch("ls_mx4_join_kernel");
+  };
+  auto by_form = [&](auto dt, auto mtc, auto pr) {
+    return cut.shared ? shared(dt, mtc, pr) : by_waves(dt, mtc, pr);
+  };
   auto by_pair = [&](auto dt, auto mtc) {
-    return silu_mul ? launch(dt, mtc, std::true_type()) : launch(dt, mtc, std::false_type());
+    return silu_mul ? by_form(dt, mtc, std::true_type()) : by_form(dt, mtc, std::false_type());
   };
   auto by_rows = [&](auto dt) {
-    if (mt == 1) return by_pair(dt, std::integral_constant<int, 1>());
-    if (mt == 2) return by_pair(dt, std::integral_constant<int, 2>());
-    return by_pair(dt, std::integral_constant<int, 4>());
+    if (cut.mt == 1) return by_pair(dt, integral_constant<int, 1>());
+    if (cut.mt == 2) return by_pair(dt, integral_constant<int, 2>());
+    if (cut.mt == 3) return by_pair(dt, integral_constant<int, 3>());
+    return by_pair(dt, integral_constant<int, 4>());
   };
-  return dtype == LS_BF16 ? by_rows(std::integral_constant<int, LS_BF16>())
-                          : by_rows(std::integral_constant<int, LS_F16>());
+  return dtype == LS_BF16 ? by_rows(integral_constant<int, LS_BF16>())
+                          : by_rows(integral_constant<int, LS_F16>());
 }
 
 extern "C" int ls_quantize_mx4(const void* weight, int64_t weight_row_stride, int64_t out_features,

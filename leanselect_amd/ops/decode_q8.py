@@ -21,6 +21,8 @@ The reference's cache is 16-bit (leanselect/models/minicpm.py:1188-1490).
 """
 from __future__ import annotations
 
+from operator import gt
+
 import torch
 
 from .. import _hip
@@ -30,8 +32,11 @@ __all__ = ["new_kvcache_q8", "kvcache_append_q8", "sparse_attention_kvcache_q8",
            "dense_attention_kvcache_q8"]
 
 PAGE, HEAD_DIM = 64, 128
+_E4M3 = torch.float8_e4m3fn
+_CODES = {torch.bfloat16: _hip.LS_BF16, torch.float16: _hip.LS_F16}
 _PAGE_BYTES = PAGE * HEAD_DIM
 _MAX_SPLITS = 256
+_WORKGROUPS, _RAGGED_WORKGROUPS = 256, 1024
 
 
 def new_kvcache_q8(batch: int, capacity: int, num_kv_heads: int, head_dim: int = 128, *,
@@ -50,22 +55,38 @@ def new_kvcache_q8(batch: int, capacity: int, num_kv_heads: int, head_dim: int =
             torch.empty(shape, dtype=torch.uint8, device=device))
 
 
-def _check_cache_q8(k8, v8, k_scale, v_scale) -> tuple[int, int, int]:
-    if k8.ndim != 5 or k8.shape[3:] != (PAGE, HEAD_DIM) or k8.dtype != torch.float8_e4m3fn:
-        raise ValueError(f"k8 must be float8_e4m3fn [batch, pages, num_kv_heads, {PAGE}, {HEAD_DIM}]")
-    B, P, G = k8.shape[:3]
-    if v8.shape != (B, P, G, HEAD_DIM, PAGE) or v8.dtype != torch.float8_e4m3fn:
-        raise ValueError(f"v8 must be float8_e4m3fn [batch, pages, num_kv_heads, {HEAD_DIM}, {PAGE}]")
-    if k_scale.shape != (B, P, G) or v_scale.shape != (B, P, G) \
-            or k_scale.dtype != torch.uint8 or v_scale.dtype != torch.uint8:
-        raise ValueError("k_scale and v_scale must be uint8 [batch, pages, num_kv_heads]")
-    row = (G * _PAGE_BYTES, _PAGE_BYTES)
-    ks, vs = k8.stride(), v8.stride()
+def _cache_dims(k8, v8, k_scale, v_scale) -> tuple[int, int, int, int, int]:
+    """``(batch, pages, num_kv_heads, batch stride, scale batch stride)`` of a well-formed cache."""
+    if k8.ndim != 5 or k8.dtype is not _E4M3 or v8.dtype is not _E4M3 \
+            or k_scale.dtype is not torch.uint8 or v_scale.dtype is not torch.uint8:
+        _refuse_cache()
+    B, P, G, rows, cols = k8.shape
+    scales = (B, P, G)
+    if rows != PAGE or cols != HEAD_DIM or v8.shape != (B, P, G, HEAD_DIM, PAGE) \
+            or k_scale.shape != scales or v_scale.shape != scales:
+        _refuse_cache()
+    if k8.is_contiguous() and v8.is_contiguous() and k_scale.is_contiguous() \
+            and v_scale.is_contiguous():
+        return B, P, G, P * G * _PAGE_BYTES, P * G
+    ks, vs, row = k8.stride(), v8.stride(), (G * _PAGE_BYTES, _PAGE_BYTES)
     if ks[1:] != (*row, HEAD_DIM, 1) or vs[1:] != (*row, PAGE, 1) or ks[0] != vs[0] \
             or k_scale.stride()[1:] != (G, 1) or v_scale.stride() != k_scale.stride():
         raise ValueError("each sequence's pages and scales must be dense, k and v with the same "
                          "batch strides")
-    return B, P, G
+    return B, P, G, ks[0], k_scale.stride(0)
+
+
+def _refuse_cache():
+    raise ValueError(f"the cache must be k8 float8_e4m3fn [batch, pages, num_kv_heads, {PAGE}, "
+                     f"{HEAD_DIM}], v8 float8_e4m3fn [batch, pages, num_kv_heads, {HEAD_DIM}, "
+                     f"{PAGE}] and k_scale, v_scale uint8 [batch, pages, num_kv_heads]")
+
+
+def _rows16(t: torch.Tensor) -> bool:
+    """Rows ``[n, heads, 128]`` that the kernels read as they are: dense, 16-byte aligned."""
+    if t.data_ptr() % 16:
+        return False
+    return t.is_contiguous() or (t.stride()[1:] == (HEAD_DIM, 1) and t.stride(0) % 8 == 0)
 
 
 def kvcache_append_q8(k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
@@ -79,49 +100,47 @@ def kvcache_append_q8(k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
     the 8-bit cache and, with ``kc_cache [batch, kc_capacity, G, 128]`` (``k_new``'s dtype),
     the compressed windows the new tokens complete: means of the 32 keys as the cache
     holds them.  ``cache_seqlens`` is left as it is (advance it after)."""
-    B, P, G = _check_cache_q8(k8, v8, k_scale, v_scale)
-    if k_new.ndim != 3 or v_new.shape != k_new.shape or k_new.shape[1:] != (G, HEAD_DIM):
+    B, P, G, cache_stride, scale_stride = _cache_dims(k8, v8, k_scale, v_scale)
+    if k_new.ndim != 3 or k_new.shape != (k_new.shape[0], G, HEAD_DIM) or v_new.shape != k_new.shape:
         raise ValueError("k_new and v_new must be [total_new, num_kv_heads, head_dim] like the cache")
-    if k_new.dtype not in (torch.bfloat16, torch.float16) or v_new.dtype != k_new.dtype:
+    code = _CODES.get(k_new.dtype)
+    if code is None or v_new.dtype is not k_new.dtype:
         raise ValueError("new keys/values must be bf16 or fp16, k and v alike")
+    total = k_new.shape[0]
     lens = _lengths(cache_seqlens, cache_seqlens_host, "cache_seqlens")
     cu = _lengths(cu_seqlens_new, cu_seqlens_new_host, "cu_seqlens_new")
-    if len(lens) != B or cache_seqlens.numel() != B or len(cu) != B + 1 \
-            or cu_seqlens_new.numel() != B + 1 or cu[0] != 0 or cu[-1] != k_new.shape[0]:
+    if len(lens) != B or len(cu) != B + 1 or cu[0] != 0 or cu[-1] != total \
+            or cache_seqlens.numel() != B or cu_seqlens_new.numel() != B + 1:
         raise ValueError("cache_seqlens must be [batch] and cu_seqlens_new [batch + 1] offsets "
                          "of the packed new rows")
-    windows = 0
-    for b, before in enumerate(lens):
-        after = before + cu[b + 1] - cu[b]
-        if before < 0 or after < before or after > P * PAGE:
-            raise ValueError(f"appending {cu[b + 1] - cu[b]} tokens to {before} of sequence {b} "
-                             f"exceeds the capacity {P * PAGE}")
-        if kc_cache is not None and after > before:
-            nw = n_windows(after)
-            if nw > kc_cache.shape[1]:
-                raise ValueError(f"{nw} compressed windows exceed kc_capacity {kc_cache.shape[1]}")
-            windows += nw - n_windows(before)
+    after = [n + b - a for n, a, b in zip(lens, cu, cu[1:])]
+    if min(lens) < 0 or max(after) > P * PAGE or any(map(gt, lens, after)):
+        raise ValueError(f"sequences of {lens} tokens cannot become {after} in a cache with a "
+                         f"capacity of {P * PAGE}")
+    windows, kc = 0, (None, 0, 0, 0)
     if kc_cache is not None:
-        if (kernel_size, kernel_stride) != (32, 16):
+        if kernel_size != 32 or kernel_stride != 16:
             raise ValueError("the 8-bit cache forms windows of 32 keys at stride 16")
-        if kc_cache.ndim != 4 or kc_cache.shape[0] != B or kc_cache.shape[2:] != (G, HEAD_DIM) \
-                or kc_cache.dtype != k_new.dtype or kc_cache.stride()[2:] != (HEAD_DIM, 1):
+        if kc_cache.ndim != 4 or kc_cache.dtype is not k_new.dtype or kc_cache.stride()[2:] != (HEAD_DIM, 1) \
+                or kc_cache.shape != (B, kc_cache.shape[1], G, HEAD_DIM):
             raise ValueError("kc_cache must be [batch, kc_capacity, num_kv_heads, head_dim] in "
                              "k_new's dtype with dense rows")
-    dev = _hip.require_gpu(k8, v8, k_scale, v_scale, cache_seqlens, k_new, v_new, cu_seqlens_new,
+        kc = (kc_cache.data_ptr(), kc_cache.stride(0), kc_cache.stride(1), kc_cache.shape[1])
+        if n_windows(max(after)) > kc[3]:
+            raise ValueError(f"{n_windows(max(after))} compressed windows exceed kc_capacity {kc[3]}")
+        # n_windows(n) = max(1, n // 16) - 1.
+        windows = sum([n >> 4 or 1 for n in after]) - sum([n >> 4 or 1 for n in lens])
+    index = _hip.gpu_index(k8, v8, k_scale, v_scale, cache_seqlens, k_new, v_new, cu_seqlens_new,
                            kc_cache)
     # One row stride serves both: dense 16-byte aligned rows with equal strides, else copies.
-    if k_new.stride()[1:] != (HEAD_DIM, 1) or v_new.stride() != k_new.stride() \
-            or k_new.stride(0) % 8 or k_new.data_ptr() % 16 or v_new.data_ptr() % 16:
+    if not (_rows16(k_new) and _rows16(v_new) and k_new.stride() == v_new.stride()):
         k_new = k_new.clone(memory_format=torch.contiguous_format)
         v_new = v_new.clone(memory_format=torch.contiguous_format)
-    kc = (kc_cache.data_ptr(), kc_cache.stride(0), kc_cache.stride(1), kc_cache.shape[1]) \
-        if kc_cache is not None else (None, 0, 0, 0)
-    _hip.launch(dev, "ls_kvcache_append_q8", k8.data_ptr(), v8.data_ptr(), k8.stride(0),
-                k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0), P,
+    _hip.launch(index, "ls_kvcache_append_q8", k8.data_ptr(), v8.data_ptr(), cache_stride,
+                k_scale.data_ptr(), v_scale.data_ptr(), scale_stride, P,
                 cache_seqlens.contiguous().data_ptr(), k_new.data_ptr(), v_new.data_ptr(),
-                k_new.stride(0), cu_seqlens_new.contiguous().data_ptr(), k_new.shape[0], B, G,
-                HEAD_DIM, _hip.dtype_code(k_new.dtype), *kc, windows)
+                k_new.stride(0), cu_seqlens_new.contiguous().data_ptr(), total, B, G, HEAD_DIM, code,
+                *kc, windows)
 
 
 def sparse_attention_kvcache_q8(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor,
@@ -156,40 +175,53 @@ def dense_attention_kvcache_q8(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tens
 
 def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, n_pages, causal,
             softmax_scale, n_splits, return_lse, out):
-    B, P, G = _check_cache_q8(k8, v8, k_scale, v_scale)
-    if q.ndim != 3 or q.shape[2] != HEAD_DIM or q.shape[1] % G or q.shape[1] > 16 * G \
-            or q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"q must be bf16 or fp16 [total_q, H, {HEAD_DIM}], H a multiple of the "
-                         f"cache's {G} heads and at most 16 times it")
-    total_q, H, _ = q.shape
-    if cache_seqlens.dtype != torch.int32 or cache_seqlens.shape != (B,) \
-            or cu_seqlens_q.dtype != torch.int32 or cu_seqlens_q.shape != (B + 1,):
+    B, P, G, cache_stride, scale_stride = _cache_dims(k8, v8, k_scale, v_scale)
+    code = _CODES.get(q.dtype)
+    if q.ndim != 3 or code is None:
+        _refuse_queries(G)
+    total_q, H, cols = q.shape
+    if cols != HEAD_DIM or H % G or not G <= H <= 16 * G:
+        _refuse_queries(G)
+    if cache_seqlens.dtype is not torch.int32 or cache_seqlens.shape != (B,) \
+            or cu_seqlens_q.dtype is not torch.int32 or cu_seqlens_q.shape != (B + 1,):
         raise ValueError("cache_seqlens must be int32 [batch] and cu_seqlens_q int32 [batch + 1]")
+    ids = None
     if topk_idx is not None:
-        if topk_idx.shape[:2] != (G, total_q) or not 1 <= topk_idx.shape[2] <= 256:
+        g, t, n_pages = topk_idx.shape
+        if g != G or t != total_q or not 1 <= n_pages <= 256:
             raise ValueError(f"topk_idx must be [{G}, {total_q}, k] with 1 <= k <= 256")
-        topk_idx = topk_idx.to(torch.int32).contiguous()
-        n_pages = topk_idx.shape[2]
     if out is not None:
         _hip.check_out(out, (total_q, H, HEAD_DIM), q.dtype, q.device)
-    dev = _hip.require_gpu(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q)
-    if q.stride()[1:] != (HEAD_DIM, 1) or q.stride(0) % 8 or q.data_ptr() % 16:
+        if out.data_ptr() % 16:
+            raise ValueError("out must be 16-byte aligned")
+    index = _hip.gpu_index(q, k8, v8, k_scale, v_scale, cache_seqlens, cu_seqlens_q, topk_idx)
+    if topk_idx is not None:
+        topk_idx = topk_idx.to(torch.int32).contiguous()
+        ids = topk_idx.data_ptr()
+    if not _rows16(q):
         q = q.clone(memory_format=torch.contiguous_format)
     if n_splits is None:
-        # Workgroups of four waves per (row, group): enough of them to cover the
-        # device when there are few rows, at least one page per wave.
-        n_splits = max(1, min(-(-n_pages // 4), -(-256 // max(1, total_q * G))))
+        # Workgroups of four waves per (row, group): enough of them to cover the device, at
+        # least one page a wave.  Rows without a plan differ in length, so several of them
+        # are cut finer, for the longest not to run alone.
+        most = _WORKGROUPS if topk_idx is not None or total_q == 1 else _RAGGED_WORKGROUPS
+        n_splits = min(-(-n_pages // 4), -(-most // max(1, total_q * G)))
     n_splits = max(1, min(int(n_splits), _MAX_SPLITS))
     if out is None:
-        out = torch.empty((total_q, H, HEAD_DIM), dtype=q.dtype, device=dev)
-    lse = torch.empty((H, total_q), dtype=torch.float32, device=dev) if return_lse else None
-    nbytes = _hip.lib().ls_attn_kvcache_q8_workspace_size(total_q, G, n_splits)
-    ws = _hip.workspace(nbytes, dev) if nbytes else None
-    _hip.launch(dev, "ls_attn_kvcache_q8", q.data_ptr(), q.stride(0),
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty((H, total_q), dtype=torch.float32, device=q.device) if return_lse else None
+    # The slices' partial sums, maxima and weights: ls_attn_kvcache_q8_workspace_size.
+    floats = total_q * H * n_splits * (HEAD_DIM + 2) if n_splits > 1 else 0
+    ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
+    _hip.launch(index, "ls_attn_kvcache_q8", q.data_ptr(), q.stride(0),
                 cu_seqlens_q.contiguous().data_ptr(), total_q, k8.data_ptr(), v8.data_ptr(),
-                k8.stride(0), k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0), P,
-                cache_seqlens.contiguous().data_ptr(), B, H, G, HEAD_DIM, _hip.dtype_code(q.dtype),
-                _hip.ptr(topk_idx), n_pages if topk_idx is not None else 0,
+                cache_stride, k_scale.data_ptr(), v_scale.data_ptr(), scale_stride, P,
+                cache_seqlens.contiguous().data_ptr(), B, H, G, HEAD_DIM, code, ids, n_pages,
                 HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale),
-                1 if causal else 0, n_splits, out.data_ptr(), _hip.ptr(lse), _hip.ptr(ws), nbytes)
+                1 if causal else 0, n_splits, out.data_ptr(), _hip.ptr(lse), _hip.ptr(ws), 4 * floats)
     return (out, lse) if return_lse else out
+
+
+def _refuse_queries(G: int):
+    raise ValueError(f"q must be bf16 or fp16 [total_q, H, {HEAD_DIM}], H a multiple of the cache's "
+                     f"{G} heads and at most 16 times it")

@@ -23,6 +23,8 @@ import torch
 
 from .. import _hip
 
+_CODES = {torch.bfloat16: _hip.LS_BF16, torch.float16: _hip.LS_F16}
+
 __all__ = ["quantize_mx4", "lay_out_mx4", "dequantize_mx4", "linear_mx4", "linear_mx4_silu_mul"]
 
 
@@ -36,8 +38,8 @@ def _shapes(out_features: int, in_features: int) -> tuple[tuple, tuple]:
 
 def _check_weight(codes, scales, out_features: int, in_features: int) -> None:
     cs, ss = _shapes(out_features, in_features)
-    if codes.shape != cs or scales.shape != ss or codes.dtype != torch.uint8 \
-            or scales.dtype != torch.uint8 or not codes.is_contiguous() \
+    if codes.shape != cs or scales.shape != ss or codes.dtype is not torch.uint8 \
+            or scales.dtype is not torch.uint8 or not codes.is_contiguous() \
             or not scales.is_contiguous():
         raise ValueError(f"a {out_features} x {in_features} weight needs contiguous uint8 codes "
                          f"{cs} and scales {ss} (got {tuple(codes.shape)} and "
@@ -55,12 +57,12 @@ def quantize_mx4(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     n, k = weight.shape
     cs, ss = _shapes(n, k)
     code = _hip.dtype_code(weight.dtype)
-    dev = _hip.require_gpu(weight)
+    index = _hip.gpu_index(weight)
     if not bool(torch.isfinite(weight).all()):
         raise ValueError("weight must be finite: E2M1 has no infinity and no NaN")
-    codes = torch.empty(cs, dtype=torch.uint8, device=dev)
-    scales = torch.empty(ss, dtype=torch.uint8, device=dev)
-    _hip.launch(dev, "ls_quantize_mx4", weight.data_ptr(), weight.stride(0), n, k, code,
+    codes = torch.empty(cs, dtype=torch.uint8, device=weight.device)
+    scales = torch.empty(ss, dtype=torch.uint8, device=weight.device)
+    _hip.launch(index, "ls_quantize_mx4", weight.data_ptr(), weight.stride(0), n, k, code,
                 codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
@@ -94,12 +96,12 @@ def dequantize_mx4(codes: torch.Tensor, scales: torch.Tensor, out_features: int,
     _check_weight(codes, scales, out_features, in_features)
     if dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("the values are given in bf16 or fp16")
-    dev = _hip.require_gpu(codes, scales)
+    index = _hip.gpu_index(codes, scales)
     if out is None:
-        out = torch.empty((out_features, in_features), dtype=dtype, device=dev)
+        out = torch.empty((out_features, in_features), dtype=dtype, device=codes.device)
     else:
-        _hip.check_out(out, (out_features, in_features), dtype, dev)
-    _hip.launch(dev, "ls_dequantize_mx4", codes.data_ptr(), scales.data_ptr(), out_features,
+        _hip.check_out(out, (out_features, in_features), dtype, codes.device)
+    _hip.launch(index, "ls_dequantize_mx4", codes.data_ptr(), scales.data_ptr(), out_features,
                 in_features, _hip.dtype_code(dtype), out.data_ptr(), in_features)
     return out
 
@@ -108,7 +110,8 @@ def linear_mx4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_f
                out: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T`` for ``x [rows, in_features]`` (bf16 or fp16): ``[rows, out_features]`` in
     ``x``'s dtype.  Made for the few rows of a decode step; every 64 rows read the weight
-    again."""
+    again.  A row's bits do not depend on the other rows, but may on whether there are more
+    than 16 (and then than 64) of them."""
     return _linear(x, codes, scales, out_features, 0, out)
 
 
@@ -122,21 +125,29 @@ def linear_mx4_silu_mul(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
 
 
 def _linear(x, codes, scales, out_features, silu, out):
-    if x.ndim != 2 or x.dtype not in (torch.bfloat16, torch.float16):
+    code = _CODES.get(x.dtype)
+    if x.ndim != 2 or code is None:
         raise ValueError("x must be bf16 or fp16 [rows, in_features]")
     rows, k = x.shape
     _check_weight(codes, scales, out_features, k)
     n = out_features // 2 if silu else out_features
-    dev = _hip.require_gpu(x, codes, scales)
+    index = _hip.gpu_index(x, codes, scales, out)
     if out is None:
-        out = torch.empty((rows, n), dtype=x.dtype, device=dev)
-    elif out.ndim != 2 or out.stride(1) != 1 or out.shape != (rows, n) or out.dtype != x.dtype \
-            or out.device != dev:
-        raise ValueError(f"out must be ({rows}, {n}) {x.dtype} on {dev} with unit column stride, "
-                         f"got {tuple(out.shape)} {out.dtype} on {out.device}")
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    _hip.launch(dev, "ls_linear_mx4", x.data_ptr(), x.stride(0), rows, k, codes.data_ptr(),
-                scales.data_ptr(), out_features, silu, _hip.dtype_code(x.dtype), out.data_ptr(),
-                out.stride(0))
+        out = torch.empty(rows, n, dtype=x.dtype, device=x.device)
+        out_stride = n
+    else:
+        if out.shape != (rows, n) or out.stride(1) != 1 or out.dtype is not x.dtype:
+            raise ValueError(f"out must be ({rows}, {n}) {x.dtype} with unit column stride, "
+                             f"got {tuple(out.shape)} {out.dtype}")
+        out_stride = out.stride(0)
+    x_stride = k
+    if x.data_ptr() % 16 or not x.is_contiguous():
+        if x.data_ptr() % 16 or x.stride(1) != 1 or x.stride(0) % 8:
+            x = x.clone(memory_format=torch.contiguous_format)
+        x_stride = x.stride(0)
+    nbytes = _hip.lib().ls_linear_mx4_workspace_size(rows, k, out_features, silu)
+    ws = _hip.workspace(nbytes, x.device) if nbytes else None
+    _hip.launch(index, "ls_linear_mx4", x.data_ptr(), x_stride, rows, k, codes.data_ptr(),
+                scales.data_ptr(), out_features, silu, code, out.data_ptr(), out_stride,
+                _hip.ptr(ws), nbytes)
     return out

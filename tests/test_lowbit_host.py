@@ -57,11 +57,11 @@ def test_append_refusals(change, match):
 def _bad_caches():
     k8, v8, ks, vs = new_kvcache_q8(2, 128, 2, device="cpu")
     return [
-        ((k8.view(torch.uint8), v8, ks, vs), "k8 must"),
-        ((k8[..., :64], v8, ks, vs), "k8 must"),
-        ((k8, k8, ks, vs), "v8 must"),
-        ((k8, v8, ks.int(), vs), "uint8"),
-        ((k8, v8, ks[:, :1], vs), "k_scale and v_scale"),
+        ((k8.view(torch.uint8), v8, ks, vs), "the cache must be"),
+        ((k8[..., :64], v8, ks, vs), "the cache must be"),
+        ((k8, k8, ks, vs), "the cache must be"),
+        ((k8, v8, ks.int(), vs), "the cache must be"),
+        ((k8, v8, ks[:, :1], vs), "the cache must be"),
         ((k8.transpose(1, 2), v8, ks, vs), "dense"),
         ((k8, v8, ks, vs.transpose(1, 2).contiguous().transpose(1, 2)), "dense"),
         ((torch.cat([k8, k8])[::2], v8, ks, vs), "batch strides"),
@@ -159,23 +159,23 @@ def test_c_entry_points_refuse_before_any_launch():
     assert append(total=0, k8=None) == _hip.LS_OK
     attend = lambda **k: L.ls_attn_kvcache_q8(*{**dict(  # noqa: E731
         q=16, qrs=4096, cu=4, total=1, k8=16, v8=16, cbs=16384, ks=1, vs=1, sbs=2, pages=1, lens=4, batch=1,
-        H=32, G=2, D=128, dt=B, ids=None, topk=0, scale=1.0, causal=0, splits=1, out=16, lse=None, ws=None,
+        H=32, G=2, D=128, dt=B, ids=None, n_pages=1, scale=1.0, causal=0, splits=1, out=16, lse=None, ws=None,
         wsb=0, stream=None), **k}.values())
     for change, rc, word in (
             (dict(H=33), _hip.LS_ERR_INVALID, b"sizes"), (dict(H=34), _hip.LS_ERR_UNSUPPORTED, b"16 query"),
             (dict(D=64), _hip.LS_ERR_UNSUPPORTED, b"head_dim"), (dict(dt=_hip.LS_F32), _hip.LS_ERR_UNSUPPORTED, b"bf16"),
             (dict(splits=0), _hip.LS_ERR_INVALID, b"n_splits"), (dict(splits=257), _hip.LS_ERR_INVALID, b"n_splits"),
-            (dict(ids=4, topk=0), _hip.LS_ERR_INVALID, b"topk"), (dict(ids=4, topk=257), _hip.LS_ERR_UNSUPPORTED, b"plan ids"),
-            (dict(splits=2), _hip.LS_ERR_WORKSPACE, b"workspace"), (dict(splits=2, ws=16, wsb=8), _hip.LS_ERR_WORKSPACE, b"workspace"),
+            (dict(n_pages=0), _hip.LS_ERR_INVALID, b"n_pages"), (dict(ids=4, n_pages=257), _hip.LS_ERR_UNSUPPORTED, b"plan ids"),
+            (dict(splits=2, n_pages=9), _hip.LS_ERR_WORKSPACE, b"workspace"), (dict(splits=2, n_pages=9, ws=16, wsb=8), _hip.LS_ERR_WORKSPACE, b"workspace"),
             (dict(q=None), _hip.LS_ERR_INVALID, b"null"), (dict(q=18), _hip.LS_ERR_UNSUPPORTED, b"aligned"),
             (dict(qrs=4097), _hip.LS_ERR_UNSUPPORTED, b"aligned"), (dict(pages=1 << 25), _hip.LS_ERR_UNSUPPORTED, b"pages"),
             (dict(total=1 << 31), _hip.LS_ERR_UNSUPPORTED, b"rows"), (dict(batch=0), _hip.LS_ERR_INVALID, b"sizes")):
         assert attend(**change) == rc and word in L.ls_last_error(), change
     assert attend(total=0, q=None) == _hip.LS_OK
     assert L.ls_attn_kvcache_q8_workspace_size(4, 2, 1) == 0
-    assert L.ls_attn_kvcache_q8_workspace_size(4, 2, 3) >= 4 * 4 * 2 * 3 * (16 * 128 + 32)
+    assert L.ls_attn_kvcache_q8_workspace_size(4, 32, 3) == 4 * 4 * 32 * 3 * 130
     linear = lambda **k: L.ls_linear_mx4(*{**dict(  # noqa: E731
-        x=16, xrs=64, rows=1, K=64, codes=16, scales=4, N=32, silu=0, dt=B, out=2, ors=32, stream=None), **k}.values())
+        x=16, xrs=64, rows=1, K=64, codes=16, scales=4, N=32, silu=0, dt=B, out=2, ors=32, ws=None, wsb=0, stream=None), **k}.values())
     for change, rc, word in (
             (dict(K=63), _hip.LS_ERR_INVALID, b"multiple of 8"), (dict(N=0), _hip.LS_ERR_INVALID, b"out_features"),
             (dict(rows=-1), _hip.LS_ERR_INVALID, b"rows"), (dict(silu=1, N=48), _hip.LS_ERR_UNSUPPORTED, b"32"),
