@@ -645,9 +645,9 @@ int ls_dense_attn_kvcache(const void* q, int64_t q_row_stride, const int32_t* cu
  * at least the old code where it holds older rows (from before cache_seqlens[b]),
  * which are then brought under the new one; rows after the new ones are left as
  * they are.  Infinities and NaN are stored as NaN.  With kc_cache [batch]
- * [kc_rows][G][128] (the dtype of k_new), the first max_new_windows windows that
- * the new tokens complete are written: window w is the mean of the stored keys
- * [16 w, 16 w + 32), float32 sums, one rounding.  Rows past `pages` pages and
+ * [kc_rows][G][128] (the dtype of k_new), the windows that the new tokens complete
+ * are written: window w is the mean of the stored keys [16 w, 16 w + 32), float32
+ * sums, one rounding.  Rows past `pages` pages and
  * windows past kc_rows are not written.  cache_seqlens is not advanced.
  */
 int ls_kvcache_append_q8(void* k8, void* v8, int64_t cache_batch_stride, uint8_t* k_scale,
@@ -656,7 +656,7 @@ int ls_kvcache_append_q8(void* k8, void* v8, int64_t cache_batch_stride, uint8_t
                          int64_t new_row_stride, const int32_t* cu_seqlens_new, int64_t total_new,
                          int32_t batch, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
                          void* kc_cache, int64_t kc_batch_stride, int64_t kc_row_stride,
-                         int64_t kc_rows, int64_t max_new_windows, void* stream);
+                         int64_t kc_rows, void* stream);
 
 /*
  * Attention of packed decode rows over the 8-bit cache: ls_sparse_attn_kvcache

@@ -112,7 +112,7 @@ SIGNATURES = {
                _i32, _i32, _p, _p, _p, _sz, _p]),
     "ls_kvcache_append_q8": (
         _i32, [_p, _p, _i64, _p, _p, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _i32, _i32, _i32,
-               _i32, _p, _i64, _i64, _i64, _i64, _p]),
+               _i32, _p, _i64, _i64, _i64, _p]),
     "ls_attn_kvcache_q8_workspace_size": (_sz, [_i64, _i32, _i32]),
     "ls_attn_kvcache_q8": (
         _i32, [_p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _p, _i32, _i32, _i32, _i32,

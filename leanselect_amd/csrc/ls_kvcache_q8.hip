@@ -32,10 +32,6 @@ constexpr int kPageBytes = kPage * kDim;
 
 typedef float Q8F2 __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ int64_t q8_windows(int64_t len, int ks, int stride) {
-  return len >= ks ? (len - ks) / stride + 1 : 0;
-}
-
 // Largest finite magnitude of eight 16-bit values as 16 bits (their order is that of the
 // values); an infinity or NaN counts as zero.
 template <int DT>
@@ -106,14 +102,40 @@ __device__ __forceinline__ int q8_find(int64_t& unit, int batch, Count count) {
 // A page of a sequence belongs to one workgroup, so nothing is shared between them.
 // K: thread (row, c) takes the 8-channel pieces c, c + 4, c + 8, c + 12 of its row.
 // V: thread (quad, octet) takes 8 channels of the four tokens that share a 4-byte word.
+//
+// Compressed keys: window w is the mean of the 32 stored keys from token 16 w, so it is two
+// of the 16-row halves of pages.  The halves of the page are summed from the bytes in LDS,
+// with the last half of the page before and the first of the page after.  A window across
+// two pages belongs to the first one if the call writes to it: the second one's rows are
+// then all new, and their code and bytes are formed here once more from the new keys (a
+// page's older rows may be changing under another workgroup's hands, its new ones not).
+// Otherwise the first page is at rest and is read as it is.  So the windows need no second
+// launch: 3 to 5 us a call, against reading a prompt's keys twice.
 // ---------------------------------------------------------------------------
+// Eight 16-bit values as eight e4m3 bytes under a scale.
+template <int DT>
+__device__ __forceinline__ uint2 q8_pack8(ls_u32x4 x, float inv) {
+  float f[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    f[2 * e] = LsElem<DT>::to_f((uint16_t)(x[e] & 0xffffu)) * inv;
+    f[2 * e + 1] = LsElem<DT>::to_f((uint16_t)(x[e] >> 16)) * inv;
+  }
+  return make_uint2(q8_pack(f[0], f[1], f[2], f[3]), q8_pack(f[4], f[5], f[6], f[7]));
+}
+
 template <int DT>
 __global__ __launch_bounds__(256) void ls_q8_append_kernel(
     uint8_t* __restrict__ k8, uint8_t* __restrict__ v8, int64_t cbs, uint8_t* __restrict__ ks,
     uint8_t* __restrict__ vs, int64_t sbs, int64_t pages, const int32_t* __restrict__ cache_seqlens,
     const uint16_t* __restrict__ kn, const uint16_t* __restrict__ vn, int64_t nrs,
-    const int32_t* __restrict__ cu_new, int64_t total_new, int batch, int G) {
-  __shared__ uint32_t s_top[2][4];
+    const int32_t* __restrict__ cu_new, int64_t total_new, int batch, int G,
+    uint16_t* __restrict__ kcc, int64_t kbs, int64_t krs, int64_t kc_rows) {
+  __shared__ uint32_t s_top[3][4];
+  // Keys by half of a page: the last one before, the page's four, the first one after.
+  constexpr int kPitch = kDim + 4;
+  __shared__ uint32_t s_k[96 * kPitch / 4];
+  __shared__ float s_half[6][kDim];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int g = blockIdx.y;
   int64_t unit = blockIdx.x;
@@ -126,45 +148,67 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(
   const int64_t n1 = min((int64_t)cu_new[b + 1], total_new);
   const int64_t page = len / kPage + unit;
   if (page >= pages || n0 < 0) return;
-  const int64_t base = page * kPage;
-  const int r0 = (int)max<int64_t>(0, len - base);              // first new row of the page
-  const int r1 = (int)min<int64_t>(kPage, len + (n1 - n0) - base);
+  const int64_t base = page * kPage, end = len + (n1 - n0);
+  const int r0 = (int)max<int64_t>(0, len - base);  // the page's new rows: r0 <= row < r1
+  const int r1 = (int)min<int64_t>(kPage, end - base);
   const int64_t at = (int64_t)b * cbs + (page * G + g) * kPageBytes;
   const int64_t sat = (int64_t)b * sbs + page * G + g;
   const int64_t first = (n0 + base - len) * nrs + (int64_t)g * kDim;  // the page's row 0, if it were new
 
+  // The window of halves i and i + 1 (0: the page before's last and the page's first).
+  const int after = page + 1 < pages ? (int)max<int64_t>(0, min<int64_t>(kPage, end - base - kPage)) : 0;
+  auto complete = [&](int i) {
+    if (!kcc) return false;
+    if (i == 4) return after >= 16;
+    return r0 <= 16 * i + 15 && 16 * i + 15 < r1 && (i > 0 || (unit == 0 && page > 0));
+  };
+  const bool windows = complete(0) || complete(1) || complete(2) || complete(3) || complete(4);
+
   const int krow = tid >> 2, kc = 8 * (tid & 3);
   const bool knew = krow >= r0 && krow < r1;
-  const int quad = tid >> 4, oct = tid & 15;                    // quad = 4 q + t
+  const int quad = tid >> 4, oct = tid & 15;  // quad = 4 q + t
   const int tok = 16 * (quad & 3) + 4 * (quad >> 2);
-  ls_u32x4 kx[4], vx[4];
-  uint32_t ktop = 0, vtop = 0;
+  ls_u32x4 kx[4], vx[4], nx[4];
+  uint2 ko[4];
+  uint32_t ktop = 0, vtop = 0, ntop = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     kx[j] = knew ? ls_load16(kn + first + krow * nrs + 32 * j + kc) : ls_u32x4{0u, 0u, 0u, 0u};
     const bool vnew = tok + j >= r0 && tok + j < r1;
     vx[j] = vnew ? ls_load16(vn + first + (tok + j) * nrs + 8 * oct) : ls_u32x4{0u, 0u, 0u, 0u};
   }
+  if (complete(4)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      nx[j] = krow < after ? ls_load16(kn + first + (kPage + krow) * nrs + 32 * j + kc)
+                           : ls_u32x4{0u, 0u, 0u, 0u};
+  }
+  uint8_t* kp = k8 + at + krow * kDim + kc;
   uint32_t kold = 1, vold = 1;
   if (r0 > 0) {
     kold = ks[sat];
     vold = vs[sat];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ko[j] = krow < r0 ? *reinterpret_cast<const uint2*>(kp + 32 * j) : make_uint2(0, 0);
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     ktop = q8_abs_max<DT>(kx[j], ktop);
     vtop = q8_abs_max<DT>(vx[j], vtop);
+    if (complete(4)) ntop = q8_abs_max<DT>(nx[j], ntop);
   }
   ktop = ls_wave_max_u32(ktop);
   vtop = ls_wave_max_u32(vtop);
+  ntop = ls_wave_max_u32(ntop);
   if (lane == 0) {
     s_top[0][w] = ktop;
     s_top[1][w] = vtop;
+    s_top[2][w] = ntop;
   }
   __syncthreads();
-  ktop = max(max(s_top[0][0], s_top[0][1]), max(s_top[0][2], s_top[0][3]));
-  vtop = max(max(s_top[1][0], s_top[1][1]), max(s_top[1][2], s_top[1][3]));
-  const uint32_t kcode = max(q8_code<DT>(ktop), kold), vcode = max(q8_code<DT>(vtop), vold);
+  auto all_waves = [&](int i) { return max(max(s_top[i][0], s_top[i][1]), max(s_top[i][2], s_top[i][3])); };
+  const uint32_t kcode = max(q8_code<DT>(all_waves(0)), kold);
+  const uint32_t vcode = max(q8_code<DT>(all_waves(1)), vold);
   if (tid == 0) {
     ks[sat] = (uint8_t)kcode;
     vs[sat] = (uint8_t)vcode;
@@ -173,25 +217,23 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(
   const float kdown = q8_pow(max(127 + (int)kold - (int)kcode, 0));
   const float vdown = q8_pow(max(127 + (int)vold - (int)vcode, 0));
 
-  uint8_t* kp = k8 + at + krow * kDim + kc;
-  if (knew) {
+  auto keep = [&](int row, int j, uint2 v) {  // a row's bytes into LDS
+    uint32_t* p = s_k + (row * kPitch + 32 * j + kc) / 4;
+    p[0] = v.x;
+    p[1] = v.y;
+  };
+  if (krow < r1) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float f[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        f[2 * e] = LsElem<DT>::to_f((uint16_t)(kx[j][e] & 0xffffu)) * kinv;
-        f[2 * e + 1] = LsElem<DT>::to_f((uint16_t)(kx[j][e] >> 16)) * kinv;
+      uint2 v;
+      if (knew) {
+        v = q8_pack8<DT>(kx[j], kinv);
+      } else {
+        v = ko[j];
+        if (kcode > kold) v = make_uint2(q8_rescale(v.x, kdown), q8_rescale(v.y, kdown));
       }
-      *reinterpret_cast<uint2*>(kp + 32 * j) =
-          make_uint2(q8_pack(f[0], f[1], f[2], f[3]), q8_pack(f[4], f[5], f[6], f[7]));
-    }
-  } else if (krow < r0 && kcode > kold) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint2* p = reinterpret_cast<uint2*>(kp + 32 * j);
-      const uint2 v = *p;
-      *p = make_uint2(q8_rescale(v.x, kdown), q8_rescale(v.y, kdown));
+      if (knew || kcode > kold) *reinterpret_cast<uint2*>(kp + 32 * j) = v;
+      if (windows) keep(16 + krow, j, v);
     }
   }
 
@@ -221,63 +263,49 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(
       *p = v;
     }
   }
-}
 
-// Compressed keys: a wave per (window, KV head), after the rows are stored.  Window w is
-// the mean of the 32 stored keys from token 16 w, as the cache holds them; lane (c, part)
-// sums 8 channels of 8 rows in float32, then the parts are added in order.
-template <int DT>
-__global__ __launch_bounds__(256) void ls_q8_windows_kernel(
-    const uint8_t* __restrict__ k8, int64_t cbs, const uint8_t* __restrict__ ks, int64_t sbs,
-    int64_t pages, const int32_t* __restrict__ cache_seqlens, const int32_t* __restrict__ cu_new,
-    int batch, int G, int64_t max_windows, uint16_t* __restrict__ kcc, int64_t kbs, int64_t krs,
-    int64_t kc_rows) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int g = blockIdx.y;
-  int64_t unit = (int64_t)blockIdx.x * 4 + (tid >> 6);
-  if (unit >= max_windows) return;
-  const int b = q8_find(unit, batch, [&](int i) -> int64_t {
-    const int64_t len = cache_seqlens[i], n = cu_new[i + 1] - cu_new[i];
-    return n > 0 ? q8_windows(len + n, 32, 16) - q8_windows(len, 32, 16) : 0;
-  });
-  if (b < 0) return;
-  const int64_t win = q8_windows(cache_seqlens[b], 32, 16) + unit;
-  const int c = lane & 15, part = lane >> 4;
-  const int64_t tok = 16 * win + 8 * part;
-  const int64_t page = tok / kPage;  // eight rows from a multiple of eight: one page
-  if (page >= pages || win >= kc_rows) return;
-  const uint8_t* p = k8 + (int64_t)b * cbs + (page * G + g) * kPageBytes + (tok & 63) * kDim + 8 * c;
-  const float f = q8_pow(ks[(int64_t)b * sbs + page * G + g]);
-  float s[8];
+  if (!windows) return;
+  const uint32_t ncode = q8_code<DT>(all_waves(2));
+  uint32_t pcode = 1;
+  if (complete(0)) {
+    pcode = ks[sat - G];
+    if (krow >= 48) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) s[e] = 0.f;
-#pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p + r * kDim);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int x = (int)(h ? v.y : v.x);
-      const Q8F2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(x, false);
-      const Q8F2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(x, true);
-      s[4 * h] += lo[0];
-      s[4 * h + 1] += lo[1];
-      s[4 * h + 2] += hi[0];
-      s[4 * h + 3] += hi[1];
+      for (int j = 0; j < 4; ++j)
+        keep(krow - 48, j, *reinterpret_cast<const uint2*>(kp - (int64_t)G * kPageBytes + 32 * j));
     }
   }
+  if (complete(4) && krow < 16) {
+    const float ninv = q8_pow(254 - (int)ncode);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    s[e] *= f;  // the four parts may lie in two pages
-    s[e] += ls_shfl_xor(s[e], 16);
-    s[e] += ls_shfl_xor(s[e], 32);
-    s[e] *= 1.f / 32.f;
+    for (int j = 0; j < 4; ++j) keep(80 + krow, j, q8_pack8<DT>(nx[j], ninv));
   }
-  if (part == 0) {
-    ls_u32x4 o;
+  __syncthreads();
+  // Halves in float32 in token order, two channels a thread (a half that no window needs
+  // may be anything).
+  for (int u = tid; u < 6 * 64; u += 256) {
+    const int half = u >> 6, c = u & 63;
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(s_k) + half * 16 * (kPitch / 2) + c;
+    float a0 = 0.f, a1 = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      o[e] = ls_pack2(LsElem<DT>::from_f(s[2 * e]), LsElem<DT>::from_f(s[2 * e + 1]));
-    *reinterpret_cast<ls_u32x4*>(kcc + (int64_t)b * kbs + win * krs + (int64_t)g * kDim + 8 * c) = o;
+    for (int r = 0; r < 16; ++r) {
+      const Q8F2 x = __builtin_amdgcn_cvt_pk_f32_fp8((int)p[r * (kPitch / 2)], false);
+      a0 += x[0];
+      a1 += x[1];
+    }
+    const float f = q8_pow((int)(half == 0 ? pcode : half == 5 ? ncode : kcode));
+    s_half[half][2 * c] = a0 * f;
+    s_half[half][2 * c + 1] = a1 * f;
+  }
+  __syncthreads();
+  for (int u = tid; u < 5 * 64; u += 256) {
+    const int i = u >> 6, c = 2 * (u & 63);
+    const int64_t win = 4 * page - 1 + i;
+    if (!complete(i) || win >= kc_rows) continue;
+    const float a0 = (s_half[i][c] + s_half[i + 1][c]) * (1.f / 32.f);
+    const float a1 = (s_half[i][c + 1] + s_half[i + 1][c + 1]) * (1.f / 32.f);
+    *reinterpret_cast<uint32_t*>(kcc + (int64_t)b * kbs + win * krs + (int64_t)g * kDim + c) =
+        ls_pack2(LsElem<DT>::from_f(a0), LsElem<DT>::from_f(a1));
   }
 }
 
@@ -661,8 +689,7 @@ extern "C" int ls_kvcache_append_q8(void* k8, void* v8, int64_t cache_batch_stri
                                     const int32_t* cu_seqlens_new, int64_t total_new,
                                     int32_t batch, int32_t num_kv_heads, int32_t head_dim,
                                     int32_t dtype, void* kc_cache, int64_t kc_batch_stride,
-                                    int64_t kc_row_stride, int64_t kc_rows,
-                                    int64_t max_new_windows, void* stream) {
+                                    int64_t kc_row_stride, int64_t kc_rows, void* stream) {
   const char* who = "ls_kvcache_append_q8";
   LS_REQUIRE(batch >= 0 && total_new >= 0 && num_kv_heads > 0 && pages >= 0 && kc_rows >= 0,
              LS_ERR_INVALID, "%s: bad sizes", who);
@@ -681,33 +708,18 @@ extern "C" int ls_kvcache_append_q8(void* k8, void* v8, int64_t cache_batch_stri
   const int64_t nb = std::min<int64_t>(batch, total_new);
   const int64_t units = std::min(total_new, (total_new + 126 * nb) / 64);
   LS_REQUIRE(units <= 0x7fffffffLL, LS_ERR_UNSUPPORTED, "%s: too many new tokens", who);
-  const bool windows = kc_cache && max_new_windows > 0;
-  if (windows) {
-    LS_REQUIRE(ls_aligned16(kc_cache) && kc_row_stride % 8 == 0 && kc_batch_stride % 8 == 0,
-               LS_ERR_UNSUPPORTED, "%s: compressed cache must be 16-byte aligned", who);
-    LS_REQUIRE(max_new_windows <= 0x7fffffffLL, LS_ERR_UNSUPPORTED, "%s: too many windows", who);
-  }
-  hipStream_t s = (hipStream_t)stream;
+  LS_REQUIRE(!kc_cache || (ls_aligned16(kc_cache) && kc_row_stride % 8 == 0 && kc_batch_stride % 8 == 0),
+             LS_ERR_UNSUPPORTED, "%s: compressed cache must be 16-byte aligned", who);
   auto append = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)units, num_kv_heads), dim3(256), 0, s, (uint8_t*)k8,
-                       (uint8_t*)v8, cache_batch_stride, k_scale, v_scale, scale_batch_stride,
-                       pages, cache_seqlens, (const uint16_t*)k_new, (const uint16_t*)v_new,
-                       new_row_stride, cu_seqlens_new, total_new, batch, num_kv_heads);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)units, num_kv_heads), dim3(256), 0,
+                       (hipStream_t)stream, (uint8_t*)k8, (uint8_t*)v8, cache_batch_stride, k_scale,
+                       v_scale, scale_batch_stride, pages, cache_seqlens, (const uint16_t*)k_new,
+                       (const uint16_t*)v_new, new_row_stride, cu_seqlens_new, total_new, batch,
+                       num_kv_heads, (uint16_t*)kc_cache, kc_batch_stride, kc_row_stride, kc_rows);
     return ls_check_launch("ls_q8_append_kernel");
   };
-  int rc = dtype == LS_BF16 ? append(ls_q8_append_kernel<LS_BF16>)
-                            : append(ls_q8_append_kernel<LS_F16>);
-  if (rc || !windows) return rc;
-  auto pool = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((max_new_windows + 3) / 4), num_kv_heads),
-                       dim3(256), 0, s, (const uint8_t*)k8, cache_batch_stride, k_scale,
-                       scale_batch_stride, pages, cache_seqlens, cu_seqlens_new, batch,
-                       num_kv_heads, max_new_windows, (uint16_t*)kc_cache, kc_batch_stride,
-                       kc_row_stride, kc_rows);
-    return ls_check_launch("ls_q8_windows_kernel");
-  };
-  return dtype == LS_BF16 ? pool(ls_q8_windows_kernel<LS_BF16>)
-                          : pool(ls_q8_windows_kernel<LS_F16>);
+  return dtype == LS_BF16 ? append(ls_q8_append_kernel<LS_BF16>)
+                          : append(ls_q8_append_kernel<LS_F16>);
 }
 
 extern "C" size_t ls_attn_kvcache_q8_workspace_size(int64_t total_q, int32_t num_heads,

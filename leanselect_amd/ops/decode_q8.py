@@ -117,7 +117,7 @@ def kvcache_append_q8(k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
     if min(lens) < 0 or max(after) > P * PAGE or any(map(gt, lens, after)):
         raise ValueError(f"sequences of {lens} tokens cannot become {after} in a cache with a "
                          f"capacity of {P * PAGE}")
-    windows, kc = 0, (None, 0, 0, 0)
+    kc = (None, 0, 0, 0)
     if kc_cache is not None:
         if kernel_size != 32 or kernel_stride != 16:
             raise ValueError("the 8-bit cache forms windows of 32 keys at stride 16")
@@ -128,8 +128,6 @@ def kvcache_append_q8(k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
         kc = (kc_cache.data_ptr(), kc_cache.stride(0), kc_cache.stride(1), kc_cache.shape[1])
         if n_windows(max(after)) > kc[3]:
             raise ValueError(f"{n_windows(max(after))} compressed windows exceed kc_capacity {kc[3]}")
-        # n_windows(n) = max(1, n // 16) - 1.
-        windows = sum([n >> 4 or 1 for n in after]) - sum([n >> 4 or 1 for n in lens])
     index = _hip.gpu_index(k8, v8, k_scale, v_scale, cache_seqlens, k_new, v_new, cu_seqlens_new,
                            kc_cache)
     # One row stride serves both: dense 16-byte aligned rows with equal strides, else copies.
@@ -140,7 +138,7 @@ def kvcache_append_q8(k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
                 k_scale.data_ptr(), v_scale.data_ptr(), scale_stride, P,
                 cache_seqlens.contiguous().data_ptr(), k_new.data_ptr(), v_new.data_ptr(),
                 k_new.stride(0), cu_seqlens_new.contiguous().data_ptr(), total, B, G, HEAD_DIM, code,
-                *kc, windows)
+                *kc)
 
 
 def sparse_attention_kvcache_q8(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor,
@@ -196,7 +194,8 @@ def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, 
             raise ValueError("out must be 16-byte aligned")
     index = _hip.gpu_index(q, k8, v8, k_scale, v_scale, cache_seqlens, cu_seqlens_q, topk_idx)
     if topk_idx is not None:
-        topk_idx = topk_idx.to(torch.int32).contiguous()
+        if topk_idx.dtype is not torch.int32 or not topk_idx.is_contiguous():
+            topk_idx = topk_idx.to(torch.int32).contiguous()
         ids = topk_idx.data_ptr()
     if not _rows16(q):
         q = q.clone(memory_format=torch.contiguous_format)

@@ -149,12 +149,12 @@ def test_c_entry_points_refuse_before_any_launch():
     B = _hip.LS_BF16
     append = lambda **k: L.ls_kvcache_append_q8(*{**dict(  # noqa: E731
         k8=16, v8=16, cbs=16384, ks=1, vs=1, sbs=2, pages=1, lens=4, kn=16, vn=16, nrs=256, cu=4,
-        total=1, batch=1, G=2, D=128, dt=B, kc=None, kbs=0, krs=0, kcr=0, win=0, stream=None), **k}.values())
+        total=1, batch=1, G=2, D=128, dt=B, kc=None, kbs=0, krs=0, kcr=0, stream=None), **k}.values())
     for change, rc, word in (
             (dict(D=64), _hip.LS_ERR_UNSUPPORTED, b"head_dim"), (dict(dt=_hip.LS_F32), _hip.LS_ERR_UNSUPPORTED, b"bf16"),
             (dict(total=-1), _hip.LS_ERR_INVALID, b"sizes"), (dict(nrs=257), _hip.LS_ERR_UNSUPPORTED, b"aligned"),
             (dict(k8=None), _hip.LS_ERR_INVALID, b"null"), (dict(kn=18), _hip.LS_ERR_UNSUPPORTED, b"aligned"),
-            (dict(kc=18, win=1), _hip.LS_ERR_UNSUPPORTED, b"compressed"), (dict(G=70000), _hip.LS_ERR_INVALID, b"heads")):
+            (dict(kc=18), _hip.LS_ERR_UNSUPPORTED, b"compressed"), (dict(G=70000), _hip.LS_ERR_INVALID, b"heads")):
         assert append(**change) == rc and word in L.ls_last_error(), change
     assert append(total=0, k8=None) == _hip.LS_OK
     attend = lambda **k: L.ls_attn_kvcache_q8(*{**dict(  # noqa: E731
