@@ -74,23 +74,23 @@ __device__ __forceinline__ uint32_t q8_rescale(uint32_t v, float f) {
 // a wave scans 64 sequences at a time.  Every lane gets the sequence and the unit's number
 // in it; -1 past the last unit.
 template <class Count>
-__device__ __forceinline__ int q8_find(int64_t& unit, int batch, Count count) {
+__device__ __forceinline__ int q8_find(int& unit, int batch, Count count) {
   const int lane = ls_lane();
   for (int s0 = 0; s0 < batch; s0 += 64) {
-    const int64_t mine = s0 + lane < batch ? count(s0 + lane) : 0;
-    int64_t upto = mine;
+    const int mine = s0 + lane < batch ? count(s0 + lane) : 0;
+    int upto = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int64_t y = __shfl_up(upto, d, 64);
+      const int y = __shfl_up(upto, d, 64);
       if (lane >= d) upto += y;
     }
     const uint64_t past = __ballot(unit < upto);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
-      unit -= __shfl(upto - mine, at, 64);
+      unit -= __builtin_amdgcn_readlane(upto - mine, at);
       return s0 + at;
     }
-    unit -= __shfl(upto, 63, 64);
+    unit -= __builtin_amdgcn_readlane(upto, 63);
   }
   return -1;
 }
@@ -135,13 +135,15 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(
   // Keys by half of a page: the last one before, the page's four, the first one after.
   constexpr int kPitch = kDim + 4;
   __shared__ uint32_t s_k[96 * kPitch / 4];
-  __shared__ float s_half[6][kDim];
+  __shared__ ls_f32x4 s_half[6][kDim / 4];
+  constexpr int kVPitch = kPage + 4;
+  __shared__ uint32_t s_v[kDim * kVPitch / 4];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int g = blockIdx.y;
-  int64_t unit = blockIdx.x;
-  const int b = q8_find(unit, batch, [&](int i) -> int64_t {
+  int unit = blockIdx.x;
+  const int b = q8_find(unit, batch, [&](int i) {
     const int64_t len = cache_seqlens[i], n = cu_new[i + 1] - cu_new[i];
-    return n > 0 && len >= 0 ? (len + n + kPage - 1) / kPage - len / kPage : 0;
+    return n > 0 && len >= 0 ? (int)((len + n + kPage - 1) / kPage - len / kPage) : 0;
   });
   if (b < 0) return;
   const int64_t len = cache_seqlens[b], n0 = cu_new[b];
@@ -191,6 +193,19 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(
 #pragma unroll
     for (int j = 0; j < 4; ++j) ko[j] = krow < r0 ? *reinterpret_cast<const uint2*>(kp + 32 * j) : make_uint2(0, 0);
   }
+  // Bytes of a V word that are new, and those that are older; the words as they are, where
+  // not all of a word is new.
+  uint32_t is_new = 0, is_old = 0, vo[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (tok + j >= r0 && tok + j < r1) is_new |= 0xffu << (8 * j);
+    if (tok + j < r0) is_old |= 0xffu << (8 * j);
+  }
+  uint8_t* vp = v8 + at + (8 * oct) * kPage + 4 * quad;
+  if ((is_new | is_old) != 0 && is_new != 0xffffffffu) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) vo[e] = *reinterpret_cast<const uint32_t*>(vp + e * kPage);
+  }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     ktop = q8_abs_max<DT>(kx[j], ktop);
@@ -237,30 +252,33 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(
     }
   }
 
-  // Bytes of the word that are new, and those that are older.
-  uint32_t is_new = 0, is_old = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (tok + j >= r0 && tok + j < r1) is_new |= 0xffu << (8 * j);
-    if (tok + j < r0) is_old |= 0xffu << (8 * j);
-  }
   const bool lower = vcode > vold && is_old != 0;
+  const bool whole = r0 == 0 && r1 == kPage;
   if (is_new != 0 || lower) {
-    uint8_t* vp = v8 + at + (8 * oct) * kPage + 4 * quad;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float f[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         f[j] = LsElem<DT>::to_f((uint16_t)(vx[j][e >> 1] >> (16 * (e & 1)))) * vinv;
-      uint32_t* p = reinterpret_cast<uint32_t*>(vp + e * kPage);
       uint32_t v = q8_pack(f[0], f[1], f[2], f[3]);
       if (is_new != 0xffffffffu) {
-        const uint32_t o = *p;
-        const uint32_t l = lower ? q8_rescale(o, vdown) : o;
-        v = (v & is_new) | (l & is_old) | (o & ~(is_new | is_old));
+        const uint32_t l = lower ? q8_rescale(vo[e], vdown) : vo[e];
+        v = (v & is_new) | (l & is_old) | (vo[e] & ~(is_new | is_old));
       }
-      *p = v;
+      if (whole)
+        s_v[(8 * oct + e) * (kVPitch / 4) + quad] = v;
+      else
+        *reinterpret_cast<uint32_t*>(vp + e * kPage) = v;
+    }
+  }
+  if (whole) {  // through LDS, so that a wave writes whole lines
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int u = 256 * i + tid, c = u >> 2;
+      const uint32_t* p = s_v + c * (kVPitch / 4) + 4 * (u & 3);
+      *reinterpret_cast<ls_u32x4*>(v8 + at + 16 * u) = ls_u32x4{p[0], p[1], p[2], p[3]};
     }
   }
 
@@ -281,36 +299,34 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(
     for (int j = 0; j < 4; ++j) keep(80 + krow, j, q8_pack8<DT>(nx[j], ninv));
   }
   __syncthreads();
-  // Halves in float32 in token order, two channels a thread (a half that no window needs
+  // Halves in float32 in token order, four channels a thread (a half that no window needs
   // may be anything).
-  for (int u = tid; u < 6 * 64; u += 256) {
-    const int half = u >> 6, c = u & 63;
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(s_k) + half * 16 * (kPitch / 2) + c;
-    float a0 = 0.f, a1 = 0.f;
+  if (tid < 6 * 32) {
+    const int half = tid >> 5, c = tid & 31;
+    const uint32_t* p = s_k + half * 16 * (kPitch / 4) + c;
+    ls_f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const Q8F2 x = __builtin_amdgcn_cvt_pk_f32_fp8((int)p[r * (kPitch / 2)], false);
-      a0 += x[0];
-      a1 += x[1];
+      const uint32_t x = p[r * (kPitch / 4)];
+      const Q8F2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, false);
+      const Q8F2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, true);
+      a += ls_f32x4{lo[0], lo[1], hi[0], hi[1]};
     }
-    const float f = q8_pow((int)(half == 0 ? pcode : half == 5 ? ncode : kcode));
-    s_half[half][2 * c] = a0 * f;
-    s_half[half][2 * c + 1] = a1 * f;
+    s_half[half][c] = a * q8_pow((int)(half == 0 ? pcode : half == 5 ? ncode : kcode));
   }
   __syncthreads();
-  for (int u = tid; u < 5 * 64; u += 256) {
-    const int i = u >> 6, c = 2 * (u & 63);
-    const int64_t win = 4 * page - 1 + i;
-    if (!complete(i) || win >= kc_rows) continue;
-    const float a0 = (s_half[i][c] + s_half[i + 1][c]) * (1.f / 32.f);
-    const float a1 = (s_half[i][c + 1] + s_half[i + 1][c + 1]) * (1.f / 32.f);
-    *reinterpret_cast<uint32_t*>(kcc + (int64_t)b * kbs + win * krs + (int64_t)g * kDim + c) =
-        ls_pack2(LsElem<DT>::from_f(a0), LsElem<DT>::from_f(a1));
+  const int i = tid >> 5, c = tid & 31;
+  const int64_t win = 4 * page - 1 + i;
+  if (i < 5 && complete(i) && win < kc_rows) {
+    const ls_f32x4 a = (s_half[i][c] + s_half[i + 1][c]) * (1.f / 32.f);
+    *reinterpret_cast<uint2*>(kcc + (int64_t)b * kbs + win * krs + (int64_t)g * kDim + 4 * c) =
+        make_uint2(ls_pack2(LsElem<DT>::from_f(a[0]), LsElem<DT>::from_f(a[1])),
+                   ls_pack2(LsElem<DT>::from_f(a[2]), LsElem<DT>::from_f(a[3])));
   }
 }
 
 // ---------------------------------------------------------------------------
-// Attention of decode rows.  Workgroup (slice s, row t, KV head g): four waves, each a
+// Attention of decode rows.  Workgroup (slice s, row t, KV head g): NW waves, each a
 // share of the row's pages with a running maximum and sum, joined through LDS; with
 // several slices, partial results go to the workspace and a second kernel joins them.
 // Row i of sequence b sees keys j < len_b, or j <= len_b - len_q(b) + i (causal).
@@ -324,6 +340,7 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(
 // its V as soon as this page's sum is, into the same registers.
 // ---------------------------------------------------------------------------
 #define LS_Q8_MAX_SPLITS 256
+constexpr int kSplitWaves = 4, kWholeWaves = 8;  // of a workgroup: one of several slices, or the row
 #define LS_Q8_PITCH 132             // floats per head of a wave's O in LDS
 #define LS_Q8_ID_REGS 4             // plan ids held in registers: topk <= 256
 
@@ -333,7 +350,7 @@ struct Q8Part {
   float2* ml;
 };
 
-// The decode row: its sequence's length, and the keys j < limit it sees (<= 0: none).
+// The decode row: its sequence, and the keys j < limit it sees (<= 0: none).
 struct Q8Row {
   int b;
   int64_t limit;
@@ -343,6 +360,7 @@ struct Q8Row {
 __device__ __forceinline__ Q8Row q8_row(const int32_t* __restrict__ cu_q,
                                         const int32_t* __restrict__ lens, int batch, int64_t t,
                                         int64_t capacity, int causal) {
+  Q8Row r;
   int b, c0, c1, len;
   if (batch <= 64) {
     const int i = min(ls_lane(), batch - 1);
@@ -358,23 +376,23 @@ __device__ __forceinline__ Q8Row q8_row(const int32_t* __restrict__ cu_q,
     c1 = cu_q[b + 1];
     len = lens[b];
   }
-  Q8Row r;
   r.b = b;
   const int64_t held = min((int64_t)len, capacity);
   r.limit = causal ? held - (c1 - c0) + (t - c0) + 1 : held;
   return r;
 }
 
-// Pages a wave takes of a dense row, at least ppw and enough for n_splits slices of four waves,
+// Pages a wave takes of a dense row, at least ppw and enough for n_splits slices of NW waves,
 // and the slices that the row's pages then fill.
 struct Q8Share {
   int pages, share, slices;
 };
+template <int NW>
 __device__ __forceinline__ Q8Share q8_share(int64_t limit, int ppw, int n_splits) {
   Q8Share x;
   x.pages = limit <= 0 ? 0 : (int)((limit + kPage - 1) / kPage);
-  x.share = max(ppw, (x.pages + 4 * n_splits - 1) / (4 * n_splits));
-  x.slices = (x.pages + 4 * x.share - 1) / (4 * x.share);
+  x.share = max(ppw, (x.pages + NW * n_splits - 1) / (NW * n_splits));
+  x.slices = (x.pages + NW * x.share - 1) / (NW * x.share);
   return x;
 }
 
@@ -396,16 +414,16 @@ __device__ __forceinline__ ls_u32x4 q8_expand(uint32_t lo, uint32_t hi) {
   return o;
 }
 
-template <int DT, bool DENSE>
-__global__ __launch_bounds__(256) void ls_q8_attn_kernel(
+template <int DT, bool DENSE, int NW>
+__global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(
     const uint16_t* __restrict__ q, int64_t qrs, const int32_t* __restrict__ cu_q, int batch,
     int64_t total_q, const uint8_t* __restrict__ k8, const uint8_t* __restrict__ v8, int64_t cbs,
     const uint8_t* __restrict__ ks, const uint8_t* __restrict__ vs, int64_t sbs, int64_t pages,
     const int32_t* __restrict__ cache_seqlens, int gs, const int32_t* __restrict__ topk_idx,
     int topk, int ppw, int n_splits, float scale_log2, int causal, Q8Part part,
     uint16_t* __restrict__ out, float* __restrict__ lse) {
-  __shared__ __attribute__((aligned(16))) float s_o[4][16 * LS_Q8_PITCH];
-  __shared__ float s_ml[4][2][16];
+  __shared__ __attribute__((aligned(16))) float s_o[NW][16 * LS_Q8_PITCH];
+  __shared__ float s_ml[NW][2][16];
   const int64_t t = blockIdx.x / (unsigned)n_splits;
   const int s = (int)(blockIdx.x - (unsigned)t * (unsigned)n_splits);
   const int g = blockIdx.y, G = gridDim.y;
@@ -433,7 +451,7 @@ __global__ __launch_bounds__(256) void ls_q8_attn_kernel(
   const int64_t limit = row.limit;
   Q8Share cut = {topk, ppw, n_splits};
   if constexpr (DENSE) {
-    cut = q8_share(limit, ppw, n_splits);
+    cut = q8_share<NW>(limit, ppw, n_splits);
     if (s > 0 && s >= cut.slices) return;
   }
   const uint8_t* kseq = k8 + (int64_t)row.b * cbs + (int64_t)g * kPageBytes;
@@ -441,7 +459,7 @@ __global__ __launch_bounds__(256) void ls_q8_attn_kernel(
   const uint8_t* kss = ks + (int64_t)row.b * sbs + g;
   const uint8_t* vss = vs + (int64_t)row.b * sbs + g;
 
-  int slot = (4 * s + w) * cut.share;  // the wave's next plan slot (DENSE: page) and its end
+  int slot = (NW * s + w) * cut.share;  // the wave's next plan slot (DENSE: page) and its end
   const int slot1 = min(cut.pages, slot + cut.share);
   // The page of the next valid slot (-1 at the end of the share).
   auto next_page = [&]() -> int {
@@ -568,39 +586,42 @@ __global__ __launch_bounds__(256) void ls_q8_attn_kernel(
     s_ml[w][1][r] = l_run;
   }
   __syncthreads();
-  // Join the four waves, eight channels of a head a thread.  A wave without a page has sum 0
-  // and is left out; one whose sum is NaN is not.
-  const int h = tid >> 4, d = 8 * (tid & 15);
+  // Join the waves, a few channels of a head a thread.  A wave without a page has sum 0 and
+  // is left out; one whose sum is NaN is not.
+  constexpr int kCh = 16 * kDim / (64 * NW);  // channels a thread: 8 or 4
+  const int h = tid / (kDim / kCh), d = kCh * (tid % (kDim / kCh));
   if (h >= gs) return;
   float M = -INFINITY, L = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) M = fmaxf(M, s_ml[i][0][h]);
-  ls_f32x4 a[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  for (int i = 0; i < NW; ++i) M = fmaxf(M, s_ml[i][0][h]);
+  ls_f32x4 a[kCh / 4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int e = 0; e < kCh / 4; ++e) a[e] = ls_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
     const float l = s_ml[i][1][h];
     const float wt = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(s_ml[i][0][h] - M);
-    const float* so = &s_o[i][h * LS_Q8_PITCH + d];
-    a[0] += wt * *reinterpret_cast<const ls_f32x4*>(so);
-    a[1] += wt * *reinterpret_cast<const ls_f32x4*>(so + 4);
+#pragma unroll
+    for (int e = 0; e < kCh / 4; ++e)
+      a[e] += wt * *reinterpret_cast<const ls_f32x4*>(&s_o[i][h * LS_Q8_PITCH + d + 4 * e]);
     L += wt * l;
   }
   const int64_t tg = (int64_t)g * total_q + t;
   if (n_splits == 1) {
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    ls_u32x4 x;
+    uint16_t* po = out + ((t * G + g) * (int64_t)gs + h) * kDim + d;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      x[e] = ls_pack2(LsElem<DT>::from_f(a[e >> 1][2 * (e & 1)] * inv),
-                      LsElem<DT>::from_f(a[e >> 1][2 * (e & 1) + 1] * inv));
-    *reinterpret_cast<ls_u32x4*>(out + ((t * G + g) * (int64_t)gs + h) * kDim + d) = x;
+    for (int e = 0; e < kCh / 4; ++e)
+      *reinterpret_cast<uint2*>(po + 4 * e) =
+          make_uint2(ls_pack2(LsElem<DT>::from_f(a[e][0] * inv), LsElem<DT>::from_f(a[e][1] * inv)),
+                     ls_pack2(LsElem<DT>::from_f(a[e][2] * inv), LsElem<DT>::from_f(a[e][3] * inv)));
     if (lse && d == 0)
       lse[((int64_t)g * gs + h) * total_q + t] =
           L == 0.f ? INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
   } else {
     float* po = part.o + ((tg * n_splits + s) * gs + h) * kDim + d;
-    *reinterpret_cast<ls_f32x4*>(po) = a[0];
-    *reinterpret_cast<ls_f32x4*>(po + 4) = a[1];
+#pragma unroll
+    for (int e = 0; e < kCh / 4; ++e) *reinterpret_cast<ls_f32x4*>(po + 4 * e) = a[e];
     if (d == 0) part.ml[(tg * gs + h) * n_splits + s] = make_float2(M, L);
   }
 }
@@ -624,7 +645,7 @@ __global__ __launch_bounds__(256) void ls_q8_join_kernel(
   int n = n_splits;
   if constexpr (DENSE) {
     const Q8Row row = q8_row(cu_q, cache_seqlens, batch, t, pages * kPage, causal);
-    n = max(1, __builtin_amdgcn_readfirstlane(q8_share(row.limit, ppw, n_splits).slices));
+    n = max(1, __builtin_amdgcn_readfirstlane(q8_share<kSplitWaves>(row.limit, ppw, n_splits).slices));
   }
   const int64_t tg = (int64_t)g * total_q + t;
   const float2* ml = part.ml + (tg * gs + h) * n_splits;
@@ -763,10 +784,10 @@ extern "C" int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int
   LS_REQUIRE(ls_aligned16(q) && ls_aligned16(k8) && ls_aligned16(v8) && ls_aligned16(out) &&
                  ls_aligned16(workspace),
              LS_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned", who);
-  // Four waves a slice, ppw plan slots or pages a wave; with every wave's share rounded up,
-  // fewer slices may do.
-  const int ppw = (int)((n_pages + 4LL * n_splits - 1) / (4 * n_splits));
-  const int splits = (int)((n_pages + 4LL * ppw - 1) / (4 * ppw));
+  // ppw plan slots or pages a wave; with every wave's share rounded up, fewer slices may do.
+  const int waves = n_splits == 1 ? kWholeWaves : kSplitWaves;
+  const int ppw = (int)((n_pages + (int64_t)waves * n_splits - 1) / (waves * n_splits));
+  const int splits = (int)((n_pages + (int64_t)waves * ppw - 1) / (waves * ppw));
   const size_t need = ls_attn_kvcache_q8_workspace_size(total_q, num_heads, splits);
   LS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), LS_ERR_WORKSPACE,
              "%s: workspace %zu < %zu", who, workspace ? workspace_bytes : (size_t)0, need);
@@ -775,19 +796,25 @@ extern "C" int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int
   Q8Part part;
   part.o = (float*)workspace;
   part.ml = (float2*)(part.o + (splits > 1 ? (size_t)total_q * num_heads * splits * kDim : 0));
-  auto attend = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(total_q * splits), num_kv_heads), dim3(256), 0,
-                       s, (const uint16_t*)q, q_row_stride, cu_seqlens_q, batch, total_q,
+  auto attend = [&](auto dt, auto dn, auto nw) {
+    constexpr int NW = decltype(nw)::value;
+    hipLaunchKernelGGL((ls_q8_attn_kernel<decltype(dt)::value, decltype(dn)::value, NW>),
+                       dim3((unsigned)(total_q * splits), num_kv_heads), dim3(64 * NW), 0, s,
+                       (const uint16_t*)q, q_row_stride, cu_seqlens_q, batch, total_q,
                        (const uint8_t*)k8, (const uint8_t*)v8, cache_batch_stride, k_scale,
                        v_scale, scale_batch_stride, pages, cache_seqlens, gs, topk_idx, n_pages, ppw,
                        splits, scale_log2, causal, part, (uint16_t*)out, softmax_lse);
     return ls_check_launch("ls_q8_attn_kernel");
   };
-  int rc;
-  if (dtype == LS_BF16)
-    rc = dense ? attend(ls_q8_attn_kernel<LS_BF16, true>) : attend(ls_q8_attn_kernel<LS_BF16, false>);
-  else
-    rc = dense ? attend(ls_q8_attn_kernel<LS_F16, true>) : attend(ls_q8_attn_kernel<LS_F16, false>);
+  auto by_waves = [&](auto dt, auto dn) {
+    return n_splits == 1 ? attend(dt, dn, std::integral_constant<int, kWholeWaves>())
+                         : attend(dt, dn, std::integral_constant<int, kSplitWaves>());
+  };
+  auto by_plan = [&](auto dt) {
+    return dense ? by_waves(dt, std::true_type()) : by_waves(dt, std::false_type());
+  };
+  const int rc = dtype == LS_BF16 ? by_plan(std::integral_constant<int, LS_BF16>())
+                                  : by_plan(std::integral_constant<int, LS_F16>());
   if (rc || splits == 1) return rc;
   auto join = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)total_q, num_kv_heads, gs), dim3(256), 0, s, part,
