@@ -8,12 +8,18 @@ instead of concatenating, and the compressed keys are extended by the windows
 each step completes (``ls_kvcache_append``) instead of being kept as Python
 lists.  A step of new tokens is written layer by layer between ``begin`` and
 ``end``; during the step ``seqlens_after`` holds the lengths including it.
+
+``kv_format="q8"`` holds keys and values in 8 bits (e4m3 pages with a power-of-two
+scale per page and head, ``ops.decode_q8``): half the memory and half the bytes a
+step reads.  The compressed keys stay in ``dtype``; those the cache forms are means
+of the keys as it holds them.
 """
 from __future__ import annotations
 
 import torch
 
-from .ops.decode import kvcache_append, n_windows
+from .ops.decode import kvcache_append, n_windows, sparse_attention_kvcache
+from .ops.decode_q8 import kvcache_append_q8, new_kvcache_q8, sparse_attention_kvcache_q8
 
 __all__ = ["LeanSelectKVCache"]
 
@@ -21,16 +27,27 @@ __all__ = ["LeanSelectKVCache"]
 class LeanSelectKVCache:
     def __init__(self, num_layers: int, batch: int, capacity: int, num_kv_heads: int,
                  head_dim: int = 128, *, dtype: torch.dtype = torch.bfloat16, device="cuda",
-                 kernel_size: int = 32, kernel_stride: int = 16):
+                 kernel_size: int = 32, kernel_stride: int = 16, kv_format: str = "native"):
         if num_layers < 1 or batch < 1 or capacity < 1:
             raise ValueError("num_layers, batch and capacity must be positive")
+        if kv_format not in ("native", "q8"):
+            raise ValueError(f"unknown kv_format {kv_format!r}; expected 'native' or 'q8'")
+        if kv_format == "q8" and ((kernel_size, kernel_stride) != (32, 16)
+                                  or dtype not in (torch.bfloat16, torch.float16)):
+            raise ValueError("the 8-bit cache forms windows of 32 keys at stride 16, in bf16 or fp16")
+        self.kv_format = kv_format
         cap = -(-int(capacity) // 64) * 64
         self.num_layers, self.batch, self.capacity = int(num_layers), int(batch), cap
         self.kernel_size, self.kernel_stride = int(kernel_size), int(kernel_stride)
         self.device = torch.device(device)
         shape = (num_layers, batch, cap, num_kv_heads, head_dim)
-        self.k = torch.empty(shape, dtype=dtype, device=self.device)
-        self.v = torch.empty(shape, dtype=dtype, device=self.device)
+        if kv_format == "q8":  # per layer [batch, pages, ...], see ops.decode_q8
+            flat = new_kvcache_q8(num_layers * batch, cap, num_kv_heads, head_dim, device=self.device)
+            self.k8, self.v8, self.k_scale, self.v_scale = (
+                t.view(num_layers, batch, *t.shape[1:]) for t in flat)
+        else:
+            self.k = torch.empty(shape, dtype=dtype, device=self.device)
+            self.v = torch.empty(shape, dtype=dtype, device=self.device)
         cap_c = max(1, n_windows(cap, kernel_size, kernel_stride))
         self.kc = torch.empty((num_layers, batch, cap_c, num_kv_heads, head_dim), dtype=dtype,
                               device=self.device)
@@ -59,10 +76,24 @@ class LeanSelectKVCache:
         """Write layer ``layer``'s packed new keys / values ``[sum n_new, G, D]``
         (and the compressed windows they complete) into the cache."""
         st = self._require_step()
-        kvcache_append(self.k[layer], self.v[layer], self.seqlens, k_new, v_new, st["cu"],
-                       kc_cache=self.kc[layer], kernel_size=self.kernel_size,
-                       kernel_stride=self.kernel_stride, cache_seqlens_host=self.lengths,
-                       cu_seqlens_new_host=st["cu_host"])
+        append = kvcache_append_q8 if self.kv_format == "q8" else kvcache_append
+        append(*self.layer(layer), self.seqlens, k_new, v_new, st["cu"], kc_cache=self.kc[layer],
+               kernel_size=self.kernel_size, kernel_stride=self.kernel_stride,
+               cache_seqlens_host=self.lengths, cu_seqlens_new_host=st["cu_host"])
+
+    def attend(self, layer: int, q: torch.Tensor, topk_idx: torch.Tensor, cu_seqlens_q: torch.Tensor,
+               **kw) -> torch.Tensor:
+        """Attention of the open step's rows over layer ``layer``, restricted to their page
+        plans: ``ops.sparse_attention_kvcache`` (or its 8-bit form; ``kw`` are its options)."""
+        st = self._require_step()
+        attention = sparse_attention_kvcache_q8 if self.kv_format == "q8" else sparse_attention_kvcache
+        return attention(q, *self.layer(layer), st["after"], topk_idx, cu_seqlens_q, **kw)
+
+    def layer(self, layer: int) -> tuple[torch.Tensor, ...]:
+        """Layer ``layer``'s cache tensors: ``(k, v)``, or ``(k8, v8, k_scale, v_scale)``."""
+        if self.kv_format == "q8":
+            return self.k8[layer], self.v8[layer], self.k_scale[layer], self.v_scale[layer]
+        return self.k[layer], self.v[layer]
 
     def end(self) -> None:
         """Close the step: the appended tokens count from now on."""

@@ -405,15 +405,21 @@ __global__ __launch_bounds__(256) void ls_mx4_dequantize_kernel(
     int64_t kc, int64_t kc4, uint16_t* __restrict__ out, int64_t ors) {
   const int64_t nt = blockIdx.y, chunk = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
-  const int64_t row = 16 * nt + (lane & 15), k0 = 128 * chunk + 32 * (lane >> 4);
-  if (chunk >= kc || row >= N) return;
+  const int64_t row = 16 * nt + (lane & 15);
+  if (chunk >= kc) return;
   const ls_u32x4 v = ls_load16(codes + ((nt * kc + chunk) * 64 + lane) * 16);
   const uint32_t c = scales[((nt * kc4 + (chunk >> 2)) * 64 + lane) * 4 + (chunk & 3)];
   const float f = __uint_as_float(c << 23);
+  ls_u32x4 o[4];
 #pragma unroll
-  for (int s = 0; s < 4; ++s)
-    if (k0 + 8 * s < K)
-      *reinterpret_cast<ls_u32x4*>(out + row * ors + k0 + 8 * s) = mx4_expand<DT>(v[s], f);
+  for (int s = 0; s < 4; ++s) o[s] = mx4_expand<DT>(v[s], f);
+  mx4_transpose(o);  // piece q of the four groups: four lanes write 64 bytes together
+  if (row >= N) return;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const int64_t k = 128 * chunk + 32 * s + 8 * (lane >> 4);
+    if (k < K) *reinterpret_cast<ls_u32x4*>(out + row * ors + k) = o[s];
+  }
 }
 
 bool mx4_sizes(int64_t n, int64_t k) {

@@ -24,6 +24,10 @@ compressed-key cache (LeanSelect hands decode selection to it,
 minicpm.py:359-367, 2509-2512, 2718-2736) and attends the cache through those
 pages (minicpm.py:3216-3244 with ``causal=False``).
 
+``new_cache(kv_format="q8")`` keeps the cache in 8 bits and ``quantize_weights`` the
+projections, the MLPs and the head in 4 bits (``ops.mx4``): a decode step then reads
+about half and a quarter of the bytes.
+
 Weights are random-initialised (no checkpoint is loaded here).  Nothing in this
 module falls back to a non-HIP path: it raises when the library is missing or
 the tensors are not on a GPU.
@@ -32,13 +36,15 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
 
 from . import _hip
 from .cache import LeanSelectKVCache
-from .ops.decode import decode_topk_idx, sparse_attention_kvcache
+from .ops.decode import decode_topk_idx
+from .ops.mx4 import dequantize_mx4, linear_mx4, linear_mx4_silu_mul, quantize_mx4
 from .prefill import leanselect_sparse_prefill
 from .selector import LeanSelectSelector
 
@@ -356,6 +362,34 @@ def embed_scale(ids: torch.Tensor, table: torch.Tensor, scale: float,
 # ---------------------------------------------------------------------------
 # The model
 # ---------------------------------------------------------------------------
+# Rows up to which a 4-bit weight is multiplied as it is; more rows go through its 16-bit
+# values and a library GEMM (us: [gate; up] 32768 x 4096, 256 rows 118 against 146, 384 rows 177
+# against 161; 4096 x 16384, 256 rows 50 against 78, 512 rows 85 against 110).
+_MX4_ROWS = 256
+
+
+class Mx4Weight(NamedTuple):
+    """A 4-bit weight ``[out_features, in_features]`` (``ops.mx4``)."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    out_features: int
+    in_features: int
+
+
+def _mx4(w: torch.Tensor) -> Mx4Weight:
+    return Mx4Weight(*quantize_mx4(w), *w.shape)
+
+
+def _linear(x: torch.Tensor, w) -> torch.Tensor:
+    """``x @ w.T`` for a 16-bit or 4-bit weight."""
+    if not isinstance(w, Mx4Weight):
+        return F.linear(x, w)
+    if x.shape[0] <= _MX4_ROWS:
+        return linear_mx4(x, w.codes, w.scales, w.out_features)
+    return F.linear(x, dequantize_mx4(*w, dtype=x.dtype))
+
+
 class _Layer:
     __slots__ = ("input_norm", "w_qkv", "w_o", "post_norm", "w_gate_up", "w_down", "selector")
 
@@ -446,7 +480,7 @@ class MiniCPMLeanSelect:
         cfg, L = self.cfg, self.layers[li]
         H, G, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         N = h.shape[0]
-        qkv = F.linear(h, L.w_qkv)
+        qkv = _linear(h, L.w_qkv)
         cos, sin = self.rope_tables(max(cu_host[i + 1] - cu_host[i] for i in range(len(cu_host) - 1)))
         # Producer-side fusion: the queries rotate in the pass that also forms
         # the selector's query projection, the keys in the pass that also forms
@@ -477,15 +511,30 @@ class MiniCPMLeanSelect:
             init_blocks=cfg.init_blocks, block_size=cfg.block_size, kernel_size=cfg.kernel_size,
             kernel_stride=cfg.kernel_stride, cu_seqlens_host=cu_host, return_topk_idx=True,
             compressed=compressed, q_tilde=q_tilde)
-        o = F.linear(attn.view(N, H * D), L.w_o)
+        o = _linear(attn.view(N, H * D), L.w_o)
         if return_parts:
             return o, dict(qkv=qkv, attn=attn, topk_idx=ids)
         return o
 
     def mlp(self, li: int, h: torch.Tensor) -> torch.Tensor:
-        """``down(silu(gate(h)) * up(h))`` with gate and up as one GEMM."""
-        L = self.layers[li]
-        return F.linear(silu_mul(F.linear(h, L.w_gate_up), self.cfg.intermediate_size), L.w_down)
+        """``down(silu(gate(h)) * up(h))`` with gate and up as one GEMM (with few rows and
+        4-bit weights, one kernel that also applies the activation)."""
+        L, inter = self.layers[li], self.cfg.intermediate_size
+        w = L.w_gate_up
+        if isinstance(w, Mx4Weight) and h.shape[0] <= _MX4_ROWS and inter % 16 == 0:
+            return _linear(linear_mx4_silu_mul(h, w.codes, w.scales, w.out_features), L.w_down)
+        return _linear(silu_mul(_linear(h, w), inter), L.w_down)
+
+    def quantize_weights(self) -> "MiniCPMLeanSelect":
+        """Replace the projections, the MLPs' weights and the head by 4-bit ones (the embedding,
+        the norms and the selectors stay as they are)."""
+        for L in self.layers:
+            for name in ("w_qkv", "w_o", "w_gate_up", "w_down"):
+                if not isinstance(getattr(L, name), Mx4Weight):
+                    setattr(L, name, _mx4(getattr(L, name)))
+        if not isinstance(self.lm_head, Mx4Weight):
+            self.lm_head = _mx4(self.lm_head)
+        return self
 
     @staticmethod
     def positions(cu_host: list[int], device) -> torch.Tensor:
@@ -495,12 +544,14 @@ class MiniCPMLeanSelect:
         return torch.cat(parts).to(device)
 
     # -- prefill -----------------------------------------------------------------
-    def new_cache(self, batch: int, capacity: int) -> LeanSelectKVCache:
-        """An empty decode cache for ``batch`` sequences of up to ``capacity`` tokens."""
+    def new_cache(self, batch: int, capacity: int, kv_format: str = "native") -> LeanSelectKVCache:
+        """An empty decode cache for ``batch`` sequences of up to ``capacity`` tokens, in the
+        model's dtype or (``kv_format="q8"``) in 8 bits."""
         cfg = self.cfg
         return LeanSelectKVCache(cfg.num_hidden_layers, batch, capacity, cfg.num_key_value_heads,
                                  cfg.head_dim, dtype=self.dtype, device=self.device,
-                                 kernel_size=cfg.kernel_size, kernel_stride=cfg.kernel_stride)
+                                 kernel_size=cfg.kernel_size, kernel_stride=cfg.kernel_stride,
+                                 kv_format=kv_format)
 
     @torch.no_grad()
     def prefill(self, input_ids: torch.Tensor, cu_seqlens_host: list[int] | None = None,
@@ -544,7 +595,7 @@ class MiniCPMLeanSelect:
             cache.end()
         last = torch.tensor([b - 1 for b in cu_host[1:]], device=dev, dtype=torch.long)
         h_last = h.index_select(0, last) / (cfg.hidden_size / cfg.dim_model_base)
-        return F.linear(h_last, self.lm_head).float()
+        return _linear(h_last, self.lm_head).float()
 
     # -- decode ------------------------------------------------------------------
     def attention_decode(self, li: int, h: torch.Tensor, positions: torch.Tensor,
@@ -556,7 +607,7 @@ class MiniCPMLeanSelect:
         cfg, L = self.cfg, self.layers[li]
         H, G, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         B = h.shape[0]
-        qkv = F.linear(h, L.w_qkv)
+        qkv = _linear(h, L.w_qkv)
         cos, sin = self.rope_tables(max(cache.lengths_after))
         rope_inplace(qkv, positions, cos, sin, n_q_heads=H, n_k_heads=G, k_col_offset=H * D,
                      head_dim=D, check_positions=False)
@@ -570,9 +621,8 @@ class MiniCPMLeanSelect:
                               block_size=cfg.block_size, kernel_size=cfg.kernel_size,
                               kernel_stride=cfg.kernel_stride, cache_seqlens_host=after,
                               cu_seqlens_q_host=cu_q_host)
-        attn = sparse_attention_kvcache(q, cache.k[li], cache.v[li], cache.seqlens_after, ids,
-                                        cu_q, causal=False)
-        return F.linear(attn.view(B, H * D), L.w_o)
+        attn = cache.attend(li, q, ids, cu_q, causal=False)
+        return _linear(attn.view(B, H * D), L.w_o)
 
     @torch.no_grad()
     def decode_step(self, input_ids: torch.Tensor, cache: LeanSelectKVCache) -> torch.Tensor:
@@ -599,4 +649,4 @@ class MiniCPMLeanSelect:
             nxt = self.layers[li + 1].input_norm if li + 1 < cfg.num_hidden_layers else self.final_norm
             add_rms_layernorm(x, d, c, nxt, cfg.rms_norm_eps, out=h)
         cache.end()
-        return F.linear(h / (cfg.hidden_size / cfg.dim_model_base), self.lm_head).float()
+        return _linear(h / (cfg.hidden_size / cfg.dim_model_base), self.lm_head).float()

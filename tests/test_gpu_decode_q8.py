@@ -6,8 +6,10 @@ import math
 import pytest
 import torch
 
-from leanselect_amd.ops import (dense_attention_kvcache_q8, kvcache_append_q8, new_kvcache_q8,
-                                sparse_attention_kvcache_q8)
+from leanselect_amd import minicpm
+from leanselect_amd.cache import LeanSelectKVCache
+from leanselect_amd.ops import (decode_topk_idx, dense_attention_kvcache_q8, kvcache_append_q8,
+                                new_kvcache_q8, sparse_attention_kvcache_q8)
 from leanselect_amd.ops.decode import n_windows
 from oracle import lowbit_oracle as lo
 
@@ -439,3 +441,78 @@ def test_nothing_to_do():
     assert sparse_attention_kvcache_q8(q, *cache, _i32([5]), ids, _i32([0, 0])).shape == (0, 32, D)
     none = torch.empty(0, 2, D, dtype=torch.bfloat16, device=DEV)
     kvcache_append_q8(*cache, _i32([5]), none, none, _i32([0, 0]))
+
+
+# ---------------------------------------------------------------------------
+# In the cache class and the model
+# ---------------------------------------------------------------------------
+def test_cache_class_runs_the_operators_together():
+    """Prompt, then ragged steps through ``LeanSelectKVCache(kv_format="q8")``: its tensors equal
+    the definition's bytes, the plans come from its compressed keys, attention reads them."""
+    G, H, layers = 2, 32, 2
+    cache = LeanSelectKVCache(layers, 3, 600, G, kv_format="q8")
+    plain = LeanSelectKVCache(layers, 3, 600, G)
+    assert cache.k8.shape == (layers, 3, 10, G, 64, 128)
+    want = [lo.Q8Cache(*cache.layer(i)) for i in range(layers)]
+    g = torch.Generator().manual_seed(30)
+    lens = [0, 0, 0]
+    for new in ([500, 65, 31], [1, 1, 1], [1, 0, 1], [1, 1, 1]):
+        for c in (cache, plain):
+            c.begin(new)
+        rows = [b for b in range(3) for _ in range(new[b])]
+        cu = _cu(new)
+        after = [a + b for a, b in zip(lens, new)]
+        for i in range(layers):
+            k, v = _rows(cu[-1], G, torch.bfloat16, g, 0.3), _rows(cu[-1], G, torch.bfloat16, g, 0.3)
+            want[i].append(lens, k, v, cu)
+            for c in (cache, plain):
+                c.update(i, k.to(DEV), v.to(DEV))
+            _same_bytes(cache.layer(i), want[i], after)
+            if max(new) == 1:
+                q = torch.randn(len(rows), H, D, generator=g).bfloat16()
+                ids = decode_topk_idx(q.to(DEV), cache.kc[i], cache.seqlens_after, _i32(cu), topk=4,
+                                      local_blocks=1, cache_seqlens_host=after, cu_seqlens_q_host=cu)
+                out, lse = cache.attend(i, q.to(DEV), ids, _i32(cu), return_lse=True)
+                ref, ref_lse, bound = lo.attend(want[i], q, after, cu, ids.cpu())
+                _check(out, lse, ref, ref_lse, bound, torch.bfloat16)
+                assert plain.attend(i, q.to(DEV), ids, _i32(cu)).shape == out.shape
+        for c in (cache, plain):
+            c.end()
+        lens = after
+        # Each key within e4m3's half step (relative, or half a subnormal step of the page's scale),
+        # so the compressed keys within the mean of that, and a rounding on either side.
+        for i in range(layers):
+            for b in range(3):
+                n = n_windows(lens[b])
+                if not n:
+                    continue
+                x = plain.k[i, b, :lens[b]].double().cpu()
+                pages = torch.arange(lens[b]) // 64
+                step = 2.0 ** (want[i].kcode[b][pages].double() - 127 - 10)[..., None]
+                # Twice: a row may have been brought under a raised code.
+                off = 2 * (2.0 ** -4 * x.abs()).maximum(step) * (1 + 2.0 ** -4)
+                tol = off.unfold(0, 32, 16).mean(-1) + 2.0 ** -7 * (x.abs() + off).unfold(0, 32, 16).mean(-1)
+                d = (cache.kc[i, b, :n].double() - plain.kc[i, b, :n].double()).abs().cpu()
+                assert bool((d <= tol).all()), (i, b, (d - tol).max().item())
+
+
+def test_model_decodes_over_an_8_bit_cache():
+    """Logits of decode steps over both caches: close, as 8 bits of keys and values allow, and
+    the step's attention equal to the operators' on the cache."""
+    cfg = minicpm.MiniCPMConfig(hidden_size=1024, num_hidden_layers=2, num_attention_heads=8,
+                                num_key_value_heads=2, intermediate_size=2048, vocab_size=4096,
+                                topk=64, local_blocks=4)
+    model = minicpm.MiniCPMLeanSelect(cfg, device=DEV, seed=3)
+    g = torch.Generator(device=DEV).manual_seed(11)
+    ids = torch.randint(0, 4096, (817,), generator=g, device=DEV, dtype=torch.int32)
+    caches = [model.new_cache(2, 1024, kv_format=f) for f in ("native", "q8")]
+    first = [model.prefill(ids, [0, 300, 817], cache=c) for c in caches]
+    assert torch.equal(first[0], first[1])  # a prefill does not read the cache
+    for _ in range(6):
+        tok = torch.randint(0, 4096, (2,), generator=g, device=DEV, dtype=torch.int32)
+        a, b = (model.decode_step(tok, c) for c in caches)
+        assert bool(torch.isfinite(b).all())
+        rel = ((a - b).norm() / a.norm()).item()
+        # Keys and values off by 2^-4 at most each, in two of the residual stream's layers.
+        assert rel < 2 * 2 * 2.0 ** -4, rel
+    assert caches[1].lengths == [306, 523]

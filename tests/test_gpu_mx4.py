@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from leanselect_amd import minicpm
 from leanselect_amd.ops import (dequantize_mx4, lay_out_mx4, linear_mx4, linear_mx4_silu_mul,
                                 quantize_mx4)
 from oracle import lowbit_oracle as lo
@@ -179,3 +180,36 @@ def test_weights_that_are_not_finite_are_refused():
         w[3, 3] = bad
         with pytest.raises(ValueError, match="finite"):
             quantize_mx4(w)
+
+
+def _small_model(seed):
+    cfg = minicpm.MiniCPMConfig(hidden_size=1024, num_hidden_layers=2, num_attention_heads=8,
+                                num_key_value_heads=2, intermediate_size=2048, vocab_size=4100,
+                                topk=64, local_blocks=4)
+    return minicpm.MiniCPMLeanSelect(cfg, device=DEV, seed=seed)
+
+
+def test_model_with_4_bit_weights_is_the_model_of_their_values():
+    """A quantised model's prefill (library products of the values) and decode steps (4-bit
+    products) against the same model whose 16-bit weights are those values."""
+    a, b = _small_model(5).quantize_weights(), _small_model(5)
+    for L in b.layers:
+        for name in ("w_qkv", "w_o", "w_gate_up", "w_down"):
+            w = getattr(L, name)
+            setattr(L, name, dequantize_mx4(*quantize_mx4(w), *w.shape))
+    b.lm_head = dequantize_mx4(*quantize_mx4(b.lm_head), *b.lm_head.shape)
+    assert a.quantize_weights() is a  # again: nothing left to do
+    g = torch.Generator(device=DEV).manual_seed(12)
+    lens = [300, 600]
+    ids = torch.randint(0, 4100, (sum(lens),), generator=g, device=DEV, dtype=torch.int32)
+    for kv in ("native", "q8"):
+        caches = [m.new_cache(2, 1024, kv_format=kv) for m in (a, b)]
+        got, want = (m.prefill(ids, [0, 300, 900], cache=c) for m, c in zip((a, b), caches))
+        # Prefill of 900 rows: the same library products, so the same bits.
+        assert torch.equal(got, want)
+        for _ in range(3):
+            tok = torch.randint(0, 4100, (2,), generator=g, device=DEV, dtype=torch.int32)
+            got, want = (m.decode_step(tok, c) for m, c in zip((a, b), caches))
+            rel = ((got - want).norm() / want.norm()).item()
+            # Two layers whose 16-bit roundings (2^-9 each, some ten a layer) may differ.
+            assert rel < 20 * 2.0 ** -9, (kv, rel)

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from leanselect_amd import _hip, ops
+from leanselect_amd.cache import LeanSelectKVCache
 from leanselect_amd.ops import (dense_attention_kvcache_q8, kvcache_append_q8, linear_mx4,
                                 linear_mx4_silu_mul, new_kvcache_q8, quantize_mx4,
                                 sparse_attention_kvcache_q8)
@@ -187,6 +188,19 @@ def test_c_entry_points_refuse_before_any_launch():
     assert L.ls_quantize_mx4(16, 32, 1, 31, B, 16, 4, None) == _hip.LS_ERR_INVALID
     assert L.ls_dequantize_mx4(16, 4, 1, 32, _hip.LS_F32, 16, 32, None) == _hip.LS_ERR_UNSUPPORTED
     assert L.ls_dequantize_mx4(16, 4, 1, 32, B, 18, 32, None) == _hip.LS_ERR_UNSUPPORTED
+
+
+def test_cache_class_refusals():
+    for bad in (dict(kv_format="int8"), dict(kv_format="q8", kernel_size=64),
+                dict(kv_format="q8", kernel_stride=8), dict(kv_format="q8", dtype=torch.float32),
+                dict(kv_format="q8", head_dim=64)):
+        with pytest.raises(ValueError):
+            LeanSelectKVCache(1, 1, 64, 1, device="cpu", **bad)
+    c = LeanSelectKVCache(2, 3, 100, 4, device="cpu", kv_format="q8")
+    assert c.capacity == 128 and [t.shape for t in c.layer(1)] == [
+        (3, 2, 4, 64, 128), (3, 2, 4, 128, 64), (3, 2, 4), (3, 2, 4)]
+    with pytest.raises(RuntimeError, match="no cache step"):
+        c.attend(0, None, None, None)
 
 
 def test_operators_are_public():
