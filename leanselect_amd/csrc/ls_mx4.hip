@@ -79,6 +79,24 @@ __device__ __forceinline__ void mx4_transpose(ls_u32x4 (&x)[4]) {
   }
 }
 
+// Arguments of both products (one: a launch with many costs the host more).
+struct Mx4Args {
+  const uint16_t* x;
+  int64_t xrs;
+  int64_t m;
+  int64_t K;
+  const uint8_t* codes;
+  const uint32_t* scales;
+  int64_t kc;
+  int64_t kc4;
+  int64_t tiles;
+  int64_t per_half;
+  int64_t n_out;
+  uint16_t* out;
+  int64_t ors;
+  float* part;
+};
+
 // Workgroup (RT tiles of 16 outputs, block of 16 MT rows of x): NW waves share the inputs, four
 // tiles (512 inputs) at a time, and are summed through LDS in order, so a row's bits depend
 // on neither MT nor RT.  PAIR: half of the tiles are `pair` tiles later, the up projections of
@@ -90,10 +108,19 @@ __device__ __forceinline__ void mx4_transpose(ls_u32x4 (&x)[4]) {
 // quarters of the wave brings the pieces where the weights' order wants them.
 // A wave's next weights are loaded into the registers of each tile that it has used.
 template <int DT, int MT, int RT, bool PAIR, int NW>
-__global__ __launch_bounds__(64 * NW) void ls_mx4_kernel(
-    const uint16_t* __restrict__ x, int64_t xrs, int64_t m, int64_t K,
-    const uint8_t* __restrict__ codes, const uint32_t* __restrict__ scales, int64_t kc, int64_t kc4,
-    int64_t tiles, int64_t n_out, uint16_t* __restrict__ out, int64_t ors) {
+__global__ __launch_bounds__(64 * NW) void ls_mx4_kernel(const Mx4Args args) {
+  const uint16_t* __restrict__ x = args.x;
+  const int64_t xrs = args.xrs;
+  const int64_t m = args.m;
+  const int64_t K = args.K;
+  const uint8_t* __restrict__ codes = args.codes;
+  const uint32_t* __restrict__ scales = args.scales;
+  const int64_t kc = args.kc;
+  const int64_t kc4 = args.kc4;
+  const int64_t tiles = args.tiles;
+  const int64_t n_out = args.n_out;
+  uint16_t* __restrict__ out = args.out;
+  const int64_t ors = args.ors;
   constexpr int OT = PAIR ? RT / 2 : RT;  // tiles of outputs
   __shared__ __attribute__((aligned(16))) ls_f32x4 s_acc[NW][RT * MT][64];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -212,11 +239,21 @@ __global__ __launch_bounds__(64 * NW) void ls_mx4_kernel(
 // for 16 lanes.  The halves are summed through LDS; with several slices float32 parts go to the
 // workspace, [slice][row][16 tiles], and a second kernel adds them in order.
 template <int DT, int MT, bool PAIR>
-__global__ __launch_bounds__(512) void ls_mx4_rows_kernel(
-    const uint16_t* __restrict__ x, int64_t xrs, int64_t m, int64_t K,
-    const uint8_t* __restrict__ codes, const uint32_t* __restrict__ scales, int64_t kc, int64_t kc4,
-    int64_t tiles, int64_t per_half, int64_t n_out, uint16_t* __restrict__ out, int64_t ors,
-    float* __restrict__ part) {
+__global__ __launch_bounds__(512) void ls_mx4_rows_kernel(const Mx4Args args) {
+  const uint16_t* __restrict__ x = args.x;
+  const int64_t xrs = args.xrs;
+  const int64_t m = args.m;
+  const int64_t K = args.K;
+  const uint8_t* __restrict__ codes = args.codes;
+  const uint32_t* __restrict__ scales = args.scales;
+  const int64_t kc = args.kc;
+  const int64_t kc4 = args.kc4;
+  const int64_t tiles = args.tiles;
+  const int64_t per_half = args.per_half;
+  const int64_t n_out = args.n_out;
+  uint16_t* __restrict__ out = args.out;
+  const int64_t ors = args.ors;
+  float* __restrict__ part = args.part;
   constexpr int OT = PAIR ? 4 : 8;  // tiles of outputs of the workgroup
   // [buffer][half][128 inputs][16 rows][32 inputs][16 p + r]: 16 bytes, piece p of row r
   __shared__ __attribute__((aligned(16))) ls_u32x4 s_x[2][2][2][MT][4][64];
@@ -509,6 +546,9 @@ extern "C" int ls_linear_mx4(const void* x, int64_t x_row_stride, int64_t rows,
   LS_REQUIRE(cut.blocks <= 65535, LS_ERR_UNSUPPORTED, "%s: too many rows", who);
   const int64_t n_out = silu_mul ? out_features / 2 : out_features;
   hipStream_t stm = (hipStream_t)stream;
+  const Mx4Args args = {(const uint16_t*)x, x_row_stride, rows, in_features, (const uint8_t*)codes,
+                        (const uint32_t*)scales, cut.kc, cut.kc4, cut.tiles, cut.per_half, n_out,
+                        (uint16_t*)out, out_row_stride, (float*)workspace};
   using std::integral_constant;
   auto few = [&](auto dt, auto mtc, auto pr, auto rt, auto nw) {
     constexpr int RT = decltype(rt)::value, NW = decltype(nw)::value;
@@ -516,9 +556,7 @@ extern "C" int ls_linear_mx4(const void* x, int64_t x_row_stride, int64_t rows,
     constexpr int OT = PAIR ? RT / 2 : RT;
     hipLaunchKernelGGL((ls_mx4_kernel<decltype(dt)::value, decltype(mtc)::value, RT, PAIR, NW>),
                        dim3((unsigned)((cut.tiles + OT - 1) / OT), (unsigned)cut.blocks),
-                       dim3(64 * NW), 0, stm, (const uint16_t*)x, x_row_stride, rows, in_features,
-                       (const uint8_t*)codes, (const uint32_t*)scales, cut.kc, cut.kc4, cut.tiles,
-                       n_out, (uint16_t*)out, out_row_stride);
+                       dim3(64 * NW), 0, stm, args);
     return ls_check_launch("ls_mx4_kernel");
   };
   auto by_waves = [&](auto dt, auto mtc, auto pr) {
@@ -534,9 +572,7 @@ extern "C" int ls_linear_mx4(const void* x, int64_t x_row_stride, int64_t rows,
     hipLaunchKernelGGL((ls_mx4_rows_kernel<DT, decltype(mtc)::value, PAIR>),
                        dim3((unsigned)((cut.tiles + OT - 1) / OT), (unsigned)cut.blocks,
                             (unsigned)cut.slices),
-                       dim3(512), 0, stm, (const uint16_t*)x, x_row_stride, rows, in_features,
-                       (const uint8_t*)codes, (const uint32_t*)scales, cut.kc, cut.kc4, cut.tiles,
-                       cut.per_half, n_out, (uint16_t*)out, out_row_stride, (float*)workspace);
+                       dim3(512), 0, stm, args);
     const int rc = ls_check_launch("ls_mx4_rows_kernel");
     if (rc || cut.slices == 1) return rc;
     hipLaunchKernelGGL((ls_mx4_join_kernel<DT, PAIR>),
