@@ -70,14 +70,17 @@ __device__ __forceinline__ uint32_t q8_rescale(uint32_t v, float f) {
   return q8_pack(lo[0] * f, lo[1] * f, hi[0] * f, hi[1] * f);
 }
 
-// The sequence that holds work unit `unit` when sequence b has count(b) units, in order:
-// a wave scans 64 sequences at a time.  Every lane gets the sequence and the unit's number
-// in it; -1 past the last unit.
-template <class Count>
-__device__ __forceinline__ int q8_find(int& unit, int batch, Count count) {
+// The sequence that gets the `unit`-th of the batch's pages with new rows, in order, its length
+// and its new rows [n0, n1); `unit` becomes the page's number among the sequence's.  -1 past the
+// last page.  A wave scans 64 sequences at a time, and what it found stays in its lanes.
+__device__ __forceinline__ int q8_find(int& unit, int batch, const int32_t* __restrict__ lens,
+                                       const int32_t* __restrict__ cu_new, int& len, int& n0, int& n1) {
   const int lane = ls_lane();
   for (int s0 = 0; s0 < batch; s0 += 64) {
-    const int mine = s0 + lane < batch ? count(s0 + lane) : 0;
+    const int i = min(s0 + lane, batch - 1);
+    const int l = lens[i], lo = cu_new[i], hi = cu_new[i + 1];
+    const bool some = s0 + lane < batch && hi > lo && l >= 0 && lo >= 0;
+    const int mine = some ? (int)(((int64_t)l + (hi - lo) + kPage - 1) / kPage) - l / kPage : 0;
     int upto = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -88,6 +91,9 @@ __device__ __forceinline__ int q8_find(int& unit, int batch, Count count) {
     if (past != 0) {
       const int at = __builtin_ctzll(past);
       unit -= __builtin_amdgcn_readlane(upto - mine, at);
+      len = __builtin_amdgcn_readlane(l, at);
+      n0 = __builtin_amdgcn_readlane(lo, at);
+      n1 = __builtin_amdgcn_readlane(hi, at);
       return s0 + at;
     }
     unit -= __builtin_amdgcn_readlane(upto, 63);
@@ -177,16 +183,12 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
   __shared__ uint32_t s_v[kDim * kVPitch / 4];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int g = blockIdx.y;
-  int unit = blockIdx.x;
-  const int b = q8_find(unit, batch, [&](int i) {
-    const int64_t len = cache_seqlens[i], n = cu_new[i + 1] - cu_new[i];
-    return n > 0 && len >= 0 ? (int)((len + n + kPage - 1) / kPage - len / kPage) : 0;
-  });
+  int unit = blockIdx.x, len_b, n0_b, n1_b;
+  const int b = q8_find(unit, batch, cache_seqlens, cu_new, len_b, n0_b, n1_b);
   if (b < 0) return;
-  const int64_t len = cache_seqlens[b], n0 = cu_new[b];
-  const int64_t n1 = min((int64_t)cu_new[b + 1], total_new);
+  const int64_t len = len_b, n0 = n0_b, n1 = min((int64_t)n1_b, total_new);
   const int64_t page = len / kPage + unit;
-  if (page >= pages || n0 < 0) return;
+  if (page >= pages) return;
   const int64_t base = page * kPage, end = len + (n1 - n0);
   const int r0 = (int)max<int64_t>(0, len - base);  // the page's new rows: r0 <= row < r1
   const int r1 = (int)min<int64_t>(kPage, end - base);
@@ -373,7 +375,7 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
 // A page's powers of two go into the scores' scale and into the sum of O.
 //
 // A wave takes ppw plan slots, or (DENSE) pages, or more of a row that is longer than the
-// caller said; a row's later slices, past its last page, end at once.  The next page's K is loaded as soon as this page's scores are formed,
+// caller said; a row's later slices, past its last page, only say that they hold nothing.  The next page's K is loaded as soon as this page's scores are formed,
 // its V as soon as this page's sum is, into the same registers.
 // ---------------------------------------------------------------------------
 #define LS_Q8_MAX_SPLITS 256
@@ -393,7 +395,8 @@ struct Q8Row {
   int64_t limit;
 };
 
-// Row t of the batch (t < cu_q[batch]).  A batch of at most 64 is read by the lanes at once.
+// Row t of the batch, b = -1 behind the last sequence.  A batch of at most 64 is read by the
+// lanes at once.
 __device__ __forceinline__ Q8Row q8_row(const int32_t* __restrict__ cu_q,
                                         const int32_t* __restrict__ lens, int batch, int64_t t,
                                         int64_t capacity, int causal) {
@@ -403,11 +406,12 @@ __device__ __forceinline__ Q8Row q8_row(const int32_t* __restrict__ cu_q,
     const int i = min(ls_lane(), batch - 1);
     const int lo = cu_q[i], hi = cu_q[i + 1], n = lens[i];
     b = __popcll(__ballot(ls_lane() < batch && t >= hi));  // sequences that end at or before t
-    b = min(b, batch - 1);
+    if (b >= batch) return Q8Row{-1, 0};
     c0 = __builtin_amdgcn_readlane(lo, b);
     c1 = __builtin_amdgcn_readlane(hi, b);
     len = __builtin_amdgcn_readlane(n, b);
   } else {
+    if (t >= cu_q[batch]) return Q8Row{-1, 0};
     b = ls_find_segment(cu_q, batch, t);
     c0 = cu_q[b];
     c1 = cu_q[b + 1];
@@ -527,13 +531,16 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
 #pragma unroll
   for (int k4 = 0; k4 < 4; ++k4)
     qf[k4] = r < gs ? ls_load16(qrow + 8 * k4) : ls_u32x4{0u, 0u, 0u, 0u};
-  if (t >= cu_q[batch]) return;  // a row behind the last sequence
   const Q8Row row = q8_row(cu_q, cache_seqlens, batch, t, pages * kPage, causal);
+  if (row.b < 0) return;
   const int64_t limit = row.limit;
   Q8Share cut = {topk, ppw, n_splits};
   if constexpr (DENSE) {
     cut = q8_share<NW>(limit, ppw, n_splits);
-    if (s > 0 && s >= cut.slices) return;
+    if (s > 0 && s >= cut.slices) {  // nothing left for this slice
+      if (tid < gs) part.ml[(((int64_t)g * total_q + t) * gs + tid) * n_splits + s] = make_float2(-INFINITY, 0.f);
+      return;
+    }
   }
   const uint8_t* kseq = k8 + (int64_t)row.b * cbs + (int64_t)g * kPageBytes;
   const uint8_t* vseq = v8 + (int64_t)row.b * cbs + (int64_t)g * kPageBytes;
@@ -707,38 +714,26 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
   }
 }
 
-// out[t][g*gs + h] = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the slices that the
-// row fills; a row that sees no key gives zeros and lse = +inf.  A workgroup per (row, KV head,
-// query head): each wave forms the maximum and sum of all slices (at most four a lane), then
-// thread (part, c) sums four channels of every eighth slice, and the eight parts are added in
-// LDS in order.
-template <int DT, bool DENSE>
+// out[t][g*gs + h] = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s; a row that sees no key gives
+// zeros and lse = +inf.  A workgroup per (row, KV head, query head): each wave forms the maximum
+// and sum of all slices (at most four a lane), then thread (p, c) sums four channels of every
+// eighth slice, and the eight parts are added in LDS in order.  The first slices' values are
+// loaded with the maxima (a slice of sum 0 may hold anything and is left out).
+template <int DT>
 __global__ __launch_bounds__(256) void ls_q8_join_kernel(const Q8AttnArgs args) {
   const Q8Part part = args.part;
-  const int32_t* __restrict__ cu_q = args.cu_q;
-  const int32_t* __restrict__ cache_seqlens = args.cache_seqlens;
-  const int batch = args.batch;
-  const int64_t pages = args.pages;
-  const int causal = args.causal;
-  const int ppw = args.ppw;
   const int64_t total_q = args.total_q;
-  const int gs = args.gs;
-  const int n_splits = args.n_splits;
-  uint16_t* __restrict__ out = args.out;
-  float* __restrict__ lse = args.lse;
+  const int gs = args.gs, n = args.n_splits;
+  constexpr int kAhead = 8;
   __shared__ float s_w[LS_Q8_MAX_SPLITS];
   __shared__ ls_f32x4 s_a[8][32];
   const int64_t t = blockIdx.x;
   const int g = blockIdx.y, h = blockIdx.z, G = gridDim.y;
   const int tid = threadIdx.x, lane = tid & 63;
-  if (t >= cu_q[batch]) return;
-  int n = n_splits;
-  if constexpr (DENSE) {
-    const Q8Row row = q8_row(cu_q, cache_seqlens, batch, t, pages * kPage, causal);
-    n = max(1, __builtin_amdgcn_readfirstlane(q8_share<kSplitWaves>(row.limit, ppw, n_splits).slices));
-  }
+  const int c = tid & 31, p = tid >> 5;
   const int64_t tg = (int64_t)g * total_q + t;
-  const float2* ml = part.ml + (tg * gs + h) * n_splits;
+  const float2* __restrict__ ml = part.ml + (tg * gs + h) * n;
+  const float* __restrict__ po = part.o + (tg * n * gs + h) * kDim + 4 * c;
   float ms[4], sum[4], M = -INFINITY;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -746,8 +741,14 @@ __global__ __launch_bounds__(256) void ls_q8_join_kernel(const Q8AttnArgs args) 
     const float2 x = i < n ? ml[i] : make_float2(-INFINITY, 0.f);
     ms[k] = x.x;
     sum[k] = x.y;
-    M = fmaxf(M, ms[k]);
   }
+  ls_f32x4 ahead[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    ahead[k] = *reinterpret_cast<const ls_f32x4*>(po + (int64_t)min(p + 8 * k, n - 1) * gs * kDim);
+  if (t >= args.cu_q[args.batch]) return;  // a row behind the last sequence
+#pragma unroll
+  for (int k = 0; k < 4; ++k) M = fmaxf(M, ms[k]);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, ls_shfl_xor(M, o));
   float L = 0.f;
@@ -764,12 +765,23 @@ __global__ __launch_bounds__(256) void ls_q8_join_kernel(const Q8AttnArgs args) 
       if (64 * k + lane < n) s_w[64 * k + lane] = ms[k];
   }
   __syncthreads();
-  const int c = tid & 31, p = tid >> 5;
   ls_f32x4 a = {0.f, 0.f, 0.f, 0.f};
-  const float* po = part.o + (tg * n_splits * gs + h) * kDim + 4 * c;
-#pragma unroll 8
-  for (int sp = p; sp < n; sp += 8)
-    a += s_w[sp] * *reinterpret_cast<const ls_f32x4*>(po + (int64_t)sp * gs * kDim);
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    const float wt = p + 8 * k < n ? s_w[p + 8 * k] : 0.f;
+    if (wt != 0.f) a += wt * ahead[k];
+  }
+  for (int s0 = p + 8 * kAhead; s0 < n; s0 += 8 * kAhead) {
+    ls_f32x4 x[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      x[k] = *reinterpret_cast<const ls_f32x4*>(po + (int64_t)min(s0 + 8 * k, n - 1) * gs * kDim);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const float wt = s0 + 8 * k < n ? s_w[s0 + 8 * k] : 0.f;
+      if (wt != 0.f) a += wt * x[k];
+    }
+  }
   s_a[p][c] = a;
   __syncthreads();
   if (tid < 32) {
@@ -780,9 +792,9 @@ __global__ __launch_bounds__(256) void ls_q8_join_kernel(const Q8AttnArgs args) 
     uint2 x;
     x.x = ls_pack2(LsElem<DT>::from_f(a[0] * inv), LsElem<DT>::from_f(a[1] * inv));
     x.y = ls_pack2(LsElem<DT>::from_f(a[2] * inv), LsElem<DT>::from_f(a[3] * inv));
-    *reinterpret_cast<uint2*>(out + ((t * G + g) * (int64_t)gs + h) * kDim + 4 * c) = x;
-    if (lse && tid == 0)
-      lse[((int64_t)g * gs + h) * total_q + t] =
+    *reinterpret_cast<uint2*>(args.out + ((t * G + g) * (int64_t)gs + h) * kDim + 4 * c) = x;
+    if (args.lse && tid == 0)
+      args.lse[((int64_t)g * gs + h) * total_q + t] =
           L == 0.f ? INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
   }
 }
@@ -913,7 +925,5 @@ extern "C" int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int
     hipLaunchKernelGGL(kernel, dim3((unsigned)total_q, num_kv_heads, gs), dim3(256), 0, s, args);
     return ls_check_launch("ls_q8_join_kernel");
   };
-  if (dtype == LS_BF16)
-    return dense ? join(ls_q8_join_kernel<LS_BF16, true>) : join(ls_q8_join_kernel<LS_BF16, false>);
-  return dense ? join(ls_q8_join_kernel<LS_F16, true>) : join(ls_q8_join_kernel<LS_F16, false>);
+  return dtype == LS_BF16 ? join(ls_q8_join_kernel<LS_BF16>) : join(ls_q8_join_kernel<LS_F16>);
 }

@@ -509,6 +509,10 @@ Mx4Cut mx4_cut(int64_t rows, int64_t K, int64_t N, bool silu) {
   c.slices = (c.kc4 + 2 * c.per_half - 1) / (2 * c.per_half);
   c.shared = rows > 16 ? tiles * c.kc >= 2048
                        : (c.slices == 1 && wgs > 128 && wgs <= 256) || (c.kc4 >= 16 && tiles <= 256);
+  if (!c.shared && c.mt > 2) {  // few tiles and many rows: blocks of 32, their registers bound the waves
+    c.mt = 2;
+    c.blocks = (rows + 31) / 32;
+  }
   return c;
 }
 }  // namespace
@@ -582,7 +586,9 @@ extern "C" int ls_linear_mx4(const void* x, int64_t x_row_stride, int64_t rows,
     return ls_check_launch("ls_mx4_join_kernel");
   };
   auto by_form = [&](auto dt, auto mtc, auto pr) {
-    return cut.shared ? shared(dt, mtc, pr) : by_waves(dt, mtc, pr);
+    if constexpr (decltype(mtc)::value <= 2)
+      if (!cut.shared) return by_waves(dt, mtc, pr);
+    return shared(dt, mtc, pr);
   };
   auto by_pair = [&](auto dt, auto mtc) {
     return silu_mul ? by_form(dt, mtc, std::true_type()) : by_form(dt, mtc, std::false_type());
