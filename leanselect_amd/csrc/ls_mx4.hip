@@ -235,8 +235,9 @@ __global__ __launch_bounds__(64 * NW) void ls_mx4_kernel(const Mx4Args args) {
 // tiles, or four and their up projections; block of 16 MT rows; slice z of the inputs): eight
 // waves, wave (n, h) two tiles over the h-th half of the slice.  256 inputs of each half are
 // staged at a time, in two buffers: the four waves of a half load x as it lies (wave n the n-th
-// 64 bytes of each 256), and an operand is read back across the pieces, 256 contiguous bytes
-// for 16 lanes.  The halves are summed through LDS; with several slices float32 parts go to the
+// 64 bytes of each 256, four neighbouring lanes a row: 73448 x 4096, 64 rows 77 us; with a
+// row's four lanes 16 apart 84), and an operand is read back across the pieces, 256 contiguous
+// bytes for 16 lanes.  The halves are summed through LDS; with several slices float32 parts go to the
 // workspace, [slice][row][16 tiles], and a second kernel adds them in order.
 template <int DT, int MT, bool PAIR>
 __global__ __launch_bounds__(512) void ls_mx4_rows_kernel(const Mx4Args args) {
@@ -261,6 +262,7 @@ __global__ __launch_bounds__(512) void ls_mx4_rows_kernel(const Mx4Args args) {
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = w & 3, h = w >> 2;
   const int r = lane & 15, q = lane >> 4;
+  const int xr = lane >> 2, xp = lane & 3;  // row and piece of x that the lane stages
   const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
   int64_t ot[2], tile[2];  // tile of outputs, tile of the weight (past the last: the last again)
 #pragma unroll
@@ -292,10 +294,10 @@ __global__ __launch_bounds__(512) void ls_mx4_rows_kernel(const Mx4Args args) {
   auto load_x = [&](int64_t g, int st) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t k = 512 * g + 256 * st + 128 * i + 32 * wn + 8 * q;
+      const int64_t k = 512 * g + 256 * st + 128 * i + 32 * wn + 8 * xp;
 #pragma unroll
       for (int c = 0; c < MT; ++c) {
-        const int64_t row = m0 + 16 * c + r;
+        const int64_t row = m0 + 16 * c + xr;
         xs[i * MT + c] = row < m && k < K && g < g1 ? ls_load16(x + row * xrs + k)
                                                     : ls_u32x4{0u, 0u, 0u, 0u};
       }
@@ -305,7 +307,7 @@ __global__ __launch_bounds__(512) void ls_mx4_rows_kernel(const Mx4Args args) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int c = 0; c < MT; ++c) s_x[buf][h][i][c][wn][lane] = xs[i * MT + c];
+      for (int c = 0; c < MT; ++c) s_x[buf][h][i][c][wn][16 * xp + xr] = xs[i * MT + c];
   };
   load_s(g0);
   load_x(g0, 0);
