@@ -188,8 +188,8 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
   if (b < 0) return;
   const int64_t len = len_b, n0 = n0_b, n1 = min((int64_t)n1_b, total_new);
   const int64_t page = len / kPage + unit;
-  if (page >= pages) return;
   const int64_t base = page * kPage, end = len + (n1 - n0);
+  if (page >= pages || base >= end) return;  // (the second: offsets past total_new)
   const int r0 = (int)max<int64_t>(0, len - base);  // the page's new rows: r0 <= row < r1
   const int r1 = (int)min<int64_t>(kPage, end - base);
   const int64_t at = (int64_t)b * cbs + (page * G + g) * kPageBytes;

@@ -109,10 +109,12 @@ def kvcache_append_q8(k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
     total = k_new.shape[0]
     lens = _lengths(cache_seqlens, cache_seqlens_host, "cache_seqlens")
     cu = _lengths(cu_seqlens_new, cu_seqlens_new_host, "cu_seqlens_new")
-    if len(lens) != B or len(cu) != B + 1 or cu[0] != 0 or cu[-1] != total \
+    if B < 1 or len(lens) != B or len(cu) != B + 1 or cu[0] != 0 or cu[-1] != total \
             or cache_seqlens.numel() != B or cu_seqlens_new.numel() != B + 1:
         raise ValueError("cache_seqlens must be [batch] and cu_seqlens_new [batch + 1] offsets "
                          "of the packed new rows")
+    if B > 1 and (cache_stride < P * G * _PAGE_BYTES or scale_stride < P * G):
+        raise ValueError("sequences that share pages cannot be appended to")
     after = [n + b - a for n, a, b in zip(lens, cu, cu[1:])]
     if min(lens) < 0 or max(after) > P * PAGE or any(map(gt, lens, after)):
         raise ValueError(f"sequences of {lens} tokens cannot become {after} in a cache with a "
@@ -130,15 +132,15 @@ def kvcache_append_q8(k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
             raise ValueError(f"{n_windows(max(after))} compressed windows exceed kc_capacity {kc[3]}")
     index = _hip.gpu_index(k8, v8, k_scale, v_scale, cache_seqlens, k_new, v_new, cu_seqlens_new,
                            kc_cache)
+    cache_seqlens, cu_seqlens_new = cache_seqlens.contiguous(), cu_seqlens_new.contiguous()
     # One row stride serves both: dense 16-byte aligned rows with equal strides, else copies.
     if not (_rows16(k_new) and _rows16(v_new) and k_new.stride() == v_new.stride()):
         k_new = k_new.clone(memory_format=torch.contiguous_format)
         v_new = v_new.clone(memory_format=torch.contiguous_format)
     _hip.launch(index, "ls_kvcache_append_q8", k8.data_ptr(), v8.data_ptr(), cache_stride,
                 k_scale.data_ptr(), v_scale.data_ptr(), scale_stride, P,
-                cache_seqlens.contiguous().data_ptr(), k_new.data_ptr(), v_new.data_ptr(),
-                k_new.stride(0), cu_seqlens_new.contiguous().data_ptr(), total, B, G, HEAD_DIM, code,
-                *kc)
+                cache_seqlens.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0),
+                cu_seqlens_new.data_ptr(), total, B, G, HEAD_DIM, code, *kc)
 
 
 def sparse_attention_kvcache_q8(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor,
@@ -168,7 +170,7 @@ def dense_attention_kvcache_q8(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tens
     """``sparse_attention_kvcache_q8`` over every cached page; ``max_len`` is the longest
     sequence's length (it only decides how the work is cut)."""
     return _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, None, cu_seqlens_q,
-                   max(1, -(-int(max_len) // PAGE)), causal, softmax_scale, n_splits, return_lse, out)
+                   -(-int(max_len) // PAGE), causal, softmax_scale, n_splits, return_lse, out)
 
 
 def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, n_pages, causal,
@@ -188,11 +190,14 @@ def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, 
         g, t, n_pages = topk_idx.shape
         if g != G or t != total_q or not 1 <= n_pages <= 256:
             raise ValueError(f"topk_idx must be [{G}, {total_q}, k] with 1 <= k <= 256")
+    else:
+        n_pages = max(1, min(n_pages, P))
     if out is not None:
         _hip.check_out(out, (total_q, H, HEAD_DIM), q.dtype, q.device)
-        if out.data_ptr() % 16:
-            raise ValueError("out must be 16-byte aligned")
+        if out.data_ptr() % 16 or out.data_ptr() == q.data_ptr() and total_q:
+            raise ValueError("out must be 16-byte aligned and must not overlap q")
     index = _hip.gpu_index(q, k8, v8, k_scale, v_scale, cache_seqlens, cu_seqlens_q, topk_idx)
+    cache_seqlens, cu_seqlens_q = cache_seqlens.contiguous(), cu_seqlens_q.contiguous()
     if topk_idx is not None:
         if topk_idx.dtype is not torch.int32 or not topk_idx.is_contiguous():
             topk_idx = topk_idx.to(torch.int32).contiguous()
@@ -214,9 +219,9 @@ def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, 
     floats = total_q * H * n_splits * (HEAD_DIM + 2) if n_splits > 1 else 0
     ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     _hip.launch(index, "ls_attn_kvcache_q8", q.data_ptr(), q.stride(0),
-                cu_seqlens_q.contiguous().data_ptr(), total_q, k8.data_ptr(), v8.data_ptr(),
-                cache_stride, k_scale.data_ptr(), v_scale.data_ptr(), scale_stride, P,
-                cache_seqlens.contiguous().data_ptr(), B, H, G, HEAD_DIM, code, ids, n_pages,
+                cu_seqlens_q.data_ptr(), total_q, k8.data_ptr(), v8.data_ptr(), cache_stride,
+                k_scale.data_ptr(), v_scale.data_ptr(), scale_stride, P,
+                cache_seqlens.data_ptr(), B, H, G, HEAD_DIM, code, ids, n_pages,
                 HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale),
                 1 if causal else 0, n_splits, out.data_ptr(), _hip.ptr(lse), _hip.ptr(ws), 4 * floats)
     return (out, lse) if return_lse else out

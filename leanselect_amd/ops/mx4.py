@@ -110,8 +110,8 @@ def linear_mx4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_f
                out: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T`` for ``x [rows, in_features]`` (bf16 or fp16): ``[rows, out_features]`` in
     ``x``'s dtype.  Made for the few rows of a decode step; every 64 rows read the weight
-    again.  A row's bits do not depend on the other rows, but may on whether there are more
-    than 16 (and then than 64) of them."""
+    again.  ``out`` must not overlap ``x``.  A row's bits do not depend on what the other rows
+    hold, but may on how many there are: up to 16, up to 64, or each number of 64 above."""
     return _linear(x, codes, scales, out_features, 0, out)
 
 
@@ -140,6 +140,8 @@ def _linear(x, codes, scales, out_features, silu, out):
             raise ValueError(f"out must be ({rows}, {n}) {x.dtype} with unit column stride, "
                              f"got {tuple(out.shape)} {out.dtype}")
         out_stride = out.stride(0)
+        if rows > 1 and out_stride < n or out.data_ptr() == x.data_ptr() and rows:
+            raise ValueError("out's rows must not overlap each other or x")
     x_stride = k
     if x.data_ptr() % 16 or not x.is_contiguous():
         if x.data_ptr() % 16 or x.stride(1) != 1 or x.stride(0) % 8:

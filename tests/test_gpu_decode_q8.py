@@ -190,6 +190,19 @@ def test_append_to_many_sequences():
                          <= 2.0 ** -8 * ref.abs() + 2.0 ** -19 * size).all()), (b, w)
 
 
+def test_offsets_past_the_new_rows_write_nothing():
+    """Offsets on the device that pass the rows there are (the host's lists say otherwise):
+    the rows there are get written, and no page or code behind them."""
+    cache = _garbage(2, 256, 1, 5)
+    x = _rows(2, 1, torch.bfloat16, torch.Generator().manual_seed(30)).to(DEV)
+    before = [t.view(torch.uint8).clone() for t in cache]
+    kvcache_append_q8(*cache, _i32([0, 0]), x, x, _i32([0, 200, 200]), cache_seqlens_host=[0, 0],
+                      cu_seqlens_new_host=[0, 1, 2])
+    for t, old in zip(cache, before):
+        new = t.view(torch.uint8)
+        assert torch.equal(new[0, 1:], old[0, 1:]) and torch.equal(new[1], old[1])
+
+
 # ---------------------------------------------------------------------------
 # Attention
 # ---------------------------------------------------------------------------
@@ -283,6 +296,30 @@ def test_several_rows_a_sequence(sparse):
             want, _, bound = lo.attend(ref, q, lens, cu, ids if sparse else None, causal, 0.2)
             _check(out, None, want, None, bound, torch.bfloat16, slice(0, cu[-1]))
             assert bool((out[cu[-1]:] == 3.0).all())
+
+
+@pytest.mark.parametrize("sparse", [True, False])
+def test_more_sequences_than_a_wave(sparse):
+    """Rows are found by search then; sequences without a row and rows behind the last one."""
+    B, H, G = 70, 8, 2
+    lens = [(37 * b) % 200 for b in range(B)]
+    lq = [(b % 5) // 2 for b in range(B)]
+    cache = _filled(lens, G, torch.bfloat16, 31)
+    ref = lo.Q8Cache(*cache)
+    cu, total = _cu(lq), sum(lq) + 3
+    g = torch.Generator().manual_seed(32)
+    q = torch.randn(total, H, D, generator=g).to(torch.bfloat16)
+    ids = torch.randint(-1, 5, (G, total, 6), generator=g, dtype=torch.int32)
+    want, want_lse, bound = lo.attend(ref, q, lens, cu, ids if sparse else None, True)
+    for n_splits in (None, 1, 2):
+        out = torch.full((total, H, D), 3.0, dtype=torch.bfloat16, device=DEV)
+        args = dict(causal=True, n_splits=n_splits, out=out, return_lse=True)
+        if sparse:
+            _, lse = sparse_attention_kvcache_q8(q.to(DEV), *cache, _i32(lens), ids.to(DEV), _i32(cu), **args)
+        else:
+            _, lse = dense_attention_kvcache_q8(q.to(DEV), *cache, _i32(lens), _i32(cu), max(lens), **args)
+        _check(out, lse, want, want_lse, bound, torch.bfloat16, slice(0, cu[-1]))
+        assert bool((out[cu[-1]:] == 3.0).all())
 
 
 def test_values_that_are_not_seen_do_not_matter():

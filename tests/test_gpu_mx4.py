@@ -108,6 +108,27 @@ def test_silu_mul(dtype, inter, k, m):
     _check(linear_mx4_silu_mul(x.to(DEV), codes, scales, 2 * inter), x, w, silu=True)
 
 
+@pytest.mark.parametrize("n,k,m", [
+    (4608, 264, 1), (4624, 264, 9),        # two tiles a workgroup of eight waves
+    (16400, 136, 1), (16400, 136, 16),     # four tiles a workgroup of four
+    (16400, 128, 17), (16390, 120, 70),    # the same, 32 rows a workgroup
+    (16640, 512, 1), (32768, 264, 5),      # shared rows, one slice
+    (48, 8200, 3), (2048, 8192, 40),       # shared rows, slices and their join
+    (2048, 2056, 130)])
+def test_linear_in_each_form(n, k, m):
+    (codes, scales), w = _values(n, k, n + 2 * k + m)
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(m)).bfloat16()
+    _check(linear_mx4(x.to(DEV), codes, scales, n), x, w)
+
+
+@pytest.mark.parametrize("n,k,m", [(16896, 128, 2), (16896, 120, 40), (32800, 72, 16), (20480, 512, 1),
+                                   (2048, 8200, 5), (2048, 2056, 33)])
+def test_silu_mul_in_each_form(n, k, m):
+    (codes, scales), w = _values(n, k, n + 3 * k + m, 112, 122)
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(m)).bfloat16()
+    _check(linear_mx4_silu_mul(x.to(DEV), codes, scales, n), x, w, silu=True)
+
+
 def test_scales_at_the_ends_of_their_range():
     for code in (8, 60, 200, 250):
         (codes, scales), w = _values(24, 264, code, code, code)

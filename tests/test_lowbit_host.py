@@ -1,4 +1,8 @@
-"""Refusals of the 8-bit cache and the 4-bit products, before any GPU call (CPU only)."""
+"""Refusals of the 8-bit cache and the 4-bit products, before any GPU call, and what their
+wrappers hand to the library (CPU only)."""
+import contextlib
+import ctypes
+
 import pytest
 import torch
 
@@ -45,6 +49,10 @@ def test_well_formed_cpu_arguments_reach_the_device_check():
     (dict(lens=_i32([3, 126])), "capacity"),
     (dict(lens=_i32([-1, 0])), "capacity"),
     (dict(cache_seqlens_host=[3, 0, 0]), "offsets"),
+    (dict(cache=[t[:0] for t in new_kvcache_q8(1, 64, 2, device="cpu")], lens=_i32([]), cu=_i32([4])),
+     "offsets"),
+    (dict(cache=[t.expand(2, *t.shape[1:]) for t in new_kvcache_q8(1, 128, 2, device="cpu")]),
+     "share pages"),
     (dict(kc_cache=torch.zeros(2, 7, 2, 128)), "kc_cache"),
     (dict(kc_cache=torch.zeros(2, 7, 2, 64, dtype=BF16)), "kc_cache"),
     (dict(lens=_i32([100, 0]), kc_cache=torch.zeros(2, 4, 2, 128, dtype=BF16)), "kc_capacity"),
@@ -201,6 +209,86 @@ def test_cache_class_refusals():
         (3, 2, 4, 64, 128), (3, 2, 4, 128, 64), (3, 2, 4), (3, 2, 4)]
     with pytest.raises(RuntimeError, match="no cache step"):
         c.attend(0, None, None, None)
+
+
+def test_outputs_that_overlap_are_refused(monkeypatch):
+    monkeypatch.setattr(_hip, "gpu_index", lambda *t: 0)
+    codes = torch.zeros(8, 1, 64, 16, dtype=torch.uint8)
+    scales = torch.zeros(8, 1, 64, 4, dtype=torch.uint8)
+    x = torch.zeros(3, 128, dtype=BF16)
+    for out in (x, torch.zeros(1, 128, dtype=BF16).expand(3, 128),
+                torch.zeros(384, dtype=BF16).as_strided((3, 128), (64, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            linear_mx4(x, codes, scales, 128, out=out)
+    q = torch.zeros(2, 32, 128, dtype=BF16)
+    cache = new_kvcache_q8(2, 128, 2, device="cpu")
+    with pytest.raises(ValueError, match="overlap q"):
+        dense_attention_kvcache_q8(q, *cache, _i32([3, 3]), _i32([0, 1, 2]), 3, out=q)
+
+
+@pytest.fixture
+def sent(monkeypatch):
+    """What the wrappers hand to the library: (device, entry point, arguments), in turn, with
+    the int32 arrays behind the pointers read at that moment."""
+    calls = []
+
+    def launch(index, name, *args):
+        calls.append((index, name, args, [list((ctypes.c_int32 * n).from_address(args[at]))
+                                          for at, n in INT_ARGS[name]]))
+
+    monkeypatch.setattr(_hip, "gpu_index", lambda *t: 0)
+    monkeypatch.setattr(_hip, "launch", launch)
+    return calls
+
+
+# (argument, entries) of the int32 arrays, for two sequences.
+INT_ARGS = {"ls_kvcache_append_q8": [(7, 2), (11, 3)], "ls_attn_kvcache_q8": [(2, 3), (11, 2)]}
+
+
+def test_lengths_and_offsets_that_are_not_contiguous_stay_apart(sent):
+    """Each is copied to rows of its own: neither copy may be given back before the call."""
+    cache = new_kvcache_q8(2, 128, 2, device="cpu")
+    lens, cu = _i32([[3, 9], [5, 9]])[:, 0], _i32([[0, 9], [1, 9], [2, 9]])[:, 0]
+    x = torch.zeros(2, 2, 128, dtype=BF16)
+    q = torch.zeros(2, 32, 128, dtype=BF16)
+    ids = torch.zeros(2, 2, 1, dtype=torch.int32)
+    kvcache_append_q8(*cache, lens, x, x, cu)
+    dense_attention_kvcache_q8(q, *cache, lens, cu, 5)
+    sparse_attention_kvcache_q8(q, *cache, lens, ids, cu)
+    assert [c[3] for c in sent] == [[[3, 5], [0, 1, 2]], [[0, 1, 2], [3, 5]], [[0, 1, 2], [3, 5]]]
+
+
+@pytest.mark.parametrize("max_len,pages", [(-5, 1), (0, 1), (64, 1), (65, 2), (1 << 45, 2)])
+def test_the_longest_length_is_only_a_hint(sent, max_len, pages):
+    cache = new_kvcache_q8(2, 128, 2, device="cpu")
+    q = torch.zeros(2, 32, 128, dtype=BF16)
+    dense_attention_kvcache_q8(q, *cache, _i32([3, 5]), _i32([0, 1, 2]), max_len)
+    assert sent[0][2][18] == pages
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_launches_are_made_on_the_tensors_device(monkeypatch, current):
+    """With that device current while it launches, on that device's current stream."""
+    now, seen = [current], []
+
+    @contextlib.contextmanager
+    def device(index):
+        before, now[0] = now[0], index
+        yield
+        now[0] = before
+
+    class Library:
+        @staticmethod
+        def ls_linear_mx4(*args):
+            seen.append((now[0], args))
+            return _hip.LS_OK
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: now[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(_hip, "lib", lambda: Library)
+    _hip.launch(1, "ls_linear_mx4", 7, None)
+    assert seen == [(1, (7, None, 101))] and now == [current]
 
 
 def test_operators_are_public():
