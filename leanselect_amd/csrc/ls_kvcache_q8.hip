@@ -375,8 +375,19 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
 // A page's powers of two go into the scores' scale and into the sum of O.
 //
 // A wave takes ppw plan slots, or (DENSE) pages, or more of a row that is longer than the
-// caller said; a row's later slices, past its last page, only say that they hold nothing.  The next page's K is loaded as soon as this page's scores are formed,
-// its V as soon as this page's sum is, into the same registers.
+// caller said; a row's later slices, past its last page, only say that they hold nothing.
+// The next page's K and V are loaded as soon as this page's have been used, into the same
+// registers.
+//
+// What bounds it: a compute unit's reads from memory.  Operands read in their own order (lanes
+// 16 apart on neighbouring bytes) reach 50 GB/s a unit however many waves read; 1 KB a load in
+// the lanes' order (kStage), brought into the operands' order through LDS, 63 GB/s with eight
+// waves (131071 keys, one slice: 671 us, 533 us), but with four waves, alone on their SIMDs, the
+// way through LDS is in the page's chain (two slices of 256 pages: 50 us, 54 us).  So rows of
+// one slice, which need their unit's rate, take eight waves and kStage; slices take neither.
+// 131071 keys in 128 slices: 19.1 us with the join (67 MB, 3.5 TB/s; a launch, the chain of
+// lengths, page and sum, and the join are 9 us of it); 16 rows of 64 pages in eight slices:
+// 14.1 us (34 MB, 2.4 TB/s); 72 rows of 4000 keys, one slice: 33 us (150 MB, 4.6 TB/s).
 // ---------------------------------------------------------------------------
 #define LS_Q8_MAX_SPLITS 256
 constexpr int kSplitWaves = 4, kWholeWaves = 8;  // of a workgroup: one of several slices, or the row
@@ -435,6 +446,13 @@ __device__ __forceinline__ Q8Share q8_share(int64_t limit, int ppw, int n_splits
   x.share = max(ppw, (x.pages + NW * n_splits - 1) / (NW * n_splits));
   x.slices = (x.pages + NW * x.share - 1) / (NW * x.share);
   return x;
+}
+
+// Orders a wave's accesses to LDS among its lanes (its instructions reach LDS in order: no wait).
+__device__ __forceinline__ void q8_wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // Eight e4m3 bytes as eight values of the query's type.
@@ -507,8 +525,11 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
   const Q8Part part = args.part;
   uint16_t* __restrict__ out = args.out;
   float* __restrict__ lse = args.lse;
+  // Each wave's O at its end; before, where kStage, a page's K and V in turn.
   __shared__ __attribute__((aligned(16))) float s_o[NW][16 * LS_Q8_PITCH];
   __shared__ float s_ml[NW][2][16];
+  constexpr bool kStage = NW == kWholeWaves;
+  static_assert(kPageBytes <= (int)sizeof(s_o[0]), "a page fits where a wave's O lies");
   const int64_t t = blockIdx.x / (unsigned)n_splits;
   const int s = (int)(blockIdx.x - (unsigned)t * (unsigned)n_splits);
   const int g = blockIdx.y, G = gridDim.y;
@@ -574,23 +595,37 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
   ls_f32x4 o[8];
 #pragma unroll
   for (int db = 0; db < 8; ++db) o[db] = ls_f32x4{0.f, 0.f, 0.f, 0.f};
-  ls_u32x4 kf[4][2], vf[8];
+  ls_u32x4 kl[8], vl[8];
   uint32_t kcode, vcode;
   auto load_k = [&](int page) {
-    const uint8_t* kp = kseq + (int64_t)page * G * kPageBytes + r * kDim + 32 * qg;
+    const uint8_t* kp = kseq + (int64_t)page * G * kPageBytes;
 #pragma unroll
-    for (int kb = 0; kb < 4; ++kb) {
-      kf[kb][0] = ls_load16(kp + kb * 16 * kDim);
-      kf[kb][1] = ls_load16(kp + kb * 16 * kDim + 16);
-    }
+    for (int j = 0; j < 8; ++j)
+      kl[j] = ls_load16(kp + (kStage ? 1024 * j + 16 * lane
+                                     : (16 * (j >> 1) + r) * kDim + 32 * qg + 16 * (j & 1)));
     kcode = kss[(int64_t)page * G];
   };
   auto load_v = [&](int page) {
-    const uint8_t* vp = vseq + (int64_t)page * G * kPageBytes + r * kPage + 16 * qg;
+    const uint8_t* vp = vseq + (int64_t)page * G * kPageBytes;
 #pragma unroll
-    for (int db = 0; db < 8; ++db) vf[db] = ls_load16(vp + db * 16 * kPage);
+    for (int j = 0; j < 8; ++j) vl[j] = ls_load16(vp + 1024 * j + (kStage ? 16 * lane : r * kPage + 16 * qg));
     vcode = vss[(int64_t)page * G];
   };
+  // Piece p of 16 bytes of 128-byte line n lies at 8 n + (p ^ (n & 7)): both the writes (a line
+  // for eight lanes) and the reads (a piece of eight lines) then touch every bank once.
+  ls_u32x4* stage = reinterpret_cast<ls_u32x4*>(s_o[w]);
+  const int put_at = (lane & 56) | ((lane ^ (lane >> 3)) & 7);
+  auto put = [&](const ls_u32x4 (&x)[8]) {
+    q8_wave_sync();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) stage[64 * j + put_at] = x[j];
+    q8_wave_sync();
+  };
+  // K: key r of 16, channels 32 qg + 16 h + [0, 16).  V: channel r of 16, the qg-th 16 bytes.
+  int k_at[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) k_at[h] = 8 * r + ((2 * qg + h) ^ (r & 7));
+  const int v_at = 8 * (r >> 1) + ((4 * (r & 1) + qg) ^ (r >> 1));
   // One page whose K and V are in registers (or on their way), with the loads of the page
   // after it.  The last page is its own copy of this code, so that the loads are on every
   // path of the loop (a conditional load would be waited for where the paths meet).
@@ -600,29 +635,34 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
     const int nvis = left < kPage ? (int)left : kPage;
     const float kscale = scale_log2 * q8_pow(kcode);
     float sv[16], pm = -INFINITY;
+    if constexpr (kStage) {
+      put(kl);
+      if constexpr (kMore) load_k(after);
+    }
 #pragma unroll
     for (int kb = 0; kb < 4; ++kb) {
       ls_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k4 = 0; k4 < 4; ++k4) {
-        const ls_u32x4 kk = kf[kb][k4 >> 1];
-        acc = LsElem<DT>::mfma(q8_expand<DT>(kk[2 * (k4 & 1)], kk[2 * (k4 & 1) + 1]), qf[k4], acc);
+      for (int h = 0; h < 2; ++h) {
+        ls_u32x4 kk;
+        if constexpr (kStage)
+          kk = stage[128 * kb + k_at[h]];
+        else
+          kk = kl[2 * kb + h];
+        acc = LsElem<DT>::mfma(q8_expand<DT>(kk[0], kk[1]), qf[2 * h], acc);
+        acc = LsElem<DT>::mfma(q8_expand<DT>(kk[2], kk[3]), qf[2 * h + 1], acc);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) sv[4 * kb + i] = acc[i] * kscale;
     }
-    if constexpr (kMore) load_k(after);
-    if (nvis < kPage) {  // keys past the end: no weight; their values may be anything: zeros
+    if constexpr (!kStage && kMore) load_k(after);
+    const bool part_page = nvis < kPage;  // keys past the end have no weight, and may be anything
+    if (part_page) {
 #pragma unroll
-      for (int kb = 0; kb < 4; ++kb) {
+      for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (16 * kb + 4 * qg + i >= nvis) sv[4 * kb + i] = -INFINITY;
-        const int n = min(4, max(0, nvis - 16 * kb - 4 * qg));
-        const uint32_t keep = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
-#pragma unroll
-        for (int db = 0; db < 8; ++db) vf[db][kb] &= keep;
-      }
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) pm = fmaxf(pm, sv[i]);
@@ -642,15 +682,37 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
         l_run += ls_f16_to_f32(h0) + ls_f16_to_f32(h1);
         pf[c][e] = ls_pack2(h0, h1);
       }
-    const float vscale = q8_pow(vcode);
+    auto weigh = [&](ls_u32x4 (&vf)[8], uint32_t code) {
+      if (part_page) {
 #pragma unroll
-    for (int db = 0; db < 8; ++db) {
-      ls_f32x4 pv = {0.f, 0.f, 0.f, 0.f};
-      pv = LsElem<LS_F16>::mfma(q8_expand<LS_F16>(vf[db][0], vf[db][1]), pf[0], pv);
-      pv = LsElem<LS_F16>::mfma(q8_expand<LS_F16>(vf[db][2], vf[db][3]), pf[1], pv);
-      o[db] = o[db] * alpha + pv * vscale;
+        for (int kb = 0; kb < 4; ++kb) {
+          const int n = min(4, max(0, nvis - 16 * kb - 4 * qg));
+          const uint32_t keep = n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
+#pragma unroll
+          for (int db = 0; db < 8; ++db) vf[db][kb] &= keep;
+        }
+      }
+      const float vscale = q8_pow(code);
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+        ls_f32x4 pv = {0.f, 0.f, 0.f, 0.f};
+        pv = LsElem<LS_F16>::mfma(q8_expand<LS_F16>(vf[db][0], vf[db][1]), pf[0], pv);
+        pv = LsElem<LS_F16>::mfma(q8_expand<LS_F16>(vf[db][2], vf[db][3]), pf[1], pv);
+        o[db] = o[db] * alpha + pv * vscale;
+      }
+    };
+    if constexpr (kStage) {
+      put(vl);
+      const uint32_t code = vcode;
+      if constexpr (kMore) load_v(after);
+      ls_u32x4 vf[8];
+#pragma unroll
+      for (int db = 0; db < 8; ++db) vf[db] = stage[64 * db + v_at];
+      weigh(vf, code);
+    } else {
+      weigh(vl, vcode);
+      if constexpr (kMore) load_v(after);
     }
-    if constexpr (kMore) load_v(after);
   };
   int page = next_page();
   if (page >= 0) {
@@ -666,6 +728,7 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
   }
   l_run += ls_shfl_xor(l_run, 16);
   l_run += ls_shfl_xor(l_run, 32);
+  q8_wave_sync();
 #pragma unroll
   for (int db = 0; db < 8; ++db)  // o[db][i]: head r, channel 16 db + 4 qg + i
     *reinterpret_cast<ls_f32x4*>(&s_o[w][r * LS_Q8_PITCH + 16 * db + 4 * qg]) = o[db];

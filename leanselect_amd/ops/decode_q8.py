@@ -205,12 +205,14 @@ def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, 
     if not _rows16(q):
         q = q.clone(memory_format=torch.contiguous_format)
     if n_splits is None:
-        # Workgroups a (row, group), of four waves: enough of them to cover the device, at least
-        # one page a wave.  A power of two for plans (48 rows of 64 pages, 96 (row, group)s: 2
-        # slices 23.9 us, 3 slices 30.4, 4 slices 26.5).
-        pairs = max(1, total_q * G)
-        n_splits = min(-(-n_pages // 4), -(-_WORKGROUPS // pairs) if topk_idx is None
-                       else 1 << (_WORKGROUPS // pairs).bit_length() >> 1)
+        # Slices of a row: as many as leave every workgroup its compute unit, at least a page a
+        # wave.  One slice (eight waves, no join) for few pages, and where the rows fill the
+        # device meanwhile (us, one slice and several: 1000 keys, 1 row 9.5, 8.5 and a launch
+        # more, 16 rows 9.5, 10.2; 4000 keys, 40 rows 24.3, 21.8, 56 rows 24.7, 27.7).  More
+        # workgroups than units: 48 rows of 4000 keys in 2 slices 24.1, in 3 slices 30.4.
+        pairs = total_q * G
+        n_splits = 1 if n_pages <= max(16, 2 * pairs // 3) \
+            else min(-(-n_pages // 4), _WORKGROUPS // max(1, pairs))
     n_splits = max(1, min(int(n_splits), _MAX_SPLITS))
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
