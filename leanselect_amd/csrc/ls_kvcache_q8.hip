@@ -106,7 +106,7 @@ __device__ __forceinline__ int q8_find(int& unit, int batch, const int32_t* __re
 // magnitude of the page's new rows, takes the page's code (at least the old one where the
 // page holds older rows), brings older rows under a raised code, and writes the new rows.
 // A page of a sequence belongs to one workgroup, so nothing is shared between them.
-// K: thread (row, c) takes the 8-channel pieces c, c + 4, c + 8, c + 12 of its row.
+// K: thread (r, c) takes 8 channels of the rows r, r + 16, r + 32, r + 48.
 // V: thread (quad, octet) takes 8 channels of the four tokens that share a 4-byte word.
 //
 // Compressed keys: window w is the mean of the 32 stored keys from token 16 w, so it is two
@@ -205,8 +205,8 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
   };
   const bool windows = complete(0) || complete(1) || complete(2) || complete(3) || complete(4);
 
-  const int krow = tid >> 2, kc = 8 * (tid & 3);
-  const bool knew = krow >= r0 && krow < r1;
+  const int krow = tid >> 4, kc = 8 * (tid & 15);  // rows krow + 16 j
+  auto knew = [&](int j) { return krow + 16 * j >= r0 && krow + 16 * j < r1; };
   const int quad = tid >> 4, oct = tid & 15;  // quad = 4 q + t
   const int tok = 16 * (quad & 3) + 4 * (quad >> 2);
   ls_u32x4 kx[4], vx[4], nx[4];
@@ -214,15 +214,15 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
   uint32_t ktop = 0, vtop = 0, ntop = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    kx[j] = knew ? ls_load16(kn + first + krow * nrs + 32 * j + kc) : ls_u32x4{0u, 0u, 0u, 0u};
+    kx[j] = knew(j) ? ls_load16(kn + first + (krow + 16 * j) * nrs + kc) : ls_u32x4{0u, 0u, 0u, 0u};
     const bool vnew = tok + j >= r0 && tok + j < r1;
     vx[j] = vnew ? ls_load16(vn + first + (tok + j) * nrs + 8 * oct) : ls_u32x4{0u, 0u, 0u, 0u};
   }
   if (complete(4)) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      nx[j] = krow < after ? ls_load16(kn + first + (kPage + krow) * nrs + 32 * j + kc)
-                           : ls_u32x4{0u, 0u, 0u, 0u};
+      nx[j] = krow + 16 * j < after ? ls_load16(kn + first + (kPage + krow + 16 * j) * nrs + kc)
+                                    : ls_u32x4{0u, 0u, 0u, 0u};
   }
   uint8_t* kp = k8 + at + krow * kDim + kc;
   uint32_t kold = 1, vold = 1;
@@ -230,7 +230,8 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
     kold = ks[sat];
     vold = vs[sat];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ko[j] = krow < r0 ? *reinterpret_cast<const uint2*>(kp + 32 * j) : make_uint2(0, 0);
+    for (int j = 0; j < 4; ++j)
+      ko[j] = krow + 16 * j < r0 ? *reinterpret_cast<const uint2*>(kp + 16 * kDim * j) : make_uint2(0, 0);
   }
   // Bytes of a V word that are new, and those that are older; the words as they are, where
   // not all of a word is new.
@@ -271,24 +272,23 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
   const float kdown = q8_pow(max(127 + (int)kold - (int)kcode, 0));
   const float vdown = q8_pow(max(127 + (int)vold - (int)vcode, 0));
 
-  auto keep = [&](int row, int j, uint2 v) {  // a row's bytes into LDS
-    uint32_t* p = s_k + (row * kPitch + 32 * j + kc) / 4;
+  auto keep = [&](int row, uint2 v) {  // a row's bytes into LDS
+    uint32_t* p = s_k + (row * kPitch + kc) / 4;
     p[0] = v.x;
     p[1] = v.y;
   };
-  if (krow < r1) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint2 v;
-      if (knew) {
-        v = q8_pack8<DT>(kx[j], kinv);
-      } else {
-        v = ko[j];
-        if (kcode > kold) v = make_uint2(q8_rescale(v.x, kdown), q8_rescale(v.y, kdown));
-      }
-      if (knew || kcode > kold) *reinterpret_cast<uint2*>(kp + 32 * j) = v;
-      if (windows) keep(16 + krow, j, v);
+  for (int j = 0; j < 4; ++j) {
+    if (krow + 16 * j >= r1) continue;
+    uint2 v;
+    if (knew(j)) {
+      v = q8_pack8<DT>(kx[j], kinv);
+    } else {
+      v = ko[j];
+      if (kcode > kold) v = make_uint2(q8_rescale(v.x, kdown), q8_rescale(v.y, kdown));
     }
+    if (knew(j) || kcode > kold) *reinterpret_cast<uint2*>(kp + 16 * kDim * j) = v;
+    if (windows) keep(16 + krow + 16 * j, v);
   }
 
   const bool lower = vcode > vold && is_old != 0;
@@ -326,17 +326,9 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
   uint32_t pcode = 1;
   if (complete(0)) {
     pcode = ks[sat - G];
-    if (krow >= 48) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        keep(krow - 48, j, *reinterpret_cast<const uint2*>(kp - (int64_t)G * kPageBytes + 32 * j));
-    }
+    keep(krow, *reinterpret_cast<const uint2*>(kp - (int64_t)G * kPageBytes + 48 * kDim));
   }
-  if (complete(4) && krow < 16) {
-    const float ninv = q8_pow(254 - (int)ncode);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) keep(80 + krow, j, q8_pack8<DT>(nx[j], ninv));
-  }
+  if (complete(4)) keep(80 + krow, q8_pack8<DT>(nx[0], q8_pow(254 - (int)ncode)));
   __syncthreads();
   // Halves in float32 in token order, four channels a thread (a half that no window needs
   // may be anything).
