@@ -528,6 +528,8 @@ class MiniCPMLeanSelect:
     def quantize_weights(self) -> "MiniCPMLeanSelect":
         """Replace the projections, the MLPs' weights and the head by 4-bit ones (the embedding,
         the norms and the selectors stay as they are)."""
+        if self.cfg.hidden_size % 8 or self.cfg.intermediate_size % 8:
+            raise ValueError("4-bit weights need hidden_size and intermediate_size multiples of 8")
         for L in self.layers:
             for name in ("w_qkv", "w_o", "w_gate_up", "w_down"):
                 if not isinstance(getattr(L, name), Mx4Weight):

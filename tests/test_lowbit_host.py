@@ -8,6 +8,7 @@ import torch
 
 from leanselect_amd import _hip, ops
 from leanselect_amd.cache import LeanSelectKVCache
+from leanselect_amd.minicpm import MiniCPMConfig, MiniCPMLeanSelect
 from leanselect_amd.ops import (dense_attention_kvcache_q8, kvcache_append_q8, linear_mx4,
                                 linear_mx4_silu_mul, new_kvcache_q8, quantize_mx4,
                                 sparse_attention_kvcache_q8)
@@ -289,6 +290,16 @@ def test_launches_are_made_on_the_tensors_device(monkeypatch, current):
     monkeypatch.setattr(_hip, "lib", lambda: Library)
     _hip.launch(1, "ls_linear_mx4", 7, None)
     assert seen == [(1, (7, None, 101))] and now == [current]
+
+
+@pytest.mark.parametrize("sizes", [dict(hidden_size=1028), dict(intermediate_size=2050)])
+def test_a_model_whose_sizes_do_not_fit_keeps_its_weights(sizes):
+    m = object.__new__(MiniCPMLeanSelect)
+    m.cfg, m.lm_head = MiniCPMConfig(**sizes), object()
+    m.layers, head = [], m.lm_head
+    with pytest.raises(ValueError, match="multiples of 8"):
+        m.quantize_weights()
+    assert m.lm_head is head
 
 
 def test_operators_are_public():
