@@ -107,6 +107,10 @@ struct Mx4Args {
 // the kernel at 1.8 TB/s of weights at 16 rows.  Four registers' exchange between the
 // quarters of the wave brings the pieces where the weights' order wants them.
 // A wave's next weights are loaded into the registers of each tile that it has used.
+//
+// Bound by the weights' bytes where there are many tiles (73448 x 4096, 16 rows: 38.9 us in eager
+// passes, 160 MB at 4.1 TB/s; one row 35.6), by a launch and one chain of load, product, LDS and
+// store where there are few (4608 x 4096, one row: 5.9 us, 10 MB).
 template <int DT, int MT, int RT, bool PAIR, int NW>
 __global__ __launch_bounds__(64 * NW) void ls_mx4_kernel(const Mx4Args args) {
   const uint16_t* __restrict__ x = args.x;
@@ -237,8 +241,11 @@ __global__ __launch_bounds__(64 * NW) void ls_mx4_kernel(const Mx4Args args) {
 // staged at a time, in two buffers: the four waves of a half load x as it lies (wave n the n-th
 // 64 bytes of each 256, four neighbouring lanes a row: 73448 x 4096, 64 rows 77 us; with a
 // row's four lanes 16 apart 84), and an operand is read back across the pieces, 256 contiguous
-// bytes for 16 lanes.  The halves are summed through LDS; with several slices float32 parts go to the
-// workspace, [slice][row][16 tiles], and a second kernel adds them in order.
+// bytes for 16 lanes.  The halves are summed through LDS; with several slices float32 parts go
+// to the workspace, [slice][row][16 tiles], and a second kernel adds them in order.
+//
+// 16384 outputs of gate and up, 4096 inputs: one row 14.9 us, 71 MB at 4.8 TB/s; 33 rows 21.6, the
+// reads of x from LDS and the matrix instructions adding some 3 us each.
 template <int DT, int MT, bool PAIR>
 __global__ __launch_bounds__(512) void ls_mx4_rows_kernel(const Mx4Args args) {
   const uint16_t* __restrict__ x = args.x;
@@ -378,7 +385,8 @@ __global__ __launch_bounds__(512) void ls_mx4_rows_kernel(const Mx4Args args) {
   }
 }
 
-// The slices' parts, added in order: a thread per four outputs of a row.
+// The slices' parts, added in order: a thread per four outputs of a row.  Bound by its launch (4096
+// outputs, 7 rows, 8 slices: 3.0 us for 1 MB).
 template <int DT, bool PAIR>
 __global__ __launch_bounds__(256) void ls_mx4_join_kernel(const float* __restrict__ part,
                                                           int64_t slices, int64_t m, int64_t tiles,
@@ -401,7 +409,8 @@ __global__ __launch_bounds__(256) void ls_mx4_join_kernel(const float* __restric
 // Laying out: a wave per tile of 16 outputs by 128 inputs, a lane per scale group.
 // The scale code is the least c >= 8 with max |w| <= 6 2^(c - 127) (127 for a group of
 // zeros), at most 252, as 6 2^125 is the last product that bf16 holds: only magnitudes above
-// it saturate.  Values go to the nearest E2M1 one, ties to the even code.
+// it saturate.  Values go to the nearest E2M1 one, ties to the even code.  Done once for a weight,
+// so it reads single elements of any row stride (32768 x 4096: 319 us, 1.1 TB/s).
 // ---------------------------------------------------------------------------
 template <int DT>
 __global__ __launch_bounds__(64) void ls_mx4_quantize_kernel(
@@ -437,7 +446,8 @@ __global__ __launch_bounds__(64) void ls_mx4_quantize_kernel(
   *reinterpret_cast<ls_u32x4*>(codes + ((nt * kc + chunk) * 64 + lane) * 16) = o;
 }
 
-// The weight's values in 16 bits (exact in bf16; rounded to fp16), rows of K.
+// The weight's values in 16 bits (exact in bf16; rounded to fp16), rows of K.  Bound by what it
+// writes (32768 x 4096: 72 us, 340 MB at 4.7 TB/s).
 template <int DT>
 __global__ __launch_bounds__(256) void ls_mx4_dequantize_kernel(
     const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t N, int64_t K,
@@ -483,7 +493,7 @@ struct Mx4Cut {
   int64_t blocks;    // of rows
 };
 
-// Measured with weights from memory (us; floor at 5.13 TB/s), outputs x inputs, rows:
+// Measured with weights from memory (us; a large copy reaches 4.9 to 5.1 TB/s), outputs x inputs, rows:
 //   waves and tiles a workgroup (8/1, 8/2, 4/4), one row: 4096 x 4096 5.2, 6.1, 9.0; 4608 x 4096
 //   6.9, 6.2, 9.1; 16384 x 4096 12.6, 11.5, 12.7; 73448 x 4096 47, 36.5, 35.3 (floor 31).  So
 //   eight waves up to 1024 tiles of the weight, one tile up to 256 (all workgroups in one round).
