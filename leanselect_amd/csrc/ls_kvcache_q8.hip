@@ -118,9 +118,10 @@ __device__ __forceinline__ int q8_find(int& unit, int batch, const int32_t* __re
 // Otherwise the first page is at rest and is read as it is.  So the windows need no second
 // launch: 3 to 5 us a call, against reading a prompt's keys twice.
 //
-// Bound by memory for prompts (32768 tokens of two heads: 12.6 us without windows, 50 MB at 4.0
-// TB/s, a copy of the same rows 12.2; 16.2 with them), by a launch and the chain of lengths,
-// rows, code and stores for a step (16 sequences, a token each: 6.2 us, 7.0 where windows end).
+// Bound by memory for prompts (32768 tokens of two heads: 12.8 us without windows, 50 MB at 3.9
+// TB/s, a copy of the same rows 12.1; 16.8 with them), by a launch and the chain of lengths,
+// rows, code and stores for a step (16 sequences, a token each: 5.1 us, 5.9 where windows end;
+// with conditional loads, each waited for before the next, 6.2 and 7.0).
 // ---------------------------------------------------------------------------
 // Eight 16-bit values as eight e4m3 bytes under a scale.
 template <int DT>
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
   const int64_t len = len_b, n0 = n0_b, n1 = min((int64_t)n1_b, total_new);
   const int64_t page = len / kPage + unit;
   const int64_t base = page * kPage, end = len + (n1 - n0);
-  if (page >= pages || base >= end) return;  // (the second: offsets past total_new)
+  if (page >= pages || base >= end || len >= end) return;  // (the later two: offsets past total_new)
   const int r0 = (int)max<int64_t>(0, len - base);  // the page's new rows: r0 <= row < r1
   const int r1 = (int)min<int64_t>(kPage, end - base);
   const int64_t at = (int64_t)b * cbs + (page * G + g) * kPageBytes;
@@ -216,29 +217,21 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
   ls_u32x4 kx[4], vx[4], nx[4];
   uint2 ko[4];
   uint32_t ktop = 0, vtop = 0, ntop = 0;
+  // Every load is made on one path, in front of the first wait: where a row is not new, a new
+  // one takes its place (it changes no maximum and is not written).
+  auto held = [&](int row) { return (int64_t)min(max(row, r0), r1 - 1) * nrs; };
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    kx[j] = knew(j) ? ls_load16(kn + first + (krow + 16 * j) * nrs + kc) : ls_u32x4{0u, 0u, 0u, 0u};
-    const bool vnew = tok + j >= r0 && tok + j < r1;
-    vx[j] = vnew ? ls_load16(vn + first + (tok + j) * nrs + 8 * oct) : ls_u32x4{0u, 0u, 0u, 0u};
-  }
-  if (complete(4)) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      nx[j] = krow + 16 * j < after ? ls_load16(kn + first + (kPage + krow + 16 * j) * nrs + kc)
-                                    : ls_u32x4{0u, 0u, 0u, 0u};
+    kx[j] = ls_load16(kn + first + held(krow + 16 * j) + kc);
+    vx[j] = ls_load16(vn + first + held(tok + j) + 8 * oct);
   }
   uint8_t* kp = k8 + at + krow * kDim + kc;
-  uint32_t kold = 1, vold = 1;
   if (r0 > 0) {
-    kold = ks[sat];
-    vold = vs[sat];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      ko[j] = krow + 16 * j < r0 ? *reinterpret_cast<const uint2*>(kp + 16 * kDim * j) : make_uint2(0, 0);
+    for (int j = 0; j < 4; ++j) ko[j] = *reinterpret_cast<const uint2*>(kp + 16 * kDim * j);
   }
   // Bytes of a V word that are new, and those that are older; the words as they are, where
-  // not all of a word is new.
+  // some of a word is new.  (Wholly older words are read later, if the page's code rises.)
   uint32_t is_new = 0, is_old = 0, vo[8];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -246,15 +239,25 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
     if (tok + j < r0) is_old |= 0xffu << (8 * j);
   }
   uint8_t* vp = v8 + at + (8 * oct) * kPage + 4 * quad;
-  if ((is_new | is_old) != 0 && is_new != 0xffffffffu) {
+  if (is_new != 0 && is_new != 0xffffffffu) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) vo[e] = *reinterpret_cast<const uint32_t*>(vp + e * kPage);
   }
+  uint32_t kold = ks[sat], vold = vs[sat];
+  if (r0 == 0) kold = vold = 1;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     ktop = q8_abs_max<DT>(kx[j], ktop);
     vtop = q8_abs_max<DT>(vx[j], vtop);
-    if (complete(4)) ntop = q8_abs_max<DT>(nx[j], ntop);
+  }
+  // The next page's keys after this page's have come: by then its own workgroup has read them
+  // (32768 tokens: 16.8 us, and 17.3 with these loads among the first).
+  if (complete(4)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      nx[j] = ls_load16(kn + first + (kPage + min(krow + 16 * j, after - 1)) * nrs + kc);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ntop = q8_abs_max<DT>(nx[j], ntop);
   }
   ktop = ls_wave_max_u32(ktop);
   vtop = ls_wave_max_u32(vtop);
@@ -297,7 +300,7 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
 
   const bool lower = vcode > vold && is_old != 0;
   const bool whole = r0 == 0 && r1 == kPage;
-  if (is_new != 0 || lower) {
+  if (is_new != 0) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float f[4];
@@ -314,6 +317,13 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
       else
         *reinterpret_cast<uint32_t*>(vp + e * kPage) = v;
     }
+  }
+  if (lower && is_new == 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) vo[e] = *reinterpret_cast<const uint32_t*>(vp + e * kPage);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      *reinterpret_cast<uint32_t*>(vp + e * kPage) = (q8_rescale(vo[e], vdown) & is_old) | (vo[e] & ~is_old);
   }
   if (whole) {  // through LDS, so that a wave writes whole lines
     __syncthreads();

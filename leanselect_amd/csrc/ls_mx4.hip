@@ -109,7 +109,7 @@ struct Mx4Args {
 // A wave's next weights are loaded into the registers of each tile that it has used.
 //
 // Bound by the weights' bytes where there are many tiles (73448 x 4096, 16 rows: 38.9 us in eager
-// passes, 160 MB at 4.1 TB/s; one row 35.6), by a launch and one chain of load, product, LDS and
+// passes, 160 MB at 4.1 TB/s; one row 33.2, 35.5 with conditional loads of x), by a launch and one chain of load, product, LDS and
 // store where there are few (4608 x 4096, one row: 5.9 us, 10 MB).
 template <int DT, int MT, int RT, bool PAIR, int NW>
 __global__ __launch_bounds__(64 * NW) void ls_mx4_kernel(const Mx4Args args) {
@@ -158,14 +158,19 @@ __global__ __launch_bounds__(64 * NW) void ls_mx4_kernel(const Mx4Args args) {
   const uint16_t* xrow[MT];
 #pragma unroll
   for (int c = 0; c < MT; ++c) xrow[c] = x + min(m0 + 16 * c + r, m - 1) * xrs;
+  // Rows past the last are the last again (not written); inputs past the last are zero, as only
+  // a wave's last group may have (`last`).  No load is conditional: it would be waited for
+  // where the paths meet.
   ls_u32x4 xr[MT][4];
-  auto load_x = [&](int64_t j, int i) {
+  auto load_x = [&](int64_t j, int i, auto last) {
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       const int64_t k = 512 * j + 128 * i + 32 * p + 8 * q;
 #pragma unroll
-      for (int c = 0; c < MT; ++c)
-        xr[c][p] = m0 + 16 * c + r < m && k < K ? ls_load16(xrow[c] + k) : ls_u32x4{0u, 0u, 0u, 0u};
+      for (int c = 0; c < MT; ++c) {
+        xr[c][p] = ls_load16(xrow[c] + (decltype(last)::value ? min(k, K - 8) : k));
+        if (decltype(last)::value && k >= K) xr[c][p] = ls_u32x4{0u, 0u, 0u, 0u};
+      }
     }
   };
   // 512 inputs whose weights are in registers (or on their way), with the loads of the wave's
@@ -186,9 +191,9 @@ __global__ __launch_bounds__(64 * NW) void ls_mx4_kernel(const Mx4Args args) {
         mx4_transpose(xf[c]);
       }
       if (i < 3)
-        load_x(j, i + 1);
+        load_x(j, i + 1, std::bool_constant<!kMore>());
       else if constexpr (kMore)
-        load_x(j + NW, 0);
+        load_x(j + NW, 0, std::true_type());
 #pragma unroll
       for (int a = 0; a < RT; ++a) {
         const float f = __uint_as_float(((s4[a] >> (8 * i)) & 0xffu) << 23);
@@ -206,7 +211,7 @@ __global__ __launch_bounds__(64 * NW) void ls_mx4_kernel(const Mx4Args args) {
   if (j < kc4) {
     load_s(j);
     load_w(j, 0);
-    load_x(j, 0);
+    load_x(j, 0, std::true_type());
 #pragma unroll
     for (int i = 1; i < 4; ++i) load_w(j, i);
     for (; j + NW < kc4; j += NW) group(j, std::true_type());
