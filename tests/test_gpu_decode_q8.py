@@ -298,6 +298,18 @@ def test_several_rows_a_sequence(sparse):
             assert bool((out[cu[-1]:] == 3.0).all())
 
 
+@pytest.mark.parametrize("max_len", [0, 1, 65, 1 << 40])
+@pytest.mark.parametrize("n_splits", [None, 1, 2, 7])
+def test_the_longest_length_only_cuts_the_work(max_len, n_splits):
+    lens, H, G = [1300, 1, 640], 16, 2
+    cache = _filled(lens, G, torch.bfloat16, 33)
+    q = torch.randn(3, H, D, generator=torch.Generator().manual_seed(34)).to(torch.bfloat16)
+    want, want_lse, bound = lo.attend(lo.Q8Cache(*cache), q, lens, [0, 1, 2, 3])
+    out, lse = dense_attention_kvcache_q8(q.to(DEV), *cache, _i32(lens), _i32([0, 1, 2, 3]), max_len,
+                                          n_splits=n_splits, return_lse=True)
+    _check(out, lse, want, want_lse, bound, torch.bfloat16)
+
+
 @pytest.mark.parametrize("sparse", [True, False])
 def test_more_sequences_than_a_wave(sparse):
     """Rows are found by search then; sequences without a row and rows behind the last one."""

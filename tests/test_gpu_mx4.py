@@ -154,6 +154,22 @@ def test_rows_do_not_depend_on_each_other():
     assert torch.equal(linear_mx4(x, codes, scales, n), alone)
 
 
+@pytest.mark.parametrize("n,k,m", [(40, 136, 3), (40, 1032, 20), (48, 8200, 3), (16384, 264, 18)])
+def test_an_infinity_among_the_last_inputs(n, k, m):
+    """The padding past the last input is no zero times infinity: an output is NaN only where the
+    infinite input meets a weight of zero."""
+    (codes, scales), w = _values(n, k, n + k)
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(m)).bfloat16()
+    x[1, k - 1], x[m - 1, k - 3] = math.inf, -math.inf
+    got, want = linear_mx4(x.to(DEV), codes, scales, n).cpu().double(), x.double() @ w.t()
+    for row in (1, m - 1):
+        assert torch.equal(torch.isnan(got[row]), torch.isnan(want[row]))
+        finite = ~torch.isnan(want[row])
+        assert torch.equal(got[row][finite], want[row][finite])  # infinities of the same sign
+    keep = [i for i in range(m) if i not in (1, m - 1)]
+    _check(linear_mx4(x.to(DEV), codes, scales, n)[keep], x[keep], w)
+
+
 def test_strided_rows_and_outputs():
     n, k, m = 50, 264, 6
     (codes, scales), _ = _values(n, k, 8)
