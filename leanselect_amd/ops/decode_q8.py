@@ -26,7 +26,6 @@ from operator import gt
 import torch
 
 from .. import _hip
-from .decode import _lengths, n_windows
 
 __all__ = ["new_kvcache_q8", "kvcache_append_q8", "sparse_attention_kvcache_q8",
            "dense_attention_kvcache_q8"]
@@ -36,6 +35,7 @@ _E4M3 = torch.float8_e4m3fn
 _CODES = {torch.bfloat16: _hip.LS_BF16, torch.float16: _hip.LS_F16}
 _PAGE_BYTES = PAGE * HEAD_DIM
 _MAX_SPLITS = 256
+_SCALE = HEAD_DIM ** -0.5
 _WORKGROUPS = 256
 
 
@@ -82,13 +82,6 @@ def _refuse_cache():
                      f"{PAGE}] and k_scale, v_scale uint8 [batch, pages, num_kv_heads]")
 
 
-def _rows16(t: torch.Tensor) -> bool:
-    """Rows ``[n, heads, 128]`` that the kernels read as they are: dense, 16-byte aligned."""
-    if t.data_ptr() % 16:
-        return False
-    return t.is_contiguous() or (t.stride()[1:] == (HEAD_DIM, 1) and t.stride(0) % 8 == 0)
-
-
 def kvcache_append_q8(k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
                       v_scale: torch.Tensor, cache_seqlens: torch.Tensor, k_new: torch.Tensor,
                       v_new: torch.Tensor, cu_seqlens_new: torch.Tensor, *,
@@ -101,46 +94,53 @@ def kvcache_append_q8(k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
     the compressed windows the new tokens complete: means of the 32 keys as the cache
     holds them.  ``cache_seqlens`` is left as it is (advance it after)."""
     B, P, G, cache_stride, scale_stride = _cache_dims(k8, v8, k_scale, v_scale)
-    if k_new.ndim != 3 or k_new.shape != (k_new.shape[0], G, HEAD_DIM) or v_new.shape != k_new.shape:
+    shape, dtype = k_new.shape, k_new.dtype
+    if len(shape) != 3 or shape[1] != G or shape[2] != HEAD_DIM or v_new.shape != shape:
         raise ValueError("k_new and v_new must be [total_new, num_kv_heads, head_dim] like the cache")
-    code = _CODES.get(k_new.dtype)
-    if code is None or v_new.dtype is not k_new.dtype:
+    code = _CODES.get(dtype)
+    if code is None or v_new.dtype is not dtype:
         raise ValueError("new keys/values must be bf16 or fp16, k and v alike")
-    total = k_new.shape[0]
-    lens = _lengths(cache_seqlens, cache_seqlens_host, "cache_seqlens")
-    cu = _lengths(cu_seqlens_new, cu_seqlens_new_host, "cu_seqlens_new")
-    if B < 1 or len(lens) != B or len(cu) != B + 1 or cu[0] != 0 or cu[-1] != total \
-            or cache_seqlens.numel() != B or cu_seqlens_new.numel() != B + 1:
+    total = shape[0]
+    if cache_seqlens.dtype is not torch.int32 or cu_seqlens_new.dtype is not torch.int32:
+        raise ValueError("cache_seqlens and cu_seqlens_new must be int32")
+    lens = cache_seqlens.tolist() if cache_seqlens_host is None else cache_seqlens_host
+    cu = cu_seqlens_new.tolist() if cu_seqlens_new_host is None else cu_seqlens_new_host
+    if B < 1 or cache_seqlens.shape != (B,) or cu_seqlens_new.shape != (B + 1,) \
+            or len(lens) != B or len(cu) != B + 1 or cu[0] != 0 or cu[-1] != total:
         raise ValueError("cache_seqlens must be [batch] and cu_seqlens_new [batch + 1] offsets "
                          "of the packed new rows")
     if B > 1 and (cache_stride < P * G * _PAGE_BYTES or scale_stride < P * G):
         raise ValueError("sequences that share pages cannot be appended to")
     after = [n + b - a for n, a, b in zip(lens, cu, cu[1:])]
-    if min(lens) < 0 or max(after) > P * PAGE or any(map(gt, lens, after)):
+    longest = max(after)
+    if min(lens) < 0 or longest > P * PAGE or any(map(gt, lens, after)):
         raise ValueError(f"sequences of {lens} tokens cannot become {after} in a cache with a "
                          f"capacity of {P * PAGE}")
     kc = (None, 0, 0, 0)
     if kc_cache is not None:
         if kernel_size != 32 or kernel_stride != 16:
             raise ValueError("the 8-bit cache forms windows of 32 keys at stride 16")
-        if kc_cache.ndim != 4 or kc_cache.dtype is not k_new.dtype or kc_cache.stride()[2:] != (HEAD_DIM, 1) \
-                or kc_cache.shape != (B, kc_cache.shape[1], G, HEAD_DIM):
+        kc_shape, kc_stride = kc_cache.shape, kc_cache.stride()
+        if len(kc_shape) != 4 or kc_shape[0] != B or kc_shape[2] != G or kc_shape[3] != HEAD_DIM \
+                or kc_stride[2] != HEAD_DIM or kc_stride[3] != 1 or kc_cache.dtype is not dtype:
             raise ValueError("kc_cache must be [batch, kc_capacity, num_kv_heads, head_dim] in "
                              "k_new's dtype with dense rows")
-        kc = (kc_cache.data_ptr(), kc_cache.stride(0), kc_cache.stride(1), kc_cache.shape[1])
-        if n_windows(max(after)) > kc[3]:
-            raise ValueError(f"{n_windows(max(after))} compressed windows exceed kc_capacity {kc[3]}")
+        if longest >= 32 and (longest - 32) // 16 + 1 > kc_shape[1]:
+            raise ValueError(f"{(longest - 32) // 16 + 1} compressed windows exceed kc_capacity "
+                             f"{kc_shape[1]}")
+        kc = (kc_cache.data_ptr(), kc_stride[0], kc_stride[1], kc_shape[1])
     index = _hip.gpu_index(k8, v8, k_scale, v_scale, cache_seqlens, k_new, v_new, cu_seqlens_new,
                            kc_cache)
     cache_seqlens, cu_seqlens_new = cache_seqlens.contiguous(), cu_seqlens_new.contiguous()
     # One row stride serves both: dense 16-byte aligned rows with equal strides, else copies.
-    if not (_rows16(k_new) and _rows16(v_new) and k_new.stride() == v_new.stride()):
+    row, k_ptr, v_ptr = k_new.stride(), k_new.data_ptr(), v_new.data_ptr()
+    if (k_ptr | v_ptr) & 15 or row[0] & 7 or row[1] != HEAD_DIM or row[2] != 1 or v_new.stride() != row:
         k_new = k_new.clone(memory_format=torch.contiguous_format)
         v_new = v_new.clone(memory_format=torch.contiguous_format)
+        row, k_ptr, v_ptr = (G * HEAD_DIM,), k_new.data_ptr(), v_new.data_ptr()
     _hip.launch(index, "ls_kvcache_append_q8", k8.data_ptr(), v8.data_ptr(), cache_stride,
-                k_scale.data_ptr(), v_scale.data_ptr(), scale_stride, P,
-                cache_seqlens.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0),
-                cu_seqlens_new.data_ptr(), total, B, G, HEAD_DIM, code, *kc)
+                k_scale.data_ptr(), v_scale.data_ptr(), scale_stride, P, cache_seqlens.data_ptr(),
+                k_ptr, v_ptr, row[0], cu_seqlens_new.data_ptr(), total, B, G, HEAD_DIM, code, *kc)
 
 
 def sparse_attention_kvcache_q8(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor,
@@ -176,10 +176,10 @@ def dense_attention_kvcache_q8(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tens
 def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, n_pages, causal,
             softmax_scale, n_splits, return_lse, out):
     B, P, G, cache_stride, scale_stride = _cache_dims(k8, v8, k_scale, v_scale)
-    code = _CODES.get(q.dtype)
-    if q.ndim != 3 or code is None:
+    code, q_shape = _CODES.get(q.dtype), q.shape
+    if code is None or len(q_shape) != 3:
         _refuse_queries(G)
-    total_q, H, cols = q.shape
+    total_q, H, cols = q_shape
     if cols != HEAD_DIM or H % G or not G <= H <= 16 * G:
         _refuse_queries(G)
     if cache_seqlens.dtype is not torch.int32 or cache_seqlens.shape != (B,) \
@@ -202,8 +202,10 @@ def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, 
         if topk_idx.dtype is not torch.int32 or not topk_idx.is_contiguous():
             topk_idx = topk_idx.to(torch.int32).contiguous()
         ids = topk_idx.data_ptr()
-    if not _rows16(q):
+    row, q_ptr = q.stride(), q.data_ptr()
+    if q_ptr & 15 or row[0] & 7 or row[1] != HEAD_DIM or row[2] != 1:  # rows the kernels do not read
         q = q.clone(memory_format=torch.contiguous_format)
+        row, q_ptr = (H * HEAD_DIM,), q.data_ptr()
     if n_splits is None:
         # Slices of a row: as many as leave every workgroup its compute unit, at least a page a
         # wave.  One slice (eight waves, no join) for few pages, and where the rows fill the
@@ -217,15 +219,16 @@ def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, 
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((H, total_q), dtype=torch.float32, device=q.device) if return_lse else None
-    # The slices' partial sums, maxima and weights: ls_attn_kvcache_q8_workspace_size.
-    floats = total_q * H * n_splits * (HEAD_DIM + 2) if n_splits > 1 else 0
-    ws = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
-    _hip.launch(index, "ls_attn_kvcache_q8", q.data_ptr(), q.stride(0),
-                cu_seqlens_q.data_ptr(), total_q, k8.data_ptr(), v8.data_ptr(), cache_stride,
-                k_scale.data_ptr(), v_scale.data_ptr(), scale_stride, P,
-                cache_seqlens.data_ptr(), B, H, G, HEAD_DIM, code, ids, n_pages,
-                HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale),
-                1 if causal else 0, n_splits, out.data_ptr(), _hip.ptr(lse), _hip.ptr(ws), 4 * floats)
+    # The slices' partial sums, maxima and weights, ls_attn_kvcache_q8_workspace_size bytes, counted
+    # in q's 16-bit elements (the cheapest tensor to make here).
+    nbytes = 4 * total_q * H * n_splits * (HEAD_DIM + 2) if n_splits > 1 else 0
+    ws = q.new_empty(nbytes >> 1) if nbytes else None
+    _hip.launch(index, "ls_attn_kvcache_q8", q_ptr, row[0], cu_seqlens_q.data_ptr(), total_q,
+                k8.data_ptr(), v8.data_ptr(), cache_stride, k_scale.data_ptr(), v_scale.data_ptr(),
+                scale_stride, P, cache_seqlens.data_ptr(), B, H, G, HEAD_DIM, code, ids, n_pages,
+                _SCALE if softmax_scale is None else float(softmax_scale), 1 if causal else 0,
+                n_splits, out.data_ptr(), lse.data_ptr() if return_lse else None,
+                ws.data_ptr() if nbytes else None, nbytes)
     return (out, lse) if return_lse else out
 
 
