@@ -109,8 +109,9 @@ def kvcache_append_q8(k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
             or len(lens) != B or len(cu) != B + 1 or cu[0] != 0 or cu[-1] != total:
         raise ValueError("cache_seqlens must be [batch] and cu_seqlens_new [batch + 1] offsets "
                          "of the packed new rows")
-    if B > 1 and (cache_stride < P * G * _PAGE_BYTES or scale_stride < P * G):
-        raise ValueError("sequences that share pages cannot be appended to")
+    if B > 1 and (cache_stride < P * G * _PAGE_BYTES or scale_stride < P * G
+                  or kc_cache is not None and kc_cache.stride(0) == 0):
+        raise ValueError("sequences that share pages or windows cannot be appended to")
     after = [n + b - a for n, a, b in zip(lens, cu, cu[1:])]
     longest = max(after)
     if min(lens) < 0 or longest > P * PAGE or any(map(gt, lens, after)):

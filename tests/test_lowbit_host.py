@@ -54,6 +54,7 @@ def test_well_formed_cpu_arguments_reach_the_device_check():
      "offsets"),
     (dict(cache=[t.expand(2, *t.shape[1:]) for t in new_kvcache_q8(1, 128, 2, device="cpu")]),
      "share pages"),
+    (dict(kc_cache=torch.zeros(1, 7, 2, 128, dtype=BF16).expand(2, 7, 2, 128)), "share pages or windows"),
     (dict(kc_cache=torch.zeros(2, 7, 2, 128)), "kc_cache"),
     (dict(kc_cache=torch.zeros(2, 7, 2, 64, dtype=BF16)), "kc_cache"),
     (dict(lens=_i32([100, 0]), kc_cache=torch.zeros(2, 4, 2, 128, dtype=BF16)), "kc_capacity"),
