@@ -19,6 +19,8 @@ No counterpart in the reference, whose projections are 16-bit.
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from .. import _hip
@@ -28,6 +30,7 @@ _CODES = {torch.bfloat16: _hip.LS_BF16, torch.float16: _hip.LS_F16}
 __all__ = ["quantize_mx4", "lay_out_mx4", "dequantize_mx4", "linear_mx4", "linear_mx4_silu_mul"]
 
 
+@lru_cache(maxsize=4096)
 def _shapes(out_features: int, in_features: int) -> tuple[tuple, tuple]:
     if out_features < 1 or in_features < 8 or in_features % 8:
         raise ValueError(f"need out_features >= 1 and in_features a multiple of 8 "
@@ -125,32 +128,37 @@ def linear_mx4_silu_mul(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tens
     return _linear(x, codes, scales, out_features, 1, out)
 
 
+@lru_cache(maxsize=4096)
+def _workspace_bytes(rows: int, k: int, out_features: int, silu: int) -> int:
+    return _hip.lib().ls_linear_mx4_workspace_size(rows, k, out_features, silu)
+
+
 def _linear(x, codes, scales, out_features, silu, out):
-    code = _CODES.get(x.dtype)
-    if x.ndim != 2 or code is None:
+    dtype, shape = x.dtype, x.shape
+    code = _CODES.get(dtype)
+    if code is None or len(shape) != 2:
         raise ValueError("x must be bf16 or fp16 [rows, in_features]")
-    rows, k = x.shape
+    rows, k = shape
     _check_weight(codes, scales, out_features, k)
     n = out_features // 2 if silu else out_features
     index = _hip.gpu_index(x, codes, scales, out)
     if out is None:
-        out = torch.empty(rows, n, dtype=x.dtype, device=x.device)
+        out = x.new_empty((rows, n))
         out_stride = n
     else:
-        if out.shape != (rows, n) or out.stride(1) != 1 or out.dtype is not x.dtype:
+        if out.shape != (rows, n) or out.stride(1) != 1 or out.dtype is not dtype:
             raise ValueError(f"out must be ({rows}, {n}) {x.dtype} with unit column stride, "
                              f"got {tuple(out.shape)} {out.dtype}")
         out_stride = out.stride(0)
         if rows > 1 and out_stride < n or out.data_ptr() == x.data_ptr() and rows:
             raise ValueError("out's rows must not overlap each other or x")
-    x_stride = k
-    if x.data_ptr() % 16 or not x.is_contiguous():
-        if x.data_ptr() % 16 or x.stride(1) != 1 or x.stride(0) % 8:
-            x = x.clone(memory_format=torch.contiguous_format)
-        x_stride = x.stride(0)
-    nbytes = _hip.lib().ls_linear_mx4_workspace_size(rows, k, out_features, silu)
-    ws = _hip.workspace(nbytes, x.device) if nbytes else None
-    _hip.launch(index, "ls_linear_mx4", x.data_ptr(), x_stride, rows, k, codes.data_ptr(),
+    x_stride, x_ptr = x.stride(), x.data_ptr()
+    if x_ptr & 15 or x_stride[1] != 1 or x_stride[0] & 7:  # rows the kernels do not read
+        x = x.clone(memory_format=torch.contiguous_format)
+        x_stride, x_ptr = (k,), x.data_ptr()
+    nbytes = _workspace_bytes(rows, k, out_features, silu)
+    ws = x.new_empty((nbytes + 1) >> 1) if nbytes else None  # counted in x's 16-bit elements
+    _hip.launch(index, "ls_linear_mx4", x_ptr, x_stride[0], rows, k, codes.data_ptr(),
                 scales.data_ptr(), out_features, silu, code, out.data_ptr(), out_stride,
-                _hip.ptr(ws), nbytes)
+                ws.data_ptr() if nbytes else None, nbytes)
     return out
