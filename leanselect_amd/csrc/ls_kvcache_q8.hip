@@ -118,8 +118,8 @@ __device__ __forceinline__ int q8_find(int& unit, int batch, const int32_t* __re
 // Otherwise the first page is at rest and is read as it is.  So the windows need no second
 // launch: 3 to 5 us a call, against reading a prompt's keys twice.
 //
-// Bound by memory for prompts (32768 tokens of two heads: 12.8 us without windows, 50 MB at 3.9
-// TB/s, a copy of the same rows 12.1; 16.8 with them), by a launch and the chain of lengths,
+// Bound by memory for prompts (32768 tokens of two heads: 12.7 us without windows, 50 MB at 4.0
+// TB/s, a copy of the same rows 12.1; 15.3 with them), by a launch and the chain of lengths,
 // rows, code and stores for a step (16 sequences, a token each: 5.1 us, 5.9 where windows end;
 // with conditional loads, each waited for before the next, 6.2 and 7.0).
 // ---------------------------------------------------------------------------
@@ -188,7 +188,11 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
   __shared__ uint32_t s_v[kDim * kVPitch / 4];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int g = blockIdx.y;
+  // Workgroups go to the eight compute dies in turn: of each 128 pages a die takes 16 in a row, so
+  // that the next page's keys are in its cache (32768 tokens 17.0 -> 15.5 us; a die's whole share
+  // in a row 15.9, and 131072 tokens 49.2 against 44.8).
   int unit = blockIdx.x, len_b, n0_b, n1_b;
+  if (unit < (int)(gridDim.x & ~127u)) unit = (unit & ~127) | (unit & 7) << 4 | (unit >> 3 & 15);
   const int b = q8_find(unit, batch, cache_seqlens, cu_new, len_b, n0_b, n1_b);
   if (b < 0) return;
   const int64_t len = len_b, n0 = n0_b, n1 = min((int64_t)n1_b, total_new);
@@ -250,22 +254,18 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
     ktop = q8_abs_max<DT>(kx[j], ktop);
     vtop = q8_abs_max<DT>(vx[j], vtop);
   }
-  // The next page's keys after this page's have come: by then its own workgroup has read them
-  // (32768 tokens: 16.8 us, and 17.3 with these loads among the first).
+  // The next page's keys after this page's have come: by then its own workgroup has read them.
+  // They are not looked at before this page is written (131072 tokens 44.8 -> 42.7 us).
   if (complete(4)) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       nx[j] = ls_load16(kn + first + (kPage + min(krow + 16 * j, after - 1)) * nrs + kc);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) ntop = q8_abs_max<DT>(nx[j], ntop);
   }
   ktop = ls_wave_max_u32(ktop);
   vtop = ls_wave_max_u32(vtop);
-  ntop = ls_wave_max_u32(ntop);
   if (lane == 0) {
     s_top[0][w] = ktop;
     s_top[1][w] = vtop;
-    s_top[2][w] = ntop;
   }
   __syncthreads();
   auto all_waves = [&](int i) { return max(max(s_top[i][0], s_top[i][1]), max(s_top[i][2], s_top[i][3])); };
@@ -325,8 +325,14 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
     for (int e = 0; e < 8; ++e)
       *reinterpret_cast<uint32_t*>(vp + e * kPage) = (q8_rescale(vo[e], vdown) & is_old) | (vo[e] & ~is_old);
   }
+  if (complete(4)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ntop = q8_abs_max<DT>(nx[j], ntop);
+    ntop = ls_wave_max_u32(ntop);
+    if (lane == 0) s_top[2][w] = ntop;
+  }
+  if (whole || complete(4)) __syncthreads();
   if (whole) {  // through LDS, so that a wave writes whole lines
-    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int u = 256 * i + tid, c = u >> 2;
