@@ -500,13 +500,13 @@ struct Mx4Cut {
 
 // Measured with weights from memory (us; a large copy reaches 4.9 to 5.1 TB/s), outputs x inputs, rows:
 //   waves and tiles a workgroup (8/1, 8/2, 4/4), one row: 4096 x 4096 5.2, 6.1, 9.0; 4608 x 4096
-//   6.9, 6.2, 9.1; 16384 x 4096 12.6, 11.5, 12.7; 73448 x 4096 47, 36.5, 35.3 (floor 31).  So
+//   6.9, 6.2, 9.1; 16384 x 4096 12.6, 11.5, 12.7; 73448 x 4096 47, 36.5, 33.3 (floor 31).  So
 //   eight waves up to 1024 tiles of the weight, one tile up to 256 (all workgroups in one round).
 //   ls_mx4_kernel, ls_mx4_rows_kernel, above 16 rows: 4608 x 4096, 40 rows 14.7, 13.1; [gate; up]
 //   32768 x 4096, 33 rows 33.9, 23.7 (floor 13.9); 4096 x 16384, 33 rows 37.8, 18.2; but 3000 x 600,
 //   24 rows 4.3, 5.7: the second for weights from 2 MB.  Up to 16 rows: [gate; up] 32768 x 4096, one
 //   row 18.6, 17.4, 16 rows 20.1, 17.6; 4096 x 16384, one row 15.0, 12.6, 16 rows 20.1, 13.7; but
-//   4608 x 4096, 16 rows 8.0, 9.7; 73448 x 4096, one row 35.3, 41.1: the second where its
+//   4608 x 4096, 16 rows 8.0, 9.7; 73448 x 4096, one row 33.3, 41.1: the second where its
 //   workgroups just fill the chip's 256 units without slices, or where the inputs are long and
 //   the tiles few.
 Mx4Cut mx4_cut(int64_t rows, int64_t K, int64_t N, bool silu) {
