@@ -502,13 +502,18 @@ struct Mx4Cut {
 //   waves and tiles a workgroup (8/1, 8/2, 4/4), one row: 4096 x 4096 5.2, 6.1, 9.0; 4608 x 4096
 //   6.9, 6.2, 9.1; 16384 x 4096 12.6, 11.5, 12.7; 73448 x 4096 47, 36.5, 33.3 (floor 31).  So
 //   eight waves up to 1024 tiles of the weight, one tile up to 256 (all workgroups in one round).
-//   ls_mx4_kernel, ls_mx4_rows_kernel, above 16 rows: 4608 x 4096, 40 rows 14.7, 13.1; [gate; up]
-//   32768 x 4096, 33 rows 33.9, 23.7 (floor 13.9); 4096 x 16384, 33 rows 37.8, 18.2; but 3000 x 600,
-//   24 rows 4.3, 5.7: the second for weights from 2 MB.  Up to 16 rows: [gate; up] 32768 x 4096, one
-//   row 18.6, 17.4, 16 rows 20.1, 17.6; 4096 x 16384, one row 15.0, 12.6, 16 rows 20.1, 13.7; but
-//   4608 x 4096, 16 rows 8.0, 9.7; 73448 x 4096, one row 33.3, 41.1: the second where its
-//   workgroups just fill the chip's 256 units without slices, or where the inputs are long and
-//   the tiles few.
+//   ls_mx4_kernel, ls_mx4_rows_kernel (with slices: a second launch, 4 us more of the host), above
+//   16 rows: 4096 x 2048, 17 rows 5.3, 8.4, 64 rows 9.8, 12.3; 4096 x 4096, 17 rows 8.0, 10.3, 32
+//   rows 10.5, 11.1, 33 rows 13.2, 12.4, 64 rows 17.7, 14.6; 2048 x 8192, 17 rows 12.5, 9.9, 32 rows
+//   17.2, 10.4; [gate; up] 32768 x 4096, 33 rows 33.9, 23.7 (floor 13.9).  The first takes as long
+//   as its rounds of 256 workgroups and the inputs each walks: up to 4096 inputs in one round or
+//   2048 in two.  Without slices the second is as cheap to launch: 32768 x 1024, 33 rows 15.3,
+//   10.4; 8192 x 1024, 17 rows (one round) 4.8, 6.4.
+//   Up to 16 rows: [gate; up] 32768 x 4096, one row 18.6, 17.4, 16 rows 20.1, 17.6; 4608 x 4096,
+//   16 rows 8.0, 9.7; 73448 x 4096, one row 33.3, 41.1: the second where its workgroups just fill
+//   the chip's 256 units without slices.  And where inputs are long and tiles few, by rows:
+//   1024 x 16384, one row 11.7, 8.6; 1024 x 12288, one row 9.2, 8.5, 8 rows 10.6, 9.1, 16 rows 14.0,
+//   9.1; 1024 x 8192, one row 6.3, 6.9, 8 rows 7.3, 7.2, 16 rows 9.6, 7.4.
 Mx4Cut mx4_cut(int64_t rows, int64_t K, int64_t N, bool silu) {
   Mx4Cut c;
   const int64_t tiles = (N + 15) / 16;  // of the weight
@@ -524,8 +529,10 @@ Mx4Cut mx4_cut(int64_t rows, int64_t K, int64_t N, bool silu) {
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(c.kc4 / 2, 256 / wgs));
   c.per_half = (c.kc4 + 2 * want - 1) / (2 * want);
   c.slices = (c.kc4 + 2 * c.per_half - 1) / (2 * c.per_half);
-  c.shared = rows > 16 ? tiles * c.kc >= 2048
-                       : (c.slices == 1 && wgs > 128 && wgs <= 256) || (c.kc4 >= 16 && tiles <= 256);
+  const int64_t rounds = ((tiles + c.rt - 1) / c.rt * ((rows + 31) / 32) + 255) / 256;
+  c.shared = rows > 16 ? K * rounds > 4096 || (c.slices == 1 && rounds > 1)
+                       : (c.slices == 1 && wgs > 128 && wgs <= 256) ||
+                             (tiles <= 256 && c.kc4 * (rows + 16) >= 544);
   if (!c.shared && c.mt > 2) {  // few tiles and many rows: blocks of 32, their registers bound the waves
     c.mt = 2;
     c.blocks = (rows + 31) / 32;

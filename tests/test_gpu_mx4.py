@@ -114,7 +114,8 @@ def test_silu_mul(dtype, inter, k, m):
     (16400, 128, 17), (16390, 120, 70),    # the same, 32 rows a workgroup
     (16640, 512, 1), (32768, 264, 5),      # shared rows, one slice
     (48, 8200, 3), (2048, 8192, 40),       # shared rows, slices and their join
-    (2048, 2056, 130)])
+    (2048, 2056, 130), (48, 16400, 3), (100, 12296, 15),
+    (4096, 2056, 33), (16384, 1032, 40), (40, 4104, 20)])
 def test_linear_in_each_form(n, k, m):
     (codes, scales), w = _values(n, k, n + 2 * k + m)
     x = torch.randn(m, k, generator=torch.Generator().manual_seed(m)).bfloat16()
@@ -122,7 +123,8 @@ def test_linear_in_each_form(n, k, m):
 
 
 @pytest.mark.parametrize("n,k,m", [(16896, 128, 2), (16896, 120, 40), (32800, 72, 16), (20480, 512, 1),
-                                   (2048, 8200, 5), (2048, 2056, 33)])
+                                   (2048, 8200, 5), (2048, 2056, 33), (2048, 16392, 5),
+                                   (512, 4104, 17)])
 def test_silu_mul_in_each_form(n, k, m):
     (codes, scales), w = _values(n, k, n + 3 * k + m, 112, 122)
     x = torch.randn(m, k, generator=torch.Generator().manual_seed(m)).bfloat16()
@@ -154,7 +156,7 @@ def test_rows_do_not_depend_on_each_other():
     assert torch.equal(linear_mx4(x, codes, scales, n), alone)
 
 
-@pytest.mark.parametrize("n,k,m", [(40, 136, 3), (40, 1032, 20), (48, 8200, 3), (16384, 264, 18)])
+@pytest.mark.parametrize("n,k,m", [(40, 136, 3), (40, 1032, 20), (48, 8200, 3), (16384, 264, 18), (48, 16392, 3)])
 def test_an_infinity_among_the_last_inputs(n, k, m):
     """The padding past the last input is no zero times infinity: an output is NaN only where the
     infinite input meets a weight of zero."""
