@@ -209,12 +209,13 @@ def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, 
         row, q_ptr = (H * HEAD_DIM,), q.data_ptr()
     if n_splits is None:
         # Slices of a row: as many as leave every workgroup its compute unit, at least a page a
-        # wave.  One slice (eight waves, no join) for few pages, and where the rows fill the
-        # device meanwhile (us, one slice and several: 1000 keys, 1 row 9.5, 8.5 and a launch
-        # more, 16 rows 9.5, 10.2; 4000 keys, 40 rows 24.3, 21.8, 56 rows 24.7, 27.7).  More
-        # workgroups than units: 48 rows of 4000 keys in 2 slices 24.1, in 3 slices 30.4.
+        # wave.  One slice (eight waves, no join) up to three pages a wave, a launch less for the
+        # host (us, replayed and called, one slice and several: 1 row of 16 pages 9.6 / 11.5, 9.2 /
+        # 16.2, of 24 pages 11.9 / 12.1, 9.3 / 16.0, of 32 pages 14.1 / 14.2, 9.2 / 15.6); and where
+        # the rows fill the device meanwhile (replayed: 4000 keys, 40 rows 24.3, 21.8, 56 rows
+        # 24.7, 27.7).  More workgroups than units: 48 rows of 4000 keys in 2 slices 24.1, in 3 30.4.
         pairs = total_q * G
-        n_splits = 1 if n_pages <= max(16, 2 * pairs // 3) \
+        n_splits = 1 if n_pages <= max(24, 2 * pairs // 3) \
             else min(-(-n_pages // 4), _WORKGROUPS // max(1, pairs))
     n_splits = max(1, min(int(n_splits), _MAX_SPLITS))
     if out is None:
