@@ -414,24 +414,42 @@ __global__ __launch_bounds__(256) void ls_mx4_join_kernel(const float* __restric
 // Laying out: a wave per tile of 16 outputs by 128 inputs, a lane per scale group.
 // The scale code is the least c >= 8 with max |w| <= 6 2^(c - 127) (127 for a group of
 // zeros), at most 252, as 6 2^125 is the last product that bf16 holds: only magnitudes above
-// it saturate.  Values go to the nearest E2M1 one, ties to the even code.  Done once for a weight,
-// so it reads single elements of any row stride (32768 x 4096: 319 us, 1.1 TB/s).
+// it saturate.  Values go to the nearest E2M1 one, ties to the even code.  ALIGNED: rows in
+// pieces of 16 bytes (all of a piece's eight inputs exist or none), else single elements.
+// Bound by memory (32768 x 4096 bf16: 86 us, 340 MB at 4.0 TB/s; single elements 319).
 // ---------------------------------------------------------------------------
-template <int DT>
-__global__ __launch_bounds__(64) void ls_mx4_quantize_kernel(
+template <int DT, bool ALIGNED>
+__global__ __launch_bounds__(256) void ls_mx4_quantize_kernel(
     const typename LsElem<DT>::T* __restrict__ w, int64_t wrs, int64_t N, int64_t K, int64_t kc,
     int64_t kc4, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const int64_t at = blockIdx.x;  // nt * 4 kc4 + chunk, chunks rounded up to whole scale words
-  const int64_t nt = at / (4 * kc4), chunk = at - nt * 4 * kc4;
-  const int lane = threadIdx.x;
+  const int64_t nt = blockIdx.x / kc4, group = blockIdx.x - nt * kc4;  // a wave a chunk of the group
+  const int64_t chunk = 4 * group + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
   const int64_t row = 16 * nt + (lane & 15), k0 = 128 * chunk + 32 * (lane >> 4);
   float v[32];
   float top = 0.f;
+  if constexpr (ALIGNED) {
+    constexpr int kBytes = sizeof(typename LsElem<DT>::T), kEach = 16 / kBytes;  // inputs a load
+    const auto* wr = w + min(row, N - 1) * wrs;
+    ls_u32x4 x[32 / kEach];
 #pragma unroll
-  for (int e = 0; e < 32; ++e) {
-    v[e] = row < N && k0 + e < K ? LsElem<DT>::to_f(w[row * wrs + k0 + e]) : 0.f;
-    top = fmaxf(top, fabsf(v[e]));
+    for (int p = 0; p < 32 / kEach; ++p) x[p] = ls_load16(wr + min(k0 + kEach * p, K - kEach));
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      const uint32_t u = x[e / kEach][e % kEach * kBytes / 4];
+      if constexpr (kBytes == 4)
+        v[e] = __uint_as_float(u);
+      else
+        v[e] = LsElem<DT>::to_f((uint16_t)(e & 1 ? u >> 16 : u & 0xffffu));
+      if (row >= N || k0 + e >= K) v[e] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      v[e] = row < N && k0 + e < K ? LsElem<DT>::to_f(w[row * wrs + k0 + e]) : 0.f;
   }
+#pragma unroll
+  for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(v[e]));
   const uint32_t bits = __float_as_uint(top);
   // 6 = 1.5 2^2.
   int c = (int)(bits >> 23) - 2 + ((bits & 0x7fffffu) > 0x400000u ? 1 : 0);
@@ -639,13 +657,17 @@ extern "C" int ls_quantize_mx4(const void* weight, int64_t weight_row_stride, in
   LS_REQUIRE(ls_aligned16(codes), LS_ERR_UNSUPPORTED, "%s: codes must be 16-byte aligned", who);
   const int64_t tiles = (out_features + 15) / 16, kc = (in_features + 127) / 128, kc4 = (kc + 3) / 4;
   LS_REQUIRE(tiles * 4 * kc4 <= 0x7fffffffLL, LS_ERR_UNSUPPORTED, "%s: weight too large", who);
-  auto launch = [&](auto dt) {
+  auto run = [&](auto dt, auto aligned) {
     constexpr int DT = decltype(dt)::value;
-    hipLaunchKernelGGL(ls_mx4_quantize_kernel<DT>, dim3((unsigned)(tiles * 4 * kc4)), dim3(64), 0,
-                       (hipStream_t)stream, (const typename LsElem<DT>::T*)weight,
-                       weight_row_stride, out_features, in_features, kc, kc4, (uint8_t*)codes,
-                       (uint8_t*)scales);
+    hipLaunchKernelGGL((ls_mx4_quantize_kernel<DT, decltype(aligned)::value>),
+                       dim3((unsigned)(tiles * kc4)), dim3(256), 0, (hipStream_t)stream,
+                       (const typename LsElem<DT>::T*)weight, weight_row_stride, out_features,
+                       in_features, kc, kc4, (uint8_t*)codes, (uint8_t*)scales);
     return ls_check_launch("ls_mx4_quantize_kernel");
+  };
+  auto launch = [&](auto dt) {
+    return ls_aligned16(weight) && weight_row_stride % 8 == 0 ? run(dt, std::true_type())
+                                                              : run(dt, std::false_type());
   };
   if (dtype == LS_F32) return launch(std::integral_constant<int, LS_F32>());
   return dtype == LS_BF16 ? launch(std::integral_constant<int, LS_BF16>())

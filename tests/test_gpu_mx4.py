@@ -70,6 +70,18 @@ def test_quantize_is_the_definition_byte_for_byte(dtype, n, k):
     assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,k", [(1, 8), (19, 136), (33, 1048)])
+def test_quantize_reads_rows_of_any_place_and_stride(dtype, n, k):
+    w = _weight(n, k, n + k).to(dtype).to(DEV)
+    want = quantize_mx4(w)
+    for at, cols in ((0, k), (1, k + 1), (3, k + 8), (8, k + 8), (4, k + 4), (0, k + 5)):
+        wide = torch.full((n, at + cols), math.nan, dtype=dtype, device=DEV)
+        wide[:, at:at + k] = w
+        got = quantize_mx4(wide[:, at:at + k])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (at, cols)
+
+
 @pytest.mark.parametrize("n,k", [(1, 8), (17, 136), (40, 520)])
 def test_dequantize_gives_the_values(n, k):
     (codes, scales), w = _values(n, k, n + k, 8, 252)
