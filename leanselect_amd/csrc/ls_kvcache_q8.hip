@@ -792,17 +792,18 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
 // out[t][g*gs + h] = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s; a row that sees no key gives
 // zeros and lse = +inf.  A workgroup per (row, KV head, query head): each wave forms the maximum
 // and sum of all slices (at most four a lane), then thread (p, c) sums four channels of every
-// eighth slice, and the eight parts are added in LDS in order.  The first slices' values are
+// P-th slice, and the P parts are added in LDS in order.  The first 8 P slices' values are
 // loaded with the maxima (a slice of sum 0 may hold anything and is left out).  Bound by its launch
-// and the two reads of its chain: 3.5 us for 16 slices of a row, 3.9 for 128.
-template <int DT>
-__global__ __launch_bounds__(256) void ls_q8_join_kernel(const Q8AttnArgs args) {
+// and the reads of its chain: 3.5 us for 16 slices of a row; P = 8 up to 64 slices, 16 above (131071
+// keys in 128 slices, with the attention: 19.0 us, and 19.5 with P = 8).
+template <int DT, int P>
+__global__ __launch_bounds__(32 * P) void ls_q8_join_kernel(const Q8AttnArgs args) {
   const Q8Part part = args.part;
   const int64_t total_q = args.total_q;
   const int gs = args.gs, n = args.n_splits;
   constexpr int kAhead = 8;
   __shared__ float s_w[LS_Q8_MAX_SPLITS];
-  __shared__ ls_f32x4 s_a[8][32];
+  __shared__ ls_f32x4 s_a[P][32];
   const int64_t t = blockIdx.x;
   const int g = blockIdx.y, h = blockIdx.z, G = gridDim.y;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -821,7 +822,7 @@ __global__ __launch_bounds__(256) void ls_q8_join_kernel(const Q8AttnArgs args) 
   ls_f32x4 ahead[kAhead];
 #pragma unroll
   for (int k = 0; k < kAhead; ++k)
-    ahead[k] = *reinterpret_cast<const ls_f32x4*>(po + (int64_t)min(p + 8 * k, n - 1) * gs * kDim);
+    ahead[k] = *reinterpret_cast<const ls_f32x4*>(po + (int64_t)min(p + P * k, n - 1) * gs * kDim);
   if (t >= args.cu_q[args.batch]) return;  // a row behind the last sequence
 #pragma unroll
   for (int k = 0; k < 4; ++k) M = fmaxf(M, ms[k]);
@@ -844,17 +845,17 @@ __global__ __launch_bounds__(256) void ls_q8_join_kernel(const Q8AttnArgs args) 
   ls_f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < kAhead; ++k) {
-    const float wt = p + 8 * k < n ? s_w[p + 8 * k] : 0.f;
+    const float wt = p + P * k < n ? s_w[p + P * k] : 0.f;
     if (wt != 0.f) a += wt * ahead[k];
   }
-  for (int s0 = p + 8 * kAhead; s0 < n; s0 += 8 * kAhead) {
+  for (int s0 = p + P * kAhead; s0 < n; s0 += P * kAhead) {
     ls_f32x4 x[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      x[k] = *reinterpret_cast<const ls_f32x4*>(po + (int64_t)min(s0 + 8 * k, n - 1) * gs * kDim);
+      x[k] = *reinterpret_cast<const ls_f32x4*>(po + (int64_t)min(s0 + P * k, n - 1) * gs * kDim);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const float wt = s0 + 8 * k < n ? s_w[s0 + 8 * k] : 0.f;
+      const float wt = s0 + P * k < n ? s_w[s0 + P * k] : 0.f;
       if (wt != 0.f) a += wt * x[k];
     }
   }
@@ -863,7 +864,7 @@ __global__ __launch_bounds__(256) void ls_q8_join_kernel(const Q8AttnArgs args) 
   if (tid < 32) {
     a = s_a[0][c];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) a += s_a[i][c];
+    for (int i = 1; i < P; ++i) a += s_a[i][c];
     const float inv = L == 0.f ? 0.f : 1.f / L;
     uint2 x;
     x.x = ls_pack2(LsElem<DT>::from_f(a[0] * inv), LsElem<DT>::from_f(a[1] * inv));
@@ -997,9 +998,13 @@ extern "C" int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int
   const int rc = dtype == LS_BF16 ? by_plan(std::integral_constant<int, LS_BF16>())
                                   : by_plan(std::integral_constant<int, LS_F16>());
   if (rc || splits == 1) return rc;
-  auto join = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)total_q, num_kv_heads, gs), dim3(256), 0, s, args);
+  auto join = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)total_q, num_kv_heads, gs), dim3(threads), 0, s, args);
     return ls_check_launch("ls_q8_join_kernel");
   };
-  return dtype == LS_BF16 ? join(ls_q8_join_kernel<LS_BF16>) : join(ls_q8_join_kernel<LS_F16>);
+  if (splits > 64)
+    return dtype == LS_BF16 ? join(ls_q8_join_kernel<LS_BF16, 16>, 512)
+                            : join(ls_q8_join_kernel<LS_F16, 16>, 512);
+  return dtype == LS_BF16 ? join(ls_q8_join_kernel<LS_BF16, 8>, 256)
+                          : join(ls_q8_join_kernel<LS_F16, 8>, 256);
 }
