@@ -382,8 +382,9 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
 // several slices, partial results go to the workspace and a second kernel joins them.
 // Row i of sequence b sees keys j < len_b, or j <= len_b - len_q(b) + i (causal).
 // K's bytes become the query's type (exact) for S^T = K Q^T, V's become fp16 (exact) for
-// O^T = V^T P^T with P <= 1 rounded to fp16 (2^-12 of each weight; the sum of the weights
-// is taken of the rounded ones, so the result is an exact mean with those weights).
+// O^T = V^T P^T with P <= 1 as an fp16 head and an fp16 remainder, a product of each: 22 bits
+// of a weight, 2^-25 of the largest where the head is subnormal.  (The head alone holds 11: its
+// error, 2^-11 of a weight, passes a bf16 output's own rounding where values nearly cancel.)
 // A page's powers of two go into the scores' scale and into the sum of O.
 //
 // A wave takes ppw plan slots, or (DENSE) pages, or more of a row that is longer than the
@@ -684,15 +685,17 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
     const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
     m_run = m_new;
     l_run *= alpha;
-    ls_u32x4 pf[2];
+    ls_u32x4 ph[2], pl[2];  // heads and remainders of the weights
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint16_t h0 = ls_f32_to_f16(__builtin_amdgcn_exp2f(sv[8 * c + 2 * e] - m_new));
-        const uint16_t h1 = ls_f32_to_f16(__builtin_amdgcn_exp2f(sv[8 * c + 2 * e + 1] - m_new));
-        l_run += ls_f16_to_f32(h0) + ls_f16_to_f32(h1);
-        pf[c][e] = ls_pack2(h0, h1);
+        const float p0 = __builtin_amdgcn_exp2f(sv[8 * c + 2 * e] - m_new);
+        const float p1 = __builtin_amdgcn_exp2f(sv[8 * c + 2 * e + 1] - m_new);
+        const uint16_t h0 = ls_f32_to_f16(p0), h1 = ls_f32_to_f16(p1);
+        ph[c][e] = ls_pack2(h0, h1);
+        pl[c][e] = ls_pack2(ls_f32_to_f16(p0 - ls_f16_to_f32(h0)), ls_f32_to_f16(p1 - ls_f16_to_f32(h1)));
+        l_run += p0 + p1;
       }
     auto weigh = [&](ls_u32x4 (&vf)[8], uint32_t code) {
       if (part_page) {
@@ -707,9 +710,13 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
       const float vscale = q8_pow(code);
 #pragma unroll
       for (int db = 0; db < 8; ++db) {
+        const ls_u32x4 v0 = q8_expand<LS_F16>(vf[db][0], vf[db][1]);
+        const ls_u32x4 v1 = q8_expand<LS_F16>(vf[db][2], vf[db][3]);
         ls_f32x4 pv = {0.f, 0.f, 0.f, 0.f};
-        pv = LsElem<LS_F16>::mfma(q8_expand<LS_F16>(vf[db][0], vf[db][1]), pf[0], pv);
-        pv = LsElem<LS_F16>::mfma(q8_expand<LS_F16>(vf[db][2], vf[db][3]), pf[1], pv);
+        pv = LsElem<LS_F16>::mfma(v0, ph[0], pv);
+        pv = LsElem<LS_F16>::mfma(v1, ph[1], pv);
+        pv = LsElem<LS_F16>::mfma(v0, pl[0], pv);
+        pv = LsElem<LS_F16>::mfma(v1, pl[1], pv);
         o[db] = o[db] * alpha + pv * vscale;
       }
     };
