@@ -382,9 +382,11 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
 // several slices, partial results go to the workspace and a second kernel joins them.
 // Row i of sequence b sees keys j < len_b, or j <= len_b - len_q(b) + i (causal).
 // K's bytes become the query's type (exact) for S^T = K Q^T, V's become fp16 (exact) for
-// O^T = V^T P^T with P <= 1 as an fp16 head and an fp16 remainder, a product of each: 22 bits
-// of a weight, 2^-25 of the largest where the head is subnormal.  (The head alone holds 11: its
-// error, 2^-11 of a weight, passes a bf16 output's own rounding where values nearly cancel.)
+// O^T = V^T P^T with 2^15 P <= 2^15 as an fp16 head and an fp16 remainder, a product of each: 22
+// bits of a weight, 2^-40 of the largest where the head or the remainder is subnormal.  (The
+// head alone holds 11: its error, 2^-11 of a weight, passes a bf16 output's own rounding where
+// values nearly cancel.  Unscaled, weights below 2^-25 of the largest would vanish, and a row of
+// 100000 of them with it.)
 // A page's powers of two go into the scores' scale and into the sum of O.
 //
 // A wave takes ppw plan slots, or (DENSE) pages, or more of a row that is longer than the
@@ -684,7 +686,7 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
     const float m_new = fmaxf(m_run, pm);
     const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
     m_run = m_new;
-    l_run *= alpha;
+    float sum = 0.f;  // of the page alone first: small weights would be lost beside a large sum
     ls_u32x4 ph[2], pl[2];  // heads and remainders of the weights
 #pragma unroll
     for (int c = 0; c < 2; ++c)
@@ -692,11 +694,13 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
       for (int e = 0; e < 4; ++e) {
         const float p0 = __builtin_amdgcn_exp2f(sv[8 * c + 2 * e] - m_new);
         const float p1 = __builtin_amdgcn_exp2f(sv[8 * c + 2 * e + 1] - m_new);
-        const uint16_t h0 = ls_f32_to_f16(p0), h1 = ls_f32_to_f16(p1);
+        sum += p0 + p1;
+        const float u0 = p0 * 0x1p15f, u1 = p1 * 0x1p15f;
+        const uint16_t h0 = ls_f32_to_f16(u0), h1 = ls_f32_to_f16(u1);
         ph[c][e] = ls_pack2(h0, h1);
-        pl[c][e] = ls_pack2(ls_f32_to_f16(p0 - ls_f16_to_f32(h0)), ls_f32_to_f16(p1 - ls_f16_to_f32(h1)));
-        l_run += p0 + p1;
+        pl[c][e] = ls_pack2(ls_f32_to_f16(u0 - ls_f16_to_f32(h0)), ls_f32_to_f16(u1 - ls_f16_to_f32(h1)));
       }
+    l_run = l_run * alpha + sum;
     auto weigh = [&](ls_u32x4 (&vf)[8], uint32_t code) {
       if (part_page) {
 #pragma unroll
@@ -707,7 +711,7 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
           for (int db = 0; db < 8; ++db) vf[db][kb] &= keep;
         }
       }
-      const float vscale = q8_pow(code);
+      const float vscale = q8_pow(code) * 0x1p-15f;
 #pragma unroll
       for (int db = 0; db < 8; ++db) {
         const ls_u32x4 v0 = q8_expand<LS_F16>(vf[db][0], vf[db][1]);

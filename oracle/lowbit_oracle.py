@@ -99,8 +99,8 @@ def attend(cache: Q8Cache, q, lens, cu_q, ids=None, causal=False, scale=None):
     """``(out, lse, bound)`` of decode rows over the cache; rows past ``cu_q[-1]`` NaN.
 
     ``bound`` is what the kernel's own roundings may move an output by, before its rounding
-    to 16 bits: weights held as an fp16 head and remainder (2^-22 of each, or 2^-25 of the
-    largest where the head is subnormal), scores formed in float32, and float32 sums (a page
+    to 16 bits: weights held as an fp16 head and remainder (2^-22 of each, or 2^-40 of the
+    largest where either is subnormal), scores formed in float32, and float32 sums (a page
     of 64 keys an addition, the joins' beside)."""
     total, H, _ = q.shape
     G = cache.k.shape[2]
@@ -130,7 +130,7 @@ def attend(cache: Q8Cache, q, lens, cu_q, ids=None, causal=False, scale=None):
                 size = (x.abs() @ k.abs().t() * abs(scale)).amax(-1, keepdim=True)
                 e = 2.0 ** -22 + 2.0 ** -17 * size + 2.0 ** -22 * (1 + s.abs().amax(-1, keepdim=True)) \
                     + 2.0 ** -24 * (len(keep) / PAGE + PAGE)
-                lost = 2 * len(keep) * 2.0 ** -25 * p.amax(-1, keepdim=True)
+                lost = 2 * len(keep) * 2.0 ** -40 * p.amax(-1, keepdim=True)
                 bound[t, rows] = 2 * e * (p @ v.abs()) + lost * v.abs().amax(0)
     return out, lse, bound
 

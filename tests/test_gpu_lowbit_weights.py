@@ -53,3 +53,29 @@ def test_two_values_that_nearly_cancel(dtype, n, first, second):
         out, lse = sparse_attention_kvcache_q8(q.to(DEV), *cache, _i32([n]), ids, _i32([0, rows]),
                                                softmax_scale=1.0, n_splits=n_splits, return_lse=True)
         _check(out, lse, want, want_lse, bound, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("at", [0, 700, 16383])
+def test_many_keys_far_below_one(dtype, at):
+    """A key that draws nearly all the weight and whose value is 0, among 16383 keys 20 to 30 bits
+    below it: the output is theirs alone, so what is lost of their weights is lost of it."""
+    n, H = 16384, 16
+    keys = torch.zeros(n)
+    keys[at] = 20.0
+    g = torch.Generator().manual_seed(40)
+    v = (torch.randint(8, 16, (n, 1, D), generator=g) / 8.0)
+    v[at] = 0.0
+    cache, ref = _one_channel_keys(keys, v, dtype)
+    q = torch.zeros(1, H, D)
+    q[0, :, 0] = (88 + 3 * torch.arange(H)) / 128.0  # scores of 13.75 to 20.8
+    q = q.to(dtype)
+    want, want_lse, bound = lo.attend(ref, q, [n], [0, 1], scale=1.0)
+    ids = torch.arange(256, dtype=torch.int32, device=DEV).view(1, 1, 256)
+    for n_splits in (1, 7, None):
+        out, lse = dense_attention_kvcache_q8(q.to(DEV), *cache, _i32([n]), _i32([0, 1]), n,
+                                              softmax_scale=1.0, n_splits=n_splits, return_lse=True)
+        _check(out, lse, want, want_lse, bound, dtype)
+        out, lse = sparse_attention_kvcache_q8(q.to(DEV), *cache, _i32([n]), ids, _i32([0, 1]),
+                                               softmax_scale=1.0, n_splits=n_splits, return_lse=True)
+        _check(out, lse, want, want_lse, bound, dtype)
