@@ -290,7 +290,8 @@ __global__ __launch_bounds__(512) void ls_mx4_rows_kernel(const Mx4Args args) {
 #pragma unroll
     for (int c = 0; c < MT; ++c) acc[a][c] = ls_f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // Past the half's end weights are those of the last group, and x is zero.
+  // Past the half's end weights are those of the last tile under scale 1 (under another tile's
+  // scale a value might not be finite in fp16), and x is zero.
   ls_u32x4 wt[2][4];
   uint32_t sc[2];
   auto load_w = [&](int64_t g, int i) {
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(512) void ls_mx4_rows_kernel(const Mx4Args args) {
   store_x(0);
   for (int64_t j = 0; j < per_half; ++j) {
     const int64_t g = g0 + j;
-    const uint32_t s4[2] = {sc[0], sc[1]};
+    const uint32_t s4[2] = {g < g1 ? sc[0] : 0x7f7f7f7fu, g < g1 ? sc[1] : 0x7f7f7f7fu};
     load_s(g + 1);
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
