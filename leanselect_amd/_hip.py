@@ -208,6 +208,25 @@ def check_out(out: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch
     return out
 
 
+def rows_overlap(a: int, a_stride: int, a_rows: int, a_width: int, b: int, b_stride: int,
+                 b_rows: int, b_width: int) -> bool:
+    """Whether rows of ``a_width`` bytes at ``a``, ``a_stride`` bytes apart, share a byte with rows
+    of the other kind (strides of each at least its width, or a single row)."""
+    if not a_rows or not b_rows or a + (a_rows - 1) * a_stride + a_width <= b \
+            or b + (b_rows - 1) * b_stride + b_width <= a:
+        return False
+    if b_rows > a_rows:
+        a, a_stride, a_rows, a_width, b, b_stride, b_rows, b_width = \
+            b, b_stride, b_rows, b_width, a, a_stride, a_rows, a_width
+    if a_rows == 1:
+        return True
+    for at in range(b, b + b_rows * b_stride, b_stride) if b_rows > 1 else (b,):
+        i = max(0, -(-(at - a - a_width + 1) // a_stride))  # the first row that ends behind `at`
+        if i < a_rows and a + i * a_stride < at + b_width:
+            return True
+    return False
+
+
 class _StatusQueue:
     """Attention status words read without stalling the host.
 

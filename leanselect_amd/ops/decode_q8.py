@@ -193,7 +193,8 @@ def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, 
             raise ValueError(f"topk_idx must be [{G}, {total_q}, k] with 1 <= k <= 256")
     else:
         n_pages = max(1, min(n_pages, P))
-    if out is not None:
+    given = out is not None
+    if given:
         _hip.check_out(out, (total_q, H, HEAD_DIM), q.dtype, q.device)
         if out.data_ptr() % 16 or out.data_ptr() == q.data_ptr() and total_q:
             raise ValueError("out must be 16-byte aligned and must not overlap q")
@@ -207,6 +208,9 @@ def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, 
     if q_ptr & 15 or row[0] & 7 or row[1] != HEAD_DIM or row[2] != 1:  # rows the kernels do not read
         q = q.clone(memory_format=torch.contiguous_format)
         row, q_ptr = (H * HEAD_DIM,), q.data_ptr()
+    elif given and _hip.rows_overlap(out.data_ptr(), 2 * H * HEAD_DIM, total_q, 2 * H * HEAD_DIM, q_ptr,
+                                     2 * row[0], total_q if row[0] else 1, 2 * H * HEAD_DIM):
+        raise ValueError("out must be 16-byte aligned and must not overlap q")
     if n_splits is None:
         # Slices of a row: as many as leave every workgroup its compute unit, at least a page a
         # wave.  One slice (eight waves, no join) up to three pages a wave, a launch less for the
@@ -218,7 +222,7 @@ def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, 
         n_splits = 1 if n_pages <= max(24, 2 * pairs // 3) \
             else min(-(-n_pages // 4), _WORKGROUPS // max(1, pairs))
     n_splits = max(1, min(int(n_splits), _MAX_SPLITS))
-    if out is None:
+    if not given:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((H, total_q), dtype=torch.float32, device=q.device) if return_lse else None
     # The slices' partial sums, maxima and weights, ls_attn_kvcache_q8_workspace_size bytes, counted

@@ -113,7 +113,7 @@ def linear_mx4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_f
                out: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T`` for ``x [rows, in_features]`` (bf16 or fp16): ``[rows, out_features]`` in
     ``x``'s dtype.  Made for the few rows of a decode step; every 64 rows read the weight
-    again.  ``out`` must not overlap ``x``.  A row's bits do not depend on what the other rows
+    again.  ``out`` must not overlap ``x`` (rows of one buffer side by side do not).  A row's bits do not depend on what the other rows
     hold, but may on how many there are.  No gradient passes."""
     return _linear(x, codes, scales, out_features, 0, out)
 
@@ -141,7 +141,8 @@ def _linear(x, codes, scales, out_features, silu, out):
     _check_weight(codes, scales, out_features, k)
     n = out_features // 2 if silu else out_features
     index = _hip.gpu_index(x, codes, scales, out)
-    if out is None:
+    given = out is not None
+    if not given:
         out = x.new_empty((rows, n))
         out_stride = n
     else:
@@ -155,6 +156,9 @@ def _linear(x, codes, scales, out_features, silu, out):
     if x_ptr & 15 or x_stride[1] != 1 or x_stride[0] & 7:  # rows the kernels do not read
         x = x.clone(memory_format=torch.contiguous_format)
         x_stride, x_ptr = (k,), x.data_ptr()
+    elif given and _hip.rows_overlap(out.data_ptr(), 2 * out_stride, rows, 2 * n, x_ptr,
+                                       2 * x_stride[0], rows if x_stride[0] else 1, 2 * k):
+        raise ValueError("out's rows must not overlap each other or x")
     nbytes = _workspace_bytes(rows, k, out_features, silu)
     ws = x.new_empty((nbytes + 1) >> 1) if nbytes else None  # counted in x's 16-bit elements
     _hip.launch(index, "ls_linear_mx4", x_ptr, x_stride[0], rows, k, codes.data_ptr(),

@@ -1,0 +1,77 @@
+"""Memory that a call both reads and writes, or writes twice, is refused wherever it overlaps
+(CPU only: nothing is launched)."""
+import random
+
+import pytest
+import torch
+
+from leanselect_amd import _hip
+from leanselect_amd.ops import (dense_attention_kvcache_q8, linear_mx4,
+                                linear_mx4_silu_mul, new_kvcache_q8, sparse_attention_kvcache_q8)
+
+BF16 = torch.bfloat16
+
+
+@pytest.fixture(autouse=True)
+def launched(monkeypatch):
+    calls = []
+    monkeypatch.setattr(_hip, "gpu_index", lambda *t: 0)
+    monkeypatch.setattr(_hip, "launch", lambda index, name, *args: calls.append(name))
+    return calls
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+def test_rows_overlap_is_the_bytes_that_are_shared():
+    rng = random.Random(1)
+    for _ in range(3000):
+        sides = []
+        for _ in range(2):
+            width, rows = rng.randint(1, 6), rng.randint(0, 5)
+            stride = rng.choice((width, width + rng.randint(0, 12), rng.randint(1, 20)))
+            sides.append((rng.randint(0, 50), max(1, stride), rows, width))
+        at = [{start + i * stride + c for i in range(rows) for c in range(width)}
+              for start, stride, rows, width in sides]
+        assert _hip.rows_overlap(*sides[0], *sides[1]) == bool(at[0] & at[1]), sides
+
+
+@pytest.mark.parametrize("product,n_out", [(linear_mx4, 128), (linear_mx4_silu_mul, 64)])
+def test_an_output_among_the_rows_it_is_formed_of(launched, product, n_out):
+    codes = torch.zeros(8, 1, 64, 16, dtype=torch.uint8)
+    scales = torch.zeros(8, 1, 64, 4, dtype=torch.uint8)
+    buf = torch.zeros(8, 512, dtype=BF16)
+    flat = torch.zeros(4096, dtype=BF16)
+    bad = [(buf[1:, :128], buf[:-1, :n_out]), (buf[:, 128:256], buf[:, 200:200 + n_out]),
+           (flat[:1024].view(8, 128), flat[1016:1016 + 8 * n_out].view(8, n_out)),
+           (buf[0, :128].expand(3, 128), buf[:3, 120:120 + n_out]),
+           (buf[::2, :128], buf[2:6, 64:64 + n_out])]
+    for x, out in bad:
+        with pytest.raises(ValueError, match="overlap"):
+            product(x, codes, scales, 128, out=out)
+    assert not launched
+    fine = [(buf[:, :128], buf[:, 128:128 + n_out]), (buf[::2, :128], buf[1::2, :n_out]),
+            (buf[1:, :128], buf[:-1, 128:128 + n_out]), (buf[0, :128].expand(3, 128), buf[1:4, :n_out]),
+            (flat[:1024].view(8, 128), flat[1024:1024 + 8 * n_out].view(8, n_out)),
+            (buf[:1, :128], buf[:1, 256:256 + n_out]), (buf[:0, :128], buf[:0, :n_out])]
+    for x, out in fine:
+        assert product(x, codes, scales, 128, out=out) is out
+    assert len(launched) == len(fine)
+
+
+def test_an_output_among_the_queries(launched):
+    cache = new_kvcache_q8(2, 128, 2, device="cpu")
+    flat = torch.zeros(10, 16, 128, dtype=BF16)
+    wide = torch.zeros(2, 24, 128, dtype=BF16)
+    n, cu, ids = _i32([3, 3]), _i32([0, 2, 4]), torch.zeros(2, 4, 1, dtype=torch.int32)
+    for q, out in ((flat[:4], flat[1:5]), (flat[3:7], flat[:4]), (flat[:1].expand(4, 16, 128), flat[:4]),
+                   (flat[::2][:4], flat[3:7])):
+        with pytest.raises(ValueError, match="overlap q"):
+            dense_attention_kvcache_q8(q, *cache, n, cu, 3, out=out)
+        with pytest.raises(ValueError, match="overlap q"):
+            sparse_attention_kvcache_q8(q, *cache, n, ids, cu, out=out)
+    assert not launched
+    dense_attention_kvcache_q8(flat[:4], *cache, n, cu, 3, out=flat[4:8])
+    dense_attention_kvcache_q8(wide[:, :16], *cache, n, _i32([0, 1, 2]), 3, out=flat[:2])
+    assert len(launched) == 2
