@@ -112,6 +112,13 @@ def kvcache_append_q8(k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
     if B > 1 and (cache_stride < P * G * _PAGE_BYTES or scale_stride < P * G
                   or kc_cache is not None and kc_cache.stride(0) == 0):
         raise ValueError("sequences that share pages or windows cannot be appended to")
+    k8_ptr, v8_ptr = k8.data_ptr(), v8.data_ptr()
+    ks_ptr, vs_ptr = k_scale.data_ptr(), v_scale.data_ptr()
+    if abs(k8_ptr - v8_ptr) < B * cache_stride or abs(ks_ptr - vs_ptr) < B * scale_stride:
+        pages, scales = P * G * _PAGE_BYTES, P * G
+        if _hip.rows_overlap(k8_ptr, cache_stride, B, pages, v8_ptr, cache_stride, B, pages) \
+                or _hip.rows_overlap(ks_ptr, scale_stride, B, scales, vs_ptr, scale_stride, B, scales):
+            raise ValueError("keys and values must not share pages or scales")
     after = [n + b - a for n, a, b in zip(lens, cu, cu[1:])]
     longest = max(after)
     if min(lens) < 0 or longest > P * PAGE or any(map(gt, lens, after)):
@@ -129,6 +136,8 @@ def kvcache_append_q8(k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
         if longest >= 32 and (longest - 32) // 16 + 1 > kc_shape[1]:
             raise ValueError(f"{(longest - 32) // 16 + 1} compressed windows exceed kc_capacity "
                              f"{kc_shape[1]}")
+        if kc_stride[1] < G * HEAD_DIM or kc_stride[0] < kc_shape[1] * kc_stride[1]:
+            _check_windows(kc_shape, kc_stride)
         kc = (kc_cache.data_ptr(), kc_stride[0], kc_stride[1], kc_shape[1])
     index = _hip.gpu_index(k8, v8, k_scale, v_scale, cache_seqlens, k_new, v_new, cu_seqlens_new,
                            kc_cache)
@@ -139,9 +148,18 @@ def kvcache_append_q8(k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
         k_new = k_new.clone(memory_format=torch.contiguous_format)
         v_new = v_new.clone(memory_format=torch.contiguous_format)
         row, k_ptr, v_ptr = (G * HEAD_DIM,), k_new.data_ptr(), v_new.data_ptr()
-    _hip.launch(index, "ls_kvcache_append_q8", k8.data_ptr(), v8.data_ptr(), cache_stride,
-                k_scale.data_ptr(), v_scale.data_ptr(), scale_stride, P, cache_seqlens.data_ptr(),
-                k_ptr, v_ptr, row[0], cu_seqlens_new.data_ptr(), total, B, G, HEAD_DIM, code, *kc)
+    _hip.launch(index, "ls_kvcache_append_q8", k8_ptr, v8_ptr, cache_stride, ks_ptr, vs_ptr,
+                scale_stride, P, cache_seqlens.data_ptr(), k_ptr, v_ptr, row[0],
+                cu_seqlens_new.data_ptr(), total, B, G, HEAD_DIM, code, *kc)
+
+
+def _check_windows(shape, stride) -> None:
+    """Refuses compressed windows that overlap (sequences may lie within windows or around them)."""
+    width = shape[2] * HEAD_DIM
+    for step, n in sorted((step, n) for step, n in zip(stride[:2], shape) if n > 1):
+        if step < width:
+            raise ValueError("kc_cache's windows must not overlap")
+        width += (n - 1) * step
 
 
 def sparse_attention_kvcache_q8(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor,

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from leanselect_amd import _hip
-from leanselect_amd.ops import (dense_attention_kvcache_q8, linear_mx4,
+from leanselect_amd.ops import (dense_attention_kvcache_q8, kvcache_append_q8, linear_mx4,
                                 linear_mx4_silu_mul, new_kvcache_q8, sparse_attention_kvcache_q8)
 
 BF16 = torch.bfloat16
@@ -75,3 +75,41 @@ def test_an_output_among_the_queries(launched):
     dense_attention_kvcache_q8(flat[:4], *cache, n, cu, 3, out=flat[4:8])
     dense_attention_kvcache_q8(wide[:, :16], *cache, n, _i32([0, 1, 2]), 3, out=flat[:2])
     assert len(launched) == 2
+
+
+def _append(cache, kc=None, total=4):
+    x = torch.zeros(total, 2, 128, dtype=BF16)
+    kvcache_append_q8(*cache, _i32([3, 0]), x, x, _i32([0, 1, total]), kc_cache=kc)
+
+
+def test_a_cache_whose_keys_and_values_share_memory(launched):
+    k8, v8, ks, vs = new_kvcache_q8(2, 128, 2, device="cpu")
+    as_values = k8.view(2, 2, 2, 128, 64)
+    pages = torch.zeros(5, *k8.shape[1:], dtype=torch.uint8).view(torch.float8_e4m3fn)
+    codes = torch.zeros(5, 2, 2, dtype=torch.uint8)
+    for cache in ((k8, as_values, ks, vs), (k8, v8, ks, ks),
+                  (pages[:2], pages[1:3].view(2, 2, 2, 128, 64), ks, vs),
+                  (pages[:4:2], pages[2:5:2].view(2, 2, 2, 128, 64), codes[:4:2], codes[1:5:2]),
+                  (k8, v8, codes[:2], codes[1:3])):
+        with pytest.raises(ValueError, match="share pages or scales"):
+            _append(cache)
+    assert not launched
+    # Keys and values of a sequence side by side.
+    _append((pages[:4:2], pages[1:5:2].view(2, 2, 2, 128, 64), codes[:4:2], codes[1:5:2]))
+    assert len(launched) == 1
+
+
+def test_compressed_windows_that_overlap(launched):
+    cache = new_kvcache_q8(2, 128, 2, device="cpu")
+    flat = torch.zeros(8192, dtype=BF16)
+
+    def at(batch, row, capacity=7):
+        return flat.as_strided((2, capacity, 2, 128), (batch, row, 128, 1))
+
+    for kc in (at(7 * 256, 0), at(7 * 256, 128), at(6 * 256, 256), at(128, 512), at(256, 256), at(1, 256)):
+        with pytest.raises(ValueError, match="windows must not overlap"):
+            _append(cache, kc)
+    assert not launched
+    for kc in (at(7 * 256, 256), at(256, 512), at(6 * 256 + 256, 256), at(4096, 264), at(256, 0, 1)):
+        _append(cache, kc)
+    assert len(launched) == 5
