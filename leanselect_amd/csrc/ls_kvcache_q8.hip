@@ -804,7 +804,8 @@ __global__ __launch_bounds__(64 * NW) void ls_q8_attn_kernel(const Q8AttnArgs ar
 // zeros and lse = +inf.  A workgroup per (row, KV head, query head): each wave forms the maximum
 // and sum of all slices (at most four a lane), then thread (p, c) sums four channels of every
 // P-th slice, and the P parts are added in LDS in order.  The first 8 P slices' values are
-// loaded with the maxima (a slice of sum 0 may hold anything and is left out).  Bound by its launch
+// loaded with the maxima (a slice of sum 0 may hold anything and is left out); with P = 8 there
+// are no more.  Bound by its launch
 // and the reads of its chain: 3.5 us for 16 slices of a row; P = 8 up to 64 slices, 16 above (131071
 // keys in 128 slices, with the attention: 19.0 us, and 19.5 with P = 8).
 template <int DT, int P>
@@ -813,7 +814,8 @@ __global__ __launch_bounds__(32 * P) void ls_q8_join_kernel(const Q8AttnArgs arg
   const int64_t total_q = args.total_q;
   const int gs = args.gs, n = args.n_splits;
   constexpr int kAhead = 8;
-  __shared__ float s_w[LS_Q8_MAX_SPLITS];
+  constexpr int kMost = P == 8 ? 64 : LS_Q8_MAX_SPLITS;  // slices
+  __shared__ float s_w[kMost];
   __shared__ ls_f32x4 s_a[P][32];
   const int64_t t = blockIdx.x;
   const int g = blockIdx.y, h = blockIdx.z, G = gridDim.y;
@@ -822,9 +824,9 @@ __global__ __launch_bounds__(32 * P) void ls_q8_join_kernel(const Q8AttnArgs arg
   const int64_t tg = (int64_t)g * total_q + t;
   const float2* __restrict__ ml = part.ml + (tg * gs + h) * n;
   const float* __restrict__ po = part.o + (tg * n * gs + h) * kDim + 4 * c;
-  float ms[4], sum[4], M = -INFINITY;
+  float ms[kMost / 64], sum[kMost / 64], M = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < kMost / 64; ++k) {
     const int i = 64 * k + lane;
     const float2 x = i < n ? ml[i] : make_float2(-INFINITY, 0.f);
     ms[k] = x.x;
@@ -836,12 +838,12 @@ __global__ __launch_bounds__(32 * P) void ls_q8_join_kernel(const Q8AttnArgs arg
     ahead[k] = *reinterpret_cast<const ls_f32x4*>(po + (int64_t)min(p + P * k, n - 1) * gs * kDim);
   if (t >= args.cu_q[args.batch]) return;  // a row behind the last sequence
 #pragma unroll
-  for (int k = 0; k < 4; ++k) M = fmaxf(M, ms[k]);
+  for (int k = 0; k < kMost / 64; ++k) M = fmaxf(M, ms[k]);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, ls_shfl_xor(M, o));
   float L = 0.f;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < kMost / 64; ++k) {
     ms[k] = sum[k] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ms[k] - M);
     L += ms[k] * sum[k];
   }
@@ -849,7 +851,7 @@ __global__ __launch_bounds__(32 * P) void ls_q8_join_kernel(const Q8AttnArgs arg
   for (int o = 32; o >= 1; o >>= 1) L += ls_shfl_xor(L, o);
   if (tid < 64) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < kMost / 64; ++k)
       if (64 * k + lane < n) s_w[64 * k + lane] = ms[k];
   }
   __syncthreads();
@@ -859,15 +861,19 @@ __global__ __launch_bounds__(32 * P) void ls_q8_join_kernel(const Q8AttnArgs arg
     const float wt = p + P * k < n ? s_w[p + P * k] : 0.f;
     if (wt != 0.f) a += wt * ahead[k];
   }
-  for (int s0 = p + P * kAhead; s0 < n; s0 += P * kAhead) {
-    ls_f32x4 x[kAhead];
+  if constexpr (P * kAhead < kMost) {
+    const int s0 = p + P * kAhead;
+    static_assert(2 * P * kAhead == kMost, "one more round");
+    if (s0 < n) {
+      ls_f32x4 x[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      x[k] = *reinterpret_cast<const ls_f32x4*>(po + (int64_t)min(s0 + P * k, n - 1) * gs * kDim);
+      for (int k = 0; k < kAhead; ++k)
+        x[k] = *reinterpret_cast<const ls_f32x4*>(po + (int64_t)min(s0 + P * k, n - 1) * gs * kDim);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const float wt = s0 + P * k < n ? s_w[s0 + P * k] : 0.f;
-      if (wt != 0.f) a += wt * x[k];
+      for (int k = 0; k < kAhead; ++k) {
+        const float wt = s0 + P * k < n ? s_w[s0 + P * k] : 0.f;
+        if (wt != 0.f) a += wt * x[k];
+      }
     }
   }
   s_a[p][c] = a;
