@@ -608,7 +608,10 @@ extern "C" int ls_linear_mx4(const void* x, int64_t x_row_stride, int64_t rows,
   };
   auto by_waves = [&](auto dt, auto mtc, auto pr) {
     constexpr int P = decltype(pr)::value ? 2 : 1;
-    if (cut.nw == 4) return few(dt, mtc, pr, integral_constant<int, 4>(), integral_constant<int, 4>());
+    // (Over 16 rows of more than 1024 tiles take the shared form: two rounds at least, one slice.)
+    if constexpr (decltype(mtc)::value == 1)
+      if (cut.nw == 4)
+        return few(dt, mtc, pr, integral_constant<int, 4>(), integral_constant<int, 4>());
     if (cut.rt == 2) return few(dt, mtc, pr, integral_constant<int, 2>(), integral_constant<int, 8>());
     return few(dt, mtc, pr, integral_constant<int, P>(), integral_constant<int, 8>());
   };
