@@ -73,18 +73,15 @@ def quantize_mx4(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def lay_out_mx4(values: torch.Tensor, scale_codes: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(codes, scales)`` in the kernel's order from 4-bit values ``uint8 [out_features,
     in_features]`` (0..15: sign, two exponent bits, one mantissa bit) and scale codes ``uint8
-    [out_features, ceil(in_features / 32)]`` in 8..252, or in 0..254 for a group of zeros."""
+    [out_features, ceil(in_features / 32)]`` in 8..252."""
     if values.ndim != 2 or values.dtype != torch.uint8 or scale_codes.dtype != torch.uint8:
         raise ValueError("values and scale_codes must be uint8, values [out_features, in_features]")
     n, k = values.shape
     cs, ss = _shapes(n, k)
     if scale_codes.shape != (n, -(-k // 32)) or scale_codes.device != values.device:
         raise ValueError(f"scale_codes must be [{n}, {-(-k // 32)}] on {values.device}")
-    # A group of zeros is the same under any scale: checkpoints give it the least one.
-    some = (torch.nn.functional.pad(values & 7, (0, -k % 32)).view(n, -1, 32) != 0).any(-1)
-    scale_codes = scale_codes.masked_fill(~some & (scale_codes < 255), 127)
     if bool((values > 15).any()) or bool(((scale_codes < 8) | (scale_codes > 252)).any()):
-        raise ValueError("values must be 0..15 and scale codes 8..252 (0..254 for a group of zeros)")
+        raise ValueError("values must be 0..15 and scale codes 8..252")
     full = values.new_zeros(cs[0] * 16, cs[1] * 128)
     full[:n, :k] = values
     packed = (full[:, 0::2] | full[:, 1::2] << 4).view(cs[0], 16, cs[1], 4, 16)
