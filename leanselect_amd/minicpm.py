@@ -530,12 +530,14 @@ class MiniCPMLeanSelect:
         the norms and the selectors stay as they are)."""
         if self.cfg.hidden_size % 8 or self.cfg.intermediate_size % 8:
             raise ValueError("4-bit weights need hidden_size and intermediate_size multiples of 8")
-        for L in self.layers:
-            for name in ("w_qkv", "w_o", "w_gate_up", "w_down"):
-                if not isinstance(getattr(L, name), Mx4Weight):
-                    setattr(L, name, _mx4(getattr(L, name)))
-        if not isinstance(self.lm_head, Mx4Weight):
-            self.lm_head = _mx4(self.lm_head)
+        todo = [(o, name) for o, names in [(L, ("w_qkv", "w_o", "w_gate_up", "w_down"))
+                                           for L in self.layers] + [(self, ("lm_head",))]
+                for name in names if not isinstance(getattr(o, name), Mx4Weight)]
+        for o, name in todo:  # before any is replaced
+            if not bool(torch.isfinite(getattr(o, name)).all()):
+                raise ValueError(f"{name} must be finite: E2M1 has no infinity and no NaN")
+        for o, name in todo:
+            setattr(o, name, _mx4(getattr(o, name)))
         return self
 
     @staticmethod
