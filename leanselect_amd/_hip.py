@@ -208,6 +208,14 @@ def check_out(out: torch.Tensor, shape: tuple, dtype: torch.dtype, device: torch
     return out
 
 
+def page_ids(topk_idx: torch.Tensor) -> torch.Tensor:
+    """A plan as contiguous int32.  A wider id that int32 does not hold stays out of range (a
+    cast alone would make 2^32 page 0)."""
+    if topk_idx.dtype is torch.int64:
+        topk_idx = topk_idx.clamp(-1, 2 ** 31 - 1)
+    return topk_idx.to(torch.int32).contiguous()
+
+
 def rows_overlap(a: int, a_stride: int, a_rows: int, a_width: int, b: int, b_stride: int,
                  b_rows: int, b_width: int) -> bool:
     """Whether rows of ``a_width`` bytes at ``a``, ``a_stride`` bytes apart, share a byte with rows

@@ -202,9 +202,7 @@ def _attend_cache(q, k_cache, v_cache, cache_seqlens, topk_idx, cu_seqlens_q, n_
         _hip.check_out(out, (total_q, H, D), q.dtype, q.device)
     dev = _hip.require_gpu(q, k_cache, v_cache, cache_seqlens, topk_idx, cu_seqlens_q)
     if topk_idx is not None:
-        if topk_idx.dtype != torch.int32:
-            topk_idx = topk_idx.to(torch.int32)
-        topk_idx = topk_idx.contiguous()
+        topk_idx = _hip.page_ids(topk_idx)
         n_pages = topk_idx.shape[2]
     q = q if (q.stride(2) == 1 and q.stride(1) == D) else q.contiguous()
     if n_splits is None:

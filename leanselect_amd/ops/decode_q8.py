@@ -220,7 +220,7 @@ def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, 
     cache_seqlens, cu_seqlens_q = cache_seqlens.contiguous(), cu_seqlens_q.contiguous()
     if topk_idx is not None:
         if topk_idx.dtype is not torch.int32 or not topk_idx.is_contiguous():
-            topk_idx = topk_idx.to(torch.int32).contiguous()
+            topk_idx = _hip.page_ids(topk_idx)
         ids = topk_idx.data_ptr()
     row, q_ptr = q.stride(), q.data_ptr()
     if q_ptr & 15 or row[0] & 7 or row[1] != HEAD_DIM or row[2] != 1:  # rows the kernels do not read
