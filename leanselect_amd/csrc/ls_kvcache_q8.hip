@@ -898,6 +898,10 @@ __global__ __launch_bounds__(32 * P) void ls_q8_join_kernel(const Q8AttnArgs arg
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
+namespace {
+constexpr int64_t kMaxThreads = 0xffffffffLL;  // of a launch along a dimension
+}  // namespace
+
 extern "C" int ls_kvcache_append_q8(void* k8, void* v8, int64_t cache_batch_stride,
                                     uint8_t* k_scale, uint8_t* v_scale,
                                     int64_t scale_batch_stride, int64_t pages,
@@ -924,7 +928,7 @@ extern "C" int ls_kvcache_append_q8(void* k8, void* v8, int64_t cache_batch_stri
   // A sequence's n > 0 new tokens touch at most (n + 126) / 64 <= n pages.
   const int64_t nb = std::min<int64_t>(batch, total_new);
   const int64_t units = std::min(total_new, (total_new + 126 * nb) / 64);
-  LS_REQUIRE(units <= 0x7fffffffLL, LS_ERR_UNSUPPORTED, "%s: too many new tokens", who);
+  LS_REQUIRE(units * 256 <= kMaxThreads, LS_ERR_UNSUPPORTED, "%s: too many new tokens", who);
   LS_REQUIRE(!kc_cache || (ls_aligned16(kc_cache) && kc_row_stride % 8 == 0 && kc_batch_stride % 8 == 0),
              LS_ERR_UNSUPPORTED, "%s: compressed cache must be 16-byte aligned", who);
   const Q8AppendArgs args = {
@@ -971,7 +975,7 @@ extern "C" int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int
              "%s: need n_pages >= 1 and 1 <= n_splits <= %d", who, LS_Q8_MAX_SPLITS);
   LS_REQUIRE(dense || n_pages <= 64 * LS_Q8_ID_REGS, LS_ERR_UNSUPPORTED,
              "%s: at most %d plan ids per row (got %d)", who, 64 * LS_Q8_ID_REGS, n_pages);
-  LS_REQUIRE(total_q <= 0x7fffffffLL / n_splits && num_kv_heads <= 65535, LS_ERR_UNSUPPORTED,
+  LS_REQUIRE(total_q <= kMaxThreads / (512LL * n_splits) && num_kv_heads <= 65535, LS_ERR_UNSUPPORTED,
              "%s: too many rows or KV heads", who);
   LS_REQUIRE(pages <= 0x1000000, LS_ERR_UNSUPPORTED, "%s: at most 2^24 pages a sequence", who);
   LS_REQUIRE(q_row_stride % 8 == 0 && cache_batch_stride % 16 == 0, LS_ERR_UNSUPPORTED,

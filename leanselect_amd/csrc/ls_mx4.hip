@@ -495,6 +495,8 @@ __global__ __launch_bounds__(256) void ls_mx4_dequantize_kernel(
   }
 }
 
+constexpr int64_t kMaxThreads = 0xffffffffLL;  // of a launch along a dimension
+
 bool mx4_sizes(int64_t n, int64_t k) {
   return n >= 1 && k >= 8 && k % 8 == 0 && n <= 0x7fffffffLL && k <= 0x7fffffffLL;
 }
@@ -591,6 +593,9 @@ extern "C" int ls_linear_mx4(const void* x, int64_t x_row_stride, int64_t rows,
   LS_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), LS_ERR_WORKSPACE,
              "%s: workspace %zu < %zu", who, workspace ? workspace_bytes : (size_t)0, need);
   LS_REQUIRE(cut.blocks <= 65535, LS_ERR_UNSUPPORTED, "%s: too many rows", who);
+  // (A large weight has 64 threads for each of its tiles.)
+  LS_REQUIRE((out_features + 15) / 16 * 64 <= kMaxThreads - 512, LS_ERR_UNSUPPORTED,
+             "%s: too many outputs", who);
   const int64_t n_out = silu_mul ? out_features / 2 : out_features;
   hipStream_t stm = (hipStream_t)stream;
   const Mx4Args args = {(const uint16_t*)x, x_row_stride, rows, in_features, (const uint8_t*)codes,
@@ -660,7 +665,7 @@ extern "C" int ls_quantize_mx4(const void* weight, int64_t weight_row_stride, in
   LS_REQUIRE(weight && codes && scales, LS_ERR_INVALID, "%s: null pointer", who);
   LS_REQUIRE(ls_aligned16(codes), LS_ERR_UNSUPPORTED, "%s: codes must be 16-byte aligned", who);
   const int64_t tiles = (out_features + 15) / 16, kc = (in_features + 127) / 128, kc4 = (kc + 3) / 4;
-  LS_REQUIRE(tiles * 4 * kc4 <= 0x7fffffffLL, LS_ERR_UNSUPPORTED, "%s: weight too large", who);
+  LS_REQUIRE(tiles * kc4 * 256 <= kMaxThreads, LS_ERR_UNSUPPORTED, "%s: weight too large", who);
   auto run = [&](auto dt, auto aligned) {
     constexpr int DT = decltype(dt)::value;
     hipLaunchKernelGGL((ls_mx4_quantize_kernel<DT, decltype(aligned)::value>),
