@@ -235,9 +235,10 @@ def rope_inplace(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, si
         lo, hi = int(positions.min()), int(positions.max())
         if lo < 0 or hi >= cos.shape[0]:
             raise ValueError(f"positions must lie in [0, {cos.shape[0]}) (got {lo}..{hi})")
+    positions, cos, sin = positions.contiguous(), cos.contiguous(), sin.contiguous()
     _hip.check(_hip.lib().ls_rope_inplace(
-        x.data_ptr(), x.stride(0), positions.contiguous().data_ptr(), x.shape[0], n_q_heads,
-        n_k_heads, k_col_offset, head_dim, cos.contiguous().data_ptr(), sin.contiguous().data_ptr(),
+        x.data_ptr(), x.stride(0), positions.data_ptr(), x.shape[0], n_q_heads,
+        n_k_heads, k_col_offset, head_dim, cos.data_ptr(), sin.data_ptr(),
         cos.shape[0], _hip.dtype_code(x.dtype), _hip.stream_of(dev)), "ls_rope_inplace")
     return x
 
@@ -273,10 +274,12 @@ def rope_k_compress(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor,
     L = _hip.lib()
     ws = _hip.workspace(L.ls_rope_k_compress_workspace_size(x.shape[0], batch, n_k_heads,
                                                             head_dim), dev)
+    positions, cos, sin = positions.contiguous(), cos.contiguous(), sin.contiguous()
+    cu_seqlens = cu_seqlens.contiguous()
     _hip.check(L.ls_rope_k_compress(
-        x.data_ptr(), x.stride(0), positions.contiguous().data_ptr(), cu_seqlens.data_ptr(), batch,
-        x.shape[0], n_k_heads, k_col_offset, head_dim, cos.contiguous().data_ptr(),
-        sin.contiguous().data_ptr(), cos.shape[0], _hip.dtype_code(x.dtype),
+        x.data_ptr(), x.stride(0), positions.data_ptr(), cu_seqlens.data_ptr(), batch,
+        x.shape[0], n_k_heads, k_col_offset, head_dim, cos.data_ptr(),
+        sin.data_ptr(), cos.shape[0], _hip.dtype_code(x.dtype),
         kc.data_ptr() if total_atoms else None, total_atoms, cu_c.data_ptr(), ws.data_ptr(),
         ws.numel(), _hip.stream_of(dev)), "ls_rope_k_compress")
     return kc, cu_c
@@ -316,9 +319,10 @@ def rope_project_queries(x: torch.Tensor, positions: torch.Tensor, cos: torch.Te
     ws = _hip.workspace(L.ls_select_workspace_size(0, 0, 0, n_q_heads, G, head_dim,
                                                    selector.router_heads, selector.router_dim,
                                                    0, dt), dev)
+    positions, cos, sin = positions.contiguous(), cos.contiguous(), sin.contiguous()
     _hip.check(L.ls_rope_project_queries(
-        x.data_ptr(), x.stride(0), positions.contiguous().data_ptr(), n, n_q_heads, G, head_dim,
-        cos.contiguous().data_ptr(), sin.contiguous().data_ptr(), cos.shape[0], hm.data_ptr(),
+        x.data_ptr(), x.stride(0), positions.data_ptr(), n, n_q_heads, G, head_dim,
+        cos.data_ptr(), sin.data_ptr(), cos.shape[0], hm.data_ptr(),
         qp.data_ptr(), selector.router_heads, selector.router_dim, dt, out.data_ptr(),
         ws.data_ptr(), ws.numel(), _hip.stream_of(dev)), "ls_rope_project_queries")
     return out

@@ -82,9 +82,10 @@ def sparse_attention(
     dt = _hip.dtype_code(q.dtype)
     ws = _hip.workspace(L.ls_sparse_attn_workspace_size(total_k, batch, G, D, int(max_seqlen_k), dt), dev)
     scale = -1.0 if softmax_scale is None else float(softmax_scale)
+    cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
     rc = L.ls_sparse_attn_varlen(
         q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
-        cu_seqlens_q.contiguous().data_ptr(), cu_seqlens_k.contiguous().data_ptr(), batch,
+        cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), batch,
         total_q, total_k, int(max_seqlen_q), int(max_seqlen_k), H, G, D, dt,
         topk_idx.data_ptr(), topk_idx.shape[2], block_size, scale, 1 if causal else 0,
         out.data_ptr(), _hip.ptr(lse), ws.data_ptr(), ws.numel(), _hip.stream_of(dev))

@@ -90,10 +90,11 @@ def kvcache_append(k_cache: torch.Tensor, v_cache: torch.Tensor, cache_seqlens: 
     if not (k_new.stride(2) == 1 and k_new.stride(1) == D and v_new.stride() == k_new.stride()
             and k_new.stride(0) % 8 == 0):
         k_new, v_new = k_new.contiguous(), v_new.contiguous()
+    cache_seqlens, cu_seqlens_new = cache_seqlens.contiguous(), cu_seqlens_new.contiguous()
     rc = _hip.lib().ls_kvcache_append(
         k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
-        cache_seqlens.contiguous().data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0),
-        cu_seqlens_new.contiguous().data_ptr(), k_new.shape[0], B, G, D,
+        cache_seqlens.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0),
+        cu_seqlens_new.data_ptr(), k_new.shape[0], B, G, D,
         _hip.dtype_code(k_cache.dtype), _hip.ptr(kc_cache),
         kc_cache.stride(0) if kc_cache is not None else 0,
         kc_cache.stride(1) if kc_cache is not None else 0, new_windows, int(kernel_size),
@@ -147,10 +148,11 @@ def decode_topk_idx(q: torch.Tensor, kc_cache: torch.Tensor, cache_seqlens: torc
     ws = _hip.workspace(L.ls_decode_select_workspace_size(total_q, B, G, max_kc, out_len), dev)
     ids = torch.empty((G, total_q, take), dtype=torch.int32, device=dev)
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
+    cu_seqlens_q, cache_seqlens = cu_seqlens_q.contiguous(), cache_seqlens.contiguous()
     rc = L.ls_decode_select(
-        q.data_ptr(), q.stride(0), cu_seqlens_q.contiguous().data_ptr(), total_q,
+        q.data_ptr(), q.stride(0), cu_seqlens_q.data_ptr(), total_q,
         kc_cache.data_ptr(), kc_cache.stride(0), kc_cache.stride(1),
-        cache_seqlens.contiguous().data_ptr(), B, max_kc, H, G, D, _hip.dtype_code(q.dtype), scale,
+        cache_seqlens.data_ptr(), B, max_kc, H, G, D, _hip.dtype_code(q.dtype), scale,
         int(topk), int(block_size), int(kernel_size), int(kernel_stride), int(init_blocks),
         int(local_blocks), out_len, take, ids.data_ptr(), ws.data_ptr(), ws.numel(),
         _hip.stream_of(dev))
@@ -216,9 +218,10 @@ def _attend_cache(q, k_cache, v_cache, cache_seqlens, topk_idx, cu_seqlens_q, n_
     L = _hip.lib()
     ws = _hip.workspace(L.ls_sparse_attn_kvcache_workspace_size(total_q, G, n_splits), dev)
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
-    head = (q.data_ptr(), q.stride(0), cu_seqlens_q.contiguous().data_ptr(), total_q,
+    cu_seqlens_q, cache_seqlens = cu_seqlens_q.contiguous(), cache_seqlens.contiguous()
+    head = (q.data_ptr(), q.stride(0), cu_seqlens_q.data_ptr(), total_q,
             k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
-            cache_seqlens.contiguous().data_ptr(), B, H, G, D, _hip.dtype_code(q.dtype))
+            cache_seqlens.data_ptr(), B, H, G, D, _hip.dtype_code(q.dtype))
     tail = (scale, 1 if causal else 0, n_splits, out.data_ptr(), _hip.ptr(lse), ws.data_ptr(),
             ws.numel(), _hip.stream_of(dev))
     if topk_idx is None:
@@ -262,9 +265,10 @@ def stage1_scores(q: torch.Tensor, kc: torch.Tensor, cu_seqlens_q: torch.Tensor,
     L = _hip.lib()
     ws = _hip.workspace(L.ls_stage1_scores_workspace_size(total_q, G, max_kc), dev)
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
+    cu_seqlens_q, cu_seqlens_kc = cu_seqlens_q.contiguous(), cu_seqlens_kc.contiguous()
     rc = L.ls_stage1_scores(
-        q.data_ptr(), q.stride(0), cu_seqlens_q.contiguous().data_ptr(), total_q,
-        kc.data_ptr() if total_kc else None, kc.stride(0), cu_seqlens_kc.contiguous().data_ptr(),
+        q.data_ptr(), q.stride(0), cu_seqlens_q.data_ptr(), total_q,
+        kc.data_ptr() if total_kc else None, kc.stride(0), cu_seqlens_kc.data_ptr(),
         B, max_kc, H, G, D, _hip.dtype_code(q.dtype), scale, out.data_ptr(), out_cols,
         ws.data_ptr(), ws.numel(), _hip.stream_of(dev))
     _hip.check(rc, "ls_stage1_scores")

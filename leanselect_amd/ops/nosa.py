@@ -77,10 +77,11 @@ def max_pooling_1d_varlen(
         out = buf
     if out.numel() == 0 or batch == 0:
         return out
-    input = input.contiguous()
+    input, cache_lens = input.contiguous(), cache_lens.contiguous()
+    cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
     rc = _hip.lib().ls_page_maxpool_varlen(
-        input.data_ptr(), cu_seqlens_q.contiguous().data_ptr(),
-        cu_seqlens_k.contiguous().data_ptr(), cache_lens.contiguous().data_ptr(), batch, H,
+        input.data_ptr(), cu_seqlens_q.data_ptr(),
+        cu_seqlens_k.data_ptr(), cache_lens.data_ptr(), batch, H,
         total_q, int(max_seqlen_k), out_len, int(local_blocks), int(init_blocks), block_size,
         stride, clip_code, _hip.dtype_code(input.dtype), out.data_ptr(), _hip.stream_of(dev))
     _hip.check(rc, "ls_page_maxpool_varlen")
@@ -161,12 +162,14 @@ def nosa_prefill_topk_idx(
         total_q, total_atoms, batch, H, G, D, selector.router_heads, selector.router_dim,
         out_len, dt)
     ws = _hip.workspace(nbytes, dev)
+    cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
+    cu_seqlens_kc = cu_seqlens_kc.contiguous()
     rc = L.ls_nosa_select_prefill(
         q_unpad.data_ptr(), q_unpad.stride(0), total_q,
         k_compressed.data_ptr() if total_atoms else None, k_compressed.stride(0), total_atoms,
         cis.data_ptr(), cis.stride(0), _hip.dtype_code(cis.dtype),
-        cu_seqlens_q.contiguous().data_ptr(), cu_seqlens_kc.contiguous().data_ptr(),
-        cu_seqlens_k.contiguous().data_ptr(), batch, int(max_seqlen_q), H, G, D,
+        cu_seqlens_q.data_ptr(), cu_seqlens_kc.data_ptr(),
+        cu_seqlens_k.data_ptr(), batch, int(max_seqlen_q), H, G, D,
         hm.data_ptr(), khm.data_ptr(), qp.data_ptr(), kp.data_ptr(), selector.router_heads,
         selector.router_dim, dt, int(topk), block_size, kernel_stride, int(init_blocks),
         int(local_blocks), int(select_blocks), clip_code, topk_idx.data_ptr(), take, ws.data_ptr(),
@@ -235,10 +238,11 @@ def nosa_sparse_attention(
     dt = _hip.dtype_code(q.dtype)
     ws = _hip.workspace(L.ls_nosa_attn_workspace_size(total_k, batch, G, D, int(max_seqlen_k), dt), dev)
     scale = -1.0 if softmax_scale is None else float(softmax_scale)
+    cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
     rc = L.ls_nosa_attn_varlen(
         q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
         cis.data_ptr(), cis.stride(0), _hip.dtype_code(cis.dtype),
-        cu_seqlens_q.contiguous().data_ptr(), cu_seqlens_k.contiguous().data_ptr(), batch,
+        cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), batch,
         total_q, total_k, int(max_seqlen_q), int(max_seqlen_k), H, G, D, dt,
         topk_idx.data_ptr(), topk_idx.shape[2], block_size, scale, out.data_ptr(),
         _hip.ptr(lse), ws.data_ptr(), ws.numel(), _hip.stream_of(dev))

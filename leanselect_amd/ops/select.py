@@ -96,6 +96,7 @@ def leanselect_prefill_topk_idx(
         total_q, total_atoms, batch, H, G, D, selector.router_heads, selector.router_dim,
         max_pages, dt)
     ws = _hip.workspace(nbytes, dev)
+    cu_seqlens_q, cu_seqlens_k = cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous()
     if q_tilde is not None:
         F = selector.router_heads * selector.router_dim
         if tuple(q_tilde.shape) != (G, total_q, F) or q_tilde.dtype != q_unpad.dtype \
@@ -105,7 +106,7 @@ def leanselect_prefill_topk_idx(
         rc = L.ls_select_prefill_qt(
             q_tilde.data_ptr(), total_q,
             k_compressed.data_ptr() if total_atoms else None, k_compressed.stride(0), total_atoms,
-            cu_seqlens_q.contiguous().data_ptr(), cu_seqlens_k.contiguous().data_ptr(), batch,
+            cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), batch,
             max_seqlen_q, H, G, D, khm.data_ptr(), kp.data_ptr(), selector.router_heads,
             selector.router_dim, dt, int(topk), block_size, kernel_stride, int(init_blocks),
             int(local_blocks), topk_idx.data_ptr(), take, ws.data_ptr(), ws.numel(),
@@ -115,7 +116,7 @@ def leanselect_prefill_topk_idx(
     rc = L.ls_select_prefill(
         q_unpad.data_ptr(), q_unpad.stride(0), total_q,
         k_compressed.data_ptr() if total_atoms else None, k_compressed.stride(0), total_atoms,
-        cu_seqlens_q.contiguous().data_ptr(), cu_seqlens_k.contiguous().data_ptr(), batch,
+        cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), batch,
         max_seqlen_q, H, G, D, hm.data_ptr(), khm.data_ptr(), qp.data_ptr(), kp.data_ptr(),
         selector.router_heads, selector.router_dim, dt, int(topk), block_size, kernel_stride,
         int(init_blocks), int(local_blocks), topk_idx.data_ptr(), take, ws.data_ptr(),
