@@ -230,14 +230,16 @@ def _attend(q, k8, v8, k_scale, v_scale, cache_seqlens, topk_idx, cu_seqlens_q, 
                                      2 * row[0], total_q if row[0] else 1, 2 * H * HEAD_DIM):
         raise ValueError("out must be 16-byte aligned and must not overlap q")
     if n_splits is None:
-        # Slices of a row: as many as leave every workgroup its compute unit, at least a page a
-        # wave.  One slice (eight waves, no join) up to three pages a wave, a launch less for the
-        # host (us, replayed and called, one slice and several: 1 row of 16 pages 9.6 / 11.5, 9.2 /
-        # 16.2, of 24 pages 11.9 / 12.1, 9.3 / 16.0, of 32 pages 14.1 / 14.2, 9.2 / 15.6); and where
-        # the rows fill the device meanwhile (replayed: 4000 keys, 40 rows 24.3, 21.8, 56 rows
-        # 24.7, 27.7).  More workgroups than units: 48 rows of 4000 keys in 2 slices 24.1, in 3 30.4.
+        # Slices of a row: as many as leave every workgroup its compute unit, at least a page a wave.
+        # One slice (eight waves, no join) up to three pages a wave, a launch less for the host (us,
+        # replayed and called, one slice and several: 1 row of 16 pages 9.6 / 10.2, 8.8 / 14.6, of 24
+        # pages 12.2 / 12.4, 9.0 / 15.0, of 32 pages 14.6 / 14.7, 9.0 / 14.7), up to 32 pages from 48
+        # workgroups (24 rows of two heads 15.7 / 15.9, 14.0 / 19.8; 48 rows 16.6, 18.1 replayed), and
+        # where the rows nearly fill the device meanwhile (63 pages, replayed: 48 rows 29.8, 26.7, 56
+        # rows 33.6, 30.5, 64 rows 35.1, 34.6, 72 rows 36.3, 46.0).  More workgroups than units: 48
+        # rows of 63 pages in 2 slices 26.7, in 3 31.9; 65 rows of 469 in 1 slice 203, in 2 259, in 3 202.
         pairs = total_q * G
-        n_splits = 1 if n_pages <= max(24, 2 * pairs // 3) \
+        n_splits = 1 if n_pages <= max(24, min(32, 2 * pairs // 3), pairs // 2) \
             else min(-(-n_pages // 4), _WORKGROUPS // max(1, pairs))
     n_splits = max(1, min(int(n_splits), _MAX_SPLITS))
     if not given:
