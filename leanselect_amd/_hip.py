@@ -228,6 +228,10 @@ def rows_overlap(a: int, a_stride: int, a_rows: int, a_width: int, b: int, b_str
             b, b_stride, b_rows, b_width, a, a_stride, a_rows, a_width
     if a_rows == 1:
         return True
+    if a_stride == b_stride >= max(a_width, b_width):  # row j of b lies at `r` of row j + n of a
+        n, r = divmod(b - a, a_stride)
+        return (r < a_width and -b_rows < n < a_rows) \
+            or (a_stride - r < b_width and -b_rows < n + 1 < a_rows)
     for at in range(b, b + b_rows * b_stride, b_stride) if b_rows > 1 else (b,):
         i = max(0, -(-(at - a - a_width + 1) // a_stride))  # the first row that ends behind `at`
         if i < a_rows and a + i * a_stride < at + b_width:

@@ -26,12 +26,14 @@ def _i32(x):
 
 def test_rows_overlap_is_the_bytes_that_are_shared():
     rng = random.Random(1)
-    for _ in range(3000):
+    for _ in range(6000):
         sides = []
         for _ in range(2):
             width, rows = rng.randint(1, 6), rng.randint(0, 5)
             stride = rng.choice((width, width + rng.randint(0, 12), rng.randint(1, 20)))
             sides.append((rng.randint(0, 50), max(1, stride), rows, width))
+        if rng.random() < 0.5:  # rows of one buffer
+            sides[1] = (sides[1][0], sides[0][1], *sides[1][2:])
         at = [{start + i * stride + c for i in range(rows) for c in range(width)}
               for start, stride, rows, width in sides]
         assert _hip.rows_overlap(*sides[0], *sides[1]) == bool(at[0] & at[1]), sides
