@@ -648,7 +648,8 @@ int ls_dense_attn_kvcache(const void* q, int64_t q_row_stride, const int32_t* cu
  * [kc_rows][G][128] (the dtype of k_new), the windows that the new tokens complete
  * are written: window w is the mean of the stored keys [16 w, 16 w + 32), float32
  * sums, one rounding.  Rows past `pages` pages and
- * windows past kc_rows are not written.  cache_seqlens is not advanced.
+ * windows past kc_rows are not written.  cache_seqlens is not advanced.  Keys, values,
+ * scales and windows, and each sequence's, lie apart in memory.
  */
 int ls_kvcache_append_q8(void* k8, void* v8, int64_t cache_batch_stride, uint8_t* k_scale,
                          uint8_t* v_scale, int64_t scale_batch_stride, int64_t pages,

@@ -397,12 +397,13 @@ __global__ __launch_bounds__(256) void ls_q8_append_kernel(const Q8AppendArgs ar
 // What bounds it: a compute unit's reads from memory.  Operands read in their own order (lanes
 // 16 apart on neighbouring bytes) reach 50 GB/s a unit however many waves read; 1 KB a load in
 // the lanes' order (kStage), brought into the operands' order through LDS, 63 GB/s with eight
-// waves (131071 keys, one slice: 671 us, 533 us), but with four waves, alone on their SIMDs, the
-// way through LDS is in the page's chain (two slices of 256 pages: 50 us, 54 us).  So rows of
-// one slice, which need their unit's rate, take eight waves and kStage; slices take neither.
-// 131071 keys in 128 slices: 19.1 us with the join (67 MB, 3.5 TB/s; a launch, the chain of
+// waves (131071 keys, one slice, the weights' heads alone: 671 us, 538 us; with their remainders,
+// which are in a lone row's chain, 618), but with four waves, alone on their SIMDs, the way
+// through LDS is in the page's chain (two slices of 256 pages: 50 us, 54 us).  So rows of one
+// slice, which need their unit's rate, take eight waves and kStage; slices take neither.
+// 131071 keys in 128 slices: 19.0 us with the join (67 MB, 3.5 TB/s; a launch, the chain of
 // lengths, page and sum, and the join are 9 us of it); 16 rows of 64 pages in eight slices:
-// 14.1 us (34 MB, 2.4 TB/s); 72 rows of 4000 keys, one slice: 33 us (150 MB, 4.6 TB/s).
+// 14.2 us (34 MB, 2.4 TB/s); 72 rows of 4000 keys, one slice: 36 us (150 MB, 4.1 TB/s).
 // ---------------------------------------------------------------------------
 #define LS_Q8_MAX_SPLITS 256
 constexpr int kSplitWaves = 4, kWholeWaves = 8;  // of a workgroup: one of several slices, or the row

@@ -249,7 +249,7 @@ __global__ __launch_bounds__(64 * NW) void ls_mx4_kernel(const Mx4Args args) {
 // bytes for 16 lanes.  The halves are summed through LDS; with several slices float32 parts go
 // to the workspace, [slice][row][16 tiles], and a second kernel adds them in order.
 //
-// 16384 outputs of gate and up, 4096 inputs: one row 14.9 us, 71 MB at 4.8 TB/s; 33 rows 21.6, the
+// 16384 outputs of gate and up, 4096 inputs: one row 14.4 us, 71 MB at 4.9 TB/s; 33 rows 21.4, the
 // reads of x from LDS and the matrix instructions adding some 3 us each.
 template <int DT, int MT, bool PAIR>
 __global__ __launch_bounds__(512) void ls_mx4_rows_kernel(const Mx4Args args) {
@@ -471,7 +471,7 @@ __global__ __launch_bounds__(256) void ls_mx4_quantize_kernel(
 }
 
 // The weight's values in 16 bits (exact in bf16; rounded to fp16), rows of K.  Bound by what it
-// writes (32768 x 4096: 72 us, 340 MB at 4.7 TB/s).
+// writes (32768 x 4096: 70 us, 340 MB at 4.9 TB/s).
 template <int DT>
 __global__ __launch_bounds__(256) void ls_mx4_dequantize_kernel(
     const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t N, int64_t K,
@@ -534,7 +534,9 @@ struct Mx4Cut {
 //   16 rows 8.0, 9.7; 73448 x 4096, one row 33.3, 41.1: the second where its workgroups just fill
 //   the chip's 256 units without slices.  And where inputs are long and tiles few, by rows:
 //   1024 x 16384, one row 11.7, 8.6; 1024 x 12288, one row 9.2, 8.5, 8 rows 10.6, 9.1, 16 rows 14.0,
-//   9.1; 1024 x 8192, one row 6.3, 6.9, 8 rows 7.3, 7.2, 16 rows 9.6, 7.4.
+//   9.1; 1024 x 8192, one row 6.3, 6.9, 8 rows 7.3, 7.2, 16 rows 9.6, 7.4.  (These are times on the
+//   GPU.  The rule's border lies above some sizes that the second form does faster, 1024 x 8192 at
+//   16 rows among them: its second launch costs a call that is not captured 4 us more.)
 Mx4Cut mx4_cut(int64_t rows, int64_t K, int64_t N, bool silu) {
   Mx4Cut c;
   const int64_t tiles = (N + 15) / 16;  // of the weight
