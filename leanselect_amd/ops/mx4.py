@@ -113,8 +113,9 @@ def linear_mx4(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out_f
                out: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T`` for ``x [rows, in_features]`` (bf16 or fp16): ``[rows, out_features]`` in
     ``x``'s dtype.  Made for the few rows of a decode step; every 64 rows read the weight
-    again.  ``out`` must not overlap ``x`` (rows of one buffer side by side do not).  A row's bits do not depend on what the other rows
-    hold, but may on how many there are.  No gradient passes."""
+    again.  ``out`` must not overlap ``x`` (rows of one buffer side by side do not).  A row's
+    bits do not depend on what the other rows hold, but may on how many there are.  No gradient
+    passes."""
     return _linear(x, codes, scales, out_features, 0, out)
 
 
