@@ -679,6 +679,39 @@ int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int32_t* cu_se
                        int32_t causal, int32_t n_splits, void* out, float* softmax_lse,
                        void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Attention of packed rows over a 16-bit cache with capped, biased or windowed
+ * scores, the sequences beginning with one prefix that is kept once (prefix_len =
+ * 0: none).  Row i of sequence b (n_b rows, len_b = cache_seqlens[b] own keys) stands at
+ * p = prefix_len + len_b - n_b + i; key j of prefix_len + len_b (the prefix first) is
+ * visible where, with causal, j <= p, with window_left >= 0, j >= p - window_left, and with
+ * window_right >= 0, j <= p + window_right.  Scores x = softmax_scale q.k, then
+ * softcap tanh(x / softcap) where softcap > 0, then less alibi_slopes[b alibi_batch_stride + h]
+ * |p - j| where given (float32).  k_prefix / v_prefix [prefix_len][G][128], rows prefix_row_stride
+ * apart; k_cache / v_cache [batch][capacity][G][128]; lengths past capacity count as it.  out
+ * [total_q, H, 128], softmax_lse float32 [H, total_q] (natural log) or NULL; a row that sees no key,
+ * or only scores of -inf, gets zeros and +inf.  Rows at and after cu_seqlens_q[batch] are left as they are.  max_len
+ * (of the own lengths) only decides how the work is cut, n_splits (0: chosen, else <= 128) into
+ * how many slices a row's keys of either kind are.  A channel in which a row sees an infinite
+ * value becomes infinite or NaN.  bf16 or fp16, at most 16 query heads per KV head,
+ * 16-byte aligned tensors and workspace (NULL where its size is 0).
+ * Replaces infllmv2_attn_with_kvcache(..., softcap=, alibi_slopes=, window_size=) without topk_idx
+ * (third_party/infllmv2/paper1.patch:2511-2615); the reference has no shared prefix.
+ */
+size_t ls_cache_attn_workspace_size(int64_t total_q, int32_t batch, int32_t num_heads,
+                                    int32_t num_kv_heads, int64_t prefix_len, int64_t max_len,
+                                    int32_t n_splits);
+int ls_cache_attn(const void* q, int64_t q_row_stride, const int32_t* cu_seqlens_q, int64_t total_q,
+                  const void* k_prefix, const void* v_prefix, int64_t prefix_row_stride,
+                  int64_t prefix_len, const void* k_cache, const void* v_cache,
+                  int64_t cache_batch_stride, int64_t cache_row_stride, int64_t capacity,
+                  const int32_t* cache_seqlens, int32_t batch, int32_t num_heads,
+                  int32_t num_kv_heads, int32_t head_dim, int32_t dtype, int64_t max_len,
+                  float softmax_scale, int32_t causal, float softcap, const float* alibi_slopes,
+                  int64_t alibi_batch_stride, int32_t window_left, int32_t window_right,
+                  int32_t n_splits, void* out, float* softmax_lse, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------
  * Products of a few rows with 4-bit weights (no counterpart in the reference,
  * whose projections are 16-bit: leanselect/models/minicpm.py:2176-2222,

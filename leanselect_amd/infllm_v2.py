@@ -84,13 +84,17 @@ def infllmv2_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=N
     with key ``len - Sq + i``.  Returns ``out [B, Sq, H, D]`` (and
     ``softmax_lse [B, H, Sq]`` float32).  Follows the wrapper contract of
     ``third_party/infllmv2/paper1.patch:2511-2615``; rotary, paged
-    (``block_table``), batch-index, left-pad, ALiBi, softcap and local-window
-    options are not supported."""
+    (``block_table``), batch-index and left-pad options are not supported, and
+    ALiBi (float32 ``[H]`` or ``[B, H]``), softcap and local windows only
+    without ``topk_idx`` (their meaning: ``ops.cache_attention``)."""
     if any(x is not None for x in (rotary_cos, rotary_sin, cache_batch_idx, cache_leftpad,
-                                   block_table, alibi_slopes)) or softcap != 0.0 \
-            or tuple(window_size) != (-1, -1):
-        raise NotImplementedError("infllmv2_attn_with_kvcache: rotary, paged, batch-index, "
-                                  "left-pad, ALiBi, softcap and window options are not supported")
+                                   block_table)):
+        raise NotImplementedError("infllmv2_attn_with_kvcache: rotary, paged, batch-index and "
+                                  "left-pad options are not supported")
+    scored = softcap != 0.0 or alibi_slopes is not None or tuple(window_size) != (-1, -1)
+    if scored and topk_idx is not None:
+        raise NotImplementedError("infllmv2_attn_with_kvcache: ALiBi, softcap and window options "
+                                  "are not supported with topk_idx")
     if q.ndim != 4 or k_cache.ndim != 4:
         raise ValueError("q must be [B, Sq, H, D] and k_cache / v_cache [B, capacity, G, D]")
     B, Sq, H, D = q.shape
@@ -120,7 +124,9 @@ def infllmv2_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=N
     if topk_idx is None:  # every cached page
         res = dense_attention_kvcache(qr, k_cache, v_cache, cache_seqlens, cu_q, max(lens),
                                       causal=bool(causal), softmax_scale=softmax_scale,
-                                      n_splits=splits, return_lse=return_softmax_lse)
+                                      n_splits=splits, return_lse=return_softmax_lse,
+                                      softcap=softcap, alibi_slopes=alibi_slopes,
+                                      window=tuple(window_size))
     else:
         res = sparse_attention_kvcache(qr, k_cache, v_cache, cache_seqlens, topk_idx, cu_q,
                                        causal=bool(causal), softmax_scale=softmax_scale,

@@ -20,6 +20,7 @@ from __future__ import annotations
 import torch
 
 from .. import _hip
+from .cache_attention import scored_attention
 
 __all__ = ["n_windows", "kvcache_append", "decode_topk_idx", "sparse_attention_kvcache",
            "decode_out_len", "stage1_scores"]
@@ -177,9 +178,17 @@ def sparse_attention_kvcache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
 def dense_attention_kvcache(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                             cache_seqlens: torch.Tensor, cu_seqlens_q: torch.Tensor, max_len: int,
                             *, causal: bool = False, softmax_scale: float | None = None,
-                            n_splits: int | None = None, return_lse: bool = False):
+                            n_splits: int | None = None, return_lse: bool = False,
+                            softcap: float = 0.0, alibi_slopes: torch.Tensor | None = None,
+                            window: tuple[int, int] = (-1, -1)):
     """``sparse_attention_kvcache`` over every cached page; ``max_len`` is the longest
-    sequence's length."""
+    sequence's length.  With ``softcap``, ``alibi_slopes`` or ``window`` as in
+    ``ops.cache_attention`` (any capacity, head_dim 128)."""
+    if softcap != 0.0 or alibi_slopes is not None or tuple(window) != (-1, -1):
+        return scored_attention(q, k_cache, v_cache, cache_seqlens, cu_seqlens_q, max_len,
+                                causal=causal, softmax_scale=softmax_scale, softcap=softcap,
+                                alibi_slopes=alibi_slopes, window=window, n_splits=n_splits,
+                                return_lse=return_lse)
     return _attend_cache(q, k_cache, v_cache, cache_seqlens, None, cu_seqlens_q,
                          max(1, -(-int(max_len) // 64)), causal, softmax_scale, n_splits,
                          return_lse, None)
