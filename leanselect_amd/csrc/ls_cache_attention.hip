@@ -26,19 +26,38 @@
 namespace {
 
 constexpr int kDim = 128;
-constexpr int kRowB = 2 * kDim;         // a key's bytes
-constexpr int kSub = 32;                // keys of a wave's step
-constexpr int kSubB = kSub * kRowB;     // their bytes
-constexpr int kWaves = 4;
-constexpr int kUnit = kWaves * kSub;    // keys of a workgroup's step
+constexpr int kRowB = 2 * kDim;  // a key's bytes
+constexpr int kWaves = 8;
+constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
+
+// Keys form: the waves share a step's keys, 32 each, and hold all of the tile's 16 NC columns.
+constexpr int kKeysSub = 32;
+constexpr int kKeysStep = kWaves * kKeysSub;
+constexpr int kSubB = kKeysSub * kRowB;
+// Rows form: the waves share the tile's columns, 16 NC each, and walk the same 64 keys a step.
+constexpr int kRowsStep = 64;
+constexpr int kRowsB = kRowsStep * kRowB;
+constexpr int kRing = 4;
+
+constexpr int kLdsBytes = 2 * kWaves * kSubB;  // 128 KB: the keys form's, and a ring of 4 in the rows form
+static_assert(kLdsBytes == kRing * 2 * kRowsB, "one allocation serves both forms");
 
 typedef short CaS4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) CaS4* CaLdsS4;
 
 #define CA_WAIT_VM(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
 #define CA_WAIT_LDS() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
+
+// How one source's keys are cut: tiles of `tokens` query tokens, `cols` columns in the workspace.
+struct CaCut {
+  int tokens;
+  int cols;
+  int tiles;   // upper bound
+  int slices;  // of a tile; 0: by its length (keys form)
+  int items;   // workgroups
+};
 
 struct CaArgs {
   const uint16_t* q;
@@ -58,21 +77,21 @@ struct CaArgs {
   int batch;
   int G;
   int gs;
-  float scale2;        // scale log2(e)
-  float cap_a;         // cap log2(e)
-  float cap_b;         // 2 scale log2(e) / cap
+  float scale2;  // scale log2(e)
+  float cap_a;   // cap log2(e), 0: none
+  float cap_b;   // 2 scale log2(e) / cap
   const float* slopes;
   int64_t slopes_bs;
   int causal;
   int left;
   int right;
-  int tokens;          // of a tile
-  int prefix_tiles;
-  int prefix_slices;
-  int own_tiles;
-  int own_slices;
-  float* part;         // [rows][heads][slices][128], or NULL: one slice
-  float* ml;           // [rows][heads][slices][2]
+  CaCut pre;
+  CaCut own;
+  // Workspace (NULL: every row is one workgroup's): per item [cols][128] sums and [cols] (maximum, sum),
+  // the prefix's items first; per (row, head) the first of its own items and their number.
+  float* part;
+  float2* ml;
+  int2* rows;
   uint16_t* out;
   float* lse;
 };
@@ -94,23 +113,46 @@ __device__ __forceinline__ float ca_sum4(float x) {
 __device__ __forceinline__ int ca_min64(int x) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) x = min(x, __shfl_xor(x, d, 64));
-  return x;
+  return __builtin_amdgcn_readfirstlane(x);
 }
 __device__ __forceinline__ int ca_max64(int x) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) x = max(x, __shfl_xor(x, d, 64));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ int ca_upto64(int x) {
+  const int lane = ls_lane();
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
+  }
   return x;
 }
 
 // Softmax weights are held as a 16-bit head and its remainder, a product each (2^-17 of a weight in
-// bf16; in fp16, whose range is small, 2^kBias times the weight, 2^-22 of it or 2^-35 of the largest),
+// bf16; in fp16, whose range is small, 2^value times the weight, 2^-21 of it or 2^-35 of the largest),
 // so that the output's rounding is the one that shows: one bf16 a weight would add as much error again.
 template <int DT> struct CaBias { static constexpr float value = 0.f; };
 template <> struct CaBias<LS_F16> { static constexpr float value = 10.f; };
-// The maximum follows once it is this far behind (base-2 units): weights reach 2^(kLazy + kBias).
+// The maximum follows once it is this far behind (base-2 units): weights reach 2^(kLazy + value).
 constexpr float kLazy = 5.f;
 
-// What a tile's columns see, and what is carried over its keys.
+// Two weights' heads (x), cut off, and remainders (y).
+template <int DT>
+__device__ __forceinline__ uint2 ca_split(float p0, float p1) {
+  if constexpr (DT == LS_BF16) {
+    const uint32_t b0 = __float_as_uint(p0) & 0xffff0000u, b1 = __float_as_uint(p1) & 0xffff0000u;
+    return make_uint2(__builtin_amdgcn_perm(b1, b0, 0x07060302u),
+                      ls_pack2(ls_f32_to_bf16(p0 - __uint_as_float(b0)), ls_f32_to_bf16(p1 - __uint_as_float(b1))));
+  } else {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+    return make_uint2(__builtin_bit_cast(uint32_t, h),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0 - (float)h[0], p1 - (float)h[1])));
+  }
+}
+
+// What a wave's columns see, and what is carried over its keys.
 template <int NC>
 struct CaState {
   ls_u32x4 qf[NC][4];
@@ -120,16 +162,18 @@ struct CaState {
   int lo[NC], hi[NC];         // visible keys, among the source's
 };
 
-// One step: 32 keys from key0, K rows at sk and V rows at sv (LDS, swizzled), `v_ready` waits for V.
-// FULL: every column sees all of them.
-template <int DT, int NC, bool CAP, bool ALIBI, bool FULL, class VReady>
-__device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, int key0, CaState<NC>& st,
-                                        const CaArgs& a, VReady v_ready) {
+// One step: 16 KB keys from key0, K rows at sk and V rows at sv (LDS, swizzled).  `k_read` is called
+// once K has been read, `v_ready` before V is, `v_read` after.  full: every column sees all of them.
+// MADE: with cap or slopes.
+template <int DT, int NC, int KB, bool MADE, class KRead, class VReady, class VRead>
+__device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, int key0, bool full,
+                                        CaState<NC>& st, const CaArgs& a, KRead k_read, VReady v_ready,
+                                        VRead v_read) {
   const int lane = ls_lane(), r = lane & 15, q = lane >> 4;
-  ls_f32x4 s[2][NC];
+  ls_f32x4 s[KB][NC];
   const int ka = r * kRowB + 16 * (q ^ r);
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < KB; ++t) {
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) s[t][nc] = ls_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -139,40 +183,61 @@ __device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, in
       for (int nc = 0; nc < NC; ++nc) s[t][nc] = LsElem<DT>::mfma(kf, st.qf[nc][ks], s[t][nc]);
     }
   }
-  constexpr bool MADE = CAP || ALIBI;  // scores in base-2 units already
-  ls_u32x4 hi[NC], lo[NC], seen[NC];
+  k_read();
+  if (MADE) {
+    if (a.cap_a > 0.f) {
+      // cap tanh(x / cap) = cap - 2 cap / (1 + exp(2 x / cap))
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+        for (int t = 0; t < KB; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float w = __builtin_amdgcn_exp2f(s[t][nc][i] * a.cap_b);
+            s[t][nc][i] = fmaf(-2.f * a.cap_a, __builtin_amdgcn_rcpf(1.f + w), a.cap_a);
+          }
+    } else {
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc)
+#pragma unroll
+        for (int t = 0; t < KB; ++t) s[t][nc] *= a.scale2;
+    }
+    if (a.slopes) {
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc) {
+        const float d0 = st.pos[nc] - (float)(key0 + 4 * q);
+#pragma unroll
+        for (int t = 0; t < KB; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s[t][nc][i] = fmaf(-st.slope2[nc], fabsf(d0 - (float)(16 * t + i)), s[t][nc][i]);
+      }
+    }
+  }
+  if (!full) {
+#pragma unroll
+    for (int nc = 0; nc < NC; ++nc) {
+      const int l0 = st.lo[nc] - (key0 + 4 * q), h0 = st.hi[nc] - (key0 + 4 * q);
+#pragma unroll
+      for (int t = 0; t < KB; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (16 * t + i < l0 || 16 * t + i >= h0) s[t][nc][i] = -INFINITY;
+    }
+  }
+  ls_u32x4 hi[KB / 2][NC], lo[KB / 2][NC];
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) {
-    float x[8];
     float top = -INFINITY;
-    const float d0 = ALIBI ? st.pos[nc] - (float)(key0 + 4 * q) : 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int k = 16 * (e >> 2) + (e & 3);  // + key0 + 4 q
-      x[e] = s[e >> 2][nc][e & 3];
-      if (CAP) {
-        // cap tanh(x / cap) = cap - 2 cap / (1 + exp(2 x / cap))
-        const float w = __builtin_amdgcn_exp2f(x[e] * a.cap_b);
-        x[e] = fmaf(-2.f * a.cap_a, __builtin_amdgcn_rcpf(1.f + w), a.cap_a);
-      } else if (MADE) {
-        x[e] *= a.scale2;
-      }
-      if (ALIBI) x[e] = fmaf(-st.slope2[nc], fabsf(d0 - (float)k), x[e]);
-      if (!FULL) {
-        const int key = key0 + 4 * q + k;
-        const bool see = key >= st.lo[nc] && key < st.hi[nc];
-        x[e] = see ? x[e] : -INFINITY;
-        if (e & 1) seen[nc][e >> 1] |= see ? 0xffff0000u : 0u;
-        else seen[nc][e >> 1] = see ? 0xffffu : 0u;
-      }
-      top = fmaxf(top, x[e]);
-    }
+    for (int t = 0; t < KB; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][nc][i]);
     top = ca_max4(top);
     if (!MADE) top *= a.scale2;  // (scale2 is positive)
     if (__any(top > st.m[nc] + kLazy)) {
       const float m = fmaxf(st.m[nc], top);
-      const float ref = m == -INFINITY ? 0.f : m;
-      const float f = __builtin_amdgcn_exp2f(st.m[nc] - ref);
+      const float f = __builtin_amdgcn_exp2f(st.m[nc] - (m == -INFINITY ? 0.f : m));
       st.m[nc] = m;
       st.l[nc] *= f;
 #pragma unroll
@@ -181,14 +246,19 @@ __device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, in
     const float ref = (st.m[nc] == -INFINITY ? 0.f : st.m[nc]) - CaBias<DT>::value;
     float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float p0 = __builtin_amdgcn_exp2f(MADE ? x[2 * e] - ref : fmaf(x[2 * e], a.scale2, -ref));
-      const float p1 = __builtin_amdgcn_exp2f(MADE ? x[2 * e + 1] - ref : fmaf(x[2 * e + 1], a.scale2, -ref));
-      sum += p0 + p1;
-      const uint16_t h0 = LsElem<DT>::from_f(p0), h1 = LsElem<DT>::from_f(p1);
-      hi[nc][e] = ls_pack2(h0, h1);
-      lo[nc][e] = ls_pack2(LsElem<DT>::from_f(p0 - LsElem<DT>::to_f(h0)),
-                           LsElem<DT>::from_f(p1 - LsElem<DT>::to_f(h1)));
+    for (int t = 0; t < KB; ++t) {
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(MADE ? s[t][nc][i] - ref : fmaf(s[t][nc][i], a.scale2, -ref));
+        sum += p[i];
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint2 w = ca_split<DT>(p[2 * e], p[2 * e + 1]);
+        hi[t / 2][nc][2 * (t & 1) + e] = w.x;
+        lo[t / 2][nc][2 * (t & 1) + e] = w.y;
+      }
     }
     st.l[nc] += sum;
   }
@@ -197,33 +267,63 @@ __device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, in
   // and gets dim r of the rows 4 q .. 4 q + 3.
   const int row = 4 * q + (r >> 2);
   const int va = row * kRowB + 32 * (row & 7) + 8 * (r & 3);
-  auto values = [&](int db) {
-    const uint8_t* p = sv + (va ^ (32 * db));
+  auto values = [&](int half, int db) {
+    const uint8_t* p = sv + 32 * kRowB * half + (va ^ (32 * db));
     const CaS4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CaLdsS4)(p));
     const CaS4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CaLdsS4)(p + 16 * kRowB));
     const uint2 w0 = __builtin_bit_cast(uint2, v0), w1 = __builtin_bit_cast(uint2, v1);
     return ls_u32x4{w0.x, w0.y, w1.x, w1.y};
   };
-  if (!FULL) {
+  bool plain = true;
+  constexpr uint32_t kExp = DT == LS_BF16 ? 0x7f80u : 0x7c00u, kOne = DT == LS_BF16 ? 0x3f80u : 0x3c00u;
+  auto odd = [&](uint32_t w) {
+    return ((w & kExp) == kExp ? 0xffffu : 0u) | ((w >> 16 & kExp) == kExp ? 0xffff0000u : 0u);
+  };
+  if (!full) {
     // Where a key is hidden from some column, its weight there is 0 and its values must not count:
-    // 0 times an infinity or NaN would.  Such values are rare: they leave the product, and the
-    // channels of the columns that see one become NaN.
-    constexpr uint32_t kExp = DT == LS_BF16 ? 0x7f80u : 0x7c00u, kOne = DT == LS_BF16 ? 0x3f80u : 0x3c00u;
-    auto odd = [&](uint32_t w) {
-      return ((w & kExp) == kExp ? 0xffffu : 0u) | ((w >> 16 & kExp) == kExp ? 0xffff0000u : 0u);
-    };
+    // 0 times an infinity or NaN would.
     uint32_t any = 0;
 #pragma unroll
-    for (int db = 0; db < 8; ++db) {
-      const ls_u32x4 v = values(db);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) any |= odd(v[e]);
-    }
-    if (__any(any != 0)) {
-      const uint32_t one = kOne | kOne << 16;
+    for (int half = 0; half < KB / 2; ++half)
 #pragma unroll
       for (int db = 0; db < 8; ++db) {
-        ls_u32x4 v = values(db), is;
+        const ls_u32x4 v = values(half, db);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any |= odd(v[e]);
+      }
+    plain = !__any(any != 0);
+  }
+  if (plain) {
+#pragma unroll
+    for (int half = 0; half < KB / 2; ++half)
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+        const ls_u32x4 v = values(half, db);
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) {
+          st.o[db][nc] = LsElem<DT>::mfma(v, hi[half][nc], st.o[db][nc]);
+          st.o[db][nc] = LsElem<DT>::mfma(v, lo[half][nc], st.o[db][nc]);
+        }
+      }
+  } else {
+    // Such values are rare: they leave the product, and the channels of the columns that see one
+    // become NaN.
+    constexpr uint32_t one = kOne | kOne << 16;
+#pragma unroll
+    for (int half = 0; half < KB / 2; ++half) {
+      ls_u32x4 see[NC];
+#pragma unroll
+      for (int nc = 0; nc < NC; ++nc) {
+        const int l0 = st.lo[nc] - (key0 + 4 * q), h0 = st.hi[nc] - (key0 + 4 * q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = 32 * half + 16 * (e >> 1) + 2 * (e & 1);
+          see[nc][e] = (k >= l0 && k < h0 ? kOne : 0u) | (k + 1 >= l0 && k + 1 < h0 ? kOne << 16 : 0u);
+        }
+      }
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+        ls_u32x4 v = values(half, db), is;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t mask = odd(v[e]);
@@ -232,118 +332,125 @@ __device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, in
         }
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
-          ls_u32x4 see;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) see[e] = seen[nc][e] & one;
-          const ls_f32x4 hits = LsElem<DT>::mfma(is, see, ls_f32x4{0.f, 0.f, 0.f, 0.f});
-          st.o[db][nc] = LsElem<DT>::mfma(v, hi[nc], st.o[db][nc]);
-          st.o[db][nc] = LsElem<DT>::mfma(v, lo[nc], st.o[db][nc]);
+          const ls_f32x4 hits = LsElem<DT>::mfma(is, see[nc], ls_f32x4{0.f, 0.f, 0.f, 0.f});
+          st.o[db][nc] = LsElem<DT>::mfma(v, hi[half][nc], st.o[db][nc]);
+          st.o[db][nc] = LsElem<DT>::mfma(v, lo[half][nc], st.o[db][nc]);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (hits[e] > 0.f) st.o[db][nc][e] = __builtin_nanf("");
         }
       }
-      return;
     }
   }
-#pragma unroll
-  for (int db = 0; db < 8; ++db) {
-    const ls_u32x4 v = values(db);
-#pragma unroll
-    for (int nc = 0; nc < NC; ++nc) {
-      st.o[db][nc] = LsElem<DT>::mfma(v, hi[nc], st.o[db][nc]);
-      st.o[db][nc] = LsElem<DT>::mfma(v, lo[nc], st.o[db][nc]);
-    }
-  }
+  v_read();
 }
 
-// The tile of `unit` among the batch's tiles of R tokens: its sequence, or -1 past the last; `unit`
-// becomes the tile's number in it.
-__device__ __forceinline__ int ca_find(const CaArgs& a, int& unit, int& n0, int& n1) {
-  const int lane = ls_lane();
-  for (int s0 = 0; s0 < a.batch; s0 += 64) {
-    const int i = min(s0 + lane, a.batch - 1);
-    const int lo = a.cu_q[i], hi = a.cu_q[i + 1];
-    const int mine = s0 + lane < a.batch && hi > lo && lo >= 0 ? (hi - lo + a.tokens - 1) / a.tokens : 0;
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int y = __shfl_up(upto, d, 64);
-      if (lane >= d) upto += y;
-    }
-    const uint64_t past = __ballot(unit < upto);
-    if (past != 0) {
-      const int at = __builtin_ctzll(past);
-      unit -= __builtin_amdgcn_readlane(upto - mine, at);
-      n0 = __builtin_amdgcn_readlane(lo, at);
-      n1 = __builtin_amdgcn_readlane(hi, at);
-      return s0 + at;
-    }
-    unit -= __builtin_amdgcn_readlane(upto, 63);
-  }
-  return -1;
-}
-
-// A workgroup's piece of work: tokens [t0, t1) of group g against keys of one source.
+// A workgroup's piece of work: tokens [t0, t1) of group g against a slice of one source's keys.
 struct CaWork {
-  int g, t0, t1, slice, slices, slot;  // slot: of the slice among the row's
-  int seq, n0, n1, len;                // of the own keys; seq < 0: the prefix
-  int n_keys, first;                   // the source's, and its first key's position
+  int item;  // its place in the workspace
+  int g, t0, t1, slice, slices;
+  int seq, n0, n1, len;  // of the own keys; seq < 0: the prefix
+  int n_keys, first;     // the source's, and its first key's position
   const uint16_t* k;
   const uint16_t* v;
   int64_t rs;
 };
 
-// False where there is nothing to do or write.
-__device__ __forceinline__ bool ca_work(const CaArgs& a, CaWork& w) {
-  int item = blockIdx.x;
-  const int units = a.prefix_slices * a.G, n_prefix = a.prefix_tiles * units;
-  if (item < n_prefix) {
-    // Workgroups go to the eight compute dies in turn: the row tiles of a slice stay on one, whose
-    // cache then serves all but the first.
-    const int block = item / (8 * a.prefix_tiles), in = item % (8 * a.prefix_tiles);
-    const int some = min(8, units - 8 * block);
-    const int u = 8 * block + in % some;
-    w.g = u % a.G;
-    w.slice = w.slot = u / a.G;
-    w.slices = a.prefix_slices;
-    w.t0 = in / some * a.tokens;
-    w.t1 = (int)min(min((int64_t)w.t0 + a.tokens, a.total_q), (int64_t)a.cu_q[a.batch]);
-    w.seq = -1;
-    w.n_keys = a.p_len;
-    w.first = 0;
-    w.k = a.kp + (int64_t)w.g * kDim;
-    w.v = a.vp + (int64_t)w.g * kDim;
-    w.rs = a.p_rs;
-    return w.t0 < w.t1;
-  }
-  item -= n_prefix;
-  w.slice = item % a.own_slices;
-  w.slices = a.own_slices;
-  w.slot = a.prefix_slices + w.slice;
-  item /= a.own_slices;
-  w.g = item % a.G;
-  int tile = item / a.G;
-  w.seq = ca_find(a, tile, w.n0, w.n1);
-  if (w.seq < 0) return false;
-  w.t0 = w.n0 + tile * a.tokens;
-  w.t1 = (int)min(min((int64_t)w.t0 + a.tokens, a.total_q), (int64_t)w.n1);
-  w.len = w.n_keys = max(0, min(a.lens[w.seq], a.capacity));
-  w.first = a.p_len;
-  w.k = a.kc + (int64_t)w.seq * a.c_bs + (int64_t)w.g * kDim;
-  w.v = a.vc + (int64_t)w.seq * a.c_bs + (int64_t)w.g * kDim;
-  w.rs = a.c_rs;
+// The item-th workgroup of the prefix.  They go to the eight compute dies in turn: the row tiles of a
+// slice stay on one, whose cache then serves all but the first.
+__device__ __forceinline__ bool ca_prefix_work(const CaArgs& a, int item, CaWork& w) {
+  const int units = a.pre.slices * a.G, block = item / (8 * a.pre.tiles), in = item % (8 * a.pre.tiles);
+  const int some = min(8, units - 8 * block), u = 8 * block + in % some;
+  w.item = item;
+  w.g = u % a.G;
+  w.slice = u / a.G;
+  w.slices = a.pre.slices;
+  w.t0 = in / some * a.pre.tokens;
+  w.t1 = (int)min(min((int64_t)w.t0 + a.pre.tokens, a.total_q), (int64_t)a.cu_q[a.batch]);
+  w.seq = -1;
+  w.n_keys = a.p_len;
+  w.first = 0;
+  w.k = a.kp + (int64_t)w.g * kDim;
+  w.v = a.vp + (int64_t)w.g * kDim;
+  w.rs = a.p_rs;
   return w.t0 < w.t1;
 }
 
-// What column c (token c / gs, head c % gs) sees.
-template <int NC, bool ALIBI>
-__device__ __forceinline__ void ca_columns(const CaArgs& a, const CaWork& w, int c0, CaState<NC>& st) {
+// The item-th workgroup of the own keys.  Keys form: a sequence's tiles are cut into slices of about
+// the same length, as many as the workgroups allow: rows of a batch differ much in length.
+__device__ __forceinline__ bool ca_own_work(const CaArgs& a, int item, CaWork& w) {
+  const int lane = ls_lane();
+  w.item = a.pre.items + item;
+  int64_t length = 0;  // of a slice, in steps; 0: fixed numbers of slices
+  auto tiles_of = [&](int s0, int& lo, int& hi, int& len) {
+    const int i = min(s0 + lane, a.batch - 1);
+    lo = a.cu_q[i];
+    hi = a.cu_q[i + 1];
+    len = max(0, min(a.lens[i], a.capacity));
+    return s0 + lane < a.batch && hi > lo && lo >= 0 ? (hi - lo + a.own.tokens - 1) / a.own.tokens : 0;
+  };
+  auto steps_of = [&](int lo, int hi, int len) {
+    const int from = a.left >= 0 ? min(len, max(0, len - (hi - lo) - a.left)) : 0;
+    return (len - from + kKeysStep - 1) / kKeysStep;
+  };
+  if (a.own.slices == 0 && !a.part) {
+    length = (int64_t)1 << 40;
+  } else if (a.own.slices == 0) {
+    int64_t work = 0;
+    int tiles = 0;
+    for (int s0 = 0; s0 < a.batch; s0 += 64) {
+      int lo, hi, len;
+      const int n = tiles_of(s0, lo, hi, len);
+      tiles += __builtin_amdgcn_readlane(ca_upto64(n), 63);
+      // (steps of 64 sequences and tiles of 2^20 tokens: fewer than 2^31)
+      int64_t mine = (int64_t)n * steps_of(lo, hi, len);
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) mine += __shfl_xor(mine, d, 64);
+      work += mine;
+    }
+    const int spare = a.own.items - tiles * a.G;
+    length = spare <= 0 ? (int64_t)1 << 40 : max((int64_t)1, (work * a.G + spare - 1) / spare);
+  }
+  for (int s0 = 0; s0 < a.batch; s0 += 64) {
+    int lo, hi, len;
+    const int n = tiles_of(s0, lo, hi, len);
+    const int slices = length ? (int)max((int64_t)1, (steps_of(lo, hi, len) + length - 1) / length) : a.own.slices;
+    const int mine = n * a.G * slices, upto = ca_upto64(mine);
+    const uint64_t past = __ballot(item < upto);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      item -= __builtin_amdgcn_readlane(upto - mine, at);
+      w.seq = s0 + at;
+      w.n0 = __builtin_amdgcn_readlane(lo, at);
+      w.n1 = __builtin_amdgcn_readlane(hi, at);
+      w.len = w.n_keys = __builtin_amdgcn_readlane(len, at);
+      w.slices = __builtin_amdgcn_readlane(slices, at);
+      w.slice = item % w.slices;
+      item /= w.slices;
+      w.g = item % a.G;
+      // The last tiles, which see the most keys where causal, first.
+      const int tile = __builtin_amdgcn_readlane(n, at) - 1 - item / a.G;
+      w.t0 = w.n0 + tile * a.own.tokens;
+      w.t1 = (int)min(min((int64_t)w.t0 + a.own.tokens, a.total_q), (int64_t)w.n1);
+      w.first = a.p_len;
+      w.k = a.kc + (int64_t)w.seq * a.c_bs + (int64_t)w.g * kDim;
+      w.v = a.vc + (int64_t)w.seq * a.c_bs + (int64_t)w.g * kDim;
+      w.rs = a.c_rs;
+      return w.t0 < w.t1;
+    }
+    item -= __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
+
+// The tile's columns c0 + 16 nc + r (token c / gs, head c % gs) and what they see.
+template <int NC>
+__device__ __forceinline__ void ca_columns(const CaArgs& a, const CaWork& w, int tokens, int c0, CaState<NC>& st) {
   const int lane = ls_lane(), r = lane & 15, q = lane >> 4;
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) {
     const int c = c0 + 16 * nc + r, tk = c / a.gs, h = c - tk * a.gs;
-    const bool valid = tk < a.tokens && w.t0 + tk < w.t1;
+    const bool valid = tk < tokens && w.t0 + tk < w.t1;
     const int t = valid ? w.t0 + tk : w.t0;
     const uint16_t* qp = a.q + (int64_t)t * a.q_rs + ((int64_t)w.g * a.gs + h) * kDim + 8 * q;
 #pragma unroll
@@ -352,7 +459,8 @@ __device__ __forceinline__ void ca_columns(const CaArgs& a, const CaWork& w, int
     st.hi[nc] = w.n_keys;
     st.m[nc] = -INFINITY;
     st.l[nc] = 0.f;
-    if (ALIBI || a.causal || a.left >= 0 || a.right >= 0) {
+    st.pos[nc] = st.slope2[nc] = 0.f;
+    if (a.slopes || a.causal || a.left >= 0 || a.right >= 0) {
       int n0 = w.n0, n1 = w.n1, len = w.len, b = w.seq;
       if (b < 0) {
         b = ls_find_segment(a.cu_q, a.batch, t);
@@ -361,10 +469,8 @@ __device__ __forceinline__ void ca_columns(const CaArgs& a, const CaWork& w, int
         len = max(0, min(a.lens[b], a.capacity));
       }
       const int p = a.p_len + len - (n1 - n0) + (t - n0) - w.first;
-      if (ALIBI) {
-        st.pos[nc] = (float)p;
-        st.slope2[nc] = a.slopes[b * a.slopes_bs + w.g * a.gs + h] * kLog2e;
-      }
+      st.pos[nc] = (float)p;
+      if (a.slopes) st.slope2[nc] = a.slopes[b * a.slopes_bs + w.g * a.gs + h] * kLog2e;
       if (a.causal) st.hi[nc] = min(st.hi[nc], p + 1);
       if (a.left >= 0) st.lo[nc] = max(0, p - a.left);
       if (a.right >= 0) st.hi[nc] = min(st.hi[nc], p + a.right + 1);
@@ -376,8 +482,8 @@ __device__ __forceinline__ void ca_columns(const CaArgs& a, const CaWork& w, int
   }
 }
 
-// The keys that some column sees, [klo, khi), and those that all do, [flo, fhi).  Columns beyond the
-// tile's (lo = -1) see everything and count for neither.
+// The keys that some column of the wave sees, [klo, khi), and those that all do, [flo, fhi).  Columns
+// beyond the tile's (lo = -1) see everything and count for neither.
 template <int NC>
 __device__ __forceinline__ void ca_range(CaState<NC>& st, int& klo, int& khi, int& flo, int& fhi) {
   klo = fhi = 0x7fffffff;
@@ -397,29 +503,36 @@ __device__ __forceinline__ void ca_range(CaState<NC>& st, int& klo, int& khi, in
   fhi = ca_min64(fhi);
 }
 
-// 32 rows from `row0` of one tensor into LDS: row i at 256 i, its 16-byte chunk C at place C ^ x(i),
-// x(i) = i & 15 for K (a lane reads chunk 4 ks + q of row r) and 2 (i & 7) for V (the transposing
-// read takes 32 bytes of each of 16 rows).  Rows past the last are the last one again.
-template <bool IS_V>
-__device__ __forceinline__ void ca_fetch(const uint16_t* base, int64_t rs, int row0, int n_keys, uint32_t lds) {
+// The slice's steps of `step` keys of the tile's [klo, khi).
+__device__ __forceinline__ void ca_steps(const CaWork& w, int klo, int khi, int step, int& it, int& end) {
+  it = end = 0;
+  if (khi <= klo) return;
+  const int u0 = klo / step, n = (khi + step - 1) / step - u0;
+  it = u0 + (int)((int64_t)n * w.slice / w.slices);
+  end = u0 + (int)((int64_t)n * (w.slice + 1) / w.slices);
+}
+
+// 4 N rows from `row0` of one tensor into LDS, whose place there is row i0 of a tile (a multiple of 4): row i
+// at 256 i, its 16-byte chunk C at place C ^ x(i), x(i) = i & 15 for K (a lane reads chunk 4 ks + q of row
+// r) and 2 (i & 7) for V (the transposing read takes 32 bytes of each of 16 rows).  Rows past the
+// last are the last one again.
+template <bool IS_V, int N>
+__device__ __forceinline__ void ca_fetch(const uint16_t* base, int64_t rs, int row0, int n_keys, int i0, uint32_t lds) {
   const int lane = ls_lane(), i4 = lane >> 4;
   const uint32_t rb = 2 * (uint32_t)rs;
   const uint16_t* p = base + (int64_t)row0 * rs;
-  const bool whole = row0 + kSub <= n_keys;
+  const bool whole = row0 + 4 * N <= n_keys;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int i = 4 * j + i4;
-    const uint32_t chunk = (uint32_t)(lane & 15) ^ (uint32_t)(IS_V ? 2 * (i & 7) : i & 15);
+  for (int j = 0; j < N; ++j) {
+    const int i = i0 + 4 * j + i4;
+    const uint32_t chunk = 16 * ((uint32_t)(lane & 15) ^ (uint32_t)(IS_V ? 2 * (i & 7) : i & 15));
     if (whole)
-      ls_dma16(p + 4 * j * rs, (uint32_t)i4 * rb + 16 * chunk, lds + 1024 * j);
-    else
-      ls_dma16(p, (uint32_t)min(i, n_keys - 1 - row0) * rb + 16 * chunk, lds + 1024 * j);
+      ls_dma16(p + 4 * j * rs, (uint32_t)i4 * rb + chunk, lds + 1024 * j);
+    else if (row0 < n_keys)
+      ls_dma16(p, (uint32_t)min(4 * j + i4, n_keys - 1 - row0) * rb + chunk, lds + 1024 * j);
+    else  // (none: the last row of all, for every row)
+      ls_dma16(base + (int64_t)(n_keys - 1) * rs, chunk, lds + 1024 * j);
   }
-}
-
-// The final values or the slice's part of column c.
-__device__ __forceinline__ void ca_store4(const CaArgs& a, int64_t row, int slot, int d, ls_f32x4 v) {
-  *reinterpret_cast<ls_f32x4*>(a.part + (row * (a.prefix_slices + a.own_slices) + slot) * kDim + d) = v;
 }
 
 template <int DT>
@@ -430,187 +543,362 @@ __device__ __forceinline__ void ca_out4(uint16_t* p, ls_f32x4 v, float inv) {
   *reinterpret_cast<uint2*>(p) = w;
 }
 
-// Few columns (16 NC): the waves share a step's keys, 32 each, and hold every column.  So each key's
-// bytes are read from LDS once, by one wave, in a ring of its own with no barrier; the waves' sums
-// are joined through LDS at the end.
-template <int DT, int NC, bool CAP, bool ALIBI>
-__global__ __launch_bounds__(256) void ls_cache_attn_keys_kernel(const CaArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint8_t ring[kWaves][2][2 * kSubB];
-  __shared__ float s_ml[kWaves][2][16 * NC];
+__device__ __forceinline__ float ca_lse(float M, float L) {
+  return L == 0.f ? INFINITY : (M + log2f(L)) * kLn2;
+}
+
+// Whether the workgroup's rows are its own alone; else the first of a tile's tells the join.
+__device__ __forceinline__ bool ca_alone(const CaArgs& a, const CaWork& w) {
+  return a.part == nullptr || (a.pre.items == 0 && w.slices == 1);
+}
+
+// ---------------------------------------------------------------------------
+// Keys form, few columns (16 NC).  Each key's bytes are read from LDS once, by one wave, from a place of
+// the wave's own, with no barrier: the next step's K is on its way from when this one's has been
+// read, V likewise.  The waves' sums are joined through LDS at the end.
+// ---------------------------------------------------------------------------
+template <int DT, int NC, bool MADE>
+__device__ __forceinline__ void ca_keys_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint8_t* lds,
+                                             float* s_m, float* s_l) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
-  CaWork w;
-  if (!ca_work(a, w)) return;
   CaState<NC> st;
-  ca_columns<NC, ALIBI>(a, w, 0, st);
-  int klo, khi, flo, fhi;
+  ca_columns<NC>(a, w, cut.tokens, 0, st);
+  int klo, khi, flo, fhi, it, end;
   ca_range<NC>(st, klo, khi, flo, fhi);
-  // The slice's steps of 128 keys.
-  int it = 0, end = 0;
-  if (khi > klo) {
-    const int u0 = klo / kUnit, n = (khi + kUnit - 1) / kUnit - u0;
-    it = u0 + (int)((int64_t)n * w.slice / w.slices);
-    end = u0 + (int)((int64_t)n * (w.slice + 1) / w.slices);
-    if (end * kUnit - kUnit + wave * kSub >= khi) --end;  // the last step's keys may not reach this wave
+  ca_steps(w, klo, khi, kKeysStep, it, end);
+  const int sub = wave * kKeysSub;
+  while (it < end && (end - 1) * kKeysStep + sub >= khi) --end;  // the last step may not reach this wave
+  while (it < end && it * kKeysStep + sub + kKeysSub <= klo) ++it;
+  uint8_t* mine = lds + 2 * wave * kSubB;
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)mine;
+  auto fetch_k = [&](int i) { ca_fetch<false, 8>(w.k, w.rs, i * kKeysStep + sub, w.n_keys, 0, at); };
+  auto fetch_v = [&](int i) { ca_fetch<true, 8>(w.v, w.rs, i * kKeysStep + sub, w.n_keys, 0, at + kSubB); };
+  if (it < end) {
+    fetch_k(it);
+    fetch_v(it);
   }
-  uint8_t* mine = ring[wave][0];
-  const uint32_t mine_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)mine;
-  auto fetch = [&](int step) {
-    const int row0 = step * kUnit + wave * kSub;
-    const uint32_t at = mine_at + (step & 1) * 2 * kSubB;
-    ca_fetch<false>(w.k, w.rs, row0, w.n_keys, at);
-    ca_fetch<true>(w.v, w.rs, row0, w.n_keys, at + kSubB);
-  };
-  if (it < end) fetch(it);
   for (; it < end; ++it) {
     const bool more = it + 1 < end;
-    const uint8_t* sk = mine + (it & 1) * 2 * kSubB;
-    if (more) {
-      CA_WAIT_LDS();  // the other half has been read
-      fetch(it + 1);
-      CA_WAIT_VM(24);
-    } else {
-      CA_WAIT_VM(8);
-    }
-    auto v_ready = [&]() {
-      if (more) CA_WAIT_VM(16);
-      else CA_WAIT_VM(0);
-    };
-    const int key0 = it * kUnit + wave * kSub;
-    if (key0 >= flo && key0 + kSub <= fhi)
-      ca_step<DT, NC, CAP, ALIBI, true>(sk, sk + kSubB, key0, st, a, v_ready);
-    else
-      ca_step<DT, NC, CAP, ALIBI, false>(sk, sk + kSubB, key0, st, a, v_ready);
+    const int key0 = it * kKeysStep + sub;
+    CA_WAIT_VM(8);  // V behind K
+    ca_step<DT, NC, 2, MADE>(
+        mine, mine + kSubB, key0, key0 >= flo && key0 + kKeysSub <= fhi, st, a,
+        [&]() {
+          CA_WAIT_LDS();
+          if (more) fetch_k(it + 1);
+        },
+        [&]() {
+          if (more) CA_WAIT_VM(8);
+          else CA_WAIT_VM(0);
+        },
+        [&]() {
+          CA_WAIT_LDS();
+          if (more) fetch_v(it + 1);
+        });
   }
-  CA_WAIT_LDS();
   // The waves' sums: column c's 128 values at 512 c, 16-byte chunk C at place C ^ (c & 15).
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) {
     const int c = 16 * nc + r;
     const float l = ca_sum4(st.l[nc]);
     if (q == 0) {
-      s_ml[wave][0][c] = st.m[nc];
-      s_ml[wave][1][c] = l;
+      s_m[wave * 32 + c] = st.m[nc];
+      s_l[wave * 32 + c] = l;
     }
 #pragma unroll
     for (int db = 0; db < 8; ++db)
       *reinterpret_cast<ls_f32x4*>(mine + 512 * c + 16 * ((4 * db + q) ^ r)) = st.o[db][nc];
   }
   __syncthreads();
-  const int H = a.G * a.gs, slots = a.prefix_slices + a.own_slices;
-  for (int e = tid; e < 16 * NC * 32; e += 256) {
-    const int c = e >> 5, ch = e & 31, tk = c / a.gs, h = c - tk * a.gs;
-    if (tk >= a.tokens || w.t0 + tk >= w.t1) break;  // (later columns are beyond the tile's, too)
+  const int H = a.G * a.gs;
+  const bool alone = ca_alone(a, w);
+#pragma unroll
+  for (int e0 = 0; e0 < NC; ++e0) {
+    const int c = 16 * e0 + (tid >> 5), ch = tid & 31, tk = c / a.gs, h = c - tk * a.gs;
+    if (tk >= cut.tokens || w.t0 + tk >= w.t1) break;  // (later columns are beyond the tile's, too)
     float M = -INFINITY, L = 0.f;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) M = fmaxf(M, s_ml[i][0][c]);
+    for (int i = 0; i < kWaves; ++i) M = fmaxf(M, s_m[i * 32 + c]);
     ls_f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
-      const float m = s_ml[i][0][c], l = s_ml[i][1][c];
+      const float m = s_m[i * 32 + c], l = s_l[i * 32 + c];
       if (l == 0.f) continue;  // nothing visible
       const float f = m == M ? 1.f : __builtin_amdgcn_exp2f(m - M);
       L += f * l;
-      v += f * *reinterpret_cast<const ls_f32x4*>(ring[i][0] + 512 * c + 16 * (ch ^ (c & 15)));
+      v += f * *reinterpret_cast<const ls_f32x4*>(lds + 2 * i * kSubB + 512 * c + 16 * (ch ^ (c & 15)));
     }
     const int64_t row = (int64_t)(w.t0 + tk) * H + w.g * a.gs + h;
     M -= CaBias<DT>::value;
-    if (a.part) {
-      if (L != 0.f) ca_store4(a, row, w.slot, 4 * ch, v);
-      if (ch == 0) *reinterpret_cast<float2*>(a.ml + 2 * (row * slots + w.slot)) = make_float2(M, L);
-    } else {
+    if (alone) {
       ca_out4<DT>(a.out + row * kDim + 4 * ch, v, L == 0.f ? 0.f : 1.f / L);
-      if (ch == 0 && a.lse)
-        a.lse[(int64_t)(w.g * a.gs + h) * a.total_q + w.t0 + tk] = L == 0.f ? INFINITY : (M + log2f(L)) * kLn2;
+      if (ch == 0 && a.lse) a.lse[(int64_t)(w.g * a.gs + h) * a.total_q + w.t0 + tk] = ca_lse(M, L);
+    } else {
+      const int64_t place = (int64_t)w.item * cut.cols + c + (w.seq < 0 ? 0 : (int64_t)a.pre.items * (a.pre.cols - cut.cols));
+      if (L != 0.f) *reinterpret_cast<ls_f32x4*>(a.part + place * kDim + 4 * ch) = v;
+      if (ch == 0) a.ml[place] = make_float2(M, L);
     }
+    if (ch == 0 && a.part && w.seq >= 0 && w.slice == 0)
+      a.rows[row] = alone ? make_int2(0, 0) : make_int2(w.item - a.pre.items, w.slices);
   }
 }
 
-// out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over a row's slices; a wave per (row, head), two
-// channels a lane, each lane the weights of up to four slices.
+// ---------------------------------------------------------------------------
+// Rows form, many columns (kWaves x 16 NC).  A ring of four steps of 64 keys; each wave fetches 8
+// rows of a step's K and V, and a barrier a step tells that the step has come and the one before has been
+// read.
+// ---------------------------------------------------------------------------
+template <int DT, int NC, bool MADE>
+__device__ __forceinline__ void ca_rows_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint8_t* lds,
+                                             int* s_range) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  CaState<NC> st;
+  ca_columns<NC>(a, w, cut.tokens, 16 * NC * wave, st);
+  int klo, khi, flo, fhi, it, end;
+  ca_range<NC>(st, klo, khi, flo, fhi);
+  if (lane == 0) {
+    s_range[wave] = klo;
+    s_range[kWaves + wave] = khi;
+  }
+  __syncthreads();
+  int lo_all = s_range[0], hi_all = s_range[kWaves];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) {
+    lo_all = min(lo_all, s_range[i]);
+    hi_all = max(hi_all, s_range[kWaves + i]);
+  }
+  lo_all = __builtin_amdgcn_readfirstlane(lo_all);
+  hi_all = __builtin_amdgcn_readfirstlane(hi_all);
+  ca_steps(w, lo_all, hi_all, kRowsStep, it, end);
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  auto fetch = [&](int i) {
+    const uint32_t to = at + (uint32_t)(i & (kRing - 1)) * 2 * kRowsB + 2048 * wave;
+    ca_fetch<false, 2>(w.k, w.rs, i * kRowsStep + 8 * wave, w.n_keys, 8 * wave, to);
+    ca_fetch<true, 2>(w.v, w.rs, i * kRowsStep + 8 * wave, w.n_keys, 8 * wave, to + kRowsB);
+  };
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i)
+    if (it + i < end) fetch(it + i);
+  for (; it < end; ++it) {
+    const int left = end - it;
+    if (left > 2) CA_WAIT_VM(8);
+    else if (left == 2) CA_WAIT_VM(4);
+    else CA_WAIT_VM(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (left >= kRing) fetch(it + kRing - 1);
+    const int key0 = it * kRowsStep;
+    const uint8_t* sk = lds + (it & (kRing - 1)) * 2 * kRowsB;
+    if (key0 < khi && key0 + kRowsStep > klo)
+      ca_step<DT, NC, 4, MADE>(sk, sk + kRowsB, key0, key0 >= flo && key0 + kRowsStep <= fhi, st, a, []() {}, []() {},
+                               []() { CA_WAIT_LDS(); });
+  }
+  const int H = a.G * a.gs;
+  const bool alone = ca_alone(a, w);
+#pragma unroll
+  for (int nc = 0; nc < NC; ++nc) {
+    const int c = 16 * (NC * wave + nc) + r, tk = c / a.gs, h = c - tk * a.gs;
+    const float L = ca_sum4(st.l[nc]), M = st.m[nc] - CaBias<DT>::value;
+    if (tk >= cut.tokens || w.t0 + tk >= w.t1) continue;
+    const int64_t row = (int64_t)(w.t0 + tk) * H + w.g * a.gs + h;
+    if (alone) {
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+      for (int db = 0; db < 8; ++db) ca_out4<DT>(a.out + row * kDim + 16 * db + 4 * q, st.o[db][nc], inv);
+      if (q == 0 && a.lse) a.lse[(int64_t)(w.g * a.gs + h) * a.total_q + w.t0 + tk] = ca_lse(M, L);
+    } else {
+      const int64_t place = (int64_t)w.item * cut.cols + c + (w.seq < 0 ? 0 : (int64_t)a.pre.items * (a.pre.cols - cut.cols));
+      if (L != 0.f) {
+#pragma unroll
+        for (int db = 0; db < 8; ++db)
+          *reinterpret_cast<ls_f32x4*>(a.part + place * kDim + 16 * db + 4 * q) = st.o[db][nc];
+      }
+      if (q == 0) a.ml[place] = make_float2(M, L);
+    }
+    if (q == 0 && a.part && w.seq >= 0 && w.slice == 0)
+      a.rows[row] = alone ? make_int2(0, 0) : make_int2(w.item - a.pre.items, w.slices);
+  }
+}
+
+// Forms: 1, 2: keys, NC 1 or 2; 3, 4: rows, NC 1 or 2; 0: no such items.
+template <int FORM> constexpr int ca_cols() { return FORM == 0 ? 0 : FORM <= 2 ? 16 * FORM : kWaves * 16 * (FORM - 2); }
+
+template <int DT, int FORM, bool MADE>
+__device__ __forceinline__ void ca_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint8_t* lds, float* small) {
+  if constexpr (FORM == 1 || FORM == 2) ca_keys_form<DT, FORM, MADE>(a, w, cut, lds, small, small + 32 * kWaves);
+  if constexpr (FORM == 3 || FORM == 4) ca_rows_form<DT, FORM - 2, MADE>(a, w, cut, lds, reinterpret_cast<int*>(small));
+}
+
+template <int DT, int PRE, int OWN, bool MADE>
+__global__ __launch_bounds__(kThreads) void ls_cache_attn_kernel(const CaArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kLdsBytes];
+  __shared__ float small[2 * 32 * kWaves];
+  const int item = blockIdx.x;
+  CaWork w;
+  if (PRE != 0 && item < a.pre.items) {
+    if (ca_prefix_work(a, item, w)) ca_form<DT, PRE, MADE>(a, w, a.pre, lds, small);
+  } else {
+    if (ca_own_work(a, item - a.pre.items, w)) ca_form<DT, OWN, MADE>(a, w, a.own, lds, small);
+  }
+}
+
+// out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over a row's slices, the prefix's and its own; a
+// wave per (row, head), two channels a lane, a slice's weight a lane.
 template <int DT>
 __global__ __launch_bounds__(256) void ls_cache_attn_join_kernel(const CaArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int H = a.G * a.gs, slots = a.prefix_slices + a.own_slices;
+  const int H = a.G * a.gs;
   const int64_t row = (int64_t)blockIdx.x * 4 + wave;
-  if (row >= a.total_q * H || row / H >= a.cu_q[a.batch]) return;
-  const float2* ml = reinterpret_cast<const float2*>(a.ml) + row * slots;
-  float m[4], l[4], M = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int s = 64 * i + lane;
-    const float2 x = s < slots ? ml[s] : make_float2(-INFINITY, 0.f);
-    m[i] = x.x;
-    l[i] = x.y;
-    M = fmaxf(M, m[i]);
-  }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, ls_shfl_xor(M, o));
-  float L = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    // A slice's weight; one without a visible key has no sums.
-    m[i] = l[i] == 0.f ? 0.f : m[i] == M ? 1.f : __builtin_amdgcn_exp2f(m[i] - M);
-    L += l[i] == 0.f ? 0.f : m[i] * l[i];
-  }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) L += ls_shfl_xor(L, o);
-  const float2* p = reinterpret_cast<const float2*>(a.part) + row * slots * (kDim / 2) + lane;
+  if (row >= a.total_q * H) return;
+  const int t = (int)(row / H), head = (int)(row % H), g = head / a.gs, h = head % a.gs;
+  if (t >= a.cu_q[a.batch]) return;
+  int2 own = a.rows[row];
+  own.y = min(max(own.y, 0), a.own.items);  // (in bounds whatever cu_seqlens_q holds)
+  own.x = min(max(own.x, 0), a.own.items - own.y);
+  const int slots = (a.pre.items ? a.pre.slices : 0) + own.y;
+  if (own.y == 0) return;  // written already
+  const int b = ls_find_segment(a.cu_q, a.batch, t);
+  const int own_col = (t - a.cu_q[b]) % a.own.tokens * a.gs + h;
+  auto place = [&](int s) -> int64_t {
+    if (s >= slots - own.y)
+      return (int64_t)a.pre.items * a.pre.cols + (int64_t)(own.x + s - (slots - own.y)) * a.own.cols + own_col;
+    const int u = s * a.G + g, block = u / 8, some = min(8, a.pre.slices * a.G - 8 * block);
+    return ((int64_t)block * 8 * a.pre.tiles + t / a.pre.tokens * some + u % 8) * a.pre.cols +
+           t % a.pre.tokens * a.gs + h;
+  };
+  float M = -INFINITY, L = 0.f;
   float2 acc = make_float2(0.f, 0.f);
+  for (int s0 = 0; s0 < slots; s0 += 64) {
+    const bool in = s0 + lane < slots;
+    const int64_t at = in ? place(s0 + lane) : 0;
+    const float2 x = in ? a.ml[at] : make_float2(-INFINITY, 0.f);
+    float top = x.x;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int n = min(64, slots - 64 * i);
+    for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, ls_shfl_xor(top, o));
+    top = fmaxf(top, M);
+    const float keep = L == 0.f ? 0.f : M == top ? 1.f : __builtin_amdgcn_exp2f(M - top);
+    // A slice's weight; one without a visible key has no sums.
+    const float f = x.y == 0.f ? 0.f : x.x == top ? 1.f : __builtin_amdgcn_exp2f(x.x - top);
+    float l = x.y == 0.f ? 0.f : f * x.y;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) l += ls_shfl_xor(l, o);
+    L = (L == 0.f ? 0.f : L * keep) + l;
+    M = top;
+    acc.x *= keep;
+    acc.y *= keep;
+    const int n = min(64, slots - s0);
+    const int at_lo = (int)(uint32_t)at, at_hi = (int)(at >> 32);
+#pragma unroll 8
     for (int s = 0; s < n; ++s) {
-      const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m[i]), s));
-      if (f == 0.f) continue;
-      const float2 x = p[(64 * i + s) * (kDim / 2)];
-      acc.x = fmaf(f, x.x, acc.x);
-      acc.y = fmaf(f, x.y, acc.y);
+      const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s));
+      const int64_t p = (int64_t)(uint32_t)__builtin_amdgcn_readlane(at_lo, s) |
+                        (int64_t)__builtin_amdgcn_readlane(at_hi, s) << 32;
+      if (fs != 0.f) {
+        const float2 v = reinterpret_cast<const float2*>(a.part + p * kDim)[lane];
+        acc.x = fmaf(fs, v.x, acc.x);
+        acc.y = fmaf(fs, v.y, acc.y);
+      }
     }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   reinterpret_cast<uint32_t*>(a.out)[row * (kDim / 2) + lane] =
       ls_pack2(LsElem<DT>::from_f(acc.x * inv), LsElem<DT>::from_f(acc.y * inv));
-  if (lane == 0 && a.lse)
-    a.lse[(row % H) * a.total_q + row / H] = L == 0.f ? INFINITY : (M + log2f(L)) * kLn2;
+  if (lane == 0 && a.lse) a.lse[(int64_t)head * a.total_q + t] = ca_lse(M, L);
 }
 
-// How a call is cut.
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+constexpr int kUnits = 256;  // compute units
+constexpr int kMaxSplits = 128;
+
+int ca_form_of(int64_t cols) { return cols <= 16 ? 1 : cols <= 32 ? 2 : cols <= 128 ? 3 : 4; }
+int ca_form_cols(int form) { return form == 0 ? 0 : form <= 2 ? 16 * form : kWaves * 16 * (form - 2); }
+
 struct CaPlan {
-  int nc, tokens;
-  int prefix_tiles, prefix_slices, own_tiles, own_slices;
-  int64_t items;
-  size_t part, total;
+  int pre_form, own_form;
+  CaCut pre, own;
+  size_t part, ml, total;  // total 0: no join
 };
 
-constexpr int kMaxSlots = 256;
-
 CaPlan ca_plan(int64_t total_q, int batch, int H, int G, int64_t p_len, int64_t max_len, int n_splits) {
-  CaPlan p;
+  CaPlan p = {};
   const int gs = H / G;
-  const int64_t rows = batch > 0 ? (total_q + batch - 1) / batch : 0;  // of a sequence
-  const int64_t cols = (p_len > 0 ? total_q : rows) * gs;
-  p.nc = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
-  p.tokens = std::max(1, 16 * p.nc / gs);
-  p.own_tiles = (int)std::min<int64_t>(total_q, total_q / p.tokens + batch);
-  p.prefix_tiles = p_len > 0 ? (int)((total_q + p.tokens - 1) / p.tokens) : 0;
-  const int64_t own_steps = std::max<int64_t>(1, (max_len + kUnit - 1) / kUnit);
-  const int64_t prefix_steps = (p_len + kUnit - 1) / kUnit;
-  auto cut = [&](int64_t tiles, int64_t steps) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>({steps, 256 / std::max<int64_t>(1, tiles * G), kMaxSlots / 2}));
-  };
-  if (n_splits > 0) {
-    p.prefix_slices = p_len > 0 ? std::min(n_splits, kMaxSlots / 2) : 0;
-    p.own_slices = std::min(n_splits, kMaxSlots / 2);
-  } else {
-    p.prefix_slices = p_len > 0 ? cut(p.prefix_tiles, prefix_steps) : 0;
-    p.own_slices = cut(p.own_tiles, own_steps);
+  const int64_t rows = (total_q + batch - 1) / batch;  // of a sequence
+  auto tokens_of = [&](int cols) { return std::max(1, cols / gs); };
+  if (p_len > 0) {
+    p.pre_form = ca_form_of(total_q * gs);
+    p.pre.cols = ca_form_cols(p.pre_form);
+    p.pre.tokens = tokens_of(p.pre.cols);
+    p.pre.tiles = (int)((total_q + p.pre.tokens - 1) / p.pre.tokens);
+    const int64_t steps = (p_len + kRowsStep - 1) / kRowsStep;
+    p.pre.slices = (int)std::max<int64_t>(
+        1, std::min<int64_t>({n_splits > 0 ? n_splits : kUnits / std::max(1, p.pre.tiles * G), steps, kMaxSplits}));
+    p.pre.items = p.pre.tiles * p.pre.slices * G;
   }
-  const int slots = p.prefix_slices + p.own_slices;
-  p.items = ((int64_t)p.prefix_tiles * p.prefix_slices + (int64_t)p.own_tiles * p.own_slices) * G;
-  p.part = slots > 1 ? ls_align256(4 * (size_t)total_q * H * slots * kDim) : 0;
-  p.total = slots > 1 ? p.part + 8 * (size_t)total_q * H * slots : 0;
+  p.own_form = ca_form_of(rows * gs);
+  p.own.cols = ca_form_cols(p.own_form);
+  p.own.tokens = tokens_of(p.own.cols);
+  p.own.tiles = (int)std::min<int64_t>(total_q, total_q / p.own.tokens + batch);
+  const int64_t tiles = (int64_t)p.own.tiles * G;
+  const int step = p.own_form <= 2 ? kKeysStep : kRowsStep;
+  const int64_t steps = std::max<int64_t>(1, (max_len + step - 1) / step);
+  if (n_splits > 0) {
+    p.own.slices = n_splits;
+    p.own.items = (int)std::min<int64_t>(tiles * n_splits, 0x7fffffff);
+  } else if (p.own_form <= 2) {
+    p.own.slices = 0;
+    p.own.items = (int)std::min<int64_t>(tiles * steps, std::max<int64_t>(kUnits, tiles + kUnits / 2));
+  } else {
+    // Rounds of a workgroup a unit: as many slices as make them even.
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 8 && s <= steps; ++s) {
+      const double rounds = (double)((tiles * s + kUnits - 1) / kUnits) / s + 0.02 * s;
+      if (rounds < least) least = rounds, best = s;
+    }
+    p.own.slices = best;
+    p.own.items = (int)std::min<int64_t>(tiles * best, 0x7fffffff);
+  }
+  if (p.pre.items > 0 || p.own.items > tiles) {
+    const size_t places = (size_t)p.pre.items * p.pre.cols + (size_t)p.own.items * p.own.cols;
+    p.part = ls_align256(4 * places * kDim);
+    p.ml = ls_align256(8 * places);
+    p.total = p.part + p.ml + 8 * (size_t)total_q * H;
+  }
   return p;
+}
+
+template <int DT, int PRE, int OWN>
+void ca_launch(const CaArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)(a.pre.items + a.own.items));
+  if (a.cap_a > 0.f || a.slopes)
+    hipLaunchKernelGGL((ls_cache_attn_kernel<DT, PRE, OWN, true>), grid, dim3(kThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL((ls_cache_attn_kernel<DT, PRE, OWN, false>), grid, dim3(kThreads), 0, s, a);
+}
+
+template <int DT>
+void ca_by_form(const CaArgs& a, int pre, int own, hipStream_t s) {
+#define CA_PAIR(P, O) \
+  if (pre == P && own == O) return ca_launch<DT, P, O>(a, s)
+  CA_PAIR(0, 1);
+  CA_PAIR(0, 2);
+  CA_PAIR(0, 3);
+  CA_PAIR(0, 4);
+  CA_PAIR(1, 1);
+  CA_PAIR(2, 1);
+  CA_PAIR(3, 1);
+  CA_PAIR(4, 1);
+  CA_PAIR(2, 2);
+  CA_PAIR(3, 2);
+  CA_PAIR(4, 2);
+  CA_PAIR(3, 3);
+  CA_PAIR(4, 3);
+  CA_PAIR(4, 4);
+#undef CA_PAIR
 }
 
 }  // namespace
@@ -642,8 +930,8 @@ extern "C" int ls_cache_attn(const void* q, int64_t q_row_stride, const int32_t*
   LS_REQUIRE(dtype == LS_BF16 || dtype == LS_F16, LS_ERR_UNSUPPORTED, "%s: bf16 or fp16", who);
   LS_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY && softcap >= 0.f && softcap < INFINITY,
              LS_ERR_INVALID, "%s: softmax_scale must be positive and softcap not negative", who);
-  LS_REQUIRE(n_splits >= 0 && n_splits <= kMaxSlots / 2, LS_ERR_INVALID, "%s: 0 <= n_splits <= %d", who,
-             kMaxSlots / 2);
+  LS_REQUIRE(n_splits >= 0 && n_splits <= kMaxSplits, LS_ERR_INVALID, "%s: 0 <= n_splits <= %d", who,
+             kMaxSplits);
   LS_REQUIRE(prefix_len + capacity < (1 << 30) && total_q < (1 << 30), LS_ERR_UNSUPPORTED,
              "%s: fewer than 2^30 keys a sequence and rows", who);
   LS_REQUIRE(q_row_stride % 8 == 0 && cache_row_stride % 8 == 0 && cache_batch_stride % 8 == 0 &&
@@ -662,8 +950,8 @@ extern "C" int ls_cache_attn(const void* q, int64_t q_row_stride, const int32_t*
   const CaPlan p = ca_plan(total_q, batch, num_heads, num_kv_heads, prefix_len, max_len, n_splits);
   LS_REQUIRE(workspace_bytes >= p.total && (p.total == 0 || workspace), LS_ERR_WORKSPACE,
              "%s: workspace %zu < %zu", who, workspace_bytes, p.total);
-  LS_REQUIRE(p.items < (1 << 23) && total_q * num_heads < (1 << 25), LS_ERR_UNSUPPORTED,
-             "%s: more workgroups than a launch holds", who);
+  LS_REQUIRE((int64_t)p.pre.items + p.own.items < (1 << 22) && total_q * num_heads < (1 << 25),
+             LS_ERR_UNSUPPORTED, "%s: more workgroups than a launch holds", who);
   CaArgs a = {};
   a.q = (const uint16_t*)q;
   a.q_rs = q_row_stride;
@@ -690,39 +978,24 @@ extern "C" int ls_cache_attn(const void* q, int64_t q_row_stride, const int32_t*
   a.causal = causal != 0;
   a.left = window_left < 0 ? -1 : std::min(window_left, 1 << 30);
   a.right = window_right < 0 ? -1 : std::min(window_right, (1 << 30) - 1);
-  a.tokens = p.tokens;
-  a.prefix_tiles = p.prefix_tiles;
-  a.prefix_slices = p.prefix_slices;
-  a.own_tiles = p.own_tiles;
-  a.own_slices = p.own_slices;
-  a.part = p.total ? (float*)workspace : nullptr;
-  a.ml = p.total ? (float*)((uint8_t*)workspace + p.part) : nullptr;
+  a.pre = p.pre;
+  a.own = p.own;
+  if (p.total) {
+    a.part = (float*)workspace;
+    a.ml = (float2*)((uint8_t*)workspace + p.part);
+    a.rows = (int2*)((uint8_t*)workspace + p.part + p.ml);
+  }
   a.out = (uint16_t*)out;
   a.lse = softmax_lse;
   hipStream_t s = (hipStream_t)stream;
-  auto by_type = [&](auto dt) {
-    constexpr int DT = decltype(dt)::value;
-    auto by_score = [&](auto nc) {
-      constexpr int NC = decltype(nc)::value;
-      auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)p.items), dim3(256), 0, s, a);
-      };
-      if (softcap > 0.f)
-        alibi_slopes ? go(ls_cache_attn_keys_kernel<DT, NC, true, true>)
-                     : go(ls_cache_attn_keys_kernel<DT, NC, true, false>);
-      else
-        alibi_slopes ? go(ls_cache_attn_keys_kernel<DT, NC, false, true>)
-                     : go(ls_cache_attn_keys_kernel<DT, NC, false, false>);
-    };
-    if (p.nc == 1) by_score(std::integral_constant<int, 1>());
-    else if (p.nc == 2) by_score(std::integral_constant<int, 2>());
-    else by_score(std::integral_constant<int, 4>());
-    int rc = ls_check_launch("ls_cache_attn_keys_kernel");
-    if (rc || !p.total) return rc;
-    hipLaunchKernelGGL(ls_cache_attn_join_kernel<DT>, dim3((unsigned)((total_q * num_heads + 3) / 4)),
-                       dim3(256), 0, s, a);
-    return ls_check_launch("ls_cache_attn_join_kernel");
-  };
-  return dtype == LS_BF16 ? by_type(std::integral_constant<int, LS_BF16>())
-                          : by_type(std::integral_constant<int, LS_F16>());
+  dtype == LS_BF16 ? ca_by_form<LS_BF16>(a, p.pre_form, p.own_form, s)
+                   : ca_by_form<LS_F16>(a, p.pre_form, p.own_form, s);
+  int rc = ls_check_launch("ls_cache_attn_kernel");
+  if (rc || !p.total) return rc;
+  const dim3 grid((unsigned)((total_q * num_heads + 3) / 4));
+  if (dtype == LS_BF16)
+    hipLaunchKernelGGL(ls_cache_attn_join_kernel<LS_BF16>, grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(ls_cache_attn_join_kernel<LS_F16>, grid, dim3(256), 0, s, a);
+  return ls_check_launch("ls_cache_attn_join_kernel");
 }
