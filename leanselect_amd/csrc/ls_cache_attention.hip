@@ -163,12 +163,11 @@ struct CaState {
 };
 
 // One step: 16 KB keys from key0, K rows at sk and V rows at sv (LDS, swizzled).  `k_read` is called
-// once K has been read, `v_ready` before V is, `v_read` after.  full: every column sees all of them.
+// once K has been read, `v_ready` before V is, `v_read` after.  FULL: every column sees all of them.
 // MADE: with cap or slopes.
-template <int DT, int NC, int KB, bool MADE, class KRead, class VReady, class VRead>
-__device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, int key0, bool full,
-                                        CaState<NC>& st, const CaArgs& a, KRead k_read, VReady v_ready,
-                                        VRead v_read) {
+template <int DT, int NC, int KB, bool MADE, bool FULL, class KRead, class VReady, class VRead>
+__device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, int key0, CaState<NC>& st,
+                                        const CaArgs& a, KRead k_read, VReady v_ready, VRead v_read) {
   const int lane = ls_lane(), r = lane & 15, q = lane >> 4;
   ls_f32x4 s[KB][NC];
   const int ka = r * kRowB + 16 * (q ^ r);
@@ -214,7 +213,7 @@ __device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, in
       }
     }
   }
-  if (!full) {
+  if (!FULL) {
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
       const int l0 = st.lo[nc] - (key0 + 4 * q), h0 = st.hi[nc] - (key0 + 4 * q);
@@ -274,41 +273,22 @@ __device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, in
     const uint2 w0 = __builtin_bit_cast(uint2, v0), w1 = __builtin_bit_cast(uint2, v1);
     return ls_u32x4{w0.x, w0.y, w1.x, w1.y};
   };
-  bool plain = true;
-  constexpr uint32_t kExp = DT == LS_BF16 ? 0x7f80u : 0x7c00u, kOne = DT == LS_BF16 ? 0x3f80u : 0x3c00u;
-  auto odd = [&](uint32_t w) {
-    return ((w & kExp) == kExp ? 0xffffu : 0u) | ((w >> 16 & kExp) == kExp ? 0xffff0000u : 0u);
-  };
-  if (!full) {
-    // Where a key is hidden from some column, its weight there is 0 and its values must not count:
-    // 0 times an infinity or NaN would.
-    uint32_t any = 0;
+  if (FULL) {
 #pragma unroll
     for (int half = 0; half < KB / 2; ++half)
 #pragma unroll
       for (int db = 0; db < 8; ++db) {
         const ls_u32x4 v = values(half, db);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) any |= odd(v[e]);
-      }
-    plain = !__any(any != 0);
-  }
-  if (plain) {
+        for (int nc = 0; nc < NC; ++nc) st.o[db][nc] = LsElem<DT>::mfma(v, hi[half][nc], st.o[db][nc]);
 #pragma unroll
-    for (int half = 0; half < KB / 2; ++half)
-#pragma unroll
-      for (int db = 0; db < 8; ++db) {
-        const ls_u32x4 v = values(half, db);
-#pragma unroll
-        for (int nc = 0; nc < NC; ++nc) {
-          st.o[db][nc] = LsElem<DT>::mfma(v, hi[half][nc], st.o[db][nc]);
-          st.o[db][nc] = LsElem<DT>::mfma(v, lo[half][nc], st.o[db][nc]);
-        }
+        for (int nc = 0; nc < NC; ++nc) st.o[db][nc] = LsElem<DT>::mfma(v, lo[half][nc], st.o[db][nc]);
       }
   } else {
-    // Such values are rare: they leave the product, and the channels of the columns that see one
-    // become NaN.
-    constexpr uint32_t one = kOne | kOne << 16;
+    // Where a key is hidden from some column, its weight there is 0 and its values must not count:
+    // 0 times an infinity or NaN would.  Such values leave the product, and the channels of the columns
+    // that see one become NaN.
+    constexpr uint32_t kExp = DT == LS_BF16 ? 0x7f80u : 0x7c00u, kOne = DT == LS_BF16 ? 0x3f80u : 0x3c00u;
 #pragma unroll
     for (int half = 0; half < KB / 2; ++half) {
       ls_u32x4 see[NC];
@@ -326,9 +306,9 @@ __device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, in
         ls_u32x4 v = values(half, db), is;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t mask = odd(v[e]);
-          v[e] &= ~mask;
-          is[e] = mask & one;
+          const uint32_t odd = ((v[e] & kExp) == kExp ? 0xffffu : 0u) | ((v[e] >> 16 & kExp) == kExp ? 0xffff0000u : 0u);
+          v[e] &= ~odd;
+          is[e] = odd & (kOne | kOne << 16);
         }
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
@@ -582,20 +562,23 @@ __device__ __forceinline__ void ca_keys_form(const CaArgs& a, const CaWork& w, c
     const bool more = it + 1 < end;
     const int key0 = it * kKeysStep + sub;
     CA_WAIT_VM(8);  // V behind K
-    ca_step<DT, NC, 2, MADE>(
-        mine, mine + kSubB, key0, key0 >= flo && key0 + kKeysSub <= fhi, st, a,
-        [&]() {
-          CA_WAIT_LDS();
-          if (more) fetch_k(it + 1);
-        },
-        [&]() {
-          if (more) CA_WAIT_VM(8);
-          else CA_WAIT_VM(0);
-        },
-        [&]() {
-          CA_WAIT_LDS();
-          if (more) fetch_v(it + 1);
-        });
+    auto step = [&](auto full) {
+      ca_step<DT, NC, 2, MADE, decltype(full)::value>(
+          mine, mine + kSubB, key0, st, a,
+          [&]() {
+            CA_WAIT_LDS();
+            if (more) fetch_k(it + 1);
+          },
+          [&]() {
+            if (more) CA_WAIT_VM(8);
+            else CA_WAIT_VM(0);
+          },
+          [&]() {
+            CA_WAIT_LDS();
+            if (more) fetch_v(it + 1);
+          });
+    };
+    key0 >= flo && key0 + kKeysSub <= fhi ? step(std::true_type()) : step(std::false_type());
   }
   // The waves' sums: column c's 128 values at 512 c, 16-byte chunk C at place C ^ (c & 15).
 #pragma unroll
@@ -691,9 +674,11 @@ __device__ __forceinline__ void ca_rows_form(const CaArgs& a, const CaWork& w, c
     if (left >= kRing) fetch(it + kRing - 1);
     const int key0 = it * kRowsStep;
     const uint8_t* sk = lds + (it & (kRing - 1)) * 2 * kRowsB;
-    if (key0 < khi && key0 + kRowsStep > klo)
-      ca_step<DT, NC, 4, MADE>(sk, sk + kRowsB, key0, key0 >= flo && key0 + kRowsStep <= fhi, st, a, []() {}, []() {},
-                               []() { CA_WAIT_LDS(); });
+    auto step = [&](auto full) {
+      ca_step<DT, NC, 4, MADE, decltype(full)::value>(sk, sk + kRowsB, key0, st, a, []() {}, []() {}, []() { CA_WAIT_LDS(); });
+    };
+    if (key0 >= flo && key0 + kRowsStep <= fhi) step(std::true_type());
+    else if (key0 < khi && key0 + kRowsStep > klo) step(std::false_type());
   }
   const int H = a.G * a.gs;
   const bool alone = ca_alone(a, w);
