@@ -43,6 +43,8 @@ FILE_FLAGS = {
     # The decoder kernels round every float32 product and sum separately, as
     # the reference's torch expressions do.
     "ls_model": ["-ffp-contract=off"],
+    # As for ls_select: the running sums are rescaled by ordinary instructions.
+    "ls_cache_attention": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

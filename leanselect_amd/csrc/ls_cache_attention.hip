@@ -44,8 +44,11 @@ constexpr int kRing = 4;
 constexpr int kLdsBytes = 2 * kWaves * kSubB;  // 128 KB: the keys form's, and a ring of 4 in the rows form
 static_assert(kLdsBytes == kRing * 2 * kRowsB, "one allocation serves both forms");
 
+// LDS by 32-bit offsets: a pointer of the general kind takes two registers.
 typedef short CaS4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) CaS4* CaLdsS4;
+typedef __attribute__((address_space(3))) CaS4 CaLdsS4;
+typedef __attribute__((address_space(3))) const ls_u32x4 CaLdsU4;
+typedef __attribute__((address_space(3))) ls_f32x4 CaLdsF4;
 
 #define CA_WAIT_VM(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
 #define CA_WAIT_LDS() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
@@ -77,9 +80,12 @@ struct CaArgs {
   int batch;
   int G;
   int gs;
-  float scale2;  // scale log2(e)
-  float cap_a;   // cap log2(e), 0: none
-  float cap_b;   // 2 scale log2(e) / cap
+  // Base-2 scores are alpha z + beta: z = q.k, alpha = scale log2(e), beta = 0, or with a cap
+  // z = -1 / (1 + 2^(cap_b q.k)), alpha = 2 cap log2(e), beta = alpha / 2, cap_b = 2 scale log2(e) / cap
+  // (cap tanh(x / cap) = cap - 2 cap / (1 + exp(2 x / cap))); with slopes the score itself, less its bias.
+  float alpha;
+  float beta;
+  float cap_b;  // 0: no cap
   const float* slopes;
   int64_t slopes_bs;
   int causal;
@@ -103,13 +109,6 @@ __device__ __forceinline__ float ca_max4(float x) {
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ float ca_sum4(float x) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 __device__ __forceinline__ int ca_min64(int x) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) x = min(x, __shfl_xor(x, d, 64));
@@ -138,13 +137,20 @@ template <> struct CaBias<LS_F16> { static constexpr float value = 10.f; };
 // The maximum follows once it is this far behind (base-2 units): weights reach 2^(kLazy + value).
 constexpr float kLazy = 5.f;
 
+// Two floats as bf16, to nearest even.
+__device__ __forceinline__ uint32_t ca_bf16x2(float a, float b) {
+  typedef float F2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((F2{a, b}), B2));
+}
+
 // Two weights' heads (x), cut off, and remainders (y).
 template <int DT>
 __device__ __forceinline__ uint2 ca_split(float p0, float p1) {
   if constexpr (DT == LS_BF16) {
     const uint32_t b0 = __float_as_uint(p0) & 0xffff0000u, b1 = __float_as_uint(p1) & 0xffff0000u;
     return make_uint2(__builtin_amdgcn_perm(b1, b0, 0x07060302u),
-                      ls_pack2(ls_f32_to_bf16(p0 - __uint_as_float(b0)), ls_f32_to_bf16(p1 - __uint_as_float(b1))));
+                      ca_bf16x2(p0 - __uint_as_float(b0), p1 - __uint_as_float(b1)));
   } else {
     const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
     return make_uint2(__builtin_bit_cast(uint32_t, h),
@@ -157,61 +163,62 @@ template <int NC>
 struct CaState {
   ls_u32x4 qf[NC][4];
   ls_f32x4 o[8][NC];
-  float m[NC], l[NC];
+  ls_f32x4 l[NC];             // the sum of a column's weights, by a product with ones: four times the same
+  float m[NC];
   float slope2[NC], pos[NC];  // position among the source's keys
   int lo[NC], hi[NC];         // visible keys, among the source's
 };
 
 // One step: 16 KB keys from key0, K rows at sk and V rows at sv (LDS, swizzled).  `k_read` is called
 // once K has been read, `v_ready` before V is, `v_read` after.  FULL: every column sees all of them.
-// MADE: with cap or slopes.
-template <int DT, int NC, int KB, bool MADE, bool FULL, class KRead, class VReady, class VRead>
-__device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, int key0, CaState<NC>& st,
+template <int DT, int NC, int KB, bool FULL, class KRead, class VReady, class VRead>
+__device__ __forceinline__ void ca_step(uint32_t sk, uint32_t sv, int key0, CaState<NC>& st,
                                         const CaArgs& a, KRead k_read, VReady v_ready, VRead v_read) {
   const int lane = ls_lane(), r = lane & 15, q = lane >> 4;
+  // Left operands are read one block ahead of their products, and no further: registers.
   ls_f32x4 s[KB][NC];
-  const int ka = r * kRowB + 16 * (q ^ r);
+  const uint32_t ka = r * kRowB + 16 * (q ^ r);
+  ls_u32x4 kf[2][4];
+  auto keys = [&](int t, ls_u32x4(&f)[4]) {
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+      f[ks] = *(CaLdsU4*)(sk + 16 * kRowB * t + (ka ^ (64 * ks)));
+  };
+  keys(0, kf[0]);
 #pragma unroll
   for (int t = 0; t < KB; ++t) {
+    if (t + 1 < KB) keys(t + 1, kf[(t + 1) & 1]);
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) s[t][nc] = ls_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const ls_u32x4 kf = *reinterpret_cast<const ls_u32x4*>(sk + 16 * kRowB * t + (ka ^ (64 * ks)));
+    for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-      for (int nc = 0; nc < NC; ++nc) s[t][nc] = LsElem<DT>::mfma(kf, st.qf[nc][ks], s[t][nc]);
-    }
+      for (int nc = 0; nc < NC; ++nc) s[t][nc] = LsElem<DT>::mfma(kf[t & 1][ks], st.qf[nc][ks], s[t][nc]);
+    __builtin_amdgcn_sched_barrier(0);
   }
   k_read();
-  if (MADE) {
-    if (a.cap_a > 0.f) {
-      // cap tanh(x / cap) = cap - 2 cap / (1 + exp(2 x / cap))
+  float alpha = a.alpha, beta = a.beta;
+  if (a.cap_b > 0.f) {
 #pragma unroll
-      for (int nc = 0; nc < NC; ++nc)
+    for (int nc = 0; nc < NC; ++nc)
 #pragma unroll
-        for (int t = 0; t < KB; ++t)
+      for (int t = 0; t < KB; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float w = __builtin_amdgcn_exp2f(s[t][nc][i] * a.cap_b);
-            s[t][nc][i] = fmaf(-2.f * a.cap_a, __builtin_amdgcn_rcpf(1.f + w), a.cap_a);
-          }
-    } else {
+        for (int i = 0; i < 4; ++i)
+          s[t][nc][i] = __builtin_amdgcn_rcpf(-1.f - __builtin_amdgcn_exp2f(s[t][nc][i] * a.cap_b));
+  }
+  if (a.slopes) {
 #pragma unroll
-      for (int nc = 0; nc < NC; ++nc)
+    for (int nc = 0; nc < NC; ++nc) {
+      const float d0 = st.pos[nc] - (float)(key0 + 4 * q);
 #pragma unroll
-        for (int t = 0; t < KB; ++t) s[t][nc] *= a.scale2;
+      for (int t = 0; t < KB; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[t][nc][i] = fmaf(-st.slope2[nc], fabsf(d0 - (float)(16 * t + i)), fmaf(s[t][nc][i], alpha, beta));
     }
-    if (a.slopes) {
-#pragma unroll
-      for (int nc = 0; nc < NC; ++nc) {
-        const float d0 = st.pos[nc] - (float)(key0 + 4 * q);
-#pragma unroll
-        for (int t = 0; t < KB; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            s[t][nc][i] = fmaf(-st.slope2[nc], fabsf(d0 - (float)(16 * t + i)), s[t][nc][i]);
-      }
-    }
+    alpha = 1.f;
+    beta = 0.f;
   }
   if (!FULL) {
 #pragma unroll
@@ -227,13 +234,12 @@ __device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, in
   ls_u32x4 hi[KB / 2][NC], lo[KB / 2][NC];
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) {
-    float top = -INFINITY;
+    float top = s[0][nc][0];
 #pragma unroll
     for (int t = 0; t < KB; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][nc][i]);
-    top = ca_max4(top);
-    if (!MADE) top *= a.scale2;  // (scale2 is positive)
+      for (int i = 0; i < 4; ++i) top = ls_fmax_nan(top, s[t][nc][i]);
+    top = fmaf(ca_max4(top), alpha, beta);
     if (__any(top > st.m[nc] + kLazy)) {
       const float m = fmaxf(st.m[nc], top);
       const float f = __builtin_amdgcn_exp2f(st.m[nc] - (m == -INFINITY ? 0.f : m));
@@ -242,16 +248,12 @@ __device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, in
 #pragma unroll
       for (int db = 0; db < 8; ++db) st.o[db][nc] *= f;
     }
-    const float ref = (st.m[nc] == -INFINITY ? 0.f : st.m[nc]) - CaBias<DT>::value;
-    float sum = 0.f;
+    const float ref = beta + CaBias<DT>::value - (st.m[nc] == -INFINITY ? 0.f : st.m[nc]);
 #pragma unroll
     for (int t = 0; t < KB; ++t) {
       float p[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(MADE ? s[t][nc][i] - ref : fmaf(s[t][nc][i], a.scale2, -ref));
-        sum += p[i];
-      }
+      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(s[t][nc][i], alpha, ref));
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const uint2 w = ca_split<DT>(p[2 * e], p[2 * e + 1]);
@@ -259,36 +261,56 @@ __device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, in
         lo[t / 2][nc][2 * (t & 1) + e] = w.y;
       }
     }
-    st.l[nc] += sum;
   }
   v_ready();
   // Lane (r, q) of the transposing read gives its group of 16 the rows 4 q + (r >> 2), 8 bytes each,
   // and gets dim r of the rows 4 q .. 4 q + 3.
   const int row = 4 * q + (r >> 2);
-  const int va = row * kRowB + 32 * (row & 7) + 8 * (r & 3);
+  const uint32_t va = row * kRowB + 32 * (row & 7) + 8 * (r & 3);
   auto values = [&](int half, int db) {
-    const uint8_t* p = sv + 32 * kRowB * half + (va ^ (32 * db));
-    const CaS4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CaLdsS4)(p));
-    const CaS4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CaLdsS4)(p + 16 * kRowB));
+    const uint32_t p = sv + 32 * kRowB * half + (va ^ (32 * db));
+    const CaS4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CaLdsS4*)p);
+    const CaS4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((CaLdsS4*)(p + 16 * kRowB));
     const uint2 w0 = __builtin_bit_cast(uint2, v0), w1 = __builtin_bit_cast(uint2, v1);
     return ls_u32x4{w0.x, w0.y, w1.x, w1.y};
   };
-  if (FULL) {
+  constexpr uint32_t kExp = DT == LS_BF16 ? 0x7f80u : 0x7c00u, kOne = DT == LS_BF16 ? 0x3f80u : 0x3c00u;
+  {
+    constexpr uint32_t kOnes = kOne | kOne << 16;
+    const ls_u32x4 ones = {kOnes, kOnes, kOnes, kOnes};
 #pragma unroll
     for (int half = 0; half < KB / 2; ++half)
 #pragma unroll
-      for (int db = 0; db < 8; ++db) {
-        const ls_u32x4 v = values(half, db);
-#pragma unroll
-        for (int nc = 0; nc < NC; ++nc) st.o[db][nc] = LsElem<DT>::mfma(v, hi[half][nc], st.o[db][nc]);
-#pragma unroll
-        for (int nc = 0; nc < NC; ++nc) st.o[db][nc] = LsElem<DT>::mfma(v, lo[half][nc], st.o[db][nc]);
+      for (int nc = 0; nc < NC; ++nc) {
+        st.l[nc] = LsElem<DT>::mfma(ones, hi[half][nc], st.l[nc]);
+        st.l[nc] = LsElem<DT>::mfma(ones, lo[half][nc], st.l[nc]);
       }
+  }
+  if (FULL) {
+    constexpr int kBlocks = 4 * KB;  // (half, db)
+    ls_u32x4 vf[2][2];
+    auto pair = [&](int i, ls_u32x4(&f)[2]) {
+      f[0] = values(i >> 3, i & 7);
+      f[1] = values(i >> 3, (i & 7) + 1);
+    };
+    pair(0, vf[0]);
+#pragma unroll
+    for (int i = 0; i < kBlocks; i += 2) {
+      if (i + 2 < kBlocks) pair(i + 2, vf[(i / 2 + 1) & 1]);
+      const int half = i >> 3, db = i & 7;
+#pragma unroll
+      for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int nc = 0; nc < NC; ++nc)
+            st.o[db + e][nc] = LsElem<DT>::mfma(vf[(i / 2) & 1][e], part ? lo[half][nc] : hi[half][nc], st.o[db + e][nc]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   } else {
     // Where a key is hidden from some column, its weight there is 0 and its values must not count:
     // 0 times an infinity or NaN would.  Such values leave the product, and the channels of the columns
     // that see one become NaN.
-    constexpr uint32_t kExp = DT == LS_BF16 ? 0x7f80u : 0x7c00u, kOne = DT == LS_BF16 ? 0x3f80u : 0x3c00u;
 #pragma unroll
     for (int half = 0; half < KB / 2; ++half) {
       ls_u32x4 see[NC];
@@ -319,6 +341,7 @@ __device__ __forceinline__ void ca_step(const uint8_t* sk, const uint8_t* sv, in
           for (int e = 0; e < 4; ++e)
             if (hits[e] > 0.f) st.o[db][nc][e] = __builtin_nanf("");
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -438,7 +461,7 @@ __device__ __forceinline__ void ca_columns(const CaArgs& a, const CaWork& w, int
     st.lo[nc] = 0;
     st.hi[nc] = w.n_keys;
     st.m[nc] = -INFINITY;
-    st.l[nc] = 0.f;
+    st.l[nc] = ls_f32x4{0.f, 0.f, 0.f, 0.f};
     st.pos[nc] = st.slope2[nc] = 0.f;
     if (a.slopes || a.causal || a.left >= 0 || a.right >= 0) {
       int n0 = w.n0, n1 = w.n1, len = w.len, b = w.seq;
@@ -498,20 +521,24 @@ __device__ __forceinline__ void ca_steps(const CaWork& w, int klo, int khi, int 
 // last are the last one again.
 template <bool IS_V, int N>
 __device__ __forceinline__ void ca_fetch(const uint16_t* base, int64_t rs, int row0, int n_keys, int i0, uint32_t lds) {
-  const int lane = ls_lane(), i4 = lane >> 4;
+  int lane = ls_lane();
+  asm volatile("" : "+v"(lane));  // offsets are formed here, not kept in registers over a loop
+  const int i4 = lane >> 4;
   const uint32_t rb = 2 * (uint32_t)rs;
-  const uint16_t* p = base + (int64_t)row0 * rs;
-  const bool whole = row0 + 4 * N <= n_keys;
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
+  auto chunk = [&](int j) {
     const int i = i0 + 4 * j + i4;
-    const uint32_t chunk = 16 * ((uint32_t)(lane & 15) ^ (uint32_t)(IS_V ? 2 * (i & 7) : i & 15));
-    if (whole)
-      ls_dma16(p + 4 * j * rs, (uint32_t)i4 * rb + chunk, lds + 1024 * j);
-    else if (row0 < n_keys)
-      ls_dma16(p, (uint32_t)min(4 * j + i4, n_keys - 1 - row0) * rb + chunk, lds + 1024 * j);
-    else  // (none: the last row of all, for every row)
-      ls_dma16(base + (int64_t)(n_keys - 1) * rs, chunk, lds + 1024 * j);
+    return 16 * ((uint32_t)(lane & 15) ^ (uint32_t)(IS_V ? 2 * (i & 7) : i & 15));
+  };
+  if (row0 + 4 * N <= n_keys) {
+    const uint16_t* p = base + (int64_t)row0 * rs;
+#pragma unroll
+    for (int j = 0; j < N; ++j) ls_dma16(p + 4 * j * rs, (uint32_t)i4 * rb + chunk(j), lds + 1024 * j);
+  } else {
+    const int first = min(row0, n_keys - 1);
+    const uint16_t* p = base + (int64_t)first * rs;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      ls_dma16(p, (uint32_t)(min(row0 + 4 * j + i4, n_keys - 1) - first) * rb + chunk(j), lds + 1024 * j);
   }
 }
 
@@ -537,8 +564,8 @@ __device__ __forceinline__ bool ca_alone(const CaArgs& a, const CaWork& w) {
 // the wave's own, with no barrier: the next step's K is on its way from when this one's has been
 // read, V likewise.  The waves' sums are joined through LDS at the end.
 // ---------------------------------------------------------------------------
-template <int DT, int NC, bool MADE>
-__device__ __forceinline__ void ca_keys_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint8_t* lds,
+template <int DT, int NC>
+__device__ __forceinline__ void ca_keys_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint32_t lds,
                                              float* s_m, float* s_l) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
@@ -550,48 +577,48 @@ __device__ __forceinline__ void ca_keys_form(const CaArgs& a, const CaWork& w, c
   const int sub = wave * kKeysSub;
   while (it < end && (end - 1) * kKeysStep + sub >= khi) --end;  // the last step may not reach this wave
   while (it < end && it * kKeysStep + sub + kKeysSub <= klo) ++it;
-  uint8_t* mine = lds + 2 * wave * kSubB;
-  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)mine;
-  auto fetch_k = [&](int i) { ca_fetch<false, 8>(w.k, w.rs, i * kKeysStep + sub, w.n_keys, 0, at); };
-  auto fetch_v = [&](int i) { ca_fetch<true, 8>(w.v, w.rs, i * kKeysStep + sub, w.n_keys, 0, at + kSubB); };
+  const uint32_t mine = lds + 2 * wave * kSubB;
+  auto fetch_k = [&](int i) { ca_fetch<false, 8>(w.k, w.rs, i * kKeysStep + sub, w.n_keys, 0, mine); };
+  auto fetch_v = [&](int i) { ca_fetch<true, 8>(w.v, w.rs, i * kKeysStep + sub, w.n_keys, 0, mine + kSubB); };
   if (it < end) {
     fetch_k(it);
     fetch_v(it);
   }
-  for (; it < end; ++it) {
+  auto full = [&](int i) { return i * kKeysStep + sub >= flo && i * kKeysStep + sub + kKeysSub <= fhi; };
+  auto step = [&](auto is_full) {
     const bool more = it + 1 < end;
-    const int key0 = it * kKeysStep + sub;
     CA_WAIT_VM(8);  // V behind K
-    auto step = [&](auto full) {
-      ca_step<DT, NC, 2, MADE, decltype(full)::value>(
-          mine, mine + kSubB, key0, st, a,
-          [&]() {
-            CA_WAIT_LDS();
-            if (more) fetch_k(it + 1);
-          },
-          [&]() {
-            if (more) CA_WAIT_VM(8);
-            else CA_WAIT_VM(0);
-          },
-          [&]() {
-            CA_WAIT_LDS();
-            if (more) fetch_v(it + 1);
-          });
-    };
-    key0 >= flo && key0 + kKeysSub <= fhi ? step(std::true_type()) : step(std::false_type());
+    ca_step<DT, NC, 2, decltype(is_full)::value>(
+        mine, mine + kSubB, it * kKeysStep + sub, st, a,
+        [&]() {
+          CA_WAIT_LDS();
+          if (more) fetch_k(it + 1);
+        },
+        [&]() {
+          if (more) CA_WAIT_VM(8);
+          else CA_WAIT_VM(0);
+        },
+        [&]() {
+          CA_WAIT_LDS();
+          if (more) fetch_v(it + 1);
+        });
+  };
+  while (it < end) {  // (loops of their own: the sums stay in one set of registers)
+    for (; it < end && !full(it); ++it) step(std::false_type());
+    for (; it < end && full(it); ++it) step(std::true_type());
   }
   // The waves' sums: column c's 128 values at 512 c, 16-byte chunk C at place C ^ (c & 15).
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) {
     const int c = 16 * nc + r;
-    const float l = ca_sum4(st.l[nc]);
+    const float l = st.l[nc][0];
     if (q == 0) {
       s_m[wave * 32 + c] = st.m[nc];
       s_l[wave * 32 + c] = l;
     }
 #pragma unroll
     for (int db = 0; db < 8; ++db)
-      *reinterpret_cast<ls_f32x4*>(mine + 512 * c + 16 * ((4 * db + q) ^ r)) = st.o[db][nc];
+      *(CaLdsF4*)(mine + 512 * c + 16 * ((4 * db + q) ^ r)) = st.o[db][nc];
   }
   __syncthreads();
   const int H = a.G * a.gs;
@@ -610,7 +637,7 @@ __device__ __forceinline__ void ca_keys_form(const CaArgs& a, const CaWork& w, c
       if (l == 0.f) continue;  // nothing visible
       const float f = m == M ? 1.f : __builtin_amdgcn_exp2f(m - M);
       L += f * l;
-      v += f * *reinterpret_cast<const ls_f32x4*>(lds + 2 * i * kSubB + 512 * c + 16 * (ch ^ (c & 15)));
+      v += f * *(CaLdsF4*)(lds + 2 * i * kSubB + 512 * c + 16 * (ch ^ (c & 15)));
     }
     const int64_t row = (int64_t)(w.t0 + tk) * H + w.g * a.gs + h;
     M -= CaBias<DT>::value;
@@ -629,11 +656,11 @@ __device__ __forceinline__ void ca_keys_form(const CaArgs& a, const CaWork& w, c
 
 // ---------------------------------------------------------------------------
 // Rows form, many columns (kWaves x 16 NC).  A ring of four steps of 64 keys; each wave fetches 8
-// rows of a step's K and V, and a barrier a step tells that the step has come and the one before has been
-// read.
+// rows of a step's K and V.  A barrier every two steps tells that the next two have come and the two
+// before have been read.
 // ---------------------------------------------------------------------------
-template <int DT, int NC, bool MADE>
-__device__ __forceinline__ void ca_rows_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint8_t* lds,
+template <int DT, int NC>
+__device__ __forceinline__ void ca_rows_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint32_t lds,
                                              int* s_range) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
@@ -655,37 +682,46 @@ __device__ __forceinline__ void ca_rows_form(const CaArgs& a, const CaWork& w, c
   lo_all = __builtin_amdgcn_readfirstlane(lo_all);
   hi_all = __builtin_amdgcn_readfirstlane(hi_all);
   ca_steps(w, lo_all, hi_all, kRowsStep, it, end);
-  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
   auto fetch = [&](int i) {
-    const uint32_t to = at + (uint32_t)(i & (kRing - 1)) * 2 * kRowsB + 2048 * wave;
+    const uint32_t to = lds + (uint32_t)(i & (kRing - 1)) * 2 * kRowsB + 2048 * wave;
     ca_fetch<false, 2>(w.k, w.rs, i * kRowsStep + 8 * wave, w.n_keys, 8 * wave, to);
     ca_fetch<true, 2>(w.v, w.rs, i * kRowsStep + 8 * wave, w.n_keys, 8 * wave, to + kRowsB);
   };
-#pragma unroll
-  for (int i = 0; i < kRing - 1; ++i)
-    if (it + i < end) fetch(it + i);
-  for (; it < end; ++it) {
-    const int left = end - it;
-    if (left > 2) CA_WAIT_VM(8);
-    else if (left == 2) CA_WAIT_VM(4);
-    else CA_WAIT_VM(0);
+  auto fetch_pair = [&](int i) {
+    if (i < end) fetch(i);
+    if (i + 1 < end) fetch(i + 1);
+  };
+  const int begin = it;
+  fetch_pair(it);
+  auto next = [&]() {
+    if ((it - begin) & 1) return;
+    CA_WAIT_VM(0);
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (left >= kRing) fetch(it + kRing - 1);
-    const int key0 = it * kRowsStep;
-    const uint8_t* sk = lds + (it & (kRing - 1)) * 2 * kRowsB;
-    auto step = [&](auto full) {
-      ca_step<DT, NC, 4, MADE, decltype(full)::value>(sk, sk + kRowsB, key0, st, a, []() {}, []() {}, []() { CA_WAIT_LDS(); });
-    };
-    if (key0 >= flo && key0 + kRowsStep <= fhi) step(std::true_type());
-    else if (key0 < khi && key0 + kRowsStep > klo) step(std::false_type());
+    fetch_pair(it + 2);
+  };
+  auto full = [&](int i) { return i * kRowsStep >= flo && i * kRowsStep + kRowsStep <= fhi; };
+  auto step = [&](auto is_full) {
+    const uint32_t sk = lds + (uint32_t)(it & (kRing - 1)) * 2 * kRowsB;
+    ca_step<DT, NC, 4, decltype(is_full)::value>(sk, sk + kRowsB, it * kRowsStep, st, a, []() {}, []() {},
+                                                 []() { CA_WAIT_LDS(); });
+  };
+  while (it < end) {  // (loops of their own: the sums stay in one set of registers)
+    for (; it < end && !full(it); ++it) {
+      next();
+      if (it * kRowsStep < khi && it * kRowsStep + kRowsStep > klo) step(std::false_type());
+    }
+    for (; it < end && full(it); ++it) {
+      next();
+      step(std::true_type());
+    }
   }
   const int H = a.G * a.gs;
   const bool alone = ca_alone(a, w);
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) {
     const int c = 16 * (NC * wave + nc) + r, tk = c / a.gs, h = c - tk * a.gs;
-    const float L = ca_sum4(st.l[nc]), M = st.m[nc] - CaBias<DT>::value;
+    const float L = st.l[nc][0], M = st.m[nc] - CaBias<DT>::value;
     if (tk >= cut.tokens || w.t0 + tk >= w.t1) continue;
     const int64_t row = (int64_t)(w.t0 + tk) * H + w.g * a.gs + h;
     if (alone) {
@@ -710,22 +746,23 @@ __device__ __forceinline__ void ca_rows_form(const CaArgs& a, const CaWork& w, c
 // Forms: 1, 2: keys, NC 1 or 2; 3, 4: rows, NC 1 or 2; 0: no such items.
 template <int FORM> constexpr int ca_cols() { return FORM == 0 ? 0 : FORM <= 2 ? 16 * FORM : kWaves * 16 * (FORM - 2); }
 
-template <int DT, int FORM, bool MADE>
-__device__ __forceinline__ void ca_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint8_t* lds, float* small) {
-  if constexpr (FORM == 1 || FORM == 2) ca_keys_form<DT, FORM, MADE>(a, w, cut, lds, small, small + 32 * kWaves);
-  if constexpr (FORM == 3 || FORM == 4) ca_rows_form<DT, FORM - 2, MADE>(a, w, cut, lds, reinterpret_cast<int*>(small));
+template <int DT, int FORM>
+__device__ __forceinline__ void ca_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint32_t lds, float* small) {
+  if constexpr (FORM == 1 || FORM == 2) ca_keys_form<DT, FORM>(a, w, cut, lds, small, small + 32 * kWaves);
+  if constexpr (FORM == 3 || FORM == 4) ca_rows_form<DT, FORM - 2>(a, w, cut, lds, reinterpret_cast<int*>(small));
 }
 
-template <int DT, int PRE, int OWN, bool MADE>
+template <int DT, int PRE, int OWN>
 __global__ __launch_bounds__(kThreads) void ls_cache_attn_kernel(const CaArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kLdsBytes];
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[kLdsBytes];
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ring;
   __shared__ float small[2 * 32 * kWaves];
   const int item = blockIdx.x;
   CaWork w;
   if (PRE != 0 && item < a.pre.items) {
-    if (ca_prefix_work(a, item, w)) ca_form<DT, PRE, MADE>(a, w, a.pre, lds, small);
+    if (ca_prefix_work(a, item, w)) ca_form<DT, PRE>(a, w, a.pre, lds, small);
   } else {
-    if (ca_own_work(a, item - a.pre.items, w)) ca_form<DT, OWN, MADE>(a, w, a.own, lds, small);
+    if (ca_own_work(a, item - a.pre.items, w)) ca_form<DT, OWN>(a, w, a.own, lds, small);
   }
 }
 
@@ -858,11 +895,8 @@ CaPlan ca_plan(int64_t total_q, int batch, int H, int G, int64_t p_len, int64_t 
 
 template <int DT, int PRE, int OWN>
 void ca_launch(const CaArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.pre.items + a.own.items));
-  if (a.cap_a > 0.f || a.slopes)
-    hipLaunchKernelGGL((ls_cache_attn_kernel<DT, PRE, OWN, true>), grid, dim3(kThreads), 0, s, a);
-  else
-    hipLaunchKernelGGL((ls_cache_attn_kernel<DT, PRE, OWN, false>), grid, dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL((ls_cache_attn_kernel<DT, PRE, OWN>), dim3((unsigned)(a.pre.items + a.own.items)),
+                     dim3(kThreads), 0, s, a);
 }
 
 template <int DT>
@@ -955,8 +989,8 @@ extern "C" int ls_cache_attn(const void* q, int64_t q_row_stride, const int32_t*
   a.batch = batch;
   a.G = num_kv_heads;
   a.gs = gs;
-  a.scale2 = softmax_scale * kLog2e;
-  a.cap_a = softcap * kLog2e;
+  a.alpha = softcap > 0.f ? 2.f * softcap * kLog2e : softmax_scale * kLog2e;
+  a.beta = softcap > 0.f ? softcap * kLog2e : 0.f;
   a.cap_b = softcap > 0.f ? 2.f * softmax_scale * kLog2e / softcap : 0.f;
   a.slopes = alibi_slopes;
   a.slopes_bs = alibi_batch_stride;
