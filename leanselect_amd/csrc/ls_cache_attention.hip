@@ -158,6 +158,15 @@ __device__ __forceinline__ uint2 ca_split(float p0, float p1) {
   }
 }
 
+// All ones in each half that holds an infinity or NaN: an exponent of ones plus its lowest bit carries
+// into the sign.
+template <int DT>
+__device__ __forceinline__ uint32_t ca_odd(uint32_t w) {
+  typedef short S2 __attribute__((ext_vector_type(2)));
+  constexpr uint32_t kExp = DT == LS_BF16 ? 0x7f807f80u : 0x7c007c00u, kLow = DT == LS_BF16 ? 0x00800080u : 0x04000400u;
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(S2, (w & kExp) + kLow) >> 15);
+}
+
 // What a wave's columns see, and what is carried over its keys.
 template <int NC>
 struct CaState {
@@ -184,6 +193,9 @@ __device__ __forceinline__ void ca_step(uint32_t sk, uint32_t sv, int key0, CaSt
     for (int ks = 0; ks < 4; ++ks)
       f[ks] = *(CaLdsU4*)(sk + 16 * kRowB * t + (ka ^ (64 * ks)));
   };
+  // A wave that feeds the matrix unit goes first; the other one of its SIMD has vector work to do
+  // (a 1024-row chunk behind 32K tokens 1076 -> 1025 us).
+  __builtin_amdgcn_s_setprio(1);
   keys(0, kf[0]);
 #pragma unroll
   for (int t = 0; t < KB; ++t) {
@@ -196,6 +208,7 @@ __device__ __forceinline__ void ca_step(uint32_t sk, uint32_t sv, int key0, CaSt
       for (int nc = 0; nc < NC; ++nc) s[t][nc] = LsElem<DT>::mfma(kf[t & 1][ks], st.qf[nc][ks], s[t][nc]);
     __builtin_amdgcn_sched_barrier(0);
   }
+  __builtin_amdgcn_s_setprio(0);
   k_read();
   float alpha = a.alpha, beta = a.beta;
   if (a.cap_b > 0.f) {
@@ -263,6 +276,7 @@ __device__ __forceinline__ void ca_step(uint32_t sk, uint32_t sv, int key0, CaSt
     }
   }
   v_ready();
+  __builtin_amdgcn_s_setprio(1);
   // Lane (r, q) of the transposing read gives its group of 16 the rows 4 q + (r >> 2), 8 bytes each,
   // and gets dim r of the rows 4 q .. 4 q + 3.
   const int row = 4 * q + (r >> 2);
@@ -274,7 +288,7 @@ __device__ __forceinline__ void ca_step(uint32_t sk, uint32_t sv, int key0, CaSt
     const uint2 w0 = __builtin_bit_cast(uint2, v0), w1 = __builtin_bit_cast(uint2, v1);
     return ls_u32x4{w0.x, w0.y, w1.x, w1.y};
   };
-  constexpr uint32_t kExp = DT == LS_BF16 ? 0x7f80u : 0x7c00u, kOne = DT == LS_BF16 ? 0x3f80u : 0x3c00u;
+  constexpr uint32_t kOne = DT == LS_BF16 ? 0x3f80u : 0x3c00u;
   {
     constexpr uint32_t kOnes = kOne | kOne << 16;
     const ls_u32x4 ones = {kOnes, kOnes, kOnes, kOnes};
@@ -309,42 +323,57 @@ __device__ __forceinline__ void ca_step(uint32_t sk, uint32_t sv, int key0, CaSt
     }
   } else {
     // Where a key is hidden from some column, its weight there is 0 and its values must not count:
-    // 0 times an infinity or NaN would.  Such values leave the product, and the channels of the columns
-    // that see one become NaN.
+    // 0 times an infinity or NaN would.  Such values leave the product.
+    uint32_t some = 0;
 #pragma unroll
-    for (int half = 0; half < KB / 2; ++half) {
-      ls_u32x4 see[NC];
-#pragma unroll
-      for (int nc = 0; nc < NC; ++nc) {
-        const int l0 = st.lo[nc] - (key0 + 4 * q), h0 = st.hi[nc] - (key0 + 4 * q);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = 32 * half + 16 * (e >> 1) + 2 * (e & 1);
-          see[nc][e] = (k >= l0 && k < h0 ? kOne : 0u) | (k + 1 >= l0 && k + 1 < h0 ? kOne << 16 : 0u);
-        }
-      }
+    for (int half = 0; half < KB / 2; ++half)
 #pragma unroll
       for (int db = 0; db < 8; ++db) {
-        ls_u32x4 v = values(half, db), is;
+        ls_u32x4 v = values(half, db);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t odd = ((v[e] & kExp) == kExp ? 0xffffu : 0u) | ((v[e] >> 16 & kExp) == kExp ? 0xffff0000u : 0u);
+          const uint32_t odd = ca_odd<DT>(v[e]);
           v[e] &= ~odd;
-          is[e] = odd & (kOne | kOne << 16);
+          some |= odd;
         }
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) st.o[db][nc] = LsElem<DT>::mfma(v, hi[half][nc], st.o[db][nc]);
+#pragma unroll
+        for (int nc = 0; nc < NC; ++nc) st.o[db][nc] = LsElem<DT>::mfma(v, lo[half][nc], st.o[db][nc]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    if (__any(some != 0)) {
+      // The channels of the columns that see one become NaN.
+#pragma unroll
+      for (int half = 0; half < KB / 2; ++half) {
+        ls_u32x4 see[NC];
 #pragma unroll
         for (int nc = 0; nc < NC; ++nc) {
-          const ls_f32x4 hits = LsElem<DT>::mfma(is, see[nc], ls_f32x4{0.f, 0.f, 0.f, 0.f});
-          st.o[db][nc] = LsElem<DT>::mfma(v, hi[half][nc], st.o[db][nc]);
-          st.o[db][nc] = LsElem<DT>::mfma(v, lo[half][nc], st.o[db][nc]);
+          const int l0 = st.lo[nc] - (key0 + 4 * q), h0 = st.hi[nc] - (key0 + 4 * q);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (hits[e] > 0.f) st.o[db][nc][e] = __builtin_nanf("");
+          for (int e = 0; e < 4; ++e) {
+            const int k = 32 * half + 16 * (e >> 1) + 2 * (e & 1);
+            see[nc][e] = (k >= l0 && k < h0 ? kOne : 0u) | (k + 1 >= l0 && k + 1 < h0 ? kOne << 16 : 0u);
+          }
         }
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int db = 0; db < 8; ++db) {
+          ls_u32x4 is = values(half, db);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) is[e] = ca_odd<DT>(is[e]) & (kOne | kOne << 16);
+#pragma unroll
+          for (int nc = 0; nc < NC; ++nc) {
+            const ls_f32x4 hits = LsElem<DT>::mfma(is, see[nc], ls_f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (hits[e] > 0.f) st.o[db][nc][e] = __builtin_nanf("");
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
   }
+  __builtin_amdgcn_s_setprio(0);
   v_read();
 }
 
