@@ -700,7 +700,7 @@ int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int32_t* cu_se
  */
 size_t ls_cache_attn_workspace_size(int64_t total_q, int32_t batch, int32_t num_heads,
                                     int32_t num_kv_heads, int64_t prefix_len, int64_t max_len,
-                                    int32_t n_splits);
+                                    int32_t window_left, int32_t n_splits);
 int ls_cache_attn(const void* q, int64_t q_row_stride, const int32_t* cu_seqlens_q, int64_t total_q,
                   const void* k_prefix, const void* v_prefix, int64_t prefix_row_stride,
                   int64_t prefix_len, const void* k_cache, const void* v_cache,

@@ -117,7 +117,7 @@ SIGNATURES = {
     "ls_attn_kvcache_q8": (
         _i32, [_p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _p, _i32, _i32, _i32, _i32,
                _i32, _p, _i32, _f32, _i32, _i32, _p, _p, _p, _sz, _p]),
-    "ls_cache_attn_workspace_size": (_sz, [_i64, _i32, _i32, _i32, _i64, _i64, _i32]),
+    "ls_cache_attn_workspace_size": (_sz, [_i64, _i32, _i32, _i32, _i64, _i64, _i32, _i32]),
     "ls_cache_attn": (
         _i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i32, _i32, _i32,
                _i32, _i32, _i64, _f32, _i32, _f32, _p, _i64, _i32, _i32, _i32, _p, _p, _p, _sz, _p]),

@@ -32,11 +32,13 @@ constexpr int kThreads = 64 * kWaves;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
 
-// Keys form: the waves share a step's keys, 32 each, and hold all of the tile's 16 NC columns.
+// Keys form: the waves share a step's keys, 32 each, and hold all of the tile's 16 columns.
 constexpr int kKeysSub = 32;
 constexpr int kKeysStep = kWaves * kKeysSub;
 constexpr int kSubB = kKeysSub * kRowB;
-// Rows form: the waves share the tile's columns, 16 NC each, and walk the same 64 keys a step.
+constexpr int kKeysCols = 16;
+// Rows form: the waves share the tile's 256 columns, 32 each, and walk the same keys, 64 a step.
+constexpr int kRowsCols = 32 * kWaves;
 constexpr int kRowsStep = 64;
 constexpr int kRowsB = kRowsStep * kRowB;
 constexpr int kRing = 4;
@@ -588,14 +590,33 @@ __device__ __forceinline__ bool ca_alone(const CaArgs& a, const CaWork& w) {
   return a.part == nullptr || (a.pre.items == 0 && w.slices == 1);
 }
 
+// Four channels (chunk ch of 32) of a column's sums: the final values, or the item's for the join.
+template <int DT>
+__device__ __forceinline__ void ca_store(const CaArgs& a, const CaWork& w, const CaCut& cut, bool alone, int c, int tk,
+                                         int h, int ch, float M, float L, ls_f32x4 v) {
+  const int64_t row = (int64_t)(w.t0 + tk) * (a.G * a.gs) + w.g * a.gs + h;
+  if (alone) {
+    ca_out4<DT>(a.out + row * kDim + 4 * ch, v, L == 0.f ? 0.f : 1.f / L);
+    if (ch == 0 && a.lse) a.lse[(int64_t)(w.g * a.gs + h) * a.total_q + w.t0 + tk] = ca_lse(M, L);
+  } else {
+    const int64_t place = (w.seq < 0 ? (int64_t)w.item * cut.cols
+                                     : (int64_t)a.pre.items * a.pre.cols + (int64_t)(w.item - a.pre.items) * cut.cols) + c;
+    if (L != 0.f) *reinterpret_cast<ls_f32x4*>(a.part + place * kDim + 4 * ch) = v;
+    if (ch == 0) a.ml[place] = make_float2(M, L);
+  }
+  if (ch == 0 && a.part && w.seq >= 0 && w.slice == 0)
+    a.rows[row] = alone ? make_int2(0, 0) : make_int2(w.item - a.pre.items, w.slices);
+}
+
 // ---------------------------------------------------------------------------
-// Keys form, few columns (16 NC).  Each key's bytes are read from LDS once, by one wave, from a place of
+// Keys form, few columns (16).  Each key's bytes are read from LDS once, by one wave, from a place of
 // the wave's own, with no barrier: the next step's K is on its way from when this one's has been
 // read, V likewise.  The waves' sums are joined through LDS at the end.
 // ---------------------------------------------------------------------------
-template <int DT, int NC>
+template <int DT>
 __device__ __forceinline__ void ca_keys_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint32_t lds,
                                              float* s_m, float* s_l) {
+  constexpr int NC = 1;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
   CaState<NC> st;
@@ -642,55 +663,40 @@ __device__ __forceinline__ void ca_keys_form(const CaArgs& a, const CaWork& w, c
     const int c = 16 * nc + r;
     const float l = st.l[nc][0];
     if (q == 0) {
-      s_m[wave * 32 + c] = st.m[nc];
-      s_l[wave * 32 + c] = l;
+      s_m[wave * kKeysCols + c] = st.m[nc];
+      s_l[wave * kKeysCols + c] = l;
     }
 #pragma unroll
     for (int db = 0; db < 8; ++db)
       *(CaLdsF4*)(mine + 512 * c + 16 * ((4 * db + q) ^ r)) = st.o[db][nc];
   }
   __syncthreads();
-  const int H = a.G * a.gs;
-  const bool alone = ca_alone(a, w);
+  const int c = tid >> 5, ch = tid & 31, tk = c / a.gs, h = c - tk * a.gs;
+  if (tk >= cut.tokens || w.t0 + tk >= w.t1) return;
+  float M = -INFINITY, L = 0.f;
 #pragma unroll
-  for (int e0 = 0; e0 < NC; ++e0) {
-    const int c = 16 * e0 + (tid >> 5), ch = tid & 31, tk = c / a.gs, h = c - tk * a.gs;
-    if (tk >= cut.tokens || w.t0 + tk >= w.t1) break;  // (later columns are beyond the tile's, too)
-    float M = -INFINITY, L = 0.f;
+  for (int i = 0; i < kWaves; ++i) M = fmaxf(M, s_m[i * kKeysCols + c]);
+  ls_f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) M = fmaxf(M, s_m[i * 32 + c]);
-    ls_f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      const float m = s_m[i * 32 + c], l = s_l[i * 32 + c];
-      if (l == 0.f) continue;  // nothing visible
-      const float f = m == M ? 1.f : __builtin_amdgcn_exp2f(m - M);
-      L += f * l;
-      v += f * *(CaLdsF4*)(lds + 2 * i * kSubB + 512 * c + 16 * (ch ^ (c & 15)));
-    }
-    const int64_t row = (int64_t)(w.t0 + tk) * H + w.g * a.gs + h;
-    M -= CaBias<DT>::value;
-    if (alone) {
-      ca_out4<DT>(a.out + row * kDim + 4 * ch, v, L == 0.f ? 0.f : 1.f / L);
-      if (ch == 0 && a.lse) a.lse[(int64_t)(w.g * a.gs + h) * a.total_q + w.t0 + tk] = ca_lse(M, L);
-    } else {
-      const int64_t place = (int64_t)w.item * cut.cols + c + (w.seq < 0 ? 0 : (int64_t)a.pre.items * (a.pre.cols - cut.cols));
-      if (L != 0.f) *reinterpret_cast<ls_f32x4*>(a.part + place * kDim + 4 * ch) = v;
-      if (ch == 0) a.ml[place] = make_float2(M, L);
-    }
-    if (ch == 0 && a.part && w.seq >= 0 && w.slice == 0)
-      a.rows[row] = alone ? make_int2(0, 0) : make_int2(w.item - a.pre.items, w.slices);
+  for (int i = 0; i < kWaves; ++i) {
+    const float m = s_m[i * kKeysCols + c], l = s_l[i * kKeysCols + c];
+    if (l == 0.f) continue;  // nothing visible
+    const float f = m == M ? 1.f : __builtin_amdgcn_exp2f(m - M);
+    L += f * l;
+    v += f * *(CaLdsF4*)(lds + 2 * i * kSubB + 512 * c + 16 * (ch ^ (c & 15)));
   }
+  ca_store<DT>(a, w, cut, ca_alone(a, w), c, tk, h, ch, M - CaBias<DT>::value, L, v);
 }
 
 // ---------------------------------------------------------------------------
-// Rows form, many columns (kWaves x 16 NC).  A ring of four steps of 64 keys; each wave fetches 8
+// Rows form, many columns.  A ring of four steps of 64 keys; each wave fetches 8
 // rows of a step's K and V.  A barrier every two steps tells that the next two have come and the two
 // before have been read.
 // ---------------------------------------------------------------------------
-template <int DT, int NC>
+template <int DT>
 __device__ __forceinline__ void ca_rows_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint32_t lds,
                                              int* s_range) {
+  constexpr int NC = 2;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, q = lane >> 4;
   CaState<NC> st;
@@ -729,7 +735,8 @@ __device__ __forceinline__ void ca_rows_form(const CaArgs& a, const CaWork& w, c
     asm volatile("" ::: "memory");
     fetch_pair(it + 2);
   };
-  auto full = [&](int i) { return i * kRowsStep >= flo && i * kRowsStep + kRowsStep <= fhi; };
+  // (a wave without columns only fetches)
+  auto full = [&](int i) { return khi > klo && i * kRowsStep >= flo && i * kRowsStep + kRowsStep <= fhi; };
   auto step = [&](auto is_full) {
     const uint32_t sk = lds + (uint32_t)(it & (kRing - 1)) * 2 * kRowsB;
     ca_step<DT, NC, 4, decltype(is_full)::value>(sk, sk + kRowsB, it * kRowsStep, st, a, []() {}, []() {},
@@ -745,118 +752,112 @@ __device__ __forceinline__ void ca_rows_form(const CaArgs& a, const CaWork& w, c
       step(std::true_type());
     }
   }
-  const int H = a.G * a.gs;
   const bool alone = ca_alone(a, w);
 #pragma unroll
   for (int nc = 0; nc < NC; ++nc) {
     const int c = 16 * (NC * wave + nc) + r, tk = c / a.gs, h = c - tk * a.gs;
-    const float L = st.l[nc][0], M = st.m[nc] - CaBias<DT>::value;
     if (tk >= cut.tokens || w.t0 + tk >= w.t1) continue;
-    const int64_t row = (int64_t)(w.t0 + tk) * H + w.g * a.gs + h;
-    if (alone) {
-      const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
-      for (int db = 0; db < 8; ++db) ca_out4<DT>(a.out + row * kDim + 16 * db + 4 * q, st.o[db][nc], inv);
-      if (q == 0 && a.lse) a.lse[(int64_t)(w.g * a.gs + h) * a.total_q + w.t0 + tk] = ca_lse(M, L);
-    } else {
-      const int64_t place = (int64_t)w.item * cut.cols + c + (w.seq < 0 ? 0 : (int64_t)a.pre.items * (a.pre.cols - cut.cols));
-      if (L != 0.f) {
-#pragma unroll
-        for (int db = 0; db < 8; ++db)
-          *reinterpret_cast<ls_f32x4*>(a.part + place * kDim + 16 * db + 4 * q) = st.o[db][nc];
-      }
-      if (q == 0) a.ml[place] = make_float2(M, L);
-    }
-    if (q == 0 && a.part && w.seq >= 0 && w.slice == 0)
-      a.rows[row] = alone ? make_int2(0, 0) : make_int2(w.item - a.pre.items, w.slices);
+    for (int db = 0; db < 8; ++db)
+      ca_store<DT>(a, w, cut, alone, c, tk, h, 4 * db + q, st.m[nc] - CaBias<DT>::value, st.l[nc][0], st.o[db][nc]);
   }
 }
 
-// Forms: 1, 2: keys, NC 1 or 2; 3, 4: rows, NC 1 or 2; 0: no such items.
-template <int FORM> constexpr int ca_cols() { return FORM == 0 ? 0 : FORM <= 2 ? 16 * FORM : kWaves * 16 * (FORM - 2); }
-
+// Forms: 0: no such items, 1: keys, 2: rows.
 template <int DT, int FORM>
 __device__ __forceinline__ void ca_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint32_t lds, float* small) {
-  if constexpr (FORM == 1 || FORM == 2) ca_keys_form<DT, FORM>(a, w, cut, lds, small, small + 32 * kWaves);
-  if constexpr (FORM == 3 || FORM == 4) ca_rows_form<DT, FORM - 2>(a, w, cut, lds, reinterpret_cast<int*>(small));
+  if constexpr (FORM == 1) ca_keys_form<DT>(a, w, cut, lds, small, small + kKeysCols * kWaves);
+  if constexpr (FORM == 2) ca_rows_form<DT>(a, w, cut, lds, reinterpret_cast<int*>(small));
 }
 
 template <int DT, int PRE, int OWN>
 __global__ __launch_bounds__(kThreads) void ls_cache_attn_kernel(const CaArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t ring[kLdsBytes];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)ring;
-  __shared__ float small[2 * 32 * kWaves];
+  __shared__ float small[2 * kKeysCols * kWaves];
   const int item = blockIdx.x;
+  const bool prefix = PRE != 0 && item < a.pre.items;
   CaWork w;
-  if (PRE != 0 && item < a.pre.items) {
-    if (ca_prefix_work(a, item, w)) ca_form<DT, PRE>(a, w, a.pre, lds, small);
-  } else {
-    if (ca_own_work(a, item - a.pre.items, w)) ca_form<DT, OWN>(a, w, a.own, lds, small);
-  }
+  if (!(prefix ? ca_prefix_work(a, item, w) : ca_own_work(a, item - a.pre.items, w))) return;
+  if constexpr (PRE == OWN || PRE == 0)
+    ca_form<DT, OWN>(a, w, prefix ? a.pre : a.own, lds, small);
+  else if (prefix)
+    ca_form<DT, PRE>(a, w, a.pre, lds, small);
+  else
+    ca_form<DT, OWN>(a, w, a.own, lds, small);
 }
 
-// out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over a row's slices, the prefix's and its own; a
-// wave per (row, head), two channels a lane, a slice's weight a lane.
-template <int DT>
+// out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over a row's slices, the prefix's and its own.  SHARE
+// half waves per (row, head), each every SHARE-th slice, four channels a lane: 8 where a row has many slices, so
+// that 32 of them are on their way at once, 1 where it has few (a workgroup a row costs 0.6 ns each).
+template <int DT, int SHARE>
 __global__ __launch_bounds__(256) void ls_cache_attn_join_kernel(const CaArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tid = threadIdx.x;
   const int H = a.G * a.gs;
-  const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+  const int64_t row = SHARE == 8 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 8 + (tid >> 5);
   if (row >= a.total_q * H) return;
   const int t = (int)(row / H), head = (int)(row % H), g = head / a.gs, h = head % a.gs;
   if (t >= a.cu_q[a.batch]) return;
   int2 own = a.rows[row];
-  own.y = min(max(own.y, 0), a.own.items);  // (in bounds whatever cu_seqlens_q holds)
+  if (own.y <= 0) return;               // written already
+  own.y = min(own.y, a.own.items);      // (in bounds whatever cu_seqlens_q holds)
   own.x = min(max(own.x, 0), a.own.items - own.y);
-  const int slots = (a.pre.items ? a.pre.slices : 0) + own.y;
-  if (own.y == 0) return;  // written already
+  const int before = a.pre.items ? a.pre.slices : 0, slots = before + own.y;
   const int b = ls_find_segment(a.cu_q, a.batch, t);
-  const int own_col = (t - a.cu_q[b]) % a.own.tokens * a.gs + h;
+  const int own_col = max(0, t - a.cu_q[b]) % a.own.tokens * a.gs + h;
   auto place = [&](int s) -> int64_t {
-    if (s >= slots - own.y)
-      return (int64_t)a.pre.items * a.pre.cols + (int64_t)(own.x + s - (slots - own.y)) * a.own.cols + own_col;
+    if (s >= before)
+      return (int64_t)a.pre.items * a.pre.cols + (int64_t)(own.x + s - before) * a.own.cols + own_col;
     const int u = s * a.G + g, block = u / 8, some = min(8, a.pre.slices * a.G - 8 * block);
     return ((int64_t)block * 8 * a.pre.tiles + t / a.pre.tokens * some + u % 8) * a.pre.cols +
            t % a.pre.tokens * a.gs + h;
   };
-  float M = -INFINITY, L = 0.f;
-  float2 acc = make_float2(0.f, 0.f);
-  for (int s0 = 0; s0 < slots; s0 += 64) {
-    const bool in = s0 + lane < slots;
-    const int64_t at = in ? place(s0 + lane) : 0;
-    const float2 x = in ? a.ml[at] : make_float2(-INFINITY, 0.f);
-    float top = x.x;
+  // The maximum of all, a slice a thread.
+  const int ch = tid & 31, at = SHARE == 8 ? tid >> 5 : 0;
+  float M = -INFINITY;
+  for (int s = SHARE == 8 ? tid : ch; s < slots; s += 32 * SHARE) M = fmaxf(M, a.ml[place(s)].x);
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, ls_shfl_xor(top, o));
-    top = fmaxf(top, M);
-    const float keep = L == 0.f ? 0.f : M == top ? 1.f : __builtin_amdgcn_exp2f(M - top);
-    // A slice's weight; one without a visible key has no sums.
-    const float f = x.y == 0.f ? 0.f : x.x == top ? 1.f : __builtin_amdgcn_exp2f(x.x - top);
-    float l = x.y == 0.f ? 0.f : f * x.y;
+  for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, ls_shfl_xor(M, o));
+  __shared__ float s_m[8], s_l[8];
+  __shared__ ls_f32x4 s_o[8][32];
+  if (SHARE == 8) {
+    if (ch == 0) s_m[at] = M;
+    __syncthreads();
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) l += ls_shfl_xor(l, o);
-    L = (L == 0.f ? 0.f : L * keep) + l;
-    M = top;
-    acc.x *= keep;
-    acc.y *= keep;
-    const int n = min(64, slots - s0);
-    const int at_lo = (int)(uint32_t)at, at_hi = (int)(at >> 32);
-#pragma unroll 8
-    for (int s = 0; s < n; ++s) {
-      const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s));
-      const int64_t p = (int64_t)(uint32_t)__builtin_amdgcn_readlane(at_lo, s) |
-                        (int64_t)__builtin_amdgcn_readlane(at_hi, s) << 32;
-      if (fs != 0.f) {
-        const float2 v = reinterpret_cast<const float2*>(a.part + p * kDim)[lane];
-        acc.x = fmaf(fs, v.x, acc.x);
-        acc.y = fmaf(fs, v.y, acc.y);
-      }
+    for (int i = 0; i < 8; ++i) M = fmaxf(M, s_m[i]);
+  }
+  ls_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float L = 0.f;
+  for (int s0 = at; s0 < slots; s0 += 4 * SHARE) {
+    ls_f32x4 v[4];
+    float2 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t p = place(min(s0 + SHARE * i, slots - 1));
+      x[i] = a.ml[p];
+      v[i] = *reinterpret_cast<const ls_f32x4*>(a.part + p * kDim + 4 * ch);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (s0 + SHARE * i >= slots || x[i].y == 0.f) continue;  // (one without a visible key has no sums)
+      const float f = x[i].x == M ? 1.f : __builtin_amdgcn_exp2f(x[i].x - M);
+      L += f * x[i].y;
+      acc += f * v[i];
     }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  reinterpret_cast<uint32_t*>(a.out)[row * (kDim / 2) + lane] =
-      ls_pack2(LsElem<DT>::from_f(acc.x * inv), LsElem<DT>::from_f(acc.y * inv));
-  if (lane == 0 && a.lse) a.lse[(int64_t)head * a.total_q + t] = ca_lse(M, L);
+  if (SHARE == 8) {
+    s_o[at][ch] = acc;
+    if (ch == 0) s_l[at] = L;
+    __syncthreads();
+    if (tid >= 32) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      acc += s_o[i][ch];
+      L += s_l[i];
+    }
+  }
+  ca_out4<DT>(a.out + row * kDim + 4 * ch, acc, L == 0.f ? 0.f : 1.f / L);
+  if (ch == 0 && a.lse) a.lse[(int64_t)head * a.total_q + t] = ca_lse(M, L);
 }
 
 // ---------------------------------------------------------------------------
@@ -865,50 +866,59 @@ __global__ __launch_bounds__(256) void ls_cache_attn_join_kernel(const CaArgs a)
 constexpr int kUnits = 256;  // compute units
 constexpr int kMaxSplits = 128;
 
-int ca_form_of(int64_t cols) { return cols <= 16 ? 1 : cols <= 32 ? 2 : cols <= 128 ? 3 : 4; }
-int ca_form_cols(int form) { return form == 0 ? 0 : form <= 2 ? 16 * form : kWaves * 16 * (form - 2); }
-
 struct CaPlan {
-  int pre_form, own_form;
   CaCut pre, own;
   size_t part, ml, total;  // total 0: no join
 };
 
-CaPlan ca_plan(int64_t total_q, int batch, int H, int G, int64_t p_len, int64_t max_len, int n_splits) {
+CaPlan ca_plan(int64_t total_q, int batch, int H, int G, int64_t p_len, int64_t max_len, int left, int n_splits) {
+  // A workgroup has a unit to itself.  What one takes, in us: a step of 256 keys of 16 columns, or of 64
+  // keys of 256; and what stands in front of and behind its steps.
+  constexpr double kKeysUs = 1.6, kRowsUs = 3.0, kItemUs = 8.0;
   CaPlan p = {};
   const int gs = H / G;
   const int64_t rows = (total_q + batch - 1) / batch;  // of a sequence
-  auto tokens_of = [&](int cols) { return std::max(1, cols / gs); };
-  if (p_len > 0) {
-    p.pre_form = ca_form_of(total_q * gs);
-    p.pre.cols = ca_form_cols(p.pre_form);
-    p.pre.tokens = tokens_of(p.pre.cols);
-    p.pre.tiles = (int)((total_q + p.pre.tokens - 1) / p.pre.tokens);
-    const int64_t steps = (p_len + kRowsStep - 1) / kRowsStep;
-    p.pre.slices = (int)std::max<int64_t>(
-        1, std::min<int64_t>({n_splits > 0 ? n_splits : kUnits / std::max(1, p.pre.tiles * G), steps, kMaxSplits}));
-    p.pre.items = p.pre.tiles * p.pre.slices * G;
-  }
-  p.own_form = ca_form_of(rows * gs);
-  p.own.cols = ca_form_cols(p.own_form);
-  p.own.tokens = tokens_of(p.own.cols);
-  p.own.tiles = (int)std::min<int64_t>(total_q, total_q / p.own.tokens + batch);
+  auto shape = [&](CaCut& c, int64_t cols) {
+    c.cols = cols <= kKeysCols ? kKeysCols : kRowsCols;
+    c.tokens = std::max(1, c.cols / gs);
+    return c.cols == kKeysCols ? kKeysStep : kRowsStep;
+  };
+  auto count = [](int64_t n, int64_t of) { return (n + of - 1) / of; };
+  const int own_step = shape(p.own, rows * gs);
+  const double own_us = p.own.cols == kKeysCols ? kKeysUs : kRowsUs;
+  p.own.tiles = (int)std::min<int64_t>(total_q, (total_q + (int64_t)batch * (p.own.tokens - 1)) / p.own.tokens);
   const int64_t tiles = (int64_t)p.own.tiles * G;
-  const int step = p.own_form <= 2 ? kKeysStep : kRowsStep;
-  const int64_t steps = std::max<int64_t>(1, (max_len + step - 1) / step);
-  if (n_splits > 0) {
+  const int64_t seen = left >= 0 ? std::min<int64_t>(max_len, (int64_t)left + p.own.tokens) : max_len;
+  const int64_t steps = std::max<int64_t>(1, count(seen, own_step));
+  if (p_len > 0) {
+    const int step = shape(p.pre, total_q * gs);
+    p.pre.tiles = (int)count(total_q, p.pre.tokens);
+    const int64_t pre_tiles = (int64_t)p.pre.tiles * G, pre_steps = count(p_len, step);
+    // Some units take the own keys' items one after the other while the rest take a slice of the prefix each.
+    const double pre_us = pre_tiles * pre_steps * (p.pre.cols == kKeysCols ? kKeysUs : kRowsUs);
+    const double each = (tiles * (steps * own_us + kItemUs) + pre_us) / kUnits + kItemUs;
+    const int64_t slices = n_splits > 0 ? n_splits : std::max<int64_t>(1, (int64_t)(2 * steps * own_us / each));
+    p.own.slices = (int)std::min<int64_t>({slices, std::max<int64_t>(steps, n_splits), kMaxSplits});
+    const double busy = tiles * (steps * own_us + p.own.slices * kItemUs) / each;
+    const int64_t spare = std::max<int64_t>(1, kUnits - (int64_t)busy - 1);
+    p.pre.slices = (int)std::max<int64_t>(
+        1, std::min<int64_t>({n_splits > 0 ? n_splits : spare / pre_tiles, pre_steps, kMaxSplits}));
+    p.pre.items = p.pre.tiles * p.pre.slices * G;
+    p.own.items = (int)std::min<int64_t>(tiles * p.own.slices, 0x7fffffff);
+  } else if (n_splits > 0) {
     p.own.slices = n_splits;
     p.own.items = (int)std::min<int64_t>(tiles * n_splits, 0x7fffffff);
-  } else if (p.own_form <= 2) {
+  } else if (p.own.cols == kKeysCols) {
     p.own.slices = 0;
     p.own.items = (int)std::min<int64_t>(tiles * steps, std::max<int64_t>(kUnits, tiles + kUnits / 2));
   } else {
-    // Rounds of a workgroup a unit: as many slices as make them even.
+    // Rounds of a workgroup a unit: the number of slices that makes them shortest (more than one
+    // are also written, and joined).
     int best = 1;
     double least = 1e30;
-    for (int s = 1; s <= 8 && s <= steps; ++s) {
-      const double rounds = (double)((tiles * s + kUnits - 1) / kUnits) / s + 0.02 * s;
-      if (rounds < least) least = rounds, best = s;
+    for (int s = 1; s <= 64 && s <= steps; ++s) {
+      const double us = count(tiles * s, kUnits) * (kRowsUs * count(steps, s) + kItemUs) + (s > 1 ? 2 * kItemUs : 0.0);
+      if (us < least) least = us, best = s;
     }
     p.own.slices = best;
     p.own.items = (int)std::min<int64_t>(tiles * best, 0x7fffffff);
@@ -929,33 +939,20 @@ void ca_launch(const CaArgs& a, hipStream_t s) {
 }
 
 template <int DT>
-void ca_by_form(const CaArgs& a, int pre, int own, hipStream_t s) {
-#define CA_PAIR(P, O) \
-  if (pre == P && own == O) return ca_launch<DT, P, O>(a, s)
-  CA_PAIR(0, 1);
-  CA_PAIR(0, 2);
-  CA_PAIR(0, 3);
-  CA_PAIR(0, 4);
-  CA_PAIR(1, 1);
-  CA_PAIR(2, 1);
-  CA_PAIR(3, 1);
-  CA_PAIR(4, 1);
-  CA_PAIR(2, 2);
-  CA_PAIR(3, 2);
-  CA_PAIR(4, 2);
-  CA_PAIR(3, 3);
-  CA_PAIR(4, 3);
-  CA_PAIR(4, 4);
-#undef CA_PAIR
+void ca_by_form(const CaArgs& a, hipStream_t s) {
+  const bool keys = a.own.cols == kKeysCols;
+  if (a.pre.items == 0) return keys ? ca_launch<DT, 0, 1>(a, s) : ca_launch<DT, 0, 2>(a, s);
+  if (a.pre.cols == kKeysCols) return ca_launch<DT, 1, 1>(a, s);  // (then the own ones, too)
+  keys ? ca_launch<DT, 2, 1>(a, s) : ca_launch<DT, 2, 2>(a, s);
 }
 
 }  // namespace
 
 extern "C" size_t ls_cache_attn_workspace_size(int64_t total_q, int32_t batch, int32_t num_heads,
                                                int32_t num_kv_heads, int64_t prefix_len, int64_t max_len,
-                                               int32_t n_splits) {
+                                               int32_t window_left, int32_t n_splits) {
   if (total_q <= 0 || batch <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || prefix_len < 0) return 0;
-  return ca_plan(total_q, batch, num_heads, num_kv_heads, prefix_len, max_len, n_splits).total;
+  return ca_plan(total_q, batch, num_heads, num_kv_heads, prefix_len, max_len, window_left, n_splits).total;
 }
 
 extern "C" int ls_cache_attn(const void* q, int64_t q_row_stride, const int32_t* cu_seqlens_q,
@@ -995,10 +992,10 @@ extern "C" int ls_cache_attn(const void* q, int64_t q_row_stride, const int32_t*
   LS_REQUIRE(ls_aligned16(q) && ls_aligned16(k_cache) && ls_aligned16(v_cache) && ls_aligned16(k_prefix) &&
                  ls_aligned16(v_prefix) && ls_aligned16(out) && ls_aligned16(workspace),
              LS_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned", who);
-  const CaPlan p = ca_plan(total_q, batch, num_heads, num_kv_heads, prefix_len, max_len, n_splits);
+  const CaPlan p = ca_plan(total_q, batch, num_heads, num_kv_heads, prefix_len, max_len, window_left, n_splits);
   LS_REQUIRE(workspace_bytes >= p.total && (p.total == 0 || workspace), LS_ERR_WORKSPACE,
              "%s: workspace %zu < %zu", who, workspace_bytes, p.total);
-  LS_REQUIRE((int64_t)p.pre.items + p.own.items < (1 << 22) && total_q * num_heads < (1 << 25),
+  LS_REQUIRE((int64_t)p.pre.items + p.own.items < (1 << 22) && total_q * num_heads < (1 << 23),
              LS_ERR_UNSUPPORTED, "%s: more workgroups than a launch holds", who);
   CaArgs a = {};
   a.q = (const uint16_t*)q;
@@ -1036,14 +1033,18 @@ extern "C" int ls_cache_attn(const void* q, int64_t q_row_stride, const int32_t*
   a.out = (uint16_t*)out;
   a.lse = softmax_lse;
   hipStream_t s = (hipStream_t)stream;
-  dtype == LS_BF16 ? ca_by_form<LS_BF16>(a, p.pre_form, p.own_form, s)
-                   : ca_by_form<LS_F16>(a, p.pre_form, p.own_form, s);
+  dtype == LS_BF16 ? ca_by_form<LS_BF16>(a, s)
+                   : ca_by_form<LS_F16>(a, s);
   int rc = ls_check_launch("ls_cache_attn_kernel");
   if (rc || !p.total) return rc;
-  const dim3 grid((unsigned)((total_q * num_heads + 3) / 4));
+  const int64_t all = total_q * num_heads;
+  const bool few = p.own.slices > 0 && p.pre.slices + p.own.slices <= 8;
+  auto join = [&](auto one, auto eight) {
+    hipLaunchKernelGGL(few ? one : eight, dim3((unsigned)(few ? (all + 7) / 8 : all)), dim3(256), 0, s, a);
+  };
   if (dtype == LS_BF16)
-    hipLaunchKernelGGL(ls_cache_attn_join_kernel<LS_BF16>, grid, dim3(256), 0, s, a);
+    join(ls_cache_attn_join_kernel<LS_BF16, 1>, ls_cache_attn_join_kernel<LS_BF16, 8>);
   else
-    hipLaunchKernelGGL(ls_cache_attn_join_kernel<LS_F16>, grid, dim3(256), 0, s, a);
+    join(ls_cache_attn_join_kernel<LS_F16, 1>, ls_cache_attn_join_kernel<LS_F16, 8>);
   return ls_check_launch("ls_cache_attn_join_kernel");
 }

@@ -61,8 +61,8 @@ def scored_attention(q, k_cache, v_cache, cache_seqlens, cu_seqlens_q, max_len, 
 
 @lru_cache(maxsize=4096)
 def _workspace_bytes(total_q: int, batch: int, H: int, G: int, prefix_len: int, max_len: int,
-                     n_splits: int) -> int:
-    return _hip.lib().ls_cache_attn_workspace_size(total_q, batch, H, G, prefix_len, max_len, n_splits)
+                     left: int, n_splits: int) -> int:
+    return _hip.lib().ls_cache_attn_workspace_size(total_q, batch, H, G, prefix_len, max_len, left, n_splits)
 
 
 def _key_strides(k: torch.Tensor, v: torch.Tensor, name: str) -> tuple[int, ...]:
@@ -115,7 +115,7 @@ def _attend(q, k_prefix, v_prefix, k_cache, v_cache, cache_seqlens, cu_seqlens_q
     softcap = float(softcap)
     if not 0.0 < scale < math.inf or not 0.0 <= softcap < math.inf:
         raise ValueError("softmax_scale must be positive and softcap not negative, both finite")
-    left, right = map(int, window)
+    left, right = (min(max(int(x), -1), 1 << 30) for x in window)
     slopes_stride = 0
     if alibi_slopes is not None:
         if alibi_slopes.dtype is not torch.float32 or alibi_slopes.shape not in ((H,), (B, H)):
@@ -138,7 +138,7 @@ def _attend(q, k_prefix, v_prefix, k_cache, v_cache, cache_seqlens, cu_seqlens_q
     lse = torch.empty((H, total_q), dtype=torch.float32, device=q.device) if return_lse else None
     splits = 0 if n_splits is None else max(1, min(int(n_splits), _MAX_SPLITS))
     max_len = -(-max(0, min(int(max_len), capacity)) // _STEP) * _STEP
-    nbytes = _workspace_bytes(total_q, B, H, G, P, max_len, splits)
+    nbytes = _workspace_bytes(total_q, B, H, G, P, max_len, left, splits)
     ws = q.new_empty((nbytes + 1) >> 1) if nbytes else None  # counted in q's 16-bit elements
     _hip.launch(index, "ls_cache_attn", q_ptr, row[0], cu_seqlens_q.data_ptr(), total_q,
                 k_prefix.data_ptr() if P else None, v_prefix.data_ptr() if P else None, p_row, P,

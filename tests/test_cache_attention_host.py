@@ -122,6 +122,6 @@ def test_entry_point_refusals(change, code, match):
 def test_no_rows_launch_nothing():
     assert _entry(total=0)[0] == _hip.LS_OK
     lib = _hip.lib()
-    assert lib.ls_cache_attn_workspace_size(0, 1, 8, 2, 0, 8, 0) == 0
-    assert lib.ls_cache_attn_workspace_size(1, 1, 8, 2, 0, 100, 1) == 0
-    assert lib.ls_cache_attn_workspace_size(1, 1, 8, 2, 0, 100, 4) >= 4 * 8 * 4 * 130
+    assert lib.ls_cache_attn_workspace_size(0, 1, 8, 2, 0, 8, -1, 0) == 0
+    assert lib.ls_cache_attn_workspace_size(1, 1, 8, 2, 0, 100, -1, 1) == 0
+    assert lib.ls_cache_attn_workspace_size(1, 1, 8, 2, 0, 100, -1, 4) >= 4 * 8 * 4 * 130
