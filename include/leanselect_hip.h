@@ -712,6 +712,24 @@ int ls_cache_attn(const void* q, int64_t q_row_stride, const int32_t* cu_seqlens
                   int32_t n_splits, void* out, float* softmax_lse, void* workspace,
                   size_t workspace_bytes, void* stream);
 
+/*
+ * The next token of each row of logits [rows, vocab] (float32, bf16 or fp16, rows row_stride
+ * elements apart) from the random number u[row] in [0, 1).  With w_i = exp((x_i - max x) /
+ * temperature), ordered by x descending, ties to the lower index: the first top_k are kept (0 or
+ * less: all), of these the shortest run, of one at least, whose sum reaches top_p times theirs (from 1:
+ * all), of these w_i >= min_p; the token is the lowest index at which the running sum of the kept
+ * weights in the vocabulary's order exceeds u times their sum.  temperature 0: the largest
+ * logit's lowest index.  NaN counts as -inf, which has no weight; where the largest is +inf only
+ * those have.  A row without weight gets token -1 and -inf.  temperatures, top_ks, top_ps and
+ * min_ps (NULL or one a row) replace the settings; a temperature that is not above 0 counts as 0.
+ * logprobs (or NULL): ln of the kept share of the token's weight, 0 for temperature 0.  At
+ * most 2^19 tokens.  The reference has no such call.
+ */
+int ls_sample_logits(const void* logits, int64_t row_stride, int64_t rows, int64_t vocab, int32_t dtype,
+                     const float* u, double temperature, int32_t top_k, double top_p, double min_p,
+                     const float* temperatures, const int32_t* top_ks, const float* top_ps,
+                     const float* min_ps, int32_t* tokens, float* logprobs, void* stream);
+
 /* ------------------------------------------------------------------------
  * Products of a few rows with 4-bit weights (no counterpart in the reference,
  * whose projections are 16-bit: leanselect/models/minicpm.py:2176-2222,

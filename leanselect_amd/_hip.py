@@ -27,6 +27,7 @@ def pool_clip_code(clip: str) -> int:
         raise ValueError(f"unknown pool clip {clip!r}; expected 'sequence' or 'row'") from None
 
 _i32, _i64, _f32, _sz = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
+_f64 = ctypes.c_double
 _p = ctypes.c_void_p
 
 # name -> (restype, argtypes); mirrors include/leanselect_hip.h.
@@ -121,6 +122,8 @@ SIGNATURES = {
     "ls_cache_attn": (
         _i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i32, _i32, _i32,
                _i32, _i32, _i64, _f32, _i32, _f32, _p, _i64, _i32, _i32, _i32, _p, _p, _p, _sz, _p]),
+    "ls_sample_logits": (
+        _i32, [_p, _i64, _i64, _i64, _i32, _p, _f64, _i32, _f64, _f64, _p, _p, _p, _p, _p, _p, _p]),
     "ls_quantize_mx4": (_i32, [_p, _i64, _i64, _i64, _i32, _p, _p, _p]),
     "ls_dequantize_mx4": (_i32, [_p, _p, _i64, _i64, _i32, _p, _i64, _p]),
     "ls_linear_mx4_workspace_size": (_sz, [_i64, _i64, _i64, _i32]),

@@ -10,6 +10,7 @@ from .decode import (decode_topk_idx, dense_attention_kvcache, kvcache_append,
 from .decode_q8 import (dense_attention_kvcache_q8, kvcache_append_q8, new_kvcache_q8,
                         sparse_attention_kvcache_q8)
 from .mx4 import dequantize_mx4, lay_out_mx4, linear_mx4, linear_mx4_silu_mul, quantize_mx4
+from .sampling import sample_logits
 from . import profiling
 
 __all__ = [
@@ -37,5 +38,6 @@ __all__ = [
     "dequantize_mx4",
     "linear_mx4",
     "linear_mx4_silu_mul",
+    "sample_logits",
     "profiling",
 ]

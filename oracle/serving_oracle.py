@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import math
 
+import numpy as np
 import torch
 
 __all__ = ["cache_attention", "sample_row"]
@@ -79,47 +80,43 @@ def cache_attention(q, k_cache, v_cache, lens, cu, *, k_prefix=None, v_prefix=No
 
 
 def sample_row(logits, u, temperature, top_k, top_p, min_p):
-    """``(token, logprob, margin)`` of one row of float logits: Python floats throughout.  ``margin`` is how
-    near, in probability, the nearest border of the draw or of a cut lies (a kernel's sums may fall on
-    either side of one within its own error)."""
-    x = [float(v) for v in logits]
-    x = [-math.inf if math.isnan(v) else v for v in x]
-    order = sorted(range(len(x)), key=lambda i: (-x[i], i))
+    """``(token, logprob, sure, off)`` of one row of float logits, in 64 bits.
+
+    ``off``: the share of the sums by which a kernel's may be off: 2e-7 of the weights below 2^-12 (a power
+    in float32, of one unit) and 1e-10 of the others (whole numbers of 2^-43).  ``sure``: whether the token is the same with ``top_p`` and ``u`` moved
+    by that much either way (equal weights are exact)."""
+    x = np.asarray(logits, dtype=np.float64)
+    x = np.where(np.isnan(x), -np.inf, x)
+    order = np.lexsort((np.arange(x.size), -x))
     top = x[order[0]]
-    if top == -math.inf:
-        return -1, -math.inf, 1.0
-    if temperature == 0:
-        return order[0], 0.0, 1.0
-    if top == math.inf:
-        weight = {i: 1.0 if x[i] == math.inf else 0.0 for i in order}
-    else:
-        weight = {i: math.exp((x[i] - top) / temperature) for i in order}
-    margin = 1.0
-    if 0 < top_k < len(order):
+    if top == -np.inf:
+        return -1, -math.inf, True, 0.0
+    if not temperature > 0:
+        return int(order[0]), 0.0, True, 0.0
+    with np.errstate(invalid="ignore"):
+        y = np.where(x == top, 0.0, (x - top) / temperature)
+    weight = np.exp(y)
+    if 0 < top_k < order.size:
         order = order[:top_k]
-    total = math.fsum(weight[i] for i in order)
-    if top_p < 1:
-        kept, so_far = [], 0.0
-        for i in order:
-            if kept and so_far >= top_p * total:
-                break
-            kept.append(i)
-            so_far = math.fsum((so_far, weight[i]))
-            margin = min(margin, abs(so_far / total - top_p))
-        order = kept
-    if min_p > 0:
-        for i in order:
-            if weight[i] > 0:
-                margin = min(margin, abs(math.log(weight[i] / min_p)) if min_p < 1 else 1.0)
-        order = [i for i in order if weight[i] >= min_p]
-    order.sort()
-    total = math.fsum(weight[i] for i in order)
-    so_far, token = 0.0, None
-    for i in order:
-        so_far = math.fsum((so_far, weight[i]))
-        margin = min(margin, abs(so_far / total - u))
-        if token is None and so_far > u * total:
-            token = i
-    if token is None:
-        token = max(i for i in order if weight[i] > 0)
-    return token, math.log(weight[token] / total), margin
+    run = weight[order]
+    total = run.sum()
+    off = 1e-10 + 2e-7 * run[y[order] < -8.31].sum() / total
+
+    def draw(p, u):
+        n = order.size
+        if top_p < 1:
+            n = min(n, 1 + int(np.searchsorted(np.cumsum(run), p * total, side="left")))
+        keep = run[:n] >= min_p
+        kept = np.sort(order[:n][keep])
+        w = weight[kept]
+        upto = np.cumsum(w)
+        i = int(np.searchsorted(upto, u * upto[-1], side="right"))
+        if i >= kept.size:
+            i = int(np.nonzero(w > 0)[0][-1])
+        return int(kept[i]), math.log(w[i] / upto[-1])
+
+    token, logprob = draw(top_p, u)
+    if np.ptp(run[run > 0]) == 0:
+        return token, logprob, True, off
+    near = {draw(top_p + a * off, max(0.0, u + b * off) if u > 0 else 0.0)[0] for a in (-1, 0, 1) for b in (-1, 0, 1)}
+    return token, logprob, near == {token}, off
