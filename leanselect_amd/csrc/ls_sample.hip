@@ -8,15 +8,18 @@
 // Every cut keeps a run of that order, so the kept set is "x above a border, and the first m of those at
 // it": top_k and top_p each give a border (a logit and a number), min_p a logit; the tightest holds.
 //
-// A workgroup a row.  The first pass takes the maximum.  top_k <= 1024 gives a lower bound of its border
-// from the threads' maxima, top_p alone one from a histogram of the weights over the distance from the
-// maximum; the logits above the bound, usually few, are gathered into LDS, and all else is done there.
-// Where there is no such bound, or more than 8192 are above it, the same code reads the row again.
+// A workgroup a row.  The first pass takes each thread's four largest.  top_k <= 2048 gets a lower bound of
+// its border from those; top_p alone gets one from the row's sum S: all logits of a weight below (1 - top_p)
+// S / vocab are in the rest that it leaves.  The logits above the bound, usually few, are gathered into
+// LDS, and all else is done there: up to 256 by comparing each with each.  Where more than 8192 are
+// above it, top_p's border comes from a histogram of the weights over the distance from the maximum and
+// the logits of its bin; where there is no bound, the same code reads the row again.
 //
 // A border is found by a radix search, 11 bits a round, in a histogram in LDS of how many keys, or how much
-// weight, each value of the bits has; the draw is the same search over the indices.  Weights are summed
-// as whole numbers of 2^-s, s such that a row's sum stays under 2^62 (2^-45 for 73448 tokens): sums do
-// not depend on their order, so neither does the token.
+// weight, each value of the bits has; a draw from what was gathered is the same search over the
+// indices, one from the row takes the sums of 256 tokens each.  Weights are summed as whole numbers of 2^-s, s
+// such that a row's sum stays under 2^62 (2^-45 for 73448 tokens): sums do not depend on their order, so
+// neither does the token.
 //
 // The reference draws with torch's multinomial on the host's settings; it has no such kernel.
 #include <algorithm>
@@ -30,6 +33,9 @@ constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2048;
 constexpr int kList = 8192;
+constexpr int kFew = 256;
+constexpr int kMaxima = 4;  // of each thread
+constexpr int kBounded = 2048;  // the largest top_k that gets a bound from them
 constexpr int kSlot = 4 * kThreads;  // tokens of a round over the row
 constexpr int kIndexBits = 19;
 constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
@@ -138,9 +144,10 @@ struct SaRow {
       for (int e = 0; e < 4; ++e) k[e] = i + e < vocab ? sa_key<DT>(x[i + e]) : 0u;
     }
   }
+  // (nine rounds' loads are under way at once: 73448 tokens are two times that)
   template <class F>
   __device__ __forceinline__ void each4(F f) const {
-#pragma unroll 4
+#pragma unroll 9
     for (int i0 = 0; i0 < vocab; i0 += kSlot) {
       const int i = i0 + 4 * (int)threadIdx.x;
       uint32_t k[4];
@@ -265,64 +272,94 @@ struct SaRule {
   }
 };
 
-// The cuts and the draw over the row or what was gathered of it.  `total`: the weights of the whole row, for
-// top_p without top_k.
+// Kept are the keys above `cut`, and the first `ties` of those at it: with an index up to `last`.
+struct SaKept {
+  uint32_t cut, last;
+  uint64_t ties;
+  __device__ __forceinline__ bool operator()(int i, uint32_t key) const {
+    return key > cut || (ties != 0 && key == cut && (uint32_t)i <= last);
+  }
+};
+
+__device__ __forceinline__ uint32_t sa_by_index(int i, uint32_t) { return ~(uint32_t)i & kIndexMask; }  // lowest first
+__device__ __forceinline__ uint32_t sa_by_key(int, uint32_t key) { return key; }
+
+// `last`, from a row or list that has all keys at the border.
 template <class Row>
-__device__ __forceinline__ void sa_draw(const Row& row, SaShared& s, const SaRule& rule, uint64_t total, double u,
-                                        int32_t* token, float* logprob) {
-  auto by_key = [](int, uint32_t key) { return key; };
-  auto by_index = [](int i, uint32_t) { return ~(uint32_t)i & kIndexMask; };  // (the lowest index first)
-  // Kept are the keys above `cut`, and the first `ties` of those at it.
-  uint32_t cut = rule.least;
-  uint64_t ties = 0, above;
+__device__ __forceinline__ void sa_last(const Row& row, SaShared& s, SaKept& kept) {
+  kept.last = 0x7fffffff;
+  if (kept.ties == 0) return;
+  uint64_t n = 0, above;
+  row.each([&](int, uint32_t key) { n += key == kept.cut; });
+  n = sa_sum(n, s);
+  if (n > kept.ties)
+    kept.last = ~sa_border<kIndexBits>(row, s, kept.ties, above, sa_by_index,
+                                       [&](int, uint32_t key) -> uint64_t { return key == kept.cut ? 1 : 0; }) &
+                kIndexMask;
+}
+
+// What top_p keeps: the keys from a border, found in a row or list of which `counts` says what is summed up; the
+// sum of all larger ones is `front`.
+template <class Row, class Counts>
+__device__ __forceinline__ void sa_top_p(const Row& row, SaShared& s, const SaRule& rule, uint64_t need, uint64_t front,
+                                         SaKept& kept, Counts counts) {
+  uint64_t above;
+  const uint32_t c = sa_border<32>(row, s, need - front, above, sa_by_key, [&](int, uint32_t key) -> uint64_t {
+    const uint64_t w = rule.weight(key);
+    return counts(key) ? w : 0;
+  });
+  const uint64_t w = rule.weight(c), n = (need - front - above + w - 1) / w;
+  if (c > kept.cut || n < kept.ties) kept.cut = c, kept.ties = n;
+}
+
+// The cuts over the row or what was gathered of it.  `total`: the weights of the whole row, for top_p without
+// top_k.
+template <class Row>
+__device__ __forceinline__ SaKept sa_cuts(const Row& row, SaShared& s, const SaRule& rule, uint64_t total) {
+  SaKept kept{rule.least, 0x7fffffff, 0};
   if (rule.k > 0) {
-    uint64_t n = 0;
+    uint64_t n = 0, above;
     row.each([&](int, uint32_t key) { n += key > rule.least; });
     n = sa_sum(n, s);
     if (n > (uint64_t)rule.k) {
-      cut = sa_border<32>(row, s, rule.k, above, by_key,
-                          [&](int, uint32_t key) -> uint64_t { return key > rule.least ? 1 : 0; });
-      ties = rule.k - above;
+      kept.cut = sa_border<32>(row, s, rule.k, above, sa_by_key,
+                               [&](int, uint32_t key) -> uint64_t { return key > rule.least ? 1 : 0; });
+      kept.ties = rule.k - above;
     }
   }
   if (rule.p < 1.0) {
-    const uint64_t at_cut = rule.weight(cut);
+    const uint64_t at_cut = rule.weight(kept.cut);
     uint64_t here = 0;
     row.each([&](int, uint32_t key) {
       const uint64_t w = rule.weight(key);
-      here += key > cut ? w : 0;
+      here += key > kept.cut ? w : 0;
     });
-    here = sa_sum(here, s) + ties * at_cut;
+    here = sa_sum(here, s) + kept.ties * at_cut;
     if (rule.k > 0) total = here;
-    const double goal = ceil(rule.p * (double)total);
-    const uint64_t need = max((uint64_t)goal, (uint64_t)1);
-    if (need <= here) {  // (else more than what is here is kept)
-      const uint32_t c = sa_border<32>(row, s, need, above, by_key, [&](int, uint32_t key) -> uint64_t {
-        const uint64_t w = rule.weight(key);
-        return key > cut || (key == cut && ties) ? w : 0;
-      });
-      const uint64_t w = rule.weight(c), n = (need - above + w - 1) / w;
-      if (c > cut || n < ties) cut = c, ties = n;
-    }
+    const uint64_t need = max((uint64_t)ceil(rule.p * (double)total), (uint64_t)1);
+    if (need <= here)  // (else more than what is here is kept)
+      sa_top_p(row, s, rule, need, 0, kept,
+               [&](uint32_t key) { return key > kept.cut || (key == kept.cut && kept.ties); });
   }
-  if (rule.min_cut > cut) cut = rule.min_cut - 1, ties = 0;
-  uint32_t last = 0x7fffffff;  // the last index of those at the border
-  if (ties) {
-    uint64_t n = 0;
-    row.each([&](int, uint32_t key) { n += key == cut; });
-    n = sa_sum(n, s);
-    if (n > ties)
-      last = ~sa_border<kIndexBits>(row, s, ties, above, by_index,
-                            [&](int, uint32_t key) -> uint64_t { return key == cut ? 1 : 0; }) & kIndexMask;
-  }
-  auto kept = [&](int i, uint32_t key) { return key > cut || (ties != 0 && key == cut && (uint32_t)i <= last); };
+  if (rule.min_cut > kept.cut) kept.cut = rule.min_cut - 1, kept.ties = 0;
+  sa_last(row, s, kept);
+  return kept;
+}
+
+// The draw.
+template <class Row>
+__device__ __forceinline__ void sa_draw(const Row& row, SaShared& s, const SaRule& rule, const SaKept& kept, double u,
+                                        int32_t* token, float* logprob) {
+  uint64_t above;
   auto any = [&](int i, uint32_t key) {  // whether there is a weight at all, however small
     return kept(i, key) && (key == rule.top ||
                             (key > rule.least && ((double)sa_value(key) - rule.x_max) * rule.scale > -745.0));
   };
   auto measure = [&](int i, uint32_t key) -> uint64_t {
+    const bool k = kept(i, key);
+    if (!__any(k)) return 0;
     const uint64_t w = rule.weight(key);
-    return kept(i, key) ? w : 0;
+    return k ? w : 0;
   };
   // u sum < a running sum  <=>  floor(u sum) < it, a whole number.
   auto goal_of = [&](uint64_t sum) {
@@ -341,8 +378,8 @@ __device__ __forceinline__ void sa_draw(const Row& row, SaShared& s, const SaRul
     row.each([&](int i, uint32_t key) { sum += measure(i, key); });
     sum = sa_sum(sum, s);
     const uint32_t i =
-        ~(u > 0.0 ? sa_border<kIndexBits>(row, s, goal_of(sum) + 1, above, by_index, measure)
-                  : sa_border<kIndexBits>(row, s, 1, above, by_index,
+        ~(u > 0.0 ? sa_border<kIndexBits>(row, s, goal_of(sum) + 1, above, sa_by_index, measure)
+                  : sa_border<kIndexBits>(row, s, 1, above, sa_by_index,
                                           [&](int i, uint32_t key) -> uint64_t { return any(i, key) ? 1 : 0; })) &
         kIndexMask;
     row.each([&](int j, uint32_t key) {
@@ -382,6 +419,54 @@ __device__ __forceinline__ void sa_draw(const Row& row, SaShared& s, const SaRul
   }
 }
 
+// The same for at most kFew gathered logits, one a thread: what is in front of it in either order is found by
+// looking at each of the others, without a search or a histogram.
+__device__ __forceinline__ void sa_draw_few(int n, SaShared& s, const SaRule& rule, uint64_t total, double u,
+                                            int32_t* token, float* logprob) {
+  const int tid = threadIdx.x;
+  const bool in = tid < n;
+  const uint32_t key = in ? s.key[tid] : 0u, i = in ? s.index[tid] : 0u;
+  uint64_t w = 0;
+  if (tid < kFew) {
+    w = rule.weight(key);
+    s.bins[tid] = w;
+  }
+  __syncthreads();
+  uint32_t rank = 0;
+  uint64_t before = 0;
+  if (in) {
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const bool first = s.key[j] > key || (s.key[j] == key && s.index[j] < i);
+      rank += first;
+      before += first ? s.bins[j] : 0;
+    }
+  }
+  bool kept = in && key > rule.least && (rule.k == 0 || rank < (uint32_t)rule.k);
+  if (rule.p < 1.0) {
+    if (rule.k > 0) total = sa_sum(kept ? w : 0, s);
+    const double goal = ceil(rule.p * (double)total);
+    kept = kept && before < max((uint64_t)goal, (uint64_t)1);
+  }
+  kept = kept && key >= rule.min_cut;
+  const uint64_t sum = sa_sum(kept ? w : 0, s);
+  const double y = key == rule.top ? 0.0 : ((double)sa_value(key) - rule.x_max) * rule.scale;
+  // u = 0: the lowest index with any weight, however small.
+  const uint64_t m = !kept ? 0 : u > 0.0 ? w : y > -745.0 ? 1 : 0;
+  if (tid < kFew) s.bins[tid] = m;
+  __syncthreads();
+  if (m == 0) return;
+  uint64_t goal = u > 0.0 ? (uint64_t)(u * (double)sum) : 0;
+  goal = goal < sum ? goal : sum - 1;
+  before = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) before += s.index[j] < i ? s.bins[j] : 0;
+  if (before <= goal && goal < before + m) {
+    *token = (int32_t)i;
+    if (logprob) *logprob = (float)(y - log(ldexp((double)sum, -rule.shift)));
+  }
+}
+
 template <int DT>
 __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
   __shared__ SaShared s;
@@ -392,15 +477,16 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
   row.vocab = a.vocab;
   row.wide = ((uintptr_t)row.x & (DT == LS_F32 ? 15 : 7)) == 0;
   if (tid < 16) s.table[tid] = exp2((double)tid / 16.0);
-  if (tid == 0) s.n = 0;
-  uint32_t mine = 0, at = 0;
+  uint32_t best[kMaxima] = {}, at = 0;
   row.each([&](int i, uint32_t key) {
-    at = key > mine ? (uint32_t)i : at;
-    mine = max(mine, key);
+    at = key > best[0] ? (uint32_t)i : at;
+#pragma unroll
+    for (int m = kMaxima - 1; m > 0; --m) best[m] = max(best[m], min(best[m - 1], key));
+    best[0] = max(best[0], key);
   });
-  const uint64_t best = sa_max((uint64_t)mine << 32 | (uint32_t)~at, s);
+  const uint64_t first = sa_max((uint64_t)best[0] << 32 | (uint32_t)~at, s);
   SaRule rule;
-  rule.top = (uint32_t)(best >> 32);
+  rule.top = (uint32_t)(first >> 32);
   rule.least = ls_order_key32(0xff800000u);  // -inf: no weight
   rule.x_max = sa_value(rule.top);
   const double t = a.ts ? (double)a.ts[r] : a.t;
@@ -409,7 +495,7 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
     // Nothing to draw from, or the largest alone.
     if (tid == 0) {
       const bool none = rule.top <= rule.least;
-      a.tokens[r] = none ? -1 : (int32_t)~(uint32_t)best;
+      a.tokens[r] = none ? -1 : (int32_t)~(uint32_t)first;
       if (logprob) *logprob = none ? -INFINITY : 0.f;
     }
     return;
@@ -432,52 +518,117 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
     rule.min_cut = min(c, rule.top);
   }
   const double u = (double)a.u[r];
-  // A lower bound of what is kept, or has to be summed up.
+  // What is kept, or has to be summed up, is among the keys from `low` that are no more than `far` bins of
+  // 1 / `to_bins` from the maximum.
   uint32_t low = rule.least + 1;
-  uint64_t total = 0, above;
-  if (rule.k > 0 && rule.k <= kThreads) {
-    // The k-th largest of the threads' maxima.
-    SaList maxima{s.key, s.key, kThreads};
-    s.key[tid] = mine;
-    __syncthreads();
-    low = max(low, sa_border<32>(maxima, s, rule.k, above, [](int, uint32_t key) { return key; },
-                                 [](int, uint32_t) -> uint64_t { return 1; }));
-    __syncthreads();
-  } else if (rule.k == 0 && rule.p < 1.0) {
-    // Bins of 1/32 of a temperature below the maximum; the last takes all that is further off.
-    const float to_bins = (float)(32.0 * rule.scale);
-    sa_clear(s);
-    row.each([&](int, uint32_t key) {
-      const uint64_t w = rule.weight(key);
-      total += w;
-      const float d = (rule.x_max - sa_value(key)) * to_bins;
-      if (w != 0) atomicAdd(&s.bins[kBins - 1 - (d < kBins - 1 ? (int)d : kBins - 1)], (unsigned long long)w);
-    });
-    total = sa_sum(total, s);
-    const double goal = ceil(rule.p * (double)total);
-    uint64_t before;
-    const uint32_t bin = kBins - 1 - sa_find(s, min(max((uint64_t)goal, (uint64_t)1), total), before);
-    if (bin + 2 < kBins) {  // (a bin more: the bound is a rounded product)
-      const float f = (float)((double)rule.x_max - (bin + 2) * (1.0 / 32.0) * t);
-      low = max(low, ls_order_key32(__float_as_uint(f == 0.f ? 0.f : f)));
+  float to_bins = 0.f;
+  int far = 0;
+  auto bin_of = [&](uint32_t key) {  // (falls as the key rises)
+    const float d = (rule.x_max - sa_value(key)) * to_bins;
+    return d < kBins - 1 ? (int)d : kBins - 1;
+  };
+  uint64_t total = 0, need = 0;
+  bool bounded = false;
+  if (rule.k > 0 && rule.k <= kBounded) {
+    // Some of the threads' largest are the k-th largest or more; their k-th largest is a bound.
+    static_assert(kBounded <= 2 * kThreads && kMaxima >= 2, "");
+    const uint32_t mine = rule.k <= kThreads ? best[0] : best[1];
+    const uint32_t least = ~(uint32_t)sa_max(~mine, s);
+    const float range = rule.x_max - sa_value(least);
+    bounded = true;
+    if (least > rule.least && range > 0.f && range < INFINITY) {
+      to_bins = (kBins - 2) / range;
+      sa_clear(s);
+#pragma unroll
+      for (int m = 0; m < kMaxima; ++m)
+        if (best[m] >= least) atomicAdd(&s.bins[kBins - 1 - bin_of(best[m])], 1ull);
+      uint64_t before;
+      far = kBins - 1 - (int)sa_find(s, rule.k, before);
+    } else if (least > rule.least) {
+      low = least;
     }
+  } else if (rule.k == 0 && rule.p < 1.0) {
+    row.each([&](int, uint32_t key) { total += rule.weight(key); });
+    total = sa_sum(total, s);
+    need = min(max((uint64_t)ceil(rule.p * (double)total), (uint64_t)1), total);
+    // (a hundredth below it: the bound is rounded)
+    const double least = (1.0 - rule.p) * ldexp((double)total, -rule.shift) / a.vocab;
+    const float f = (float)((double)rule.x_max + t * (log(least) - 0.01));
+    low = max(low, ls_order_key32(__float_as_uint(f == 0.f ? 0.f : f)));
+    bounded = true;
   }
   // (What top_p sums up is more than what min_p leaves.)
-  if (!(rule.k > 0 && rule.p < 1.0)) low = max(low, rule.min_cut);
-  if (low > rule.least + 1) {
+  if (!(rule.k > 0 && rule.p < 1.0)) {
+    low = max(low, rule.min_cut);
+    bounded = bounded || rule.min_cut > rule.least + 1;
+  }
+  // Logits into LDS, a wave's in one go.
+  auto gather = [&](auto take) {
+    __syncthreads();
+    if (tid == 0) s.n = 0;
+    __syncthreads();
     row.each([&](int i, uint32_t key) {
-      if (key >= low) {
-        const uint32_t n = atomicAdd(&s.n, 1u);
-        if (n < kList) s.key[n] = key, s.index[n] = (uint32_t)i;
-      }
+      const uint64_t mask = __ballot(take(key));
+      if (mask == 0) return;
+      uint32_t n = 0;
+      if (ls_lane() == 0) n = atomicAdd(&s.n, (uint32_t)__popcll(mask));
+      n = __builtin_amdgcn_readfirstlane(n) + ls_lanes_below(mask);
+      if (take(key) && n < kList) s.key[n] = key, s.index[n] = (uint32_t)i;
     });
     __syncthreads();
-    if (s.n <= kList) {
-      sa_draw(SaList{s.key, s.index, (int)s.n}, s, rule, total, u, a.tokens + r, logprob);
+    return (int)s.n;
+  };
+  int32_t* token = a.tokens + r;
+  if (bounded) {
+    const int n = gather([&](uint32_t key) { return key >= low && (to_bins == 0.f || bin_of(key) <= far); });
+    if (n <= kFew) {
+      sa_draw_few(n, s, rule, total, u, token, logprob);
+      return;
+    }
+    if (n <= kList) {
+      const SaList list{s.key, s.index, n};
+      sa_draw(list, s, rule, sa_cuts(list, s, rule, total), u, token, logprob);
       return;
     }
   }
-  sa_draw(row, s, rule, total, u, a.tokens + r, logprob);
+  if (need > 0) {
+    // Bins of 1/32 of a temperature; then, where too many logits are in the border's, of 1/65536.
+    to_bins = (float)(32.0 / t);
+    sa_clear(s);
+    row.each([&](int, uint32_t key) {
+      const uint64_t w = rule.weight(key);
+      if (w != 0) atomicAdd(&s.bins[kBins - 1 - bin_of(key)], (unsigned long long)w);
+    });
+    uint64_t front;
+    const int bin = kBins - 1 - (int)sa_find(s, need, front);
+    auto in_bin = [&](uint32_t key) { return key > rule.least && bin_of(key) == bin; };
+    int n = gather(in_bin), sub = -1;
+    auto sub_of = [&](uint32_t key) {
+      const float d = ((rule.x_max - sa_value(key)) * to_bins - (float)bin) * kBins;
+      return d < kBins - 1 ? max((int)d, 0) : kBins - 1;
+    };
+    if (n > kList) {
+      sa_clear(s);
+      row.each([&](int, uint32_t key) {
+        const uint64_t w = rule.weight(key);
+        if (w != 0 && in_bin(key)) atomicAdd(&s.bins[kBins - 1 - sub_of(key)], (unsigned long long)w);
+      });
+      uint64_t before;
+      sub = kBins - 1 - (int)sa_find(s, need - front, before);
+      front += before;
+      n = gather([&](uint32_t key) { return in_bin(key) && sub_of(key) == sub; });
+    }
+    if (n <= kList) {
+      const SaList list{s.key, s.index, n};
+      SaKept kept{rule.least, 0x7fffffff, 0};
+      sa_top_p(list, s, rule, need, front, kept, [](uint32_t) { return true; });
+      if (rule.min_cut > kept.cut) kept.cut = rule.min_cut - 1, kept.ties = 0;
+      sa_last(list, s, kept);
+      sa_draw(row, s, rule, kept, u, token, logprob);
+      return;
+    }
+  }
+  sa_draw(row, s, rule, sa_cuts(row, s, rule, total), u, token, logprob);
 }
 
 }  // namespace
