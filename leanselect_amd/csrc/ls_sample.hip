@@ -34,12 +34,12 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2048;
 constexpr int kList = 8192;
 constexpr int kFew = 256;
-constexpr int kMaxima = 4;  // of each thread
-constexpr int kBounded = 2048;  // the largest top_k that gets a bound from them
+constexpr int kBounded = 2048;   // the largest top_k that gets a bound from the threads' two largest
 constexpr int kSlot = 4 * kThreads;  // tokens of a round over the row
 constexpr int kIndexBits = 19;
 constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
 static_assert((1 << kIndexBits) / kSlot * kWaves <= kBins, "a bin for what a wave takes in each round");
+static_assert(kBounded <= 2 * kThreads, "");
 
 struct SaArgs {
   const void* x;
@@ -58,39 +58,16 @@ struct SaArgs {
   float* logprobs;
 };
 
-
-// 2^y, y = (x - x_max) log2(e) / t, in whole numbers of 2^-shift.  The power of y's fraction: below 2^-12 in
-// float32 (1.5e-7 of it); above, where that would show, from a table of 2^(k / 16) and exp(g) to the
-// seventh power (|g| < 0.022: 2^-54).
-__device__ __forceinline__ uint64_t sa_exp(float x, float x_max, double scale2, int shift, const double* table) {
-  const double y = fmax(((double)x - (double)x_max) * scale2, -200.0);
-  const double n = rint(y), f = y - n;
-  uint64_t w = (uint64_t)rintf(ldexpf(__builtin_amdgcn_exp2f((float)f), (int)n + shift));
-  if (__any(y > -12.0)) {
-    const double m = rint(16.0 * y), g = fma(m, -1.0 / 16.0, y) * 0.69314718055994530942;
-    double p = fma(g, 1.0 / 720.0, 1.0 / 120.0);
-    p = fma(g, p, 1.0 / 24.0);
-    p = fma(g, p, 1.0 / 6.0);
-    p = fma(g, p, 0.5);
-    p = fma(g, p, 1.0);
-    p = fma(g, p, 1.0);
-    const int k = (int)m;
-    const uint64_t exact = (uint64_t)rint(ldexp(p * table[k & 15], (k >> 4) + shift));
-    w = y > -12.0 ? exact : w;
-  }
-  return w;
-}
-
-// A logit's key: their order is that of the logits, NaN as -inf.
-template <int DT>
-__device__ __forceinline__ uint32_t sa_key(typename LsElem<DT>::T v) {
-  const float x = LsElem<DT>::to_f(v);
-  return ls_order_key32(__float_as_uint(x != x ? -INFINITY : x == 0.f ? 0.f : x));
-}
+// Logits in their order as whole numbers (-0 as 0).
+__device__ __forceinline__ uint32_t sa_key(float x) { return ls_order_key32(__float_as_uint(x == 0.f ? 0.f : x)); }
 __device__ __forceinline__ float sa_value(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
+__device__ __forceinline__ uint64_t sa_lane64(uint64_t x, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane) |
+         (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32;
+}
 __device__ __forceinline__ uint64_t sa_add64(uint64_t x) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor((unsigned long long)x, o, 64);
@@ -114,59 +91,62 @@ struct SaShared {
   unsigned long long found;
   uint32_t at;
   uint32_t n;
-  uint32_t key[kList];
+  uint32_t word[kWaves];
+  float x[kList];
   uint32_t index[kList];
 };
 
-// A row in memory.  f(index, key) for this thread's logits; 0 (below every key) beyond the last.
+// A row in memory.  f(index, logit) for this thread's; NaN as -inf, which is also what lies beyond the last.
 template <int DT>
 struct SaRow {
   typedef typename LsElem<DT>::T T;
+  typedef typename std::conditional<DT == LS_F32, ls_f32x4, uint2>::type T4;
   const T* x;
   int vocab;
   bool wide;  // four may be read at once
 
-  __device__ __forceinline__ void load4(int i, uint32_t (&k)[4]) const {
+  __device__ __forceinline__ float one(int i) const { return i < vocab ? LsElem<DT>::to_f(x[i]) : -INFINITY; }
+  __device__ __forceinline__ ls_f32x4 load4(int i) const {
+    ls_f32x4 v;
     if (wide && i + 4 <= vocab) {
-      if constexpr (DT == LS_F32) {
-        const ls_f32x4 v = *reinterpret_cast<const ls_f32x4*>(x + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) k[e] = sa_key<DT>(v[e]);
-      } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(x + i);
-        k[0] = sa_key<DT>((T)(v.x & 0xffffu));
-        k[1] = sa_key<DT>((T)(v.x >> 16));
-        k[2] = sa_key<DT>((T)(v.y & 0xffffu));
-        k[3] = sa_key<DT>((T)(v.y >> 16));
-      }
+      const T4 w = *reinterpret_cast<const T4*>(x + i);
+      if constexpr (DT == LS_F32)
+        v = w;
+      else
+        v = ls_f32x4{LsElem<DT>::to_f((T)(w.x & 0xffffu)), LsElem<DT>::to_f((T)(w.x >> 16)),
+                     LsElem<DT>::to_f((T)(w.y & 0xffffu)), LsElem<DT>::to_f((T)(w.y >> 16))};
     } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) k[e] = i + e < vocab ? sa_key<DT>(x[i + e]) : 0u;
+      v = ls_f32x4{one(i), one(i + 1), one(i + 2), one(i + 3)};
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = fmaxf(v[e], -INFINITY);
+    return v;
   }
-  // (nine rounds' loads are under way at once: 73448 tokens are two times that)
+  // Two rounds' loads ahead of the one in hand.
   template <class F>
   __device__ __forceinline__ void each4(F f) const {
-#pragma unroll 9
-    for (int i0 = 0; i0 < vocab; i0 += kSlot) {
-      const int i = i0 + 4 * (int)threadIdx.x;
-      uint32_t k[4];
-      load4(i, k);
-      f(i, k);
+    int i = 4 * (int)threadIdx.x;
+    ls_f32x4 a = load4(i), b = load4(i + kSlot);
+#pragma unroll 2
+    for (int i0 = 0; i0 < vocab; i0 += kSlot, i += kSlot) {
+      const ls_f32x4 c = load4(i + 2 * kSlot);
+      f(i, a);
+      a = b;
+      b = c;
     }
   }
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-    each4([&](int i, const uint32_t(&k)[4]) {
+    each4([&](int i, const ls_f32x4& v) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f(i + e, k[e]);
+      for (int e = 0; e < 4; ++e) f(i + e, v[e]);
     });
   }
 };
 
 // What was gathered.  (Every lane runs every round: the weights are formed by whole waves.)
 struct SaList {
-  const uint32_t* key;
+  const float* x;
   const uint32_t* index;
   int n;
   template <class F>
@@ -174,22 +154,18 @@ struct SaList {
     for (int i0 = 0; i0 < n; i0 += kThreads) {
       const int i = i0 + (int)threadIdx.x;
       const bool in = i < n;
-      f(in ? (int)index[i] : 0x7fffffff, in ? key[i] : 0u);
+      f(in ? (int)index[i] : 0x7fffffff, in ? x[i] : -INFINITY);
     }
   }
 };
 
-__device__ __forceinline__ uint64_t sa_max(uint64_t x, SaShared& s) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const uint64_t y = __shfl_xor((unsigned long long)x, o, 64);
-    x = y > x ? y : x;
-  }
+__device__ __forceinline__ uint32_t sa_max(uint32_t x, SaShared& s) {
+  x = ls_wave_max_u32(x);
   __syncthreads();
-  if (ls_lane() == 0) s.part[threadIdx.x >> 6] = x;
+  if (ls_lane() == 0) s.word[threadIdx.x >> 6] = x;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) x = s.part[i] > x ? s.part[i] : x;
+  for (int i = 0; i < kWaves; ++i) x = max(x, s.word[i]);
   return x;
 }
 __device__ __forceinline__ uint64_t sa_sum(uint64_t x, SaShared& s) {
@@ -230,7 +206,7 @@ __device__ __forceinline__ uint32_t sa_find(SaShared& s, uint64_t want, uint64_t
   return s.at;
 }
 
-// The largest c such that the measures of the entries with order(index, key) >= c sum up to `need` at least
+// The largest c such that the measures of the entries with order(index, logit) >= c sum up to `need` at least
 // (0 < need <= all; a measure of 0 does not count); `above`: the sum of those > c.
 template <int BITS, class Row, class Order, class Measure>
 __device__ __forceinline__ uint32_t sa_border(const Row& row, SaShared& s, uint64_t need, uint64_t& above,
@@ -242,9 +218,9 @@ __device__ __forceinline__ uint32_t sa_border(const Row& row, SaShared& s, uint6
     const int bits = min(left, 11), low = left - bits;
     const uint32_t mask = left == 32 ? 0u : ~0u << left;
     sa_clear(s);
-    row.each([&](int i, uint32_t key) {
-      const uint32_t o = order(i, key);
-      const uint64_t w = measure(i, key);
+    row.each([&](int i, float x) {
+      const uint32_t o = order(i, x);
+      const uint64_t w = measure(i, x);
       if (w != 0 && (o & mask) == prefix) atomicAdd(&s.bins[o >> low & ((1u << bits) - 1)], (unsigned long long)w);
     });
     uint64_t before;
@@ -257,57 +233,95 @@ __device__ __forceinline__ uint32_t sa_border(const Row& row, SaShared& s, uint6
 
 // A row's settings, and what a logit weighs.
 struct SaRule {
-  uint32_t top, least;
-  float x_max;
-  double scale, scale2;  // 1 / temperature, log2(e) / temperature
+  float top;
+  double inv;         // 1 / temperature
+  double scale, off;  // a logit's base-2 exponent: scale x + off
   int shift;
   int k;          // 0: none
   double p;
-  uint32_t min_cut;  // keys from here on pass min_p
+  float min_cut;  // logits above it pass min_p
   const double* table;
 
-  __device__ __forceinline__ uint64_t weight(uint32_t key) const {
-    const uint64_t w = sa_exp(sa_value(key), x_max, scale2, shift, table);
-    return key == top ? 1ull << shift : key > least && x_max < INFINITY ? w : 0;
+  // 2^y in whole numbers of 2^-shift.  The power of y's fraction: under 2^31 of them in float32 (1.5e-7 of
+  // it); above, where that would show, from a table of 2^(k / 16) and exp(g) to the seventh power
+  // (|g| < 0.022: 2^-54).
+  __device__ __forceinline__ uint64_t weight(float x) const {
+    const double y = fma((double)x, scale, off), n = rint(y);
+    const bool near = y > 30.5 - shift;
+    const int e = (int)n + shift;
+    uint64_t w = (uint32_t)rintf(ldexpf(__builtin_amdgcn_exp2f((float)(y - n)), near ? 0 : max(e, -200)));
+    if (__any(near)) {
+      const double m = rint(16.0 * y), g = fma(m, -1.0 / 16.0, y) * 0.69314718055994530942;
+      double q = fma(g, 1.0 / 720.0, 1.0 / 120.0);
+      q = fma(g, q, 1.0 / 24.0);
+      q = fma(g, q, 1.0 / 6.0);
+      q = fma(g, q, 0.5);
+      q = fma(g, q, 1.0);
+      q = fma(g, q, 1.0);
+      const int k = (int)m;
+      const uint64_t exact = (uint64_t)rint(ldexp(q * table[k & 15], (k >> 4) + shift));
+      w = near ? exact : w;
+    }
+    return x == top ? 1ull << shift : x > -INFINITY && top < INFINITY ? w : 0;
+  }
+  // ln of the weight.
+  __device__ __forceinline__ double log_weight(float x) const {
+    return x == top ? 0.0 : ((double)x - (double)top) * inv;
+  }
+  // ln of its share of a sum.
+  __device__ __forceinline__ float share(float x, uint64_t sum) const {
+    return (float)(log_weight(x) - log(ldexp((double)sum, -shift)));
+  }
+  __device__ __forceinline__ uint64_t need(uint64_t total) const {
+    return max((uint64_t)ceil(p * (double)total), (uint64_t)1);
+  }
+  // u sum < a running sum  <=>  floor(u sum) < it, a whole number.
+  __device__ __forceinline__ static uint64_t goal(double u, uint64_t sum) {
+    const uint64_t g = u > 0.0 ? (uint64_t)(u * (double)sum) : 0;
+    return g < sum ? g : sum - 1;
   }
 };
 
-// Kept are the keys above `cut`, and the first `ties` of those at it: with an index up to `last`.
+// Kept are the logits above `cut`, and the first `ties` of those at it: with an index up to `last`.
 struct SaKept {
-  uint32_t cut, last;
+  float cut;
+  uint32_t last;
   uint64_t ties;
-  __device__ __forceinline__ bool operator()(int i, uint32_t key) const {
-    return key > cut || (ties != 0 && key == cut && (uint32_t)i <= last);
+  __device__ __forceinline__ bool operator()(int i, float x) const {
+    return x > cut || (ties != 0 && x == cut && (uint32_t)i <= last);
+  }
+  __device__ __forceinline__ void above(float c) {
+    if (c >= cut) cut = c, ties = 0;
   }
 };
 
-__device__ __forceinline__ uint32_t sa_by_index(int i, uint32_t) { return ~(uint32_t)i & kIndexMask; }  // lowest first
-__device__ __forceinline__ uint32_t sa_by_key(int, uint32_t key) { return key; }
+__device__ __forceinline__ uint32_t sa_by_index(int i, float) { return ~(uint32_t)i & kIndexMask; }  // lowest first
+__device__ __forceinline__ uint32_t sa_by_logit(int, float x) { return sa_key(x); }
 
-// `last`, from a row or list that has all keys at the border.
+// `last`, from a row or list that has all logits at the border.
 template <class Row>
 __device__ __forceinline__ void sa_last(const Row& row, SaShared& s, SaKept& kept) {
   kept.last = 0x7fffffff;
   if (kept.ties == 0) return;
   uint64_t n = 0, above;
-  row.each([&](int, uint32_t key) { n += key == kept.cut; });
+  row.each([&](int, float x) { n += x == kept.cut; });
   n = sa_sum(n, s);
   if (n > kept.ties)
     kept.last = ~sa_border<kIndexBits>(row, s, kept.ties, above, sa_by_index,
-                                       [&](int, uint32_t key) -> uint64_t { return key == kept.cut ? 1 : 0; }) &
+                                       [&](int, float x) -> uint64_t { return x == kept.cut ? 1 : 0; }) &
                 kIndexMask;
 }
 
-// What top_p keeps: the keys from a border, found in a row or list of which `counts` says what is summed up; the
-// sum of all larger ones is `front`.
+// What top_p keeps: the logits from a border, found in a row or list of which `counts` says what is summed
+// up; the sum of all larger ones is `front`.
 template <class Row, class Counts>
 __device__ __forceinline__ void sa_top_p(const Row& row, SaShared& s, const SaRule& rule, uint64_t need, uint64_t front,
                                          SaKept& kept, Counts counts) {
   uint64_t above;
-  const uint32_t c = sa_border<32>(row, s, need - front, above, sa_by_key, [&](int, uint32_t key) -> uint64_t {
-    const uint64_t w = rule.weight(key);
-    return counts(key) ? w : 0;
-  });
+  const float c = sa_value(sa_border<32>(row, s, need - front, above, sa_by_logit, [&](int, float x) -> uint64_t {
+    const uint64_t w = rule.weight(x);
+    return counts(x) ? w : 0;
+  }));
   const uint64_t w = rule.weight(c), n = (need - front - above + w - 1) / w;
   if (c > kept.cut || n < kept.ties) kept.cut = c, kept.ties = n;
 }
@@ -316,32 +330,30 @@ __device__ __forceinline__ void sa_top_p(const Row& row, SaShared& s, const SaRu
 // top_k.
 template <class Row>
 __device__ __forceinline__ SaKept sa_cuts(const Row& row, SaShared& s, const SaRule& rule, uint64_t total) {
-  SaKept kept{rule.least, 0x7fffffff, 0};
+  SaKept kept{-INFINITY, 0x7fffffff, 0};
   if (rule.k > 0) {
     uint64_t n = 0, above;
-    row.each([&](int, uint32_t key) { n += key > rule.least; });
+    row.each([&](int, float x) { n += x > -INFINITY; });
     n = sa_sum(n, s);
     if (n > (uint64_t)rule.k) {
-      kept.cut = sa_border<32>(row, s, rule.k, above, sa_by_key,
-                               [&](int, uint32_t key) -> uint64_t { return key > rule.least ? 1 : 0; });
+      kept.cut = sa_value(sa_border<32>(row, s, rule.k, above, sa_by_logit,
+                                        [&](int, float x) -> uint64_t { return x > -INFINITY ? 1 : 0; }));
       kept.ties = rule.k - above;
     }
   }
   if (rule.p < 1.0) {
     const uint64_t at_cut = rule.weight(kept.cut);
     uint64_t here = 0;
-    row.each([&](int, uint32_t key) {
-      const uint64_t w = rule.weight(key);
-      here += key > kept.cut ? w : 0;
+    row.each([&](int, float x) {
+      const uint64_t w = rule.weight(x);
+      here += x > kept.cut ? w : 0;
     });
     here = sa_sum(here, s) + kept.ties * at_cut;
-    if (rule.k > 0) total = here;
-    const uint64_t need = max((uint64_t)ceil(rule.p * (double)total), (uint64_t)1);
+    const uint64_t need = rule.need(rule.k > 0 ? here : total);
     if (need <= here)  // (else more than what is here is kept)
-      sa_top_p(row, s, rule, need, 0, kept,
-               [&](uint32_t key) { return key > kept.cut || (key == kept.cut && kept.ties); });
+      sa_top_p(row, s, rule, need, 0, kept, [&](float x) { return x > kept.cut || (x == kept.cut && kept.ties); });
   }
-  if (rule.min_cut > kept.cut) kept.cut = rule.min_cut - 1, kept.ties = 0;
+  kept.above(rule.min_cut);
   sa_last(row, s, kept);
   return kept;
 }
@@ -351,39 +363,27 @@ template <class Row>
 __device__ __forceinline__ void sa_draw(const Row& row, SaShared& s, const SaRule& rule, const SaKept& kept, double u,
                                         int32_t* token, float* logprob) {
   uint64_t above;
-  auto any = [&](int i, uint32_t key) {  // whether there is a weight at all, however small
-    return kept(i, key) && (key == rule.top ||
-                            (key > rule.least && ((double)sa_value(key) - rule.x_max) * rule.scale > -745.0));
-  };
-  auto measure = [&](int i, uint32_t key) -> uint64_t {
-    const bool k = kept(i, key);
+  auto measure = [&](int i, float x) -> uint64_t {
+    const bool k = kept(i, x);
     if (!__any(k)) return 0;
-    const uint64_t w = rule.weight(key);
+    const uint64_t w = rule.weight(x);
     return k ? w : 0;
   };
-  // u sum < a running sum  <=>  floor(u sum) < it, a whole number.
-  auto goal_of = [&](uint64_t sum) {
-    const uint64_t goal = u > 0.0 ? (uint64_t)(u * (double)sum) : 0;
-    return goal < sum ? goal : sum - 1;
-  };
-  auto answer = [&](uint32_t i, uint32_t key, uint64_t sum) {
+  auto answer = [&](uint32_t i, float x, uint64_t sum) {
     *token = (int32_t)i;
-    if (logprob) {
-      const double y = key == rule.top ? 0.0 : ((double)sa_value(key) - rule.x_max) * rule.scale;
-      *logprob = (float)(y - log(ldexp((double)sum, -rule.shift)));
-    }
+    if (logprob) *logprob = rule.share(x, sum);
   };
   if (std::is_same<Row, SaList>::value || !(u > 0.0)) {
     uint64_t sum = 0;
-    row.each([&](int i, uint32_t key) { sum += measure(i, key); });
+    row.each([&](int i, float x) { sum += measure(i, x); });
     sum = sa_sum(sum, s);
-    const uint32_t i =
-        ~(u > 0.0 ? sa_border<kIndexBits>(row, s, goal_of(sum) + 1, above, sa_by_index, measure)
-                  : sa_border<kIndexBits>(row, s, 1, above, sa_by_index,
-                                          [&](int i, uint32_t key) -> uint64_t { return any(i, key) ? 1 : 0; })) &
-        kIndexMask;
-    row.each([&](int j, uint32_t key) {
-      if ((uint32_t)j == i && key != 0) answer(i, key, sum);
+    // (u = 0: the lowest index with any weight, however small)
+    auto any = [&](int i, float x) -> uint64_t { return kept(i, x) && rule.log_weight(x) > -745.0 ? 1 : 0; };
+    const uint32_t i = ~(u > 0.0 ? sa_border<kIndexBits>(row, s, rule.goal(u, sum) + 1, above, sa_by_index, measure)
+                                 : sa_border<kIndexBits>(row, s, 1, above, sa_by_index, any)) &
+                       kIndexMask;
+    row.each([&](int j, float x) {
+      if ((uint32_t)j == i) answer(i, x, sum);
     });
     return;
   }
@@ -391,79 +391,84 @@ __device__ __forceinline__ void sa_draw(const Row& row, SaShared& s, const SaRul
     // The sums of what a wave takes in each round, 256 tokens in a row; then the one in which u falls.
     const int tid = threadIdx.x, wave = tid >> 6, rounds = (row.vocab + kSlot - 1) / kSlot;
     sa_clear(s);
-    row.each4([&](int i, const uint32_t(&key)[4]) {
-      uint64_t x = 0;
+    row.each4([&](int i, const ls_f32x4& x) {
+      uint64_t sum = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x += measure(i + e, key[e]);
-      x = sa_add64(x);
-      if (ls_lane() == 0) s.bins[kBins - 1 - (i / kSlot * kWaves + wave)] = x;
+      for (int e = 0; e < 4; ++e) sum += measure(i + e, x[e]);
+      sum = sa_add64(sum);
+      if (ls_lane() == 0) s.bins[kBins - 1 - (i / kSlot * kWaves + wave)] = sum;
     });
-    uint64_t sum = 0;
     __syncthreads();
-    sum = sa_sum(s.bins[tid] + s.bins[tid + kThreads], s);
-    const uint64_t goal = goal_of(sum);
+    const uint64_t sum = sa_sum(s.bins[tid] + s.bins[tid + kThreads], s);
+    const uint64_t goal = rule.goal(u, sum);
     const uint32_t bin = kBins - 1 - sa_find(s, goal + 1, above);
     if ((int)(bin % kWaves) != wave || (int)(bin / kWaves) >= rounds) return;
     const int i = (int)(bin / kWaves) * kSlot + 4 * tid;
-    uint32_t key[4];
-    uint64_t w[4], x = 0;
-    row.load4(i, key);
+    const ls_f32x4 x = row.load4(i);
+    uint64_t w[4], mine = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x += w[e] = measure(i + e, key[e]);
-    uint64_t before = above + sa_upto64(x) - x;
+    for (int e = 0; e < 4; ++e) mine += w[e] = measure(i + e, x[e]);
+    uint64_t before = above + sa_upto64(mine) - mine;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (before <= goal && goal < before + w[e]) answer(i + e, key[e], sum);
+      if (before <= goal && goal < before + w[e]) answer(i + e, x[e], sum);
       before += w[e];
     }
   }
 }
 
-// The same for at most kFew gathered logits, one a thread: what is in front of it in either order is found by
-// looking at each of the others, without a search or a histogram.
+// All of it for at most kFew gathered logits, one a thread: what is in front of it in either order is found
+// by looking at each of the others.  WAVE: at most 64, by the first wave from its lanes.
+template <bool WAVE>
 __device__ __forceinline__ void sa_draw_few(int n, SaShared& s, const SaRule& rule, uint64_t total, double u,
                                             int32_t* token, float* logprob) {
   const int tid = threadIdx.x;
+  if (WAVE && tid >= 64) return;
   const bool in = tid < n;
-  const uint32_t key = in ? s.key[tid] : 0u, i = in ? s.index[tid] : 0u;
-  uint64_t w = 0;
-  if (tid < kFew) {
-    w = rule.weight(key);
-    s.bins[tid] = w;
+  const float x = in ? s.x[tid] : -INFINITY;
+  const uint32_t i = in ? s.index[tid] : 0x7fffffffu;
+  const uint64_t w = WAVE || tid < kFew ? rule.weight(x) : 0;
+  if (!WAVE) {
+    if (tid < kFew) s.bins[tid] = w;
+    __syncthreads();
   }
-  __syncthreads();
+  auto add = [&](uint64_t v) { return WAVE ? sa_add64(v) : sa_sum(v, s); };
   uint32_t rank = 0;
   uint64_t before = 0;
-  if (in) {
+  if (WAVE || in) {
 #pragma unroll 4
     for (int j = 0; j < n; ++j) {
-      const bool first = s.key[j] > key || (s.key[j] == key && s.index[j] < i);
+      const float xj = WAVE ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), j)) : s.x[j];
+      const uint32_t ij = WAVE ? (uint32_t)__builtin_amdgcn_readlane((int)i, j) : s.index[j];
+      const bool first = xj > x || (xj == x && ij < i);
       rank += first;
-      before += first ? s.bins[j] : 0;
+      before += first ? (WAVE ? sa_lane64(w, j) : s.bins[j]) : 0;
     }
   }
-  bool kept = in && key > rule.least && (rule.k == 0 || rank < (uint32_t)rule.k);
+  bool kept = in && x > -INFINITY && (rule.k == 0 || rank < (uint32_t)rule.k);
   if (rule.p < 1.0) {
-    if (rule.k > 0) total = sa_sum(kept ? w : 0, s);
-    const double goal = ceil(rule.p * (double)total);
-    kept = kept && before < max((uint64_t)goal, (uint64_t)1);
+    if (rule.k > 0) total = add(kept ? w : 0);
+    kept = kept && before < rule.need(total);
   }
-  kept = kept && key >= rule.min_cut;
-  const uint64_t sum = sa_sum(kept ? w : 0, s);
-  const double y = key == rule.top ? 0.0 : ((double)sa_value(key) - rule.x_max) * rule.scale;
+  kept = kept && x > rule.min_cut;
+  const uint64_t sum = add(kept ? w : 0);
   // u = 0: the lowest index with any weight, however small.
-  const uint64_t m = !kept ? 0 : u > 0.0 ? w : y > -745.0 ? 1 : 0;
-  if (tid < kFew) s.bins[tid] = m;
-  __syncthreads();
-  if (m == 0) return;
-  uint64_t goal = u > 0.0 ? (uint64_t)(u * (double)sum) : 0;
-  goal = goal < sum ? goal : sum - 1;
+  const uint64_t m = !kept ? 0 : u > 0.0 ? w : rule.log_weight(x) > -745.0 ? 1 : 0;
+  if (!WAVE) {
+    if (tid < kFew) s.bins[tid] = m;
+    __syncthreads();
+    if (m == 0) return;
+  }
+  const uint64_t goal = u > 0.0 ? rule.goal(u, sum) : 0;
   before = 0;
 #pragma unroll 4
-  for (int j = 0; j < n; ++j) before += s.index[j] < i ? s.bins[j] : 0;
+  for (int j = 0; j < n; ++j) {
+    const uint32_t ij = WAVE ? (uint32_t)__builtin_amdgcn_readlane((int)i, j) : s.index[j];
+    before += ij < i ? (WAVE ? sa_lane64(m, j) : s.bins[j]) : 0;
+  }
   if (before <= goal && goal < before + m) {
     *token = (int32_t)i;
-    if (logprob) *logprob = (float)(y - log(ldexp((double)sum, -rule.shift)));
+    if (logprob) *logprob = rule.share(x, sum);
   }
 }
 
@@ -477,116 +482,118 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
   row.vocab = a.vocab;
   row.wide = ((uintptr_t)row.x & (DT == LS_F32 ? 15 : 7)) == 0;
   if (tid < 16) s.table[tid] = exp2((double)tid / 16.0);
-  uint32_t best[kMaxima] = {}, at = 0;
-  row.each([&](int i, uint32_t key) {
-    at = key > best[0] ? (uint32_t)i : at;
-#pragma unroll
-    for (int m = kMaxima - 1; m > 0; --m) best[m] = max(best[m], min(best[m - 1], key));
-    best[0] = max(best[0], key);
+  float best[2] = {-INFINITY, -INFINITY};
+  row.each([&](int, float x) {
+    best[1] = __builtin_amdgcn_fmed3f(best[0], best[1], x);
+    best[0] = fmaxf(best[0], x);
   });
-  const uint64_t first = sa_max((uint64_t)best[0] << 32 | (uint32_t)~at, s);
   SaRule rule;
-  rule.top = (uint32_t)(first >> 32);
-  rule.least = ls_order_key32(0xff800000u);  // -inf: no weight
-  rule.x_max = sa_value(rule.top);
+  rule.top = sa_value(sa_max(sa_key(best[0]), s));
   const double t = a.ts ? (double)a.ts[r] : a.t;
+  int32_t* token = a.tokens + r;
   float* logprob = a.logprobs ? a.logprobs + r : nullptr;
-  if (rule.top <= rule.least || !(t > 0.0)) {
-    // Nothing to draw from, or the largest alone.
+  if (!(rule.top > -INFINITY) || !(t > 0.0)) {
+    // Nothing to draw from, or the lowest index of the largest.
+    uint32_t first = 0;
+    if (rule.top > -INFINITY)
+      row.each([&](int i, float x) { first = x == rule.top ? max(first, ~(uint32_t)i) : first; });
+    first = sa_max(first, s);
     if (tid == 0) {
-      const bool none = rule.top <= rule.least;
-      a.tokens[r] = none ? -1 : (int32_t)~(uint32_t)first;
-      if (logprob) *logprob = none ? -INFINITY : 0.f;
+      *token = (int32_t)~first;  // (0: -1)
+      if (logprob) *logprob = first ? 0.f : -INFINITY;
     }
     return;
   }
-  rule.scale = 1.0 / t;
-  rule.scale2 = 1.4426950408889634074 / t;
+  rule.inv = 1.0 / t;
+  rule.scale = 1.4426950408889634074 / t;
+  rule.off = -(double)rule.top * rule.scale;
   rule.shift = a.shift;
+  rule.table = s.table;
   rule.k = a.top_ks ? a.top_ks[r] : a.top_k;
   if (rule.k <= 0 || rule.k >= a.vocab) rule.k = 0;
   rule.p = a.top_ps ? (double)a.top_ps[r] : a.top_p;
-  rule.table = s.table;
-  rule.min_cut = 0;
+  rule.min_cut = -INFINITY;
   const double min_p = a.min_ps ? (double)a.min_ps[r] : a.min_p;
   if (min_p > 0.0) {
-    // exp((x - max) / t) >= min_p  <=>  x >= max + t ln min_p.
-    const double border = (double)rule.x_max + log(min_p) * t;
-    const float f = (float)border;
-    uint32_t c = ls_order_key32(__float_as_uint(f == 0.f ? 0.f : f));
-    if ((double)f < border) ++c;  // the least logit that is not below it
-    rule.min_cut = min(c, rule.top);
+    // exp((x - max) / t) >= min_p  <=>  x >= max + t ln min_p; the next logit below passes not.
+    const double border = (double)rule.top + log(min_p) * t;
+    const float f = fminf((float)border, rule.top);
+    if (f > -INFINITY) rule.min_cut = (double)f < border && f < rule.top ? f : sa_value(sa_key(f) - 1);
   }
   const double u = (double)a.u[r];
-  // What is kept, or has to be summed up, is among the keys from `low` that are no more than `far` bins of
-  // 1 / `to_bins` from the maximum.
-  uint32_t low = rule.least + 1;
+  // What is kept, or has to be summed up, is among the logits above `low`.
+  float low = -INFINITY;
+  uint64_t total = 0, need = 0;
   float to_bins = 0.f;
-  int far = 0;
-  auto bin_of = [&](uint32_t key) {  // (falls as the key rises)
-    const float d = (rule.x_max - sa_value(key)) * to_bins;
+  auto bin_of = [&](float x) {  // (falls as x rises)
+    const float d = (rule.top - x) * to_bins;
     return d < kBins - 1 ? (int)d : kBins - 1;
   };
-  uint64_t total = 0, need = 0;
   bool bounded = false;
   if (rule.k > 0 && rule.k <= kBounded) {
-    // Some of the threads' largest are the k-th largest or more; their k-th largest is a bound.
-    static_assert(kBounded <= 2 * kThreads && kMaxima >= 2, "");
-    const uint32_t mine = rule.k <= kThreads ? best[0] : best[1];
-    const uint32_t least = ~(uint32_t)sa_max(~mine, s);
-    const float range = rule.x_max - sa_value(least);
+    // Each thread's largest (and second) are top_k or more in all; the border among them, by bins, is a bound.
+    const float least = sa_value(~sa_max(~sa_key(rule.k <= kThreads ? best[0] : best[1]), s));
+    const float range = rule.top - least;
     bounded = true;
-    if (least > rule.least && range > 0.f && range < INFINITY) {
+    if (least > -INFINITY && range > 0.f && range < INFINITY) {
       to_bins = (kBins - 2) / range;
       sa_clear(s);
 #pragma unroll
-      for (int m = 0; m < kMaxima; ++m)
+      for (int m = 0; m < 2; ++m)
         if (best[m] >= least) atomicAdd(&s.bins[kBins - 1 - bin_of(best[m])], 1ull);
       uint64_t before;
-      far = kBins - 1 - (int)sa_find(s, rule.k, before);
-    } else if (least > rule.least) {
-      low = least;
+      const uint32_t bin = kBins - 1 - sa_find(s, rule.k, before);
+      // (two bins more: theirs are rounded products)
+      low = fmaxf(sa_value(sa_key(least) - 1), rule.top - (bin + 2) / to_bins);
     }
   } else if (rule.k == 0 && rule.p < 1.0) {
-    row.each([&](int, uint32_t key) { total += rule.weight(key); });
+    row.each([&](int, float x) { total += rule.weight(x); });
     total = sa_sum(total, s);
-    need = min(max((uint64_t)ceil(rule.p * (double)total), (uint64_t)1), total);
+    need = min(rule.need(total), total);
     // (a hundredth below it: the bound is rounded)
-    const double least = (1.0 - rule.p) * ldexp((double)total, -rule.shift) / a.vocab;
-    const float f = (float)((double)rule.x_max + t * (log(least) - 0.01));
-    low = max(low, ls_order_key32(__float_as_uint(f == 0.f ? 0.f : f)));
+    low = (float)((double)rule.top + t * (log((1.0 - rule.p) * ldexp((double)total, -rule.shift) / a.vocab) - 0.01));
     bounded = true;
   }
   // (What top_p sums up is more than what min_p leaves.)
   if (!(rule.k > 0 && rule.p < 1.0)) {
-    low = max(low, rule.min_cut);
-    bounded = bounded || rule.min_cut > rule.least + 1;
+    low = fmaxf(low, rule.min_cut);
+    bounded = bounded || rule.min_cut > -INFINITY;
   }
+  low = fminf(low, sa_value(sa_key(rule.top) - 1));  // (the largest are kept whatever the settings hold)
   // Logits into LDS, a wave's in one go.
   auto gather = [&](auto take) {
     __syncthreads();
     if (tid == 0) s.n = 0;
     __syncthreads();
-    row.each([&](int i, uint32_t key) {
-      const uint64_t mask = __ballot(take(key));
-      if (mask == 0) return;
-      uint32_t n = 0;
-      if (ls_lane() == 0) n = atomicAdd(&s.n, (uint32_t)__popcll(mask));
-      n = __builtin_amdgcn_readfirstlane(n) + ls_lanes_below(mask);
-      if (take(key) && n < kList) s.key[n] = key, s.index[n] = (uint32_t)i;
+    row.each4([&](int i, const ls_f32x4& x) {
+      bool t4[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t4[e] = take(x[e]);
+      if (!__any(t4[0] | t4[1] | t4[2] | t4[3])) return;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint64_t mask = __ballot(t4[e]);
+        uint32_t n = 0;
+        if (ls_lane() == 0 && mask != 0) n = atomicAdd(&s.n, (uint32_t)__popcll(mask));
+        n = __builtin_amdgcn_readfirstlane(n) + ls_lanes_below(mask);
+        if (t4[e] && n < kList) s.x[n] = x[e], s.index[n] = (uint32_t)(i + e);
+      }
     });
     __syncthreads();
     return (int)s.n;
   };
-  int32_t* token = a.tokens + r;
   if (bounded) {
-    const int n = gather([&](uint32_t key) { return key >= low && (to_bins == 0.f || bin_of(key) <= far); });
+    const int n = gather([&](float x) { return x > low; });
+    if (n <= 64) {
+      sa_draw_few<true>(n, s, rule, total, u, token, logprob);
+      return;
+    }
     if (n <= kFew) {
-      sa_draw_few(n, s, rule, total, u, token, logprob);
+      sa_draw_few<false>(n, s, rule, total, u, token, logprob);
       return;
     }
     if (n <= kList) {
-      const SaList list{s.key, s.index, n};
+      const SaList list{s.x, s.index, n};
       sa_draw(list, s, rule, sa_cuts(list, s, rule, total), u, token, logprob);
       return;
     }
@@ -595,34 +602,34 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
     // Bins of 1/32 of a temperature; then, where too many logits are in the border's, of 1/65536.
     to_bins = (float)(32.0 / t);
     sa_clear(s);
-    row.each([&](int, uint32_t key) {
-      const uint64_t w = rule.weight(key);
-      if (w != 0) atomicAdd(&s.bins[kBins - 1 - bin_of(key)], (unsigned long long)w);
+    row.each([&](int, float x) {
+      const uint64_t w = rule.weight(x);
+      if (w != 0) atomicAdd(&s.bins[kBins - 1 - bin_of(x)], (unsigned long long)w);
     });
     uint64_t front;
     const int bin = kBins - 1 - (int)sa_find(s, need, front);
-    auto in_bin = [&](uint32_t key) { return key > rule.least && bin_of(key) == bin; };
+    auto in_bin = [&](float x) { return x > -INFINITY && bin_of(x) == bin; };
     int n = gather(in_bin), sub = -1;
-    auto sub_of = [&](uint32_t key) {
-      const float d = ((rule.x_max - sa_value(key)) * to_bins - (float)bin) * kBins;
+    auto sub_of = [&](float x) {
+      const float d = ((rule.top - x) * to_bins - (float)bin) * kBins;
       return d < kBins - 1 ? max((int)d, 0) : kBins - 1;
     };
     if (n > kList) {
       sa_clear(s);
-      row.each([&](int, uint32_t key) {
-        const uint64_t w = rule.weight(key);
-        if (w != 0 && in_bin(key)) atomicAdd(&s.bins[kBins - 1 - sub_of(key)], (unsigned long long)w);
+      row.each([&](int, float x) {
+        const uint64_t w = rule.weight(x);
+        if (w != 0 && in_bin(x)) atomicAdd(&s.bins[kBins - 1 - sub_of(x)], (unsigned long long)w);
       });
       uint64_t before;
       sub = kBins - 1 - (int)sa_find(s, need - front, before);
       front += before;
-      n = gather([&](uint32_t key) { return in_bin(key) && sub_of(key) == sub; });
+      n = gather([&](float x) { return in_bin(x) && sub_of(x) == sub; });
     }
     if (n <= kList) {
-      const SaList list{s.key, s.index, n};
-      SaKept kept{rule.least, 0x7fffffff, 0};
-      sa_top_p(list, s, rule, need, front, kept, [](uint32_t) { return true; });
-      if (rule.min_cut > kept.cut) kept.cut = rule.min_cut - 1, kept.ties = 0;
+      const SaList list{s.x, s.index, n};
+      SaKept kept{-INFINITY, 0x7fffffff, 0};
+      sa_top_p(list, s, rule, need, front, kept, [](float) { return true; });
+      kept.above(rule.min_cut);
       sa_last(list, s, kept);
       sa_draw(row, s, rule, kept, u, token, logprob);
       return;
