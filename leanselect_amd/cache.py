@@ -13,15 +13,19 @@ lists.  A step of new tokens is written layer by layer between ``begin`` and
 scale per page and head, ``ops.decode_q8``): half the memory and half the bytes a
 step reads.  The compressed keys stay in ``dtype``; those the cache forms are means
 of the keys as it holds them.
+
+``fork`` makes a :class:`SharedPrefixKVCache` of a cache with one sequence: several sequences that
+go on from it, its keys and values kept once.
 """
 from __future__ import annotations
 
 import torch
 
+from .ops.cache_attention import shared_prefix_attention
 from .ops.decode import kvcache_append, n_windows, sparse_attention_kvcache
 from .ops.decode_q8 import kvcache_append_q8, new_kvcache_q8, sparse_attention_kvcache_q8
 
-__all__ = ["LeanSelectKVCache"]
+__all__ = ["LeanSelectKVCache", "SharedPrefixKVCache"]
 
 
 class LeanSelectKVCache:
@@ -111,6 +115,16 @@ class LeanSelectKVCache:
     def lengths_after(self) -> list[int]:
         return list(self._require_step()["after_host"])
 
+    @property
+    def positions(self) -> list[int]:
+        """The positions that the next token of each sequence takes (outside a step)."""
+        return list(self.lengths)
+
+    def fork(self, batch: int, capacity: int) -> "SharedPrefixKVCache":
+        """``batch`` sequences that go on from this cache's one, for up to ``capacity`` tokens each.
+        The cache is the prefix of them all and must not change while they are in use."""
+        return SharedPrefixKVCache(self, batch, capacity)
+
     def get_seq_length(self) -> int:
         """Tokens of the longest sequence (outside a step)."""
         return max(self.lengths)
@@ -119,3 +133,42 @@ class LeanSelectKVCache:
         if self._step is None:
             raise RuntimeError("no cache step is open (call begin first)")
         return self._step
+
+
+class SharedPrefixKVCache(LeanSelectKVCache):
+    """Sequences that begin with what ``prefix`` (a cache of one sequence, 16-bit) holds, each with a
+    cache of its own behind it.  The step protocol is that of :class:`LeanSelectKVCache`, lengths
+    counting the own tokens; ``attend`` is dense, over the prefix and the own tokens (no page plans,
+    and no compressed keys are formed)."""
+
+    def __init__(self, prefix: LeanSelectKVCache, batch: int, capacity: int):
+        if prefix.kv_format != "native" or isinstance(prefix, SharedPrefixKVCache):
+            raise ValueError("only a 16-bit cache without a prefix of its own can be shared")
+        if prefix.batch != 1 or prefix.lengths[0] < 1 or prefix._step is not None:
+            raise ValueError("a shared prefix is one sequence, prefilled, with no step open")
+        super().__init__(prefix.num_layers, batch, capacity, prefix.k.shape[3], prefix.k.shape[4],
+                         dtype=prefix.k.dtype, device=prefix.device, kernel_size=prefix.kernel_size,
+                         kernel_stride=prefix.kernel_stride)
+        self.kc = None
+        self.prefix_len = prefix.lengths[0]
+        self.k_prefix = prefix.k[:, 0, :self.prefix_len]
+        self.v_prefix = prefix.v[:, 0, :self.prefix_len]
+
+    def update(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
+        st = self._require_step()
+        kvcache_append(*self.layer(layer), self.seqlens, k_new, v_new, st["cu"],
+                       cache_seqlens_host=self.lengths, cu_seqlens_new_host=st["cu_host"])
+
+    def attend(self, layer: int, q: torch.Tensor, cu_seqlens_q: torch.Tensor, **kw) -> torch.Tensor:
+        """Attention of the open step's rows over the prefix and their own tokens
+        (``ops.shared_prefix_attention``; ``kw`` are its options)."""
+        st = self._require_step()
+        return shared_prefix_attention(q, self.k_prefix[layer], self.v_prefix[layer], *self.layer(layer),
+                                       st["after"], cu_seqlens_q, max(st["after_host"]), **kw)
+
+    @property
+    def positions(self) -> list[int]:
+        return [self.prefix_len + n for n in self.lengths]
+
+    def fork(self, batch: int, capacity: int):
+        raise ValueError("only a 16-bit cache without a prefix of its own can be shared")

@@ -28,6 +28,10 @@ pages (minicpm.py:3216-3244 with ``causal=False``).
 projections, the MLPs and the head in 4 bits (``ops.mx4``): a decode step then reads
 about half and a quarter of the bytes.
 
+``generate`` draws several answers to one prompt: the prompt is prefilled once, its cache is
+forked (``LeanSelectKVCache.fork``), and each step attends the prompt once for all answers, densely,
+and draws their next tokens (``ops.sample_logits``).
+
 Weights are random-initialised (no checkpoint is loaded here).  Nothing in this
 module falls back to a non-HIP path: it raises when the library is missing or
 the tensors are not on a GPU.
@@ -42,9 +46,10 @@ import torch
 import torch.nn.functional as F
 
 from . import _hip
-from .cache import LeanSelectKVCache
+from .cache import LeanSelectKVCache, SharedPrefixKVCache
 from .ops.decode import decode_topk_idx
 from .ops.mx4 import dequantize_mx4, linear_mx4, linear_mx4_silu_mul, quantize_mx4
+from .ops.sampling import sample_logits
 from .prefill import leanselect_sparse_prefill
 from .selector import LeanSelectSelector
 
@@ -611,18 +616,22 @@ class MiniCPMLeanSelect:
         """Attention block of layer ``li`` for one new token per sequence
         (``h [B, hidden]``): projection, rotary embedding at each sequence's
         position, append to the cache, stage-1 page plans on the compressed-key
-        cache, block-sparse attention over the cache, output projection."""
+        cache, block-sparse attention over the cache (of a forked cache: dense
+        attention over the shared prefix and the own tokens), output projection."""
         cfg, L = self.cfg, self.layers[li]
         H, G, D = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
         B = h.shape[0]
         qkv = _linear(h, L.w_qkv)
-        cos, sin = self.rope_tables(max(cache.lengths_after))
+        shared = isinstance(cache, SharedPrefixKVCache)
+        cos, sin = self.rope_tables(max(cache.lengths_after) + (cache.prefix_len if shared else 0))
         rope_inplace(qkv, positions, cos, sin, n_q_heads=H, n_k_heads=G, k_col_offset=H * D,
                      head_dim=D, check_positions=False)
         q = qkv[:, : H * D].view(B, H, D)
         k = qkv[:, H * D: H * D + G * D].view(B, G, D)
         v = qkv[:, H * D + G * D:].view(B, G, D)
         cache.update(li, k, v)
+        if shared:
+            return _linear(cache.attend(li, q, cu_q).view(B, H * D), L.w_o)
         after = cache.lengths_after
         ids = decode_topk_idx(q, cache.kc[li], cache.seqlens_after, cu_q, topk=cfg.topk,
                               init_blocks=cfg.init_blocks, local_blocks=cfg.local_blocks,
@@ -640,10 +649,10 @@ class MiniCPMLeanSelect:
         B = input_ids.numel()
         if B != cache.batch:
             raise ValueError(f"one token per cached sequence: {B} ids for {cache.batch} slots")
-        if min(cache.lengths) < 1:
+        if min(cache.positions) < 1:
             raise ValueError("decode_step continues prefilled sequences")
         dev = _hip.require_gpu(input_ids)
-        pos = torch.tensor(cache.lengths, dtype=torch.int32, device=dev)
+        pos = torch.tensor(cache.positions, dtype=torch.int32, device=dev)
         cu_q_host = list(range(B + 1))
         cu_q = torch.tensor(cu_q_host, dtype=torch.int32, device=dev)
         cache.begin([1] * B)
@@ -658,3 +667,21 @@ class MiniCPMLeanSelect:
             add_rms_layernorm(x, d, c, nxt, cfg.rms_norm_eps, out=h)
         cache.end()
         return _linear(h / (cfg.hidden_size / cfg.dim_model_base), self.lm_head).float()
+
+    @torch.no_grad()
+    def generate(self, input_ids: torch.Tensor, u: torch.Tensor, **sampling) -> torch.Tensor:
+        """int32 ``[n, steps]``: ``n`` answers of ``steps`` tokens to the prompt ``input_ids`` (int32 ``[N]``),
+        drawn by the numbers ``u`` (float32 ``[steps, n]``, in [0, 1)) with ``ops.sample_logits``'s settings.
+
+        The prompt goes through ``prefill`` once; the answers' attention is dense, over the prompt (read
+        once for all of them) and their own tokens."""
+        if u.ndim != 2 or u.shape[0] < 1 or u.shape[1] < 1 or u.dtype != torch.float32:
+            raise ValueError("u must be float32 [steps, answers]")
+        steps, n = u.shape
+        prompt = self.new_cache(1, input_ids.numel())
+        logits = self.prefill(input_ids, cache=prompt)
+        cache = prompt.fork(n, max(1, steps - 1))
+        tokens = [sample_logits(logits.expand(n, -1), u[0], **sampling)]
+        for step in range(1, steps):
+            tokens.append(sample_logits(self.decode_step(tokens[-1], cache), u[step], **sampling))
+        return torch.stack(tokens, 1)
