@@ -17,9 +17,8 @@
 //
 // A border is found by a radix search, 11 bits a round, in a histogram in LDS of how many keys, or how much
 // weight, each value of the bits has; a draw from what was gathered is the same search over the
-// indices, one from the row takes the sums of 256 tokens each.  Weights are summed as whole numbers of 2^-s, s
-// such that a row's sum stays under 2^62 (2^-45 for 73448 tokens): sums do not depend on their order, so
-// neither does the token.
+// indices, one from the row takes the sums of 256 tokens each.  Weights are summed as whole numbers of 2^-40:
+// sums do not depend on their order, so neither does the token.
 //
 // The reference draws with torch's multinomial on the host's settings; it has no such kernel.
 #include <algorithm>
@@ -39,6 +38,7 @@ constexpr int kSlot = 4 * kThreads;  // tokens of a round over the row
 constexpr int kIndexBits = 19;
 constexpr uint32_t kIndexMask = (1u << kIndexBits) - 1;
 static_assert((1 << kIndexBits) / kSlot * kWaves <= kBins, "a bin for what a wave takes in each round");
+constexpr int kShift = 40;       // weights are whole numbers of 2^-40: a row's sum is 2^59 at most
 static_assert(kBounded <= 2 * kThreads, "");
 
 struct SaArgs {
@@ -53,7 +53,6 @@ struct SaArgs {
   const int32_t* top_ks;
   const float* top_ps;
   const float* min_ps;
-  int shift;  // weights are whole numbers of 2^-shift
   int32_t* tokens;
   float* logprobs;
 };
@@ -68,26 +67,28 @@ __device__ __forceinline__ uint64_t sa_lane64(uint64_t x, int lane) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane) |
          (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32;
 }
-__device__ __forceinline__ uint64_t sa_add64(uint64_t x) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor((unsigned long long)x, o, 64);
-  return x;
+// Inclusive sum over the lanes up to this one, by shifts within rows of 16 and broadcasts of their last.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t sa_dpp64(uint64_t x) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, true);
+  return (uint64_t)lo | (uint64_t)hi << 32;
 }
-// Inclusive sum over the lanes up to this one.
 __device__ __forceinline__ uint64_t sa_upto64(uint64_t x) {
-  const int lane = ls_lane();
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint64_t y = __shfl_up((unsigned long long)x, d, 64);
-    if (lane >= d) x += y;
-  }
+  x += sa_dpp64<0x111, 0xf>(x);
+  x += sa_dpp64<0x112, 0xf>(x);
+  x += sa_dpp64<0x114, 0xf>(x);
+  x += sa_dpp64<0x118, 0xf>(x);
+  x += sa_dpp64<0x142, 0xa>(x);
+  x += sa_dpp64<0x143, 0xc>(x);
   return x;
 }
+__device__ __forceinline__ uint64_t sa_add64(uint64_t x) { return sa_lane64(sa_upto64(x), 63); }
 
 struct SaShared {
   unsigned long long bins[kBins];
   unsigned long long part[kWaves];
-  double table[16];
+  double table[64];
   unsigned long long found;
   uint32_t at;
   uint32_t n;
@@ -144,7 +145,7 @@ struct SaRow {
   }
 };
 
-// What was gathered.  (Every lane runs every round: the weights are formed by whole waves.)
+// What was gathered.
 struct SaList {
   const float* x;
   const uint32_t* index;
@@ -236,33 +237,24 @@ struct SaRule {
   float top;
   double inv;         // 1 / temperature
   double scale, off;  // a logit's base-2 exponent: scale x + off
-  int shift;
   int k;          // 0: none
   double p;
   float min_cut;  // logits above it pass min_p
   const double* table;
 
-  // 2^y in whole numbers of 2^-shift.  The power of y's fraction: under 2^31 of them in float32 (1.5e-7 of
-  // it); above, where that would show, from a table of 2^(k / 16) and exp(g) to the seventh power
-  // (|g| < 0.022: 2^-54).
+  // 2^y in whole numbers of 2^-40, y = m / 64 + f: a table of 2^(k / 64), and 2^f to the fourth power (|f| <
+  // 2^-7: 2^-44).  Rounding to m, and of the result, by adding a number that leaves no smaller bits.
   __device__ __forceinline__ uint64_t weight(float x) const {
-    const double y = fma((double)x, scale, off), n = rint(y);
-    const bool near = y > 30.5 - shift;
-    const int e = (int)n + shift;
-    uint64_t w = (uint32_t)rintf(ldexpf(__builtin_amdgcn_exp2f((float)(y - n)), near ? 0 : max(e, -200)));
-    if (__any(near)) {
-      const double m = rint(16.0 * y), g = fma(m, -1.0 / 16.0, y) * 0.69314718055994530942;
-      double q = fma(g, 1.0 / 720.0, 1.0 / 120.0);
-      q = fma(g, q, 1.0 / 24.0);
-      q = fma(g, q, 1.0 / 6.0);
-      q = fma(g, q, 0.5);
-      q = fma(g, q, 1.0);
-      q = fma(g, q, 1.0);
-      const int k = (int)m;
-      const uint64_t exact = (uint64_t)rint(ldexp(q * table[k & 15], (k >> 4) + shift));
-      w = near ? exact : w;
-    }
-    return x == top ? 1ull << shift : x > -INFINITY && top < INFINITY ? w : 0;
+    const double y = fmax(fma((double)x, scale, off), -60.0);
+    const double m = y + 0x1.8p46, f = y - (m - 0x1.8p46);
+    const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, m);  // 64 y, rounded
+    double q = fma(f, 0.0096181291076284771619, 0.055504108664821579953);
+    q = fma(f, q, 0.24022650695910071233);
+    q = fma(f, q, 0.69314718055994530942);
+    q = fma(f, q, 1.0);
+    const double w = ldexp(q * table[k & 63], (k >> 6) + kShift) + 0x1p52;
+    const uint64_t whole = __builtin_bit_cast(uint64_t, w) & 0xfffffffffffffull;
+    return x == top ? 1ull << kShift : top < INFINITY ? whole : 0;
   }
   // ln of the weight.
   __device__ __forceinline__ double log_weight(float x) const {
@@ -270,7 +262,7 @@ struct SaRule {
   }
   // ln of its share of a sum.
   __device__ __forceinline__ float share(float x, uint64_t sum) const {
-    return (float)(log_weight(x) - log(ldexp((double)sum, -shift)));
+    return (float)(log_weight(x) - log(ldexp((double)sum, -kShift)));
   }
   __device__ __forceinline__ uint64_t need(uint64_t total) const {
     return max((uint64_t)ceil(p * (double)total), (uint64_t)1);
@@ -365,9 +357,7 @@ __device__ __forceinline__ void sa_draw(const Row& row, SaShared& s, const SaRul
   uint64_t above;
   auto measure = [&](int i, float x) -> uint64_t {
     const bool k = kept(i, x);
-    if (!__any(k)) return 0;
-    const uint64_t w = rule.weight(x);
-    return k ? w : 0;
+    return __any(k) ? (k ? rule.weight(x) : 0) : 0;
   };
   auto answer = [&](uint32_t i, float x, uint64_t sum) {
     *token = (int32_t)i;
@@ -481,7 +471,7 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
   row.x = (const typename LsElem<DT>::T*)a.x + r * a.rs;
   row.vocab = a.vocab;
   row.wide = ((uintptr_t)row.x & (DT == LS_F32 ? 15 : 7)) == 0;
-  if (tid < 16) s.table[tid] = exp2((double)tid / 16.0);
+  if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
   float best[2] = {-INFINITY, -INFINITY};
   row.each([&](int, float x) {
     best[1] = __builtin_amdgcn_fmed3f(best[0], best[1], x);
@@ -507,7 +497,6 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
   rule.inv = 1.0 / t;
   rule.scale = 1.4426950408889634074 / t;
   rule.off = -(double)rule.top * rule.scale;
-  rule.shift = a.shift;
   rule.table = s.table;
   rule.k = a.top_ks ? a.top_ks[r] : a.top_k;
   if (rule.k <= 0 || rule.k >= a.vocab) rule.k = 0;
@@ -551,7 +540,7 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
     total = sa_sum(total, s);
     need = min(rule.need(total), total);
     // (a hundredth below it: the bound is rounded)
-    low = (float)((double)rule.top + t * (log((1.0 - rule.p) * ldexp((double)total, -rule.shift) / a.vocab) - 0.01));
+    low = (float)((double)rule.top + t * (log((1.0 - rule.p) * ldexp((double)total, -kShift) / a.vocab) - 0.01));
     bounded = true;
   }
   // (What top_p sums up is more than what min_p leaves.)
@@ -565,17 +554,20 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
     __syncthreads();
     if (tid == 0) s.n = 0;
     __syncthreads();
+    bool full = false;
     row.each4([&](int i, const ls_f32x4& x) {
       bool t4[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) t4[e] = take(x[e]);
-      if (!__any(t4[0] | t4[1] | t4[2] | t4[3])) return;
+      if (!__any(t4[0] | t4[1] | t4[2] | t4[3]) || full) return;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint64_t mask = __ballot(t4[e]);
         uint32_t n = 0;
         if (ls_lane() == 0 && mask != 0) n = atomicAdd(&s.n, (uint32_t)__popcll(mask));
-        n = __builtin_amdgcn_readfirstlane(n) + ls_lanes_below(mask);
+        n = __builtin_amdgcn_readfirstlane(n);
+        full = n > kList;  // (one more than fits is all that matters)
+        n += ls_lanes_below(mask);
         if (t4[e] && n < kList) s.x[n] = x[e], s.index[n] = (uint32_t)(i + e);
       }
     });
@@ -669,8 +661,6 @@ extern "C" int ls_sample_logits(const void* logits, int64_t row_stride, int64_t 
   a.top_ks = top_ks;
   a.top_ps = top_ps;
   a.min_ps = min_ps;
-  a.shift = 62;
-  while (a.shift > 40 && (int64_t)1 << (62 - a.shift) < vocab) --a.shift;
   a.tokens = tokens;
   a.logprobs = logprobs;
   hipStream_t s = (hipStream_t)stream;

@@ -82,8 +82,8 @@ def cache_attention(q, k_cache, v_cache, lens, cu, *, k_prefix=None, v_prefix=No
 def sample_row(logits, u, temperature, top_k, top_p, min_p):
     """``(token, logprob, sure, off)`` of one row of float logits, in 64 bits.
 
-    ``off``: the share of the sums by which a kernel's may be off: 2e-7 of the weights below 2^-12 (a power
-    in float32, of one unit) and 1e-10 of the others (whole numbers of 2^-43).  ``sure``: whether the token is the same with ``top_p`` and ``u`` moved
+    ``off``: the share of the sums by which a kernel's may be off: 2^-43 of each weight, and 2^-41, as they are
+    whole numbers of 2^-40.  ``sure``: whether the token is the same with ``top_p`` and ``u`` moved
     by that much either way (equal weights are exact)."""
     x = np.asarray(logits, dtype=np.float64)
     x = np.where(np.isnan(x), -np.inf, x)
@@ -100,7 +100,7 @@ def sample_row(logits, u, temperature, top_k, top_p, min_p):
         order = order[:top_k]
     run = weight[order]
     total = run.sum()
-    off = 1e-10 + 2e-7 * run[y[order] < -8.31].sum() / total
+    off = 2.0 ** -43 + run.size * 2.0 ** -41 / total
 
     def draw(p, u):
         n = order.size
