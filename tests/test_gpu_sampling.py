@@ -132,6 +132,18 @@ def test_infinities_and_nan(dtype, settings):
     assert got[1] == 0 and got[2] == got[3] == -1 and got[5] in (7, 70, 5000) and got[6] >= 5990
 
 
+@pytest.mark.parametrize("settings", [
+    dict(temperature=1e-30), dict(temperature=1e-6), dict(temperature=1e20), dict(temperature=0.05), dict(top_p=0.5),
+    dict(top_p=1.0 - 2.0 ** -24)], ids=str)
+@pytest.mark.parametrize("scale,shift", [(1.0, 0.0), (1e-30, 0.0), (1e3, 0.0), (1.0, 1e6), (0.0, -3e38), (1e37, 0.0)])
+def test_top_p_at_odd_scales(settings, scale, shift):
+    """Where top_p's border falls far from, at or just below the maximum, or the distances overflow."""
+    g = torch.Generator().manual_seed(11)
+    x = scale * torch.randn(5, 10007, generator=g).clamp(-4, 4) + shift
+    x[1, 17], x[2, ::2], x[3, 9000] = float("inf"), -float("inf"), 3e38
+    _check(x, torch.rand(5, generator=g), **dict(dict(top_p=0.9), **settings))
+
+
 def test_masked_tokens_are_never_drawn():
     """A mask of the lowest value leaves no weight, for any number and temperature."""
     x = torch.full((64, 3000), torch.finfo(torch.float32).min)
