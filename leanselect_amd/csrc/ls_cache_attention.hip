@@ -16,6 +16,16 @@
 // keys are read once for a tile of them rather than once for each.  What the slices of the prefix
 // and of a row's own keys give (O, maximum, sum) is joined by a second kernel.
 //
+// What bounds it (4.9 TB/s is what a large copy reaches here, 1400 TFLOP/s a large bf16 product).  Few rows:
+// the keys' bytes; sixteen sequences of 2K to 64K take 66 us (4.6 TB/s), eight of up to 16K with 8 KV heads
+// 53 us (4.0), and one row with a window of 4096 16 us, which are two launches and one step's latency.  Many
+// rows: the vector units and the matrix units of a wave and its neighbour, which overlap only in part: of a
+// 1024-row chunk behind 32K tokens with capped scores (850 us, 655 TFLOP/s of plain products, 1000 with those
+// of the remainders) the matrix units are busy 35% and the vector ones 52% of the time, of two prompts
+// in fp16 with a bias (202 us) 44% and 69%.  Two groups of waves held half a step apart by barriers, so that
+// one's products meet the other's exponentials, took 898 us; the next step's scores in between this one's
+// weights and the last one's products, 1038 where the plain order took 1027.
+//
 // Extends ls_dense_attn_kvcache (options that infllmv2_attn_with_kvcache takes:
 // third_party/infllmv2/paper1.patch:2511-2615).
 #include <algorithm>
@@ -37,6 +47,7 @@ constexpr int kKeysSub = 32;
 constexpr int kKeysStep = kWaves * kKeysSub;
 constexpr int kSubB = kKeysSub * kRowB;
 constexpr int kKeysCols = 16;
+constexpr int kManyCols = 64;  // up to which tiles of 16 may take more columns
 // Rows form: the waves share the tile's 256 columns, 32 each, and walk the same keys, 64 a step.
 constexpr int kRowsCols = 32 * kWaves;
 constexpr int kRowsStep = 64;
@@ -96,7 +107,8 @@ struct CaArgs {
   CaCut pre;
   CaCut own;
   // Workspace (NULL: every row is one workgroup's): per item [cols][128] sums and [cols] (maximum, sum),
-  // the prefix's items first; per (row, head) the first of its own items and their number.
+  // the prefix's items first; per (row, head) the first of its
+  // sequence's items and the slices of a tile.
   float* part;
   float2* ml;
   int2* rows;
@@ -154,9 +166,12 @@ __device__ __forceinline__ uint2 ca_split(float p0, float p1) {
     return make_uint2(__builtin_amdgcn_perm(b1, b0, 0x07060302u),
                       ca_bf16x2(p0 - __uint_as_float(b0), p1 - __uint_as_float(b1)));
   } else {
-    const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
-    return make_uint2(__builtin_bit_cast(uint32_t, h),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0 - (float)h[0], p1 - (float)h[1])));
+    // (each weight less its half of the pair in one instruction; the pair stands behind the weights)
+    const uint32_t h = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+    float r0, r1;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(h), "v"(p0));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(h), "v"(p1));
+    return make_uint2(h, __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1)));
   }
 }
 
@@ -186,7 +201,8 @@ template <int DT, int NC, int KB, bool FULL, class KRead, class VReady, class VR
 __device__ __forceinline__ void ca_step(uint32_t sk, uint32_t sv, int key0, CaState<NC>& st,
                                         const CaArgs& a, KRead k_read, VReady v_ready, VRead v_read) {
   const int lane = ls_lane(), r = lane & 15, q = lane >> 4;
-  // Left operands are read one block ahead of their products, and no further: registers.
+  // K is read one block ahead of its products, V two: further ahead gained nothing (a 1024-row chunk
+  // behind 32K tokens 850 us either way).
   ls_f32x4 s[KB][NC];
   const uint32_t ka = r * kRowB + 16 * (q ^ r);
   ls_u32x4 kf[2][4];
@@ -291,7 +307,7 @@ __device__ __forceinline__ void ca_step(uint32_t sk, uint32_t sv, int key0, CaSt
     return ls_u32x4{w0.x, w0.y, w1.x, w1.y};
   };
   constexpr uint32_t kOne = DT == LS_BF16 ? 0x3f80u : 0x3c00u;
-  {
+  auto total = [&]() {
     constexpr uint32_t kOnes = kOne | kOne << 16;
     const ls_u32x4 ones = {kOnes, kOnes, kOnes, kOnes};
 #pragma unroll
@@ -301,18 +317,22 @@ __device__ __forceinline__ void ca_step(uint32_t sk, uint32_t sv, int key0, CaSt
         st.l[nc] = LsElem<DT>::mfma(ones, hi[half][nc], st.l[nc]);
         st.l[nc] = LsElem<DT>::mfma(ones, lo[half][nc], st.l[nc]);
       }
-  }
+  };
   if (FULL) {
     constexpr int kBlocks = 4 * KB;  // (half, db)
-    ls_u32x4 vf[2][2];
+    constexpr int kPairs = 3;
+    ls_u32x4 vf[kPairs][2];
     auto pair = [&](int i, ls_u32x4(&f)[2]) {
       f[0] = values(i >> 3, i & 7);
       f[1] = values(i >> 3, (i & 7) + 1);
     };
-    pair(0, vf[0]);
+#pragma unroll
+    for (int i = 0; i + 1 < kPairs; ++i) pair(2 * i, vf[i]);
+    total();
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < kBlocks; i += 2) {
-      if (i + 2 < kBlocks) pair(i + 2, vf[(i / 2 + 1) & 1]);
+      if (i + 2 * (kPairs - 1) < kBlocks) pair(i + 2 * (kPairs - 1), vf[(i / 2 + kPairs - 1) % kPairs]);
       const int half = i >> 3, db = i & 7;
 #pragma unroll
       for (int part = 0; part < 2; ++part)
@@ -320,13 +340,14 @@ __device__ __forceinline__ void ca_step(uint32_t sk, uint32_t sv, int key0, CaSt
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int nc = 0; nc < NC; ++nc)
-            st.o[db + e][nc] = LsElem<DT>::mfma(vf[(i / 2) & 1][e], part ? lo[half][nc] : hi[half][nc], st.o[db + e][nc]);
+            st.o[db + e][nc] = LsElem<DT>::mfma(vf[i / 2 % kPairs][e], part ? lo[half][nc] : hi[half][nc], st.o[db + e][nc]);
       __builtin_amdgcn_sched_barrier(0);
     }
   } else {
     // Where a key is hidden from some column, its weight there is 0 and its values must not count:
     // 0 times an infinity or NaN would.  Such values leave the product.
     uint32_t some = 0;
+    total();
 #pragma unroll
     for (int half = 0; half < KB / 2; ++half)
 #pragma unroll
@@ -382,6 +403,7 @@ __device__ __forceinline__ void ca_step(uint32_t sk, uint32_t sv, int key0, CaSt
 // A workgroup's piece of work: tokens [t0, t1) of group g against a slice of one source's keys.
 struct CaWork {
   int item;  // its place in the workspace
+  int base;  // the first item of the sequence
   int g, t0, t1, slice, slices;
   int seq, n0, n1, len;  // of the own keys; seq < 0: the prefix
   int n_keys, first;     // the source's, and its first key's position
@@ -390,16 +412,28 @@ struct CaWork {
   int64_t rs;
 };
 
-// The item-th workgroup of the prefix.  They go to the eight compute dies in turn: the row tiles of a
-// slice stay on one, whose cache then serves all but the first.
+// Items of `units` slices, each with the same `tiles` of rows, go to the eight compute dies in turn: the tiles of
+// a slice stay on one, whose cache then serves all but the first.
+__device__ __forceinline__ void ca_split_item(int item, int units, int tiles, int& unit, int& tile) {
+  const int block = item / (8 * tiles), in = item % (8 * tiles), some = min(8, units - 8 * block);
+  unit = 8 * block + in % some;
+  tile = in / some;
+}
+__device__ __forceinline__ int ca_join_item(int unit, int tile, int units, int tiles) {
+  const int block = unit / 8;
+  return block * 8 * tiles + tile * min(8, units - 8 * block) + unit % 8;
+}
+
+// The item-th workgroup of the prefix.
 __device__ __forceinline__ bool ca_prefix_work(const CaArgs& a, int item, CaWork& w) {
-  const int units = a.pre.slices * a.G, block = item / (8 * a.pre.tiles), in = item % (8 * a.pre.tiles);
-  const int some = min(8, units - 8 * block), u = 8 * block + in % some;
+  int u, tile;
+  ca_split_item(item, a.pre.slices * a.G, a.pre.tiles, u, tile);
   w.item = item;
+  w.base = 0;
   w.g = u % a.G;
   w.slice = u / a.G;
   w.slices = a.pre.slices;
-  w.t0 = in / some * a.pre.tokens;
+  w.t0 = tile * a.pre.tokens;
   w.t1 = (int)min(min((int64_t)w.t0 + a.pre.tokens, a.total_q), (int64_t)a.cu_q[a.batch]);
   w.seq = -1;
   w.n_keys = a.p_len;
@@ -459,12 +493,14 @@ __device__ __forceinline__ bool ca_own_work(const CaArgs& a, int item, CaWork& w
       w.n1 = __builtin_amdgcn_readlane(hi, at);
       w.len = w.n_keys = __builtin_amdgcn_readlane(len, at);
       w.slices = __builtin_amdgcn_readlane(slices, at);
-      w.slice = item % w.slices;
-      item /= w.slices;
-      w.g = item % a.G;
+      w.base = w.item - a.pre.items - item;
+      const int tiles = __builtin_amdgcn_readlane(n, at);
+      int u, tile;
+      ca_split_item(item, w.slices * a.G, tiles, u, tile);
+      w.g = u % a.G;
+      w.slice = u / a.G;
       // The last tiles, which see the most keys where causal, first.
-      const int tile = __builtin_amdgcn_readlane(n, at) - 1 - item / a.G;
-      w.t0 = w.n0 + tile * a.own.tokens;
+      w.t0 = w.n0 + (tiles - 1 - tile) * a.own.tokens;
       w.t1 = (int)min(min((int64_t)w.t0 + a.own.tokens, a.total_q), (int64_t)w.n1);
       w.first = a.p_len;
       w.k = a.kc + (int64_t)w.seq * a.c_bs + (int64_t)w.g * kDim;
@@ -605,13 +641,14 @@ __device__ __forceinline__ void ca_store(const CaArgs& a, const CaWork& w, const
     if (ch == 0) a.ml[place] = make_float2(M, L);
   }
   if (ch == 0 && a.part && w.seq >= 0 && w.slice == 0)
-    a.rows[row] = alone ? make_int2(0, 0) : make_int2(w.item - a.pre.items, w.slices);
+    a.rows[row] = alone ? make_int2(0, 0) : make_int2(w.base, w.slices);
 }
 
 // ---------------------------------------------------------------------------
 // Keys form, few columns (16).  Each key's bytes are read from LDS once, by one wave, from a place of
 // the wave's own, with no barrier: the next step's K is on its way from when this one's has been
-// read, V likewise.  The waves' sums are joined through LDS at the end.
+// read, V likewise.  The waves' sums are joined through LDS at the end.  128 KB of a unit's keys are on
+// their way at a time: 4.6 TB/s on sixteen ragged sequences.
 // ---------------------------------------------------------------------------
 template <int DT>
 __device__ __forceinline__ void ca_keys_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint32_t lds,
@@ -689,9 +726,12 @@ __device__ __forceinline__ void ca_keys_form(const CaArgs& a, const CaWork& w, c
 }
 
 // ---------------------------------------------------------------------------
-// Rows form, many columns.  A ring of four steps of 64 keys; each wave fetches 8
+// Rows form, many columns: 32 a wave, so that what is read from LDS (two bytes for every 32 multiplications
+// of a key's element) keeps up with the matrix units.  A ring of four steps of 64 keys; each wave fetches 8
 // rows of a step's K and V.  A barrier every two steps tells that the next two have come and the two
-// before have been read.
+// before have been read (every step: 1078 us for the chunk at the time, every two 1027).  The sums, scores and
+// weights of a wave take its registers; nothing may go to scratch memory, whose loads wait for the
+// keys on their way (with it: 2550).
 // ---------------------------------------------------------------------------
 template <int DT>
 __device__ __forceinline__ void ca_rows_form(const CaArgs& a, const CaWork& w, const CaCut& cut, uint32_t lds,
@@ -789,7 +829,7 @@ __global__ __launch_bounds__(kThreads) void ls_cache_attn_kernel(const CaArgs a)
 
 // out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over a row's slices, the prefix's and its own.  SHARE
 // half waves per (row, head), each every SHARE-th slice, four channels a lane: 8 where a row has many slices, so
-// that 32 of them are on their way at once, 1 where it has few (a workgroup a row costs 0.6 ns each).
+// that 32 of them are on their way at once, 1 where it has few.
 template <int DT, int SHARE>
 __global__ __launch_bounds__(256) void ls_cache_attn_join_kernel(const CaArgs a) {
   const int tid = threadIdx.x;
@@ -800,17 +840,18 @@ __global__ __launch_bounds__(256) void ls_cache_attn_join_kernel(const CaArgs a)
   if (t >= a.cu_q[a.batch]) return;
   int2 own = a.rows[row];
   if (own.y <= 0) return;               // written already
+  const int before = a.pre.items ? a.pre.slices : 0;
   own.y = min(own.y, a.own.items);      // (in bounds whatever cu_seqlens_q holds)
-  own.x = min(max(own.x, 0), a.own.items - own.y);
-  const int before = a.pre.items ? a.pre.slices : 0, slots = before + own.y;
-  const int b = ls_find_segment(a.cu_q, a.batch, t);
-  const int own_col = max(0, t - a.cu_q[b]) % a.own.tokens * a.gs + h;
+  const int slots = before + own.y;
+  const int b = ls_find_segment(a.cu_q, a.batch, t), n0 = a.cu_q[b];
+  const int tiles = max(1, (a.cu_q[b + 1] - n0 + a.own.tokens - 1) / a.own.tokens);
+  const int i = max(0, t - n0), own_tile = max(0, tiles - 1 - i / a.own.tokens), own_col = i % a.own.tokens * a.gs + h;
   auto place = [&](int s) -> int64_t {
-    if (s >= before)
-      return (int64_t)a.pre.items * a.pre.cols + (int64_t)(own.x + s - before) * a.own.cols + own_col;
-    const int u = s * a.G + g, block = u / 8, some = min(8, a.pre.slices * a.G - 8 * block);
-    return ((int64_t)block * 8 * a.pre.tiles + t / a.pre.tokens * some + u % 8) * a.pre.cols +
-           t % a.pre.tokens * a.gs + h;
+    if (s < before)
+      return (int64_t)ca_join_item(s * a.G + g, t / a.pre.tokens, a.pre.slices * a.G, a.pre.tiles) * a.pre.cols +
+             t % a.pre.tokens * a.gs + h;
+    const int at = own.x + ca_join_item((s - before) * a.G + g, own_tile, own.y * a.G, tiles);
+    return (int64_t)a.pre.items * a.pre.cols + (int64_t)min(max(at, 0), a.own.items - 1) * a.own.cols + own_col;
   };
   // The maximum of all, a slice a thread.
   const int ch = tid & 31, at = SHARE == 8 ? tid >> 5 : 0;
@@ -884,12 +925,40 @@ CaPlan ca_plan(int64_t total_q, int batch, int H, int G, int64_t p_len, int64_t 
     return c.cols == kKeysCols ? kKeysStep : kRowsStep;
   };
   auto count = [](int64_t n, int64_t of) { return (n + of - 1) / of; };
-  const int own_step = shape(p.own, rows * gs);
-  const double own_us = p.own.cols == kKeysCols ? kKeysUs : kRowsUs;
-  p.own.tiles = (int)std::min<int64_t>(total_q, (total_q + (int64_t)batch * (p.own.tokens - 1)) / p.own.tokens);
-  const int64_t tiles = (int64_t)p.own.tiles * G;
-  const int64_t seen = left >= 0 ? std::min<int64_t>(max_len, (int64_t)left + p.own.tokens) : max_len;
-  const int64_t steps = std::max<int64_t>(1, count(seen, own_step));
+  // The own keys' tiles, G groups of them, and the most steps that one has to take.
+  struct Own {
+    int step;
+    double us;
+    int64_t tiles, steps;
+  };
+  auto cut_own = [&](int64_t cols) {
+    Own o;
+    o.step = shape(p.own, cols);
+    o.us = p.own.cols == kKeysCols ? kKeysUs : kRowsUs;
+    p.own.tiles = (int)std::min<int64_t>(total_q, (total_q + (int64_t)batch * (p.own.tokens - 1)) / p.own.tokens);
+    o.tiles = (int64_t)p.own.tiles * G;
+    const int64_t seen = left >= 0 ? std::min<int64_t>(max_len, (int64_t)left + p.own.tokens) : max_len;
+    o.steps = std::max<int64_t>(1, count(seen, o.step));
+    return o;
+  };
+  auto balanced = [&](const Own& o) {
+    return std::min<int64_t>(o.tiles * o.steps, std::max<int64_t>(kUnits, o.tiles + kUnits / 2));
+  };
+  Own own = cut_own(rows * gs);
+  if (rows * gs > kKeysCols && rows * gs <= kManyCols) {
+    // Two to four tiles of 16 columns, or one of 256 that is mostly empty.  With all units at it a step of the
+    // first takes what its keys take to arrive: 3.5 us where a die's cache serves a slice's other tiles, else
+    // 5.4; the second needs no more of them, but fewer units have work and its prologue and join take 20 us.
+    // 8 and 24 sequences of 32K, 32 heads to 2, in us, the first against the second: 2 rows 49 / 88 and 202 /
+    // 263, 3 rows 52 / 98 and 288 / 238, 4 rows 81 / 99 and 375 / 236; one sequence 21 / 33.
+    const Own many = own;
+    own = cut_own(kKeysCols);
+    const double c = balanced(own) * G >= 8 * own.tiles ? 3.5 : 5.4;
+    if ((double)(own.tiles * own.steps) / kUnits * c + kItemUs > (double)(many.tiles * many.steps) / kUnits * kRowsUs + 20.0)
+      own = cut_own(rows * gs);
+  }
+  const double own_us = own.us;
+  const int64_t tiles = own.tiles, steps = own.steps;
   if (p_len > 0) {
     const int step = shape(p.pre, total_q * gs);
     p.pre.tiles = (int)count(total_q, p.pre.tokens);
@@ -900,7 +969,8 @@ CaPlan ca_plan(int64_t total_q, int batch, int H, int G, int64_t p_len, int64_t 
     const int64_t slices = n_splits > 0 ? n_splits : std::max<int64_t>(1, (int64_t)(2 * steps * own_us / each));
     p.own.slices = (int)std::min<int64_t>({slices, std::max<int64_t>(steps, n_splits), kMaxSplits});
     const double busy = tiles * (steps * own_us + p.own.slices * kItemUs) / each;
-    const int64_t spare = std::max<int64_t>(1, kUnits - (int64_t)busy - 1);
+    // (the same number of units on each of the eight dies, to which items go in turn)
+    const int64_t spare = std::max<int64_t>(1, kUnits - 8 * ((int64_t)(busy / 8) + 1));
     p.pre.slices = (int)std::max<int64_t>(
         1, std::min<int64_t>({n_splits > 0 ? n_splits : spare / pre_tiles, pre_steps, kMaxSplits}));
     p.pre.items = p.pre.tiles * p.pre.slices * G;
@@ -910,7 +980,7 @@ CaPlan ca_plan(int64_t total_q, int batch, int H, int G, int64_t p_len, int64_t 
     p.own.items = (int)std::min<int64_t>(tiles * n_splits, 0x7fffffff);
   } else if (p.own.cols == kKeysCols) {
     p.own.slices = 0;
-    p.own.items = (int)std::min<int64_t>(tiles * steps, std::max<int64_t>(kUnits, tiles + kUnits / 2));
+    p.own.items = (int)balanced(own);
   } else {
     // Rounds of a workgroup a unit: the number of slices that makes them shortest (more than one
     // are also written, and joined).
