@@ -121,6 +121,24 @@ def test_chunks(dtype, new, lens, H, G, window):
     _run(lens, new, H, G, dtype, seed=sum(new), causal=True, softcap=15.0, window=window)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("H,G,most", [(32, 2, 4), (32, 8, 16), (16, 1, 3), (10, 2, 12)])
+@pytest.mark.parametrize("prefix", [0, 700])
+@pytest.mark.parametrize("n_splits", [None, 3])
+@pytest.mark.parametrize("options", [dict(causal=True), dict(causal=True, window=(300, -1), softcap=20.0)],
+                         ids=["causal", "capped window"])
+def test_a_few_rows_a_sequence(dtype, H, G, most, prefix, n_splits, options):
+    """Guessed tokens: each sequence's rows in several narrow tiles or in one wide one."""
+    new = [most, 1, 0, most, most - 1, most]
+    lens = [1500, 700, 90, most, 257, 2049]
+    _run(lens, new, H, G, dtype, prefix=prefix, n_splits=n_splits, **options)
+
+
+@pytest.mark.parametrize("batch,length", [(24, 2000), (24, 900), (3, 2000), (70, 300)])
+def test_a_few_rows_of_many_sequences(batch, length):
+    _run([length - 37 * b % length for b in range(batch)], [4] * batch, 32, 2, BF16, causal=False)
+
+
 @pytest.mark.parametrize("prefix", [0, 40])
 def test_rows_that_see_nothing(prefix):
     """More rows than keys: with causal, the first rows stand in front of every own key (with a prefix
