@@ -98,7 +98,7 @@ struct CaArgs {
   // (cap tanh(x / cap) = cap - 2 cap / (1 + exp(2 x / cap))); with slopes the score itself, less its bias.
   float alpha;
   float beta;
-  float cap_b;  // 0: no cap
+  float cap_b;  // 0: no cap.  z is off by 2^-23, so the score by cap 2^-22: 2^-13 at the largest cap taken
   const float* slopes;
   int64_t slopes_bs;
   int causal;
@@ -837,7 +837,7 @@ __global__ __launch_bounds__(256) void ls_cache_attn_join_kernel(const CaArgs a)
   const int64_t row = SHARE == 8 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 8 + (tid >> 5);
   if (row >= a.total_q * H) return;
   const int t = (int)(row / H), head = (int)(row % H), g = head / a.gs, h = head % a.gs;
-  if (t >= a.cu_q[a.batch]) return;
+  if (t < a.cu_q[0] || t >= a.cu_q[a.batch]) return;
   int2 own = a.rows[row];
   if (own.y <= 0) return;               // written already
   const int before = a.pre.items ? a.pre.slices : 0;
@@ -906,6 +906,9 @@ __global__ __launch_bounds__(256) void ls_cache_attn_join_kernel(const CaArgs a)
 // ---------------------------------------------------------------------------
 constexpr int kUnits = 256;  // compute units
 constexpr int kMaxSplits = 128;
+// Above the largest cap the score's error would be more than the output's rounding in fp16; a form that is exact there
+// (the series of tanh near 0) in the same loop took 6% of the chunk's time from every other cap.
+constexpr float kMinCap = 1e-20f, kMaxCap = 512.f;
 
 struct CaPlan {
   CaCut pre, own;
@@ -1045,6 +1048,8 @@ extern "C" int ls_cache_attn(const void* q, int64_t q_row_stride, const int32_t*
   LS_REQUIRE(dtype == LS_BF16 || dtype == LS_F16, LS_ERR_UNSUPPORTED, "%s: bf16 or fp16", who);
   LS_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY && softcap >= 0.f && softcap < INFINITY,
              LS_ERR_INVALID, "%s: softmax_scale must be positive and softcap not negative", who);
+  LS_REQUIRE(softcap == 0.f || (softcap >= kMinCap && softcap <= kMaxCap), LS_ERR_UNSUPPORTED,
+             "%s: softcap must be 0 or from %g to %g", who, kMinCap, kMaxCap);
   LS_REQUIRE(n_splits >= 0 && n_splits <= kMaxSplits, LS_ERR_INVALID, "%s: 0 <= n_splits <= %d", who,
              kMaxSplits);
   LS_REQUIRE(prefix_len + capacity < (1 << 30) && total_q < (1 << 30), LS_ERR_UNSUPPORTED,

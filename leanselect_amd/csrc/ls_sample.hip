@@ -656,7 +656,7 @@ extern "C" int ls_sample_logits(const void* logits, int64_t row_stride, int64_t 
              "%s: at most 2^19 tokens, fewer than 2^22 rows", who);
   LS_REQUIRE(dtype == LS_F32 || dtype == LS_BF16 || dtype == LS_F16, LS_ERR_UNSUPPORTED,
              "%s: float32, bf16 or fp16", who);
-  LS_REQUIRE(temperature >= 0.0 && temperature < 1e30 && top_p > 0.0 && min_p >= 0.0 && min_p <= 1.0, LS_ERR_INVALID,
+  LS_REQUIRE(temperature >= 0.0 && temperature < INFINITY && top_p > 0.0 && min_p >= 0.0 && min_p <= 1.0, LS_ERR_INVALID,
              "%s: temperature >= 0, top_p > 0 and 0 <= min_p <= 1", who);
   if (rows == 0) return LS_OK;
   LS_REQUIRE(logits && u && tokens, LS_ERR_INVALID, "%s: null pointer", who);

@@ -17,6 +17,7 @@ from __future__ import annotations
 import torch
 
 from .ops.attention import infllmv2_attn_varlen_func
+from .ops.cache_attention import check_scores
 from .ops.decode import (dense_attention_kvcache, kvcache_append, sparse_attention_kvcache,
                          stage1_scores)
 from .ops.nosa import max_pooling_1d_varlen
@@ -99,6 +100,8 @@ def infllmv2_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=N
         raise ValueError("q must be [B, Sq, H, D] and k_cache / v_cache [B, capacity, G, D]")
     B, Sq, H, D = q.shape
     G = k_cache.shape[2]
+    if scored:  # before anything is appended
+        check_scores(softmax_scale, softcap, alibi_slopes, B, H)
     dev = q.device
     if cache_seqlens is None:
         cache_seqlens = 0

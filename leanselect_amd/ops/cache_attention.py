@@ -9,7 +9,8 @@ shares a prefix, on the GPU.
 A sequence with ``n`` query rows and ``len`` keys, the prefix's ``P`` included, has its row ``i`` at position
 ``p = len - n + i``.  Key ``j < len`` is visible where, with ``causal``, ``j <= p`` and, with ``window = (left,
 right)``, ``p - left <= j <= p + right`` (a negative side is open).  A score is ``x = scale * q.k``, then
-``softcap * tanh(x / softcap)`` (0: not capped), then less ``alibi_slopes[h] * |p - j|``: the options of
+``softcap * tanh(x / softcap)`` (0: not capped; at most 512, up to where the cap's float32 form is within
+2^-13), then less ``alibi_slopes[h] * |p - j|``: the options of
 ``infllmv2_attn_with_kvcache`` (third_party/infllmv2/paper1.patch:2511-2615).  The reference has no
 call for a shared prefix.
 """
@@ -57,6 +58,19 @@ def scored_attention(q, k_cache, v_cache, cache_seqlens, cu_seqlens_q, max_len, 
     """``shared_prefix_attention`` without a prefix."""
     return _attend(q, None, None, k_cache, v_cache, cache_seqlens, cu_seqlens_q, max_len, causal,
                    softmax_scale, softcap, alibi_slopes, window, n_splits, return_lse, out)
+
+
+def check_scores(softmax_scale, softcap, alibi_slopes, batch: int, num_heads: int) -> tuple[float, float]:
+    """The scale and the cap as numbers, or ``ValueError`` for options that no call takes."""
+    scale, softcap = _SCALE if softmax_scale is None else float(softmax_scale), float(softcap)
+    if not 0.0 < scale < math.inf or not 0.0 <= softcap < math.inf:
+        raise ValueError("softmax_scale must be positive and softcap not negative, both finite")
+    if softcap and not 1e-20 <= softcap <= 512.0:
+        raise ValueError(f"softcap must be 0 or from 1e-20 to 512 (got {softcap})")
+    if alibi_slopes is not None and (alibi_slopes.dtype is not torch.float32
+                                     or alibi_slopes.shape not in ((num_heads,), (batch, num_heads))):
+        raise ValueError(f"alibi_slopes must be float32 [{num_heads}] or [{batch}, {num_heads}]")
+    return scale, softcap
 
 
 @lru_cache(maxsize=4096)
@@ -111,15 +125,10 @@ def _attend(q, k_prefix, v_prefix, k_cache, v_cache, cache_seqlens, cu_seqlens_q
             raise ValueError(f"the prefix must be [prefix_len, {G}, {HEAD_DIM}] in q's dtype")
         if P:
             p_row, = _key_strides(k_prefix, v_prefix, "the prefix's")
-    scale = _SCALE if softmax_scale is None else float(softmax_scale)
-    softcap = float(softcap)
-    if not 0.0 < scale < math.inf or not 0.0 <= softcap < math.inf:
-        raise ValueError("softmax_scale must be positive and softcap not negative, both finite")
+    scale, softcap = check_scores(softmax_scale, softcap, alibi_slopes, B, H)
     left, right = (min(max(int(x), -1), 1 << 30) for x in window)
     slopes_stride = 0
     if alibi_slopes is not None:
-        if alibi_slopes.dtype is not torch.float32 or alibi_slopes.shape not in ((H,), (B, H)):
-            raise ValueError(f"alibi_slopes must be float32 [{H}] or [{B}, {H}]")
         alibi_slopes = alibi_slopes.contiguous()
         slopes_stride = H if alibi_slopes.ndim == 2 else 0
     given = out is not None

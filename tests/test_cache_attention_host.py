@@ -64,6 +64,8 @@ def test_well_formed_cpu_arguments_reach_the_device_check():
     (dict(softcap=-1.0), "softcap"),
     (dict(softcap=math.nan), "softcap"),
     (dict(softcap=math.inf), "softcap"),
+    (dict(softcap=1e-30), "softcap"),
+    (dict(softcap=513.0), "softcap"),
     (dict(softmax_scale=0.0), "softmax_scale"),
     (dict(softmax_scale=-0.1), "softmax_scale"),
     (dict(alibi_slopes=torch.zeros(8, dtype=BF16)), "alibi_slopes"),
@@ -103,6 +105,8 @@ def _entry(**kw):
     (dict(dtype=_hip.LS_F32), _hip.LS_ERR_UNSUPPORTED, "bf16 or fp16"),
     (dict(scale=0.0), _hip.LS_ERR_INVALID, "softmax_scale"),
     (dict(cap=-1.0), _hip.LS_ERR_INVALID, "softcap"),
+    (dict(cap=1e-30), _hip.LS_ERR_UNSUPPORTED, "softcap"),
+    (dict(cap=513.0), _hip.LS_ERR_UNSUPPORTED, "softcap"),
     (dict(splits=129), _hip.LS_ERR_INVALID, "n_splits"),
     (dict(capacity=1 << 30), _hip.LS_ERR_UNSUPPORTED, "2\\^30"),
     (dict(c_rs=1 << 24), _hip.LS_ERR_UNSUPPORTED, "2\\^24"),
@@ -125,3 +129,13 @@ def test_no_rows_launch_nothing():
     assert lib.ls_cache_attn_workspace_size(0, 1, 8, 2, 0, 8, -1, 0) == 0
     assert lib.ls_cache_attn_workspace_size(1, 1, 8, 2, 0, 100, -1, 1) == 0
     assert lib.ls_cache_attn_workspace_size(1, 1, 8, 2, 0, 100, -1, 4) >= 4 * 8 * 4 * 130
+
+
+def test_refused_options_leave_the_cache():
+    """A call with new keys that is refused for its options has not appended them."""
+    q, kv, new = torch.zeros(1, 1, 8, 128, dtype=BF16), _kv(1, 64), _kv(1, 1)
+    kept = kv.clone()
+    for more in (dict(softcap=-1.0), dict(alibi_slopes=torch.zeros(3)), dict(window_size=(3, 0), softmax_scale=-1.0)):
+        with pytest.raises(ValueError):
+            infllmv2_attn_with_kvcache(q, kv, kv, new, new, cache_seqlens=3, **more)
+    assert torch.equal(kv, kept)

@@ -278,6 +278,25 @@ def test_large_magnitudes():
     _run([700], [2], 4, 2, FP16, seed=12, strong=60.0, window=(600, -1))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("softcap", [1e-20, 0.01, 512.0])
+def test_the_least_and_largest_caps(dtype, rows, softcap):
+    _run([400, 90], [rows, 3], 32, 2, dtype, causal=True, softcap=softcap)
+
+
+def test_rows_in_front_of_the_first_sequence():
+    """They belong to none, and are left as they are where the output is given."""
+    q, k, v, kp, vp = _inputs([300], [6], 32, 2, BF16, 3, prefix=900)
+    out = torch.full((6, 32, D), 7.0, dtype=BF16, device=DEV)
+    shared_prefix_attention(q.to(DEV), kp.to(DEV), vp.to(DEV), k.to(DEV), v.to(DEV), _i32([300]), _i32([2, 5]), 300, out=out)
+    want = so.cache_attention(q[2:5], k, v, [300], [0, 3], k_prefix=kp, v_prefix=vp)
+    assert bool((out[:2] == 7).all()) and bool((out[5:] == 7).all())
+    exact, _, bound, _ = want
+    allowed = torch.finfo(BF16).eps / 2 * (exact.abs() + bound) + bound
+    assert bool(((out[2:5].cpu().double() - exact).abs() <= allowed).all())
+
+
 @pytest.mark.parametrize("options", [dict(softcap=20.0), dict(window_size=(40, 0)), dict(window_size=(30, -1), causal=True),
                                      dict(alibi_slopes=_slopes(8, 2), causal=True)], ids=str)
 def test_with_kvcache_options(options):
