@@ -108,10 +108,10 @@ struct CaArgs {
   CaCut own;
   // Workspace (NULL: every row is one workgroup's): per item [cols][128] sums and [cols] (maximum, sum),
   // the prefix's items first; per (row, head) the first of its
-  // sequence's items and the slices of a tile.
+  // sequence's items, a tile's slices times 256 plus the row's column, its tile and the sequence's tiles.
   float* part;
   float2* ml;
-  int2* rows;
+  int4* rows;
   uint16_t* out;
   float* lse;
 };
@@ -403,7 +403,8 @@ __device__ __forceinline__ void ca_step(uint32_t sk, uint32_t sv, int key0, CaSt
 // A workgroup's piece of work: tokens [t0, t1) of group g against a slice of one source's keys.
 struct CaWork {
   int item;  // its place in the workspace
-  int base;  // the first item of the sequence
+  int base;  // the first item of the sequence, its tiles and this one's place among them
+  int tiles, tile;
   int g, t0, t1, slice, slices;
   int seq, n0, n1, len;  // of the own keys; seq < 0: the prefix
   int n_keys, first;     // the source's, and its first key's position
@@ -494,13 +495,13 @@ __device__ __forceinline__ bool ca_own_work(const CaArgs& a, int item, CaWork& w
       w.len = w.n_keys = __builtin_amdgcn_readlane(len, at);
       w.slices = __builtin_amdgcn_readlane(slices, at);
       w.base = w.item - a.pre.items - item;
-      const int tiles = __builtin_amdgcn_readlane(n, at);
-      int u, tile;
-      ca_split_item(item, w.slices * a.G, tiles, u, tile);
+      w.tiles = __builtin_amdgcn_readlane(n, at);
+      int u;
+      ca_split_item(item, w.slices * a.G, w.tiles, u, w.tile);
       w.g = u % a.G;
       w.slice = u / a.G;
       // The last tiles, which see the most keys where causal, first.
-      w.t0 = w.n0 + (tiles - 1 - tile) * a.own.tokens;
+      w.t0 = w.n0 + (w.tiles - 1 - w.tile) * a.own.tokens;
       w.t1 = (int)min(min((int64_t)w.t0 + a.own.tokens, a.total_q), (int64_t)w.n1);
       w.first = a.p_len;
       w.k = a.kc + (int64_t)w.seq * a.c_bs + (int64_t)w.g * kDim;
@@ -641,7 +642,7 @@ __device__ __forceinline__ void ca_store(const CaArgs& a, const CaWork& w, const
     if (ch == 0) a.ml[place] = make_float2(M, L);
   }
   if (ch == 0 && a.part && w.seq >= 0 && w.slice == 0)
-    a.rows[row] = alone ? make_int2(0, 0) : make_int2(w.base, w.slices);
+    a.rows[row] = alone ? make_int4(0, 0, 0, 1) : make_int4(w.base, w.slices << 8 | c, w.tile, w.tiles);
 }
 
 // ---------------------------------------------------------------------------
@@ -838,19 +839,17 @@ __global__ __launch_bounds__(256) void ls_cache_attn_join_kernel(const CaArgs a)
   if (row >= a.total_q * H) return;
   const int t = (int)(row / H), head = (int)(row % H), g = head / a.gs, h = head % a.gs;
   if (t < a.cu_q[0] || t >= a.cu_q[a.batch]) return;
-  int2 own = a.rows[row];
+  const int4 own = a.rows[row];
   if (own.y <= 0) return;               // written already
   const int before = a.pre.items ? a.pre.slices : 0;
-  own.y = min(own.y, a.own.items);      // (in bounds whatever cu_seqlens_q holds)
-  const int slots = before + own.y;
-  const int b = ls_find_segment(a.cu_q, a.batch, t), n0 = a.cu_q[b];
-  const int tiles = max(1, (a.cu_q[b + 1] - n0 + a.own.tokens - 1) / a.own.tokens);
-  const int i = max(0, t - n0), own_tile = max(0, tiles - 1 - i / a.own.tokens), own_col = i % a.own.tokens * a.gs + h;
+  // (in bounds whatever cu_seqlens_q holds)
+  const int own_slices = min(own.y >> 8, a.own.items), own_col = min(own.y & 255, a.own.cols - 1);
+  const int slots = before + own_slices, tiles = max(1, own.w);
   auto place = [&](int s) -> int64_t {
     if (s < before)
       return (int64_t)ca_join_item(s * a.G + g, t / a.pre.tokens, a.pre.slices * a.G, a.pre.tiles) * a.pre.cols +
              t % a.pre.tokens * a.gs + h;
-    const int at = own.x + ca_join_item((s - before) * a.G + g, own_tile, own.y * a.G, tiles);
+    const int at = own.x + ca_join_item((s - before) * a.G + g, own.z, own_slices * a.G, tiles);
     return (int64_t)a.pre.items * a.pre.cols + (int64_t)min(max(at, 0), a.own.items - 1) * a.own.cols + own_col;
   };
   // The maximum of all, a slice a thread.
@@ -1000,7 +999,7 @@ CaPlan ca_plan(int64_t total_q, int batch, int H, int G, int64_t p_len, int64_t 
     const size_t places = (size_t)p.pre.items * p.pre.cols + (size_t)p.own.items * p.own.cols;
     p.part = ls_align256(4 * places * kDim);
     p.ml = ls_align256(8 * places);
-    p.total = p.part + p.ml + 8 * (size_t)total_q * H;
+    p.total = p.part + p.ml + 16 * (size_t)total_q * H;
   }
   return p;
 }
@@ -1103,7 +1102,7 @@ extern "C" int ls_cache_attn(const void* q, int64_t q_row_stride, const int32_t*
   if (p.total) {
     a.part = (float*)workspace;
     a.ml = (float2*)((uint8_t*)workspace + p.part);
-    a.rows = (int2*)((uint8_t*)workspace + p.part + p.ml);
+    a.rows = (int4*)((uint8_t*)workspace + p.part + p.ml);
   }
   a.out = (uint16_t*)out;
   a.lse = softmax_lse;

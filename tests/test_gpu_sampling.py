@@ -133,7 +133,7 @@ def test_infinities_and_nan(dtype, settings):
 
 
 @pytest.mark.parametrize("settings", [
-    dict(temperature=1e-30), dict(temperature=1e-6), dict(temperature=1e20), dict(temperature=0.05), dict(top_p=0.5),
+    dict(temperature=1e-30), dict(temperature=1e-6), dict(temperature=1e20), dict(temperature=1e35), dict(temperature=0.05), dict(top_p=0.5),
     dict(top_p=1.0 - 2.0 ** -24)], ids=str)
 @pytest.mark.parametrize("scale,shift", [(1.0, 0.0), (1e-30, 0.0), (1e3, 0.0), (1.0, 1e6), (0.0, -3e38), (1e37, 0.0)])
 def test_top_p_at_odd_scales(settings, scale, shift):
