@@ -59,7 +59,7 @@ def sample_logits(logits: torch.Tensor, u: torch.Tensor, *, temperature: float |
     t, k, p, m = numbers
     if t is not None and not 0.0 <= t < math.inf:
         raise ValueError(f"temperature must be 0 or more and finite (got {t})")
-    if k is not None and k != int(k):
+    if k is not None and (not math.isfinite(k) or k != int(k)):
         raise ValueError(f"top_k must be a whole number (got {k})")
     if p is not None and not p > 0.0:
         raise ValueError(f"top_p must be above 0 (got {p})")

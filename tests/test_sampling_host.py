@@ -29,6 +29,8 @@ def test_well_formed_cpu_arguments_reach_the_device_check():
     (dict(temperature=-0.1), "temperature"),
     (dict(temperature=math.nan), "temperature"),
     (dict(temperature=math.inf), "temperature"),
+    (dict(top_k=math.inf), "top_k"),
+    (dict(top_k=math.nan), "top_k"),
     (dict(temperature=torch.ones(2)), "temperature"),
     (dict(temperature=torch.ones(3, dtype=torch.bfloat16)), "temperature"),
     (dict(top_k=1.5), "top_k"),
