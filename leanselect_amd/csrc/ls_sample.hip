@@ -69,6 +69,11 @@ __device__ __forceinline__ uint32_t sa_key(float x) { return ls_order_key32(__fl
 __device__ __forceinline__ float sa_value(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
+// The next smaller logit (-inf: itself).  Below 0 stands the largest negative one: the key between them is -0's.
+__device__ __forceinline__ float sa_below(float x) {
+  const uint32_t key = sa_key(x);
+  return x > -INFINITY ? sa_value(key - (key == 0x80000000u ? 2 : 1)) : x;
+}
 
 __device__ __forceinline__ uint64_t sa_lane64(uint64_t x, int lane) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane) |
@@ -514,7 +519,7 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
     // exp((x - max) / t) >= min_p  <=>  x >= max + t ln min_p; the next logit below passes not.
     const double border = (double)rule.top + log(min_p) * t;
     const float f = fminf((float)border, rule.top);
-    if (f > -INFINITY) rule.min_cut = (double)f < border && f < rule.top ? f : sa_value(sa_key(f) - 1);
+    if (f > -INFINITY) rule.min_cut = (double)f < border && f < rule.top ? f : sa_below(f);
   }
   const double u = (double)a.u[r];
   // What is kept, or has to be summed up, is among the logits above `low`.
@@ -541,7 +546,7 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
       uint64_t before;
       const uint32_t bin = kBins - 1 - sa_find(s, rule.k, before);
       // (two bins more: theirs are rounded products)
-      low = fmaxf(sa_value(sa_key(least) - 1), rule.top - (bin + 2) / to_bins);
+      low = fmaxf(sa_below(least), rule.top - (bin + 2) / to_bins);
     }
   } else if (rule.k == 0 && rule.p < 1.0) {
     // Bins of 1/64 of a temperature: beyond the last no logit has any weight.
@@ -557,7 +562,7 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
     border = kBins - 1 - (int)sa_find(s, need, front);
     // (two bins and a step more: theirs are rounded products; the last is open)
     const float f = border < kBins - 1 ? rule.top - (border + 2) / to_bins : -INFINITY;
-    low = f > -INFINITY ? sa_value(sa_key(f) - 1) : f;
+    low = sa_below(f);
     bounded = true;
   }
   // (What top_p sums up is more than what min_p leaves.)
@@ -565,7 +570,7 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
     low = fmaxf(low, rule.min_cut);
     bounded = bounded || rule.min_cut > -INFINITY;
   }
-  low = fminf(low, sa_value(sa_key(rule.top) - 1));  // (the largest are kept whatever the settings hold)
+  low = fminf(low, sa_below(rule.top));  // (the largest are kept whatever the settings hold)
   // Logits into LDS, a wave's in one go.
   auto gather = [&](auto take) {
     __syncthreads();

@@ -1,0 +1,42 @@
+"""The bounds under which sampling looks for what is kept, where they fall on zero, on logits that lie
+close together or on the smallest numbers: the same tokens as the definition's (oracle/serving_oracle.py)."""
+import math
+
+import pytest
+import torch
+
+from leanselect_amd.ops import sample_logits
+from oracle import serving_oracle as so
+from test_gpu_sampling import DEV, DTYPES, _check
+
+pytestmark = pytest.mark.gpu
+
+_U = torch.tensor([0.0, 0.1, 0.37, 0.52, 0.7, 0.83, 0.96, 1.0 - 2.0 ** -24])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [5000, 73448])
+@pytest.mark.parametrize("settings", [dict(top_k=50), dict(top_k=1500), dict(top_k=50, top_p=0.9), dict(top_k=50, min_p=0.01),
+                                      dict(top_k=1500, top_p=0.99, temperature=2.0)], ids=str)
+def test_a_few_logits_above_zeros(dtype, vocab, settings):
+    """The border falls among logits of 0 and -0, with none below and with some."""
+    x = torch.zeros(8, vocab, dtype=dtype)
+    x[:, ::7] = -0.0
+    x[:, [10, 300, 4000]] = torch.tensor([1.0, 3.0, 2.0], dtype=dtype)
+    x[4:, 1::2] = -1.0
+    assert _check(x, _U, **settings) >= 7
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [1, 100, 5000, 73448])
+@pytest.mark.parametrize("more", [dict(), dict(top_k=50), dict(top_k=50, top_p=0.9), dict(top_p=0.9), dict(temperature=0.3)], ids=str)
+def test_a_largest_logit_of_zero_alone(dtype, vocab, more):
+    """min_p of 1 keeps the largest logits, also where they are 0 and -0."""
+    g = torch.Generator().manual_seed(vocab)
+    x = (-0.5 - torch.rand(8, vocab, generator=g)).to(dtype)
+    x[:, vocab // 2] = 0.0
+    x[4:, vocab // 3] = -0.0
+    assert _check(x, _U, min_p=1.0, **more) >= 7
+    assert _check(x, _U, min_p=torch.ones(8), **more) >= 7
+    above = sample_logits(x.to(DEV), _U.to(DEV), min_p=torch.full((8,), 1.5, device=DEV), **more).cpu()
+    assert torch.equal(above, sample_logits(x.to(DEV), _U.to(DEV), min_p=1.0, **more).cpu())
