@@ -545,8 +545,8 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
         if (best[m] >= least) atomicAdd(&s.bins[kBins - 1 - bin_of(best[m])], 1ull);
       uint64_t before;
       const uint32_t bin = kBins - 1 - sa_find(s, rule.k, before);
-      // (two bins more: theirs are rounded products)
-      low = fmaxf(sa_below(least), rule.top - (bin + 2) / to_bins);
+      // (two bins and a step more: theirs are rounded products, and the difference may be rounded up to a logit)
+      low = fmaxf(sa_below(least), sa_below(rule.top - (bin + 2) / to_bins));
     }
   } else if (rule.k == 0 && rule.p < 1.0) {
     // Bins of 1/64 of a temperature: beyond the last no logit has any weight.

@@ -40,3 +40,22 @@ def test_a_largest_logit_of_zero_alone(dtype, vocab, more):
     assert _check(x, _U, min_p=torch.ones(8), **more) >= 7
     above = sample_logits(x.to(DEV), _U.to(DEV), min_p=torch.full((8,), 1.5, device=DEV), **more).cpu()
     assert torch.equal(above, sample_logits(x.to(DEV), _U.to(DEV), min_p=1.0, **more).cpu())
+
+
+@pytest.mark.parametrize("offset,eps", [(100.0, 1e-3), (1e6, 1.0), (20.0, 1e-4), (1000.0, 1e-2), (20.0, 1e-3), (-1e6, 1.0), (3e30, 1e24)])
+@pytest.mark.parametrize("settings", [dict(top_k=1), dict(top_k=50), dict(top_k=200, top_p=0.8), dict(top_k=1500),
+                                      dict(top_k=50, min_p=0.9)], ids=str)
+def test_logits_within_a_few_steps_of_each_other(offset, eps, settings):
+    g = torch.Generator().manual_seed(3)
+    x = offset + eps * torch.randn(8, 73448, generator=g)
+    temperature = max(1.0, eps)
+    assert _check(x, _U, temperature=temperature, **settings) >= 7
+
+
+@pytest.mark.parametrize("settings", [dict(top_k=2), dict(top_k=50), dict(top_k=1500, top_p=0.5)], ids=str)
+@pytest.mark.parametrize("value", [1.0, -1.0, 20.0])
+def test_two_neighbouring_values(value, settings):
+    """One logit a step above all others, which are equal."""
+    x = torch.full((8, 9000), value)
+    x[:, 4321] = torch.nextafter(x[0, 0], torch.tensor(math.inf))
+    assert _check(x, _U, **settings) >= 7
