@@ -537,8 +537,10 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
     const float least = sa_value(~sa_max(~sa_key(rule.k <= kThreads ? best[0] : best[1]), s));
     const float range = rule.top - least;
     bounded = true;
-    if (least > -INFINITY && range > 0.f && range < INFINITY) {
-      to_bins = (kBins - 2) / range;
+    low = sa_below(least);
+    to_bins = (kBins - 2) / range;
+    // (else one value, infinities, or a range so small that its bins' width is none: the least alone is the bound)
+    if (range < INFINITY && to_bins < INFINITY) {
       sa_clear(s);
 #pragma unroll
       for (int m = 0; m < 2; ++m)
@@ -546,7 +548,7 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
       uint64_t before;
       const uint32_t bin = kBins - 1 - sa_find(s, rule.k, before);
       // (two bins and a step more: theirs are rounded products, and the difference may be rounded up to a logit)
-      low = fmaxf(sa_below(least), sa_below(rule.top - (bin + 2) / to_bins));
+      low = fmaxf(low, sa_below(rule.top - (bin + 2) / to_bins));
     }
   } else if (rule.k == 0 && rule.p < 1.0) {
     // Bins of 1/64 of a temperature: beyond the last no logit has any weight.

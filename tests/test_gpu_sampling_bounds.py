@@ -59,3 +59,19 @@ def test_two_neighbouring_values(value, settings):
     x = torch.full((8, 9000), value)
     x[:, 4321] = torch.nextafter(x[0, 0], torch.tensor(math.inf))
     assert _check(x, _U, **settings) >= 7
+
+
+@pytest.mark.parametrize("settings", [dict(top_k=50), dict(top_k=1500), dict(top_k=50, top_p=0.5)], ids=str)
+@pytest.mark.parametrize("scale", [1e-36, 1e-37, 1e-40, 1e-44])
+def test_the_smallest_logits(scale, settings):
+    """Logits whose range's reciprocal float32 does not hold, a single one above zeros among them."""
+    g = torch.Generator().manual_seed(4)
+    x = scale * torch.randn(8, 9000, generator=g)
+    x[4:] = 0.0
+    x[4:, 777] = scale
+    assert _check(x, _U, **settings) >= 7
+
+
+@pytest.mark.parametrize("settings", [dict(top_k=2), dict(top_k=50), dict(top_k=1500, top_p=0.5)], ids=str)
+def test_two_neighbouring_small_values(settings):
+    test_two_neighbouring_values(1e-30, settings)
