@@ -551,8 +551,9 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
       low = fmaxf(low, sa_below(rule.top - (bin + 2) / to_bins));
     }
   } else if (rule.k == 0 && rule.p < 1.0) {
-    // Bins of 1/64 of a temperature: beyond the last no logit has any weight.
-    to_bins = (float)(64.0 / t);
+    // Bins of 1/64 of a temperature, or more where float32 does not hold so large a factor (the largest logit's
+    // distance, 0, times infinity would be none): beyond the last no logit has any weight.
+    to_bins = (float)fmin(64.0 / t, 0x1.fffffep127);
     sa_clear(s);
     row.each([&](int, float x) {
       const uint64_t w = rule.weight(x);

@@ -75,3 +75,12 @@ def test_the_smallest_logits(scale, settings):
 @pytest.mark.parametrize("settings", [dict(top_k=2), dict(top_k=50), dict(top_k=1500, top_p=0.5)], ids=str)
 def test_two_neighbouring_small_values(settings):
     test_two_neighbouring_values(1e-30, settings)
+
+
+@pytest.mark.parametrize("scale,temperature", [(1e-38, 1e-38), (1e-37, 1e-37), (1e-40, 3e-40), (1e-38, 1e-30), (1.0, 1e-40)])
+@pytest.mark.parametrize("settings", [dict(top_p=0.5), dict(top_p=0.9, min_p=0.02), dict(top_k=5000, top_p=0.5)], ids=str)
+def test_the_smallest_temperatures(scale, temperature, settings):
+    """Temperatures whose reciprocal float32 does not hold, with weights that matter."""
+    g = torch.Generator().manual_seed(5)
+    x = scale * torch.randn(8, 10007, generator=g)
+    assert _check(x, _U, temperature=temperature, **settings) >= 7
