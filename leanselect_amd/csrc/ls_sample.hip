@@ -248,16 +248,18 @@ __device__ __forceinline__ uint32_t sa_border(const Row& row, SaShared& s, uint6
 struct SaRule {
   float top;
   double inv;         // 1 / temperature
-  double scale, off;  // a logit's base-2 exponent: scale x + off
+  double scale;       // a weight's base-2 exponent: scale (x - top)
   int k;          // 0: none
   double p;
   float min_cut;  // logits above it pass min_p
   const double* table;
 
   // 2^y in whole numbers of 2^-40, y = m / 64 + f: a table of 2^(k / 64), and 2^f to the fourth power (|f| <
-  // 2^-7: 2^-44).  Rounding to m, and of the result, by adding a number that leaves no smaller bits.
+  // 2^-7: 2^-44).  Rounding to m, and of the result, by adding a number that leaves no smaller bits.  The
+  // difference is formed first (exact, or off by 2^-53 of itself): scale x and scale top would each round by
+  // 2^-53 of what a common offset makes of them.
   __device__ __forceinline__ uint64_t weight(float x) const {
-    const double y = fmax(fma((double)x, scale, off), -60.0);
+    const double y = fmax(((double)x - (double)top) * scale, -60.0);
     const double m = y + 0x1.8p46, f = y - (m - 0x1.8p46);
     const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, m);  // 64 y, rounded
     double q = fma(f, 0.0096181291076284771619, 0.055504108664821579953);
@@ -508,7 +510,6 @@ __global__ __launch_bounds__(kThreads) void ls_sample_kernel(const SaArgs a) {
   }
   rule.inv = 1.0 / t;
   rule.scale = 1.4426950408889634074 / t;
-  rule.off = -(double)rule.top * rule.scale;
   rule.table = s.table;
   rule.k = a.top_ks ? a.top_ks[r] : a.top_k;
   if (rule.k <= 0 || rule.k >= a.vocab) rule.k = 0;

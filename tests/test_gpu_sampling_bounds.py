@@ -84,3 +84,20 @@ def test_the_smallest_temperatures(scale, temperature, settings):
     g = torch.Generator().manual_seed(5)
     x = scale * torch.randn(8, 10007, generator=g)
     assert _check(x, _U, temperature=temperature, **settings) >= 7
+
+
+@pytest.mark.parametrize("offset", [0.0, 1e6, -3e7, 1e9])
+def test_a_draw_next_to_an_edge_far_from_zero(offset):
+    """A weight goes by the distance from the largest logit, which a common offset does not change: numbers
+    2^-38 to 2^-29 from the edge between two tokens, on both sides of it."""
+    t = torch.linspace(0.5, 3.0, 60001)
+    step = 2.0 ** max(1, math.frexp(offset)[1] - 23)  # (representable apart)
+    t = t * step
+    edge = 1.0 / (1.0 + torch.exp(-step / t.double()))
+    u = edge.float()
+    gap = (u.double() - edge).abs()
+    near = (gap > 2.0 ** -38) & (gap < 2.0 ** -29)
+    t, u = t[near], u[near]
+    x = torch.tensor([[offset, offset - step]]).expand(len(t), 2).contiguous()
+    assert len(t) > 500
+    assert _check(x, u, temperature=t) == len(t)
