@@ -586,10 +586,11 @@ class MiniCPMLeanSelect:
             # Each sequence's logits are read at its last token, which an empty
             # sequence does not have.
             raise ValueError("every packed sequence must hold at least one token")
+        if cache is not None and (cache.batch != len(cu_host) - 1 or any(cache.positions)):
+            # (a fork is not empty: its sequences go on behind the prefix, which decode_step attends)
+            raise ValueError("prefill fills an empty cache with one slot per sequence")
         dev = _hip.require_gpu(input_ids)
         if cache is not None:
-            if cache.batch != len(cu_host) - 1 or any(cache.lengths):
-                raise ValueError("prefill fills an empty cache with one slot per sequence")
             cache.begin([b - a for a, b in zip(cu_host, cu_host[1:])])
         cu = torch.tensor(cu_host, dtype=torch.int32, device=dev)
         pos = self.positions(cu_host, dev)
