@@ -126,7 +126,7 @@ class LeanSelectKVCache:
         return SharedPrefixKVCache(self, batch, capacity)
 
     def get_seq_length(self) -> int:
-        """Tokens of the longest sequence (outside a step)."""
+        """Tokens of the longest sequence, a shared prefix included (outside a step)."""
         return max(self.lengths)
 
     def _require_step(self):
@@ -169,6 +169,9 @@ class SharedPrefixKVCache(LeanSelectKVCache):
     @property
     def positions(self) -> list[int]:
         return [self.prefix_len + n for n in self.lengths]
+
+    def get_seq_length(self) -> int:
+        return max(self.positions)
 
     def fork(self, batch: int, capacity: int):
         raise ValueError("only a 16-bit cache without a prefix of its own can be shared")
