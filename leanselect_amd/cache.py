@@ -52,12 +52,15 @@ class LeanSelectKVCache:
         else:
             self.k = torch.empty(shape, dtype=dtype, device=self.device)
             self.v = torch.empty(shape, dtype=dtype, device=self.device)
-        cap_c = max(1, n_windows(cap, kernel_size, kernel_stride))
-        self.kc = torch.empty((num_layers, batch, cap_c, num_kv_heads, head_dim), dtype=dtype,
-                              device=self.device)
+        self.kc = self._compressed_keys((num_layers, batch, num_kv_heads, head_dim), dtype)
         self.lengths = [0] * batch  # tokens held before the open step
         self.seqlens = torch.zeros(batch, dtype=torch.int32, device=self.device)
         self._step = None
+
+    def _compressed_keys(self, shape: tuple[int, ...], dtype: torch.dtype) -> torch.Tensor | None:
+        layers, batch, *rest = shape
+        cap_c = max(1, n_windows(self.capacity, self.kernel_size, self.kernel_stride))
+        return torch.empty((layers, batch, cap_c, *rest), dtype=dtype, device=self.device)
 
     # -- step protocol --------------------------------------------------------
     def begin(self, n_new: list[int]) -> None:
@@ -149,10 +152,12 @@ class SharedPrefixKVCache(LeanSelectKVCache):
         super().__init__(prefix.num_layers, batch, capacity, prefix.k.shape[3], prefix.k.shape[4],
                          dtype=prefix.k.dtype, device=prefix.device, kernel_size=prefix.kernel_size,
                          kernel_stride=prefix.kernel_stride)
-        self.kc = None
         self.prefix_len = prefix.lengths[0]
         self.k_prefix = prefix.k[:, 0, :self.prefix_len]
         self.v_prefix = prefix.v[:, 0, :self.prefix_len]
+
+    def _compressed_keys(self, shape, dtype):
+        return None
 
     def update(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
         st = self._require_step()
