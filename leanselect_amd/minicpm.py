@@ -49,7 +49,7 @@ from . import _hip
 from .cache import LeanSelectKVCache, SharedPrefixKVCache
 from .ops.decode import decode_topk_idx
 from .ops.mx4 import dequantize_mx4, linear_mx4, linear_mx4_silu_mul, quantize_mx4
-from .ops.sampling import sample_logits
+from .ops.sampling import check_settings, sample_logits
 from .prefill import leanselect_sparse_prefill
 from .selector import LeanSelectSelector
 
@@ -672,13 +672,16 @@ class MiniCPMLeanSelect:
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, u: torch.Tensor, **sampling) -> torch.Tensor:
         """int32 ``[n, steps]``: ``n`` answers of ``steps`` tokens to the prompt ``input_ids`` (int32 ``[N]``),
-        drawn by the numbers ``u`` (float32 ``[steps, n]``, in [0, 1)) with ``ops.sample_logits``'s settings.
+        drawn by the numbers ``u`` (float32 ``[steps, n]``, in [0, 1)) with ``ops.sample_logits``'s settings
+        (``temperature``, ``top_k``, ``top_p``, ``min_p``).
 
         The prompt goes through ``prefill`` once; the answers' attention is dense, over the prompt (read
         once for all of them) and their own tokens."""
         if u.ndim != 2 or u.shape[0] < 1 or u.shape[1] < 1 or u.dtype != torch.float32:
             raise ValueError("u must be float32 [steps, answers]")
         steps, n = u.shape
+        each, _ = check_settings(n, **sampling)  # (before the prompt's pass)
+        _hip.require_gpu(input_ids, u, *each)
         prompt = self.new_cache(1, input_ids.numel())
         logits = self.prefill(input_ids, cache=prompt)
         cache = prompt.fork(n, max(1, steps - 1))

@@ -18,6 +18,33 @@ _CODES = {torch.float32: _hip.LS_F32, torch.bfloat16: _hip.LS_BF16, torch.float1
 _MAX_VOCAB = 1 << 19
 
 
+def check_settings(rows: int, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> tuple[list, list]:
+    """The settings' tensors and their numbers (None for the other kind), or ``ValueError`` for what
+    ``sample_logits`` does not take for ``rows`` rows."""
+    each = []
+    numbers = []
+    for name, value, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                               ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if torch.is_tensor(value):
+            if value.dtype is not dtype or value.shape != (rows,):
+                raise ValueError(f"{name} must be a number or {dtype} [{rows}]")
+            each.append(value)
+            numbers.append(None)
+        else:
+            each.append(None)
+            numbers.append(value)
+    t, k, p, m = numbers
+    if t is not None and not 0.0 <= t < math.inf:
+        raise ValueError(f"temperature must be 0 or more and finite (got {t})")
+    if k is not None and (not math.isfinite(k) or k != int(k)):
+        raise ValueError(f"top_k must be a whole number (got {k})")
+    if p is not None and not p > 0.0:
+        raise ValueError(f"top_p must be above 0 (got {p})")
+    if m is not None and not 0.0 <= m <= 1.0:
+        raise ValueError(f"min_p must be 0 to 1 (got {m})")
+    return each, numbers
+
+
 def sample_logits(logits: torch.Tensor, u: torch.Tensor, *, temperature: float | torch.Tensor = 1.0,
                   top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0,
                   min_p: float | torch.Tensor = 0.0, return_logprob: bool = False):
@@ -44,27 +71,7 @@ def sample_logits(logits: torch.Tensor, u: torch.Tensor, *, temperature: float |
         raise ValueError(f"the vocabulary must hold 1 to {_MAX_VOCAB} tokens (got {vocab})")
     if u.dtype is not torch.float32 or u.shape != (rows,):
         raise ValueError(f"u must be float32 [{rows}]")
-    each = []
-    numbers = []
-    for name, value, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                               ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if torch.is_tensor(value):
-            if value.dtype is not dtype or value.shape != (rows,):
-                raise ValueError(f"{name} must be a number or {dtype} [{rows}]")
-            each.append(value)
-            numbers.append(None)
-        else:
-            each.append(None)
-            numbers.append(value)
-    t, k, p, m = numbers
-    if t is not None and not 0.0 <= t < math.inf:
-        raise ValueError(f"temperature must be 0 or more and finite (got {t})")
-    if k is not None and (not math.isfinite(k) or k != int(k)):
-        raise ValueError(f"top_k must be a whole number (got {k})")
-    if p is not None and not p > 0.0:
-        raise ValueError(f"top_p must be above 0 (got {p})")
-    if m is not None and not 0.0 <= m <= 1.0:
-        raise ValueError(f"min_p must be 0 to 1 (got {m})")
+    each, (t, k, p, m) = check_settings(rows, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     index = _hip.gpu_index(logits, u, *each)
     if vocab > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()

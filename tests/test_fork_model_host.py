@@ -30,3 +30,12 @@ def test_a_fork_is_not_prefilled(batch):
         MiniCPMLeanSelect.prefill(SimpleNamespace(cfg=None), ids, cu, cache=_prompt())
     with pytest.raises(RuntimeError, match="GPU"):  # an empty one is taken
         MiniCPMLeanSelect.prefill(SimpleNamespace(cfg=None), ids[:2], cache=_prompt(0))
+
+
+@pytest.mark.parametrize("sampling,error", [
+    (dict(return_logprob=True), TypeError), (dict(temperature=-1.0), ValueError), (dict(top_p=0.0), ValueError),
+    (dict(top_k=torch.zeros(2, dtype=torch.int32)), ValueError), (dict(), RuntimeError)], ids=str)
+def test_settings_are_checked_before_the_prompts_pass(sampling, error):
+    model = SimpleNamespace(new_cache=lambda *a: pytest.fail("a cache was made"))
+    with pytest.raises(error):
+        MiniCPMLeanSelect.generate(model, torch.zeros(5, dtype=torch.int32), torch.zeros(4, 3), **sampling)
