@@ -191,7 +191,8 @@ struct CaState {
   ls_f32x4 o[8][NC];
   ls_f32x4 l[NC];             // the sum of a column's weights, by a product with ones: four times the same
   float m[NC];
-  float slope2[NC], pos[NC];  // position among the source's keys
+  float slope2[NC];
+  int pos[NC];                // position among the source's keys, less the lane's first key of a step
   int lo[NC], hi[NC];         // visible keys, among the source's
 };
 
@@ -241,7 +242,9 @@ __device__ __forceinline__ void ca_step(uint32_t sk, uint32_t sv, int key0, CaSt
   if (a.slopes) {
 #pragma unroll
     for (int nc = 0; nc < NC; ++nc) {
-      const float d0 = st.pos[nc] - (float)(key0 + 4 * q);
+      // In whole numbers: both may be past 2^24.  (key0 said to be scalar: else the loops' counter goes to a vector
+      // register for it, and a 1024-row chunk behind 32K tokens, which has no slopes, takes 870 us, not 855.)
+      const float d0 = (float)(st.pos[nc] - __builtin_amdgcn_readfirstlane(key0));
 #pragma unroll
       for (int t = 0; t < KB; ++t)
 #pragma unroll
@@ -530,7 +533,8 @@ __device__ __forceinline__ void ca_columns(const CaArgs& a, const CaWork& w, int
     st.hi[nc] = w.n_keys;
     st.m[nc] = -INFINITY;
     st.l[nc] = ls_f32x4{0.f, 0.f, 0.f, 0.f};
-    st.pos[nc] = st.slope2[nc] = 0.f;
+    st.slope2[nc] = 0.f;
+    st.pos[nc] = 0;
     if (a.slopes || a.causal || a.left >= 0 || a.right >= 0) {
       int n0 = w.n0, n1 = w.n1, len = w.len, b = w.seq;
       if (b < 0) {
@@ -540,7 +544,7 @@ __device__ __forceinline__ void ca_columns(const CaArgs& a, const CaWork& w, int
         len = max(0, min(a.lens[b], a.capacity));
       }
       const int p = a.p_len + len - (n1 - n0) + (t - n0) - w.first;
-      st.pos[nc] = (float)p;
+      st.pos[nc] = p - 4 * q;
       if (a.slopes) st.slope2[nc] = a.slopes[b * a.slopes_bs + w.g * a.gs + h] * kLog2e;
       if (a.causal) st.hi[nc] = min(st.hi[nc], p + 1);
       if (a.left >= 0) st.lo[nc] = max(0, p - a.left);
