@@ -1095,7 +1095,9 @@ extern "C" int ls_cache_attn(const void* q, int64_t q_row_stride, const int32_t*
   a.gs = gs;
   a.alpha = softcap > 0.f ? 2.f * softcap * kLog2e : softmax_scale * kLog2e;
   a.beta = softcap > 0.f ? softcap * kLog2e : 0.f;
-  a.cap_b = softcap > 0.f ? 2.f * softmax_scale * kLog2e / softcap : 0.f;
+  // (a factor past float32's range either way gives what its end does: +-cap for any product but 0, or 0 for all)
+  a.cap_b = softcap > 0.f ? (float)std::min(std::max(2.0 * softmax_scale * kLog2e / softcap, 0x1p-126), 0x1.fffffep127)
+                          : 0.f;
   a.slopes = alibi_slopes;
   a.slopes_bs = alibi_batch_stride;
   a.causal = causal != 0;
