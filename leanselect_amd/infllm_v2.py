@@ -16,8 +16,9 @@ from __future__ import annotations
 
 import torch
 
+from . import _hip
 from .ops.attention import infllmv2_attn_varlen_func
-from .ops.cache_attention import check_scores
+from .ops.cache_attention import check_attention
 from .ops.decode import (dense_attention_kvcache, kvcache_append, sparse_attention_kvcache,
                          stage1_scores)
 from .ops.nosa import max_pooling_1d_varlen
@@ -101,7 +102,8 @@ def infllmv2_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=N
     B, Sq, H, D = q.shape
     G = k_cache.shape[2]
     if scored:  # before anything is appended
-        check_scores(softmax_scale, softcap, alibi_slopes, B, H)
+        check_attention(q.reshape(B * Sq, H, D), k_cache, v_cache, softmax_scale, softcap, alibi_slopes, window_size)
+        _hip.require_gpu(q, k_cache, v_cache, alibi_slopes)
     dev = q.device
     if cache_seqlens is None:
         cache_seqlens = 0

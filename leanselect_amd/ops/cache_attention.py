@@ -16,6 +16,7 @@ call for a shared prefix.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from functools import lru_cache
 
@@ -62,9 +63,10 @@ def scored_attention(q, k_cache, v_cache, cache_seqlens, cu_seqlens_q, max_len, 
 
 def check_scores(softmax_scale, softcap, alibi_slopes, batch: int, num_heads: int) -> tuple[float, float]:
     """The scale and the cap as numbers, or ``ValueError`` for options that no call takes."""
-    scale, softcap = _SCALE if softmax_scale is None else float(softmax_scale), float(softcap)
+    scale = _SCALE if softmax_scale is None else ctypes.c_float(float(softmax_scale)).value
+    softcap = float(softcap)
     if not 0.0 < scale < math.inf or not 0.0 <= softcap < math.inf:
-        raise ValueError("softmax_scale must be positive and softcap not negative, both finite")
+        raise ValueError("softmax_scale must be positive and softcap not negative, both finite (in float32)")
     if softcap and not 1e-20 <= softcap <= 512.0:
         raise ValueError(f"softcap must be 0 or from 1e-20 to 512 (got {softcap})")
     if alibi_slopes is not None and (alibi_slopes.dtype is not torch.float32
@@ -95,29 +97,40 @@ def _key_strides(k: torch.Tensor, v: torch.Tensor, name: str) -> tuple[int, ...]
                 strides.append(step)
             step = strides[-1] * n
         strides = tuple(reversed(strides))
-    if not ok or (k.data_ptr() | v.data_ptr()) & 15:
-        raise ValueError(f"{name} rows must be dense and 16-byte aligned, k and v with the same strides")
+    if not ok or (k.data_ptr() | v.data_ptr()) & 15 or strides[-3] >= 1 << 24:
+        raise ValueError(f"{name} rows must be dense, 16-byte aligned and less than 2^24 elements apart, k and v with the "
+                         "same strides")
     return strides[:-2]
 
 
-def _attend(q, k_prefix, v_prefix, k_cache, v_cache, cache_seqlens, cu_seqlens_q, max_len, causal,
-            softmax_scale, softcap, alibi_slopes, window, n_splits, return_lse, out):
+def check_attention(q, k_cache, v_cache, softmax_scale, softcap, alibi_slopes, window) -> tuple:
+    """The numbers of a call on ``q`` and the cache (scale, cap, window and the cache's strides), or ``ValueError``
+    for what no call takes, whatever the lengths."""
     dtype, q_shape, c_shape = q.dtype, q.shape, k_cache.shape
-    code = _CODES.get(dtype)
-    if code is None or len(q_shape) != 3 or q_shape[2] != HEAD_DIM:
+    if dtype not in _CODES or len(q_shape) != 3 or q_shape[2] != HEAD_DIM:
         raise ValueError(f"q must be bf16 or fp16 [total_q, H, {HEAD_DIM}]")
     if len(c_shape) != 4 or c_shape[3] != HEAD_DIM or v_cache.shape != c_shape:
         raise ValueError(f"k_cache and v_cache must be [batch, capacity, num_kv_heads, {HEAD_DIM}]")
-    total_q, H, _ = q_shape
-    B, capacity, G, _ = c_shape
+    H, (B, capacity, G, _) = q_shape[1], c_shape
     if B < 1 or G < 1 or H % G or not G <= H <= 16 * G:
         raise ValueError(f"q's {H} heads must be a multiple of the cache's {G}, at most 16 times")
     if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         raise ValueError("q and the cache must share a dtype")
+    if q_shape[0] * H >= 1 << 23 or capacity >= 1 << 30:
+        raise ValueError("a call takes fewer than 2^23 rows and heads, and fewer than 2^30 keys a sequence")
+    left, right = (min(max(int(x), -1), 1 << 30) for x in window)
+    scale, softcap = check_scores(softmax_scale, softcap, alibi_slopes, B, H)
+    return scale, softcap, left, right, *_key_strides(k_cache, v_cache, "the cache's")
+
+
+def _attend(q, k_prefix, v_prefix, k_cache, v_cache, cache_seqlens, cu_seqlens_q, max_len, causal,
+            softmax_scale, softcap, alibi_slopes, window, n_splits, return_lse, out):
+    scale, softcap, left, right, c_batch, c_row = check_attention(q, k_cache, v_cache, softmax_scale, softcap,
+                                                                  alibi_slopes, window)
+    dtype, (total_q, H, _), (B, capacity, G, _) = q.dtype, q.shape, k_cache.shape
     if cache_seqlens.dtype is not torch.int32 or cache_seqlens.shape != (B,) \
             or cu_seqlens_q.dtype is not torch.int32 or cu_seqlens_q.shape != (B + 1,):
         raise ValueError("cache_seqlens must be int32 [batch] and cu_seqlens_q int32 [batch + 1]")
-    c_batch, c_row = _key_strides(k_cache, v_cache, "the cache's")
     P, p_row = 0, 0
     if k_prefix is not None:
         P = k_prefix.shape[0]
@@ -125,8 +138,6 @@ def _attend(q, k_prefix, v_prefix, k_cache, v_cache, cache_seqlens, cu_seqlens_q
             raise ValueError(f"the prefix must be [prefix_len, {G}, {HEAD_DIM}] in q's dtype")
         if P:
             p_row, = _key_strides(k_prefix, v_prefix, "the prefix's")
-    scale, softcap = check_scores(softmax_scale, softcap, alibi_slopes, B, H)
-    left, right = (min(max(int(x), -1), 1 << 30) for x in window)
     slopes_stride = 0
     if alibi_slopes is not None:
         alibi_slopes = alibi_slopes.contiguous()
@@ -152,7 +163,7 @@ def _attend(q, k_prefix, v_prefix, k_cache, v_cache, cache_seqlens, cu_seqlens_q
     _hip.launch(index, "ls_cache_attn", q_ptr, row[0], cu_seqlens_q.data_ptr(), total_q,
                 k_prefix.data_ptr() if P else None, v_prefix.data_ptr() if P else None, p_row, P,
                 k_cache.data_ptr(), v_cache.data_ptr(), c_batch, c_row, capacity,
-                cache_seqlens.data_ptr(), B, H, G, HEAD_DIM, code, max_len, scale, 1 if causal else 0,
+                cache_seqlens.data_ptr(), B, H, G, HEAD_DIM, _CODES[dtype], max_len, scale, 1 if causal else 0,
                 softcap, None if alibi_slopes is None else alibi_slopes.data_ptr(), slopes_stride,
                 left, right, splits, out.data_ptr(), lse.data_ptr() if return_lse else None,
                 ws.data_ptr() if nbytes else None, nbytes)
