@@ -686,7 +686,7 @@ int ls_attn_kvcache_q8(const void* q, int64_t q_row_stride, const int32_t* cu_se
  * p = prefix_len + len_b - n_b + i; key j of prefix_len + len_b (the prefix first) is
  * visible where, with causal, j <= p, with window_left >= 0, j >= p - window_left, and with
  * window_right >= 0, j <= p + window_right.  Scores x = softmax_scale q.k, then
- * softcap tanh(x / softcap) where softcap > 0 (then 1e-20 to 512), then less alibi_slopes[b alibi_batch_stride + h]
+ * softcap tanh(x / softcap) where softcap > 0 (then 1e-20 to 512; within softcap 2^-21), then less alibi_slopes[b alibi_batch_stride + h]
  * |p - j| where given (float32).  k_prefix / v_prefix [prefix_len][G][128], rows prefix_row_stride
  * apart; k_cache / v_cache [batch][capacity][G][128]; lengths past capacity count as it.  out
  * [total_q, H, 128], softmax_lse float32 [H, total_q] (natural log) or NULL; a row that sees no key,

@@ -20,9 +20,9 @@
 // the keys' bytes; sixteen sequences of 2K to 64K take 66 us (4.6 TB/s), eight of up to 16K with 8 KV heads
 // 53 us (4.0), and one row with a window of 4096 16 us, which are two launches and one step's latency.  Many
 // rows: the vector units and the matrix units of a wave and its neighbour, which overlap only in part: of a
-// 1024-row chunk behind 32K tokens with capped scores (850 us, 655 TFLOP/s of plain products, 1000 with those
+// 1024-row chunk behind 32K tokens with capped scores (855 us, 654 TFLOP/s of plain products, 1000 with those
 // of the remainders) the matrix units are busy 35% and the vector ones 52% of the time, of two prompts
-// in fp16 with a bias (202 us) 44% and 69%.  Two groups of waves held half a step apart by barriers, so that
+// in fp16 with a bias (204 us) 44% and 69%.  Two groups of waves held half a step apart by barriers, so that
 // one's products meet the other's exponentials, took 898 us; the next step's scores in between this one's
 // weights and the last one's products, 1038 where the plain order took 1027.
 //
@@ -98,7 +98,7 @@ struct CaArgs {
   // (cap tanh(x / cap) = cap - 2 cap / (1 + exp(2 x / cap))); with slopes the score itself, less its bias.
   float alpha;
   float beta;
-  float cap_b;  // 0: no cap.  z is off by 2^-23, so the score by cap 2^-22: 2^-13 at the largest cap taken
+  float cap_b;  // 0: no cap.  z is off by 2^-23 or so, at most 2^-22, and the score by 2 cap times that
   const float* slopes;
   int64_t slopes_bs;
   int causal;

@@ -9,8 +9,8 @@ shares a prefix, on the GPU.
 A sequence with ``n`` query rows and ``len`` keys, the prefix's ``P`` included, has its row ``i`` at position
 ``p = len - n + i``.  Key ``j < len`` is visible where, with ``causal``, ``j <= p`` and, with ``window = (left,
 right)``, ``p - left <= j <= p + right`` (a negative side is open).  A score is ``x = scale * q.k``, then
-``softcap * tanh(x / softcap)`` (0: not capped; at most 512, up to where the cap's float32 form is within
-2^-13), then less ``alibi_slopes[h] * |p - j|``: the options of
+``softcap * tanh(x / softcap)`` (0: not capped; at most 512; the cap's float32 form, and with it ``lse``, is
+within ``softcap * 2^-21``), then less ``alibi_slopes[h] * |p - j|``: the options of
 ``infllmv2_attn_with_kvcache`` (third_party/infllmv2/paper1.patch:2511-2615).  The reference has no
 call for a shared prefix.
 """
