@@ -23,7 +23,7 @@
 // What bounds it: a row's passes by one CU's vector work, not the card's memory.  Of 73448 float32 logits, 2.4
 // GHz: the largest ones 13 thousand cycles (5 us), the histogram 44 (a weight is some 25 instructions in 64
 // bits, and an addition in LDS), a gather 16, all of up to 256 by comparison 16, the draw from the row 60.  One
-// row with top-k 50 and top-p takes 24 us, 16 rows of bf16 with top-p and min-p 42, 256 rows of mixed
+// row with top-k 50 and top-p takes 24 us, 16 rows of bf16 with top-p and min-p 40, 256 rows of mixed
 // settings 93 (0.8 TB/s); a greedy row 15, 256 of them 24 (3.1 TB/s).  Several workgroups a row would
 // have to join their sums through memory, a launch or a wait at each of the cuts; a row stays with one.
 //

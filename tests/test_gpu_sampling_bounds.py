@@ -6,7 +6,6 @@ import pytest
 import torch
 
 from leanselect_amd.ops import sample_logits
-from oracle import serving_oracle as so
 from test_gpu_sampling import DEV, DTYPES, _check
 
 pytestmark = pytest.mark.gpu
