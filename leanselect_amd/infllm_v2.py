@@ -101,8 +101,9 @@ def infllmv2_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=N
         raise ValueError("q must be [B, Sq, H, D] and k_cache / v_cache [B, capacity, G, D]")
     B, Sq, H, D = q.shape
     G = k_cache.shape[2]
+    qr = q.reshape(B * Sq, H, D)
     if scored:  # before anything is appended
-        check_attention(q.reshape(B * Sq, H, D), k_cache, v_cache, softmax_scale, softcap, alibi_slopes, window_size)
+        check_attention(qr, k_cache, v_cache, softmax_scale, softcap, alibi_slopes, window_size)
         _hip.require_gpu(q, k_cache, v_cache, alibi_slopes)
     dev = q.device
     if cache_seqlens is None:
@@ -124,7 +125,6 @@ def infllmv2_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=N
         lens = [x + s_new for x in lens]
         cache_seqlens = torch.tensor(lens, dtype=torch.int32, device=dev)
     cu_q = torch.arange(0, B * Sq + 1, Sq, dtype=torch.int32, device=dev)
-    qr = q.reshape(B * Sq, H, D)
     splits = num_splits if num_splits > 0 else None
     if topk_idx is None:  # every cached page
         res = dense_attention_kvcache(qr, k_cache, v_cache, cache_seqlens, cu_q, max(lens),
